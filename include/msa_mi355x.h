@@ -227,6 +227,39 @@ int msa_indexer_kl(const void* index_q, const void* index_k, const void* q, cons
                    const float* teacher_lse, float* loss, float* row_kl, float* grad_index_q,
                    float* grad_index_k, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* RMS norm of every query and key head, then the rotation of its token's position; no
+ * reference kernel (the reference takes normed and rotated inputs, docs/msa_training_flow.md:18-38).
+ * y = rotate(x / sqrt(mean x^2 + eps) * weight), the rotation over the first rotary_dim dims in
+ * pairs (i, i + rotary_dim / 2). q [T,Hq,D] and k [T,Hkv,D] with free token and head strides (in
+ * elements; unit stride along D); either side may have 0 heads and NULL pointers. q_out / k_out are
+ * contiguous. Weights [D] of the input dtype or fp32 (weight_dtype, shared). cos_sin: fp32
+ * [table_rows, rotary_dim], cosines then sines (unread, may be NULL, with rotary_dim 0). A token's
+ * position is its offset in its sequence plus context_lens of that sequence (NULL: 0); rotated dims of a
+ * position outside the table are NaN. head_dim up to 512 (status 2 above). */
+int msa_qk_norm_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t q_heads, const void* k,
+                     int64_t k_stride_t, int64_t k_stride_h, int64_t k_heads, int32_t dtype,
+                     const void* q_weight, const void* k_weight, int32_t weight_dtype, const float* cos_sin,
+                     int64_t table_rows, int64_t rotary_dim, const int32_t* cu_seqlens, int64_t num_seqs,
+                     const int32_t* context_lens, int64_t total_tokens, int64_t head_dim, double eps,
+                     void* q_out, void* k_out, void* stream);
+
+/* Workspace of msa_qk_norm_rope_bwd in bytes where it computes a weight's gradient, for the heads of the
+ * sides that get a gradient at all (0 heads for a side that gets none). */
+int64_t msa_qk_norm_rope_bwd_workspace_bytes(int64_t total_tokens, int64_t q_heads, int64_t k_heads,
+                                             int64_t head_dim);
+
+/* Gradients of msa_qk_norm_rope from contiguous grad_q_out / grad_k_out: grad_q and grad_k contiguous, in
+ * the input dtype, grad_q_weight and grad_k_weight in weight_dtype; each nullable. Deterministic: the weights'
+ * sums run in a fixed order. */
+int msa_qk_norm_rope_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t q_heads, const void* k,
+                         int64_t k_stride_t, int64_t k_stride_h, int64_t k_heads, int32_t dtype,
+                         const void* q_weight, const void* k_weight, int32_t weight_dtype, const float* cos_sin,
+                         int64_t table_rows, int64_t rotary_dim, const int32_t* cu_seqlens, int64_t num_seqs,
+                         const int32_t* context_lens, int64_t total_tokens, int64_t head_dim, double eps,
+                         const void* grad_q_out, const void* grad_k_out, void* grad_q, void* grad_k,
+                         void* grad_q_weight, void* grad_k_weight, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
 /* Testing hook; no counterpart in the reference. Overrides the byte budgets that size
  * the query-token chunks of the KV-major bf16 passes: msa_attn_fwd (default 2 GiB of
  * per-(token, head, slot) partial records per chunk), msa_attn_bwd (3 GiB) and

@@ -23,6 +23,12 @@ is the first two stages in one call (score and selection kernels back to back);
 is the indexer's KL training loss over the selected tokens (teacher: the detached
 attention probabilities; student: the index token logits);
 
+    m3_qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, *, eps=1e-6,
+                    context_lens=None) -> (q_out, k_out)
+
+norms the query and key heads and rotates them by their positions (``rope_table``), before the
+stages above, with gradients;
+
     prepare_sequences(cu_seqlens, *, block_size=128) -> PackedSequences
 
 validates ``cu_seqlens`` once and returns immutable metadata with device copies;
@@ -75,6 +81,18 @@ def m3_indexer_kl(index_q, index_k, q, k, indices, cu_seqlens, max_seqlen, *, bl
                           index_scale=index_scale, scale=scale, return_rows=return_rows, teacher_lse=teacher_lse)
 
 
+def m3_qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, *, eps=1e-6, context_lens=None):
+    from .norm_rope import m3_qk_norm_rope as implementation
+
+    return implementation(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps=eps, context_lens=context_lens)
+
+
+def rope_table(num_positions, rotary_dim, *, base=10000.0, device=None):
+    from .norm_rope import rope_table as implementation
+
+    return implementation(num_positions, rotary_dim, base=base, device=device)
+
+
 def prepare_sequences(cu_seqlens, *, block_size=128):
     from .layout import prepare_sequences as implementation
 
@@ -82,4 +100,4 @@ def prepare_sequences(cu_seqlens, *, block_size=128):
 
 
 __all__ = ["m3_index_score", "m3_topk", "m3_sparse_attention", "m3_index_score_topk", "m3_indexer_kl",
-           "prepare_sequences", "PackedSequences"]
+           "m3_qk_norm_rope", "rope_table", "prepare_sequences", "PackedSequences"]

@@ -1,0 +1,147 @@
+// A row of D elements (one head of one token) held by a run of LPR lanes, for the kernels that norm and
+// rotate rows: a lane has VEC elements of the first and VEC of the second half of the rotated part, or of the
+// two halves of the rest, so that the pairs the rotation mixes are in one lane.
+#pragma once
+#include "mfma_util.hpp"
+
+namespace msa {
+
+constexpr int kNormThreads = 256;
+
+struct RopeTable {
+  const float* table;  // [rows][2 * half]: cosines, then sines
+  int64_t rows;
+  int half;  // rotated dims / 2
+};
+
+// Sum over runs of LPR lanes.
+template <int LPR>
+__device__ __forceinline__ float run_sum(float v) {
+#define MSA_DPP_ADD(CTRL) \
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xF, 0xF, false));
+  if constexpr (LPR >= 2) MSA_DPP_ADD(0xB1)   // quad_perm [1, 0, 3, 2]
+  if constexpr (LPR >= 4) MSA_DPP_ADD(0x4E)   // quad_perm [2, 3, 0, 1]
+  if constexpr (LPR >= 8) MSA_DPP_ADD(0x141)  // row_half_mirror
+  if constexpr (LPR >= 16) MSA_DPP_ADD(0x140) // row_mirror
+#undef MSA_DPP_ADD
+  if constexpr (LPR >= 32) v += __shfl_xor(v, 16, kWave);
+  if constexpr (LPR >= 64) v += __shfl_xor(v, 32, kWave);
+  return v;
+}
+
+template <int DT, int VEC>
+__device__ __forceinline__ void load_vec(const void* __restrict__ p, int64_t i, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = load_as_f32<DT>(p, i);
+  } else if constexpr (DT == kF32) {
+    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 x = s[0], y = s[1];
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[2 * j] = lo16_f32<DT>(w[j]), v[2 * j + 1] = hi16_f32<DT>(w[j]);
+  }
+}
+
+template <int DT, int VEC>
+__device__ __forceinline__ void store_vec(void* __restrict__ p, int64_t i, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    store_from_f32<DT>(p, i, v[0]);
+  } else if constexpr (DT == kF32) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+    d[0] = make_float4(v[0], v[1], v[2], v[3]);
+    d[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = DT == kF16 ? cvt_pk_f16(v[2 * j], v[2 * j + 1]) : cvt_pk_bf16(v[2 * j], v[2 * j + 1]);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// The two element runs [a, a + VEC) and [b, b + VEC) of pair chunk `p` of a row, and whether the
+// rotation mixes them. ok: the chunk exists; b_ok: its second run does (the rest may be odd).
+struct PairChunk {
+  int a, b;
+  bool turned, ok, b_ok;
+};
+template <int VEC>
+__device__ __forceinline__ PairChunk pair_chunk(int p, int half, int dim) {
+  const int hc = half / VEC;
+  if (p < hc) return PairChunk{p * VEC, p * VEC + half, true, true, true};
+  const int rest = dim - 2 * half, rc = (rest + 2 * VEC - 1) / (2 * VEC), a = 2 * half + (p - hc) * VEC;
+  const bool ok = p - hc < rc;
+  return PairChunk{a, a + rc * VEC, false, ok, ok && a + rc * VEC < dim};
+}
+
+// One row's rotation factors for a pair chunk: (1, 0) past rot, NaN where the position has no table row.
+template <int VEC>
+__device__ __forceinline__ void load_turn(const RopeTable& R, const PairChunk& pc, int pos, float (&co)[VEC],
+                                          float (&si)[VEC]) {
+  const bool known = pos >= 0 && pos < R.rows;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) co[j] = pc.turned ? __builtin_nanf("") : 1.f, si[j] = 0.f;
+  if (pc.turned && known) {
+    const float* row = R.table + static_cast<int64_t>(pos) * (2 * R.half) + pc.a;
+    load_vec<kF32, VEC>(row, 0, co);
+    load_vec<kF32, VEC>(row, R.half, si);
+  }
+}
+
+template <int DT, int VEC, int C, int LPR>
+struct RowLanes {
+  static constexpr int kRows = kNormThreads / LPR;  // rows a workgroup holds at once
+  PairChunk pc[C];
+  float wa[C][VEC], wb[C][VEC];
+  __device__ __forceinline__ RowLanes(const void* w, bool w_f32, int half, int dim) {
+    const int l = threadIdx.x % LPR;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      pc[c] = pair_chunk<VEC>(l + c * LPR, half, dim);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) wa[c][j] = wb[c][j] = 0.f;
+      if (!w) continue;
+      if (w_f32) {
+        if (pc[c].ok) load_vec<kF32, VEC>(w, pc[c].a, wa[c]);
+        if (pc[c].b_ok) load_vec<kF32, VEC>(w, pc[c].b, wb[c]);
+      } else {
+        if (pc[c].ok) load_vec<DT, VEC>(w, pc[c].a, wa[c]);
+        if (pc[c].b_ok) load_vec<DT, VEC>(w, pc[c].b, wb[c]);
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const void* p, int64_t at, bool live, float (&a)[C][VEC], float (&b)[C][VEC]) const {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) a[c][j] = b[c][j] = 0.f;
+      if (live && pc[c].ok) load_vec<DT, VEC>(p, at + pc[c].a, a[c]);
+      if (live && pc[c].b_ok) load_vec<DT, VEC>(p, at + pc[c].b, b[c]);
+    }
+  }
+  __device__ __forceinline__ void store(void* p, int64_t at, const float (&a)[C][VEC], const float (&b)[C][VEC]) const {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (pc[c].ok) store_vec<DT, VEC>(p, at + pc[c].a, a[c]);
+      if (pc[c].b_ok) store_vec<DT, VEC>(p, at + pc[c].b, b[c]);
+    }
+  }
+};
+
+template <int C, int VEC>
+__device__ __forceinline__ float sum_products(const float (&a)[C][VEC], const float (&b)[C][VEC],
+                                              const float (&u)[C][VEC], const float (&v)[C][VEC]) {
+  float s = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s = fmaf(a[c][j], u[c][j], fmaf(b[c][j], v[c][j], s));
+  return s;
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace msa

@@ -205,3 +205,30 @@ def prepared_for(seqs: PackedSequences, *, block_size: int, total_tokens: int, d
     if seqs.device != device:
         raise ValueError("prepared sequences must be on the input device")
     return seqs.meta
+
+
+def packed_tokens(cu_seqlens: torch.Tensor | PackedSequences, total_tokens: int, device: torch.device):
+    """``cu_seqlens`` of an operator that needs token bounds only (any block size): the checked device tensor and
+    the number of sequences. A tensor is read on the host, ``PackedSequences`` are not."""
+    if isinstance(cu_seqlens, PackedSequences):
+        prepared_for(cu_seqlens, block_size=cu_seqlens.block_size, total_tokens=total_tokens, device=device)
+        return cu_seqlens.cu_seqlens, cu_seqlens.meta.num_seqs
+    if not isinstance(cu_seqlens, torch.Tensor):
+        raise TypeError("cu_seqlens must be a tensor or PackedSequences")
+    lengths = sequence_lengths(cu_seqlens, total_tokens)
+    if cu_seqlens.device != device:
+        raise ValueError("cu_seqlens must be on the input device")
+    return cu_seqlens.contiguous(), len(lengths)
+
+
+def context_of(context_lens: torch.Tensor | None, num_seqs: int, device: torch.device) -> torch.Tensor | None:
+    """``context_lens`` checked (its values stay on the device)."""
+    if context_lens is None:
+        return None
+    if not isinstance(context_lens, torch.Tensor) or context_lens.dtype != torch.int32:
+        raise TypeError("context_lens must be int32")
+    if context_lens.shape != (num_seqs,):
+        raise ValueError("context_lens must hold one length per sequence")
+    if context_lens.device != device:
+        raise ValueError("context_lens must be on the input device")
+    return context_lens.contiguous()

@@ -1,0 +1,180 @@
+"""RMS norm of query and key heads with the position rotation, in one pass, with autograd.
+
+The projections' outputs become what the indexer and the attention take: per head
+``y = rotate(x / sqrt(mean(x^2) + eps) * weight)``, with the rotation of a token's position over
+the first ``rotary_dim`` dims (pairs ``i``, ``i + rotary_dim / 2``). Positions come from the
+packed metadata that every operator takes, plus the tokens that a cache already holds
+(``context_lens``), so one call serves training, prompts and single tokens.
+
+Execution: ``msa_qk_norm_rope`` / ``msa_qk_norm_rope_bwd`` (one launch, and a second one for the
+gradients of the weights). fp32 arithmetic whatever the input type, each output rounded once.
+Saved state is the inputs; the backward recomputes the norm from them.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .layout import context_of, packed_tokens
+
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+MAX_HEAD_DIM = 512
+
+
+def rope_table(num_positions: int, rotary_dim: int, *, base: float = 10000.0, device=None) -> torch.Tensor:
+    """cos and sin of ``position * base**(-2 i / rotary_dim)``, fp32 ``[num_positions, rotary_dim]``:
+    the ``rotary_dim / 2`` cosines of a position, then its sines. Angles are formed in float64 (fp32 angles of
+    far positions are off by whole radians)."""
+    if not isinstance(num_positions, int) or num_positions < 0:
+        raise ValueError("num_positions must be a nonnegative integer")
+    if not isinstance(rotary_dim, int) or rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be a positive even integer")
+    if not (math.isfinite(base) and base > 0):
+        raise ValueError("base must be positive and finite")
+    half = rotary_dim // 2
+    freq = float(base) ** (-torch.arange(half, dtype=torch.float64, device=device) / half)
+    angle = torch.arange(num_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+def check_table(cos_sin, head_dim, device):
+    """The rotation table's checks: (contiguous table or None, rows, rotary dim)."""
+    if cos_sin is None:
+        return None, 0, 0
+    if cos_sin.ndim != 2 or cos_sin.dtype != torch.float32 or cos_sin.shape[1] % 2:
+        raise ValueError("cos_sin must be fp32 [positions, rotary_dim] with an even rotary_dim")
+    if cos_sin.shape[1] > head_dim:
+        raise ValueError("rotary_dim must not exceed the head dimension")
+    if cos_sin.device != device:
+        raise ValueError("cos_sin must be on the input device")
+    return cos_sin.contiguous(), cos_sin.shape[0], cos_sin.shape[1]
+
+
+def check_weight(weight, x, name):
+    if weight is None or weight.shape != x.shape[-1:] or weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{name} must be [head dim], of the input dtype or fp32")
+    if weight.device != x.device:
+        raise ValueError(f"{name} must be on the input device")
+
+
+def _unit_rows(x):
+    return x if x is None or x.stride(2) == 1 else x.contiguous()
+
+
+def _forward(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps):
+    side = [(x.data_ptr(), x.stride(0), x.stride(1), x.shape[1]) if x is not None else (None, 0, 0, 0) for x in (q, k)]
+    out = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if x is not None else None for x in (q, k)]
+    if q.shape[0]:
+        with _lib.on_device(q.device):
+            status = _lib.lib().msa_qk_norm_rope(
+                *side[0], *side[1], _lib.DTYPE_CODE[q.dtype], wq.data_ptr(), _lib.ptr(wk),
+                _lib.DTYPE_CODE[wq.dtype], _lib.ptr(table), rows, rot, cu.data_ptr(), num_seqs, _lib.ptr(context),
+                q.shape[0], q.shape[2], eps, out[0].data_ptr(), _lib.ptr(out[1]), _lib.stream_of(q.device))
+        _lib.check(status, "msa_qk_norm_rope")
+    return out
+
+
+def _backward(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps, dq_out, dk_out, need):
+    """Gradients (q, k, q_weight, k_weight), None where not needed or no gradient came in."""
+    total, _, dim = q.shape
+    xs, ws, gs = (q, k), (wq, wk), (dq_out, dk_out)
+    side, dx, dw, heads = [], [], [], []
+    gs = tuple(None if g is None else g.to(x.dtype).contiguous() for g, x in zip(gs, xs))
+    for x, w, g, need_x, need_w in zip(xs, ws, gs, need[:2], need[2:]):
+        on = x is not None and g is not None
+        dx.append(torch.empty(x.shape, dtype=x.dtype, device=x.device) if on and need_x else None)
+        dw.append(torch.zeros_like(w) if on and need_w and not total else
+                  torch.empty_like(w) if on and need_w else None)
+        heads.append(x.shape[1] if dx[-1] is not None or dw[-1] is not None else 0)
+        side.append((x.data_ptr(), x.stride(0), x.stride(1), x.shape[1]) if x is not None else (None, 0, 0, 0))
+    if total and any(heads):
+        lib = _lib.lib()
+        size = lib.msa_qk_norm_rope_bwd_workspace_bytes(total, heads[0], heads[1], dim) if any(
+            w is not None for w in dw) else 0
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        with _lib.on_device(q.device):
+            status = lib.msa_qk_norm_rope_bwd(
+                *side[0], *side[1], _lib.DTYPE_CODE[q.dtype], wq.data_ptr(), _lib.ptr(wk),
+                _lib.DTYPE_CODE[wq.dtype], _lib.ptr(table), rows, rot, cu.data_ptr(), num_seqs, _lib.ptr(context),
+                total, dim, eps, _lib.ptr(gs[0]), _lib.ptr(gs[1]), _lib.ptr(dx[0]), _lib.ptr(dx[1]), _lib.ptr(dw[0]),
+                _lib.ptr(dw[1]), _lib.ptr(workspace), size, _lib.stream_of(q.device))
+        _lib.check(status, "msa_qk_norm_rope_bwd")
+    return dx[0], dx[1], dw[0], dw[1]
+
+
+class _NormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, wq, wk, table, cu, context)
+        ctx.args = (rows, rot, num_seqs, eps)
+        return tuple(_forward(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, wq, wk, table, cu, context = ctx.saved_tensors
+        rows, rot, num_seqs, eps = ctx.args
+        grads = _backward(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps, dq_out, dk_out,
+                          ctx.needs_input_grad[:4])
+        return (*grads, None, None, None, None, None, None, None)
+
+
+def _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps, context_lens):
+    """m3_qk_norm_rope's checks; returns the kernels' arguments."""
+    if q.ndim != 3 or (k is not None and k.ndim != 3):
+        raise ValueError("q and k must be rank-3 TND tensors")
+    total, heads, dim = q.shape
+    if heads < 1 or dim < 1 or (k is not None and (k.shape[0] != total or k.shape[1] < 1 or k.shape[2] != dim)):
+        raise ValueError("expected q[T,Hq,D] and k[T,Hkv,D] with positive heads and D")
+    if q.dtype not in _TYPES:
+        raise TypeError("q must have BF16, FP16, or FP32 dtype")
+    if k is not None and (k.dtype != q.dtype or k.device != q.device):
+        raise ValueError("q and k must share dtype and device")
+    check_weight(q_weight, q, "q_weight")
+    if k is None:
+        if k_weight is not None:
+            raise ValueError("k_weight without k")
+    else:
+        check_weight(k_weight, k, "k_weight")
+        if k_weight.dtype != q_weight.dtype:
+            raise ValueError("q_weight and k_weight must share a dtype")
+    table, rows, rot = check_table(cos_sin, dim, q.device)
+    if not (isinstance(eps, (int, float)) and math.isfinite(eps) and eps >= 0):
+        raise ValueError("eps must be nonnegative and finite")
+    cu, num_seqs = packed_tokens(cu_seqlens, total, q.device)
+    context = context_of(context_lens, num_seqs, q.device)
+    if dim > MAX_HEAD_DIM:
+        raise NotImplementedError(f"m3_qk_norm_rope takes head dims up to {MAX_HEAD_DIM}")
+    _lib.require_gpu(q, "m3_qk_norm_rope")
+    return (_unit_rows(q), _unit_rows(k), q_weight.contiguous(), None if k is None else k_weight.contiguous(), table,
+            rows, rot, cu, num_seqs, context, float(eps))
+
+
+def m3_qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor | None,
+    cos_sin: torch.Tensor | None,
+    cu_seqlens,
+    *,
+    eps: float = 1e-6,
+    context_lens: torch.Tensor | None = None,
+):
+    """Per-head RMS norm of ``q[T,Hq,D]`` and ``k[T,Hkv,D]`` with their weights ``[D]``, then the
+    rotation of each token's position: ``(q_out, k_out)``, differentiable in all four.
+
+    ``k`` (and ``k_weight``) may be None; then ``k_out`` is None. ``cos_sin`` (``rope_table``) is fp32
+    ``[positions, rotary_dim]``; None leaves the rotation out. A token's position is its offset in its
+    packed sequence plus ``context_lens`` of that sequence (int32 ``[N]`` on the device, default 0); where the
+    table has no row for it, the rotated dims are NaN. Token and head strides of ``q`` and ``k`` are free
+    (slices of a fused projection are read in place). The index heads go through the same call."""
+    args = _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps, context_lens)
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in args[:4]):
+        return _NormRope.apply(*args)
+    return tuple(_forward(*args))
