@@ -260,6 +260,30 @@ int msa_qk_norm_rope_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
                          void* grad_q_weight, void* grad_k_weight, void* workspace, int64_t workspace_bytes,
                          void* stream);
 
+/* New tokens' keys, values and index keys into a paged cache; no reference kernel (the reference has no
+ * cache). k and v [T,H,D], index_k [T,1,Di] (NULL: none; index_cache, index_weight and index_dim are then
+ * unread), bf16 or fp16, packed by cu_seqlens behind context_lens[s] tokens that the cache holds already
+ * (negative: the sequence is not there, nothing is written). Position j of sequence s is slot
+ * j % page_size of page page_table[s * table_stride + j / page_size]; tokens of pages outside [0, num_pages), or
+ * past pages_per_seq, are left out. page_size: a power of two from 16 to 256. Keys and index keys are normed
+ * where their weight is given and rotated by position where rotary_dim > 0, as msa_qk_norm_rope does.
+ * Caches [num_pages, H, page_size, D] (index: 1 head): of `dtype`, or k_cache / v_cache in e4m3
+ * (cache_is_fp8) with fp32 scales [num_pages, H], contiguous: value = byte * scale, the scale the smallest power of
+ * two that holds the page's largest magnitude in 448 of it. A page's scale covers the tokens that it holds in front of
+ * the new ones (its first new token at slot 0 starts it over); where it grows they are rounded again. What is not
+ * finite becomes NaN. strides (host array, elements): k token, head; v token, head; index_k token; k_cache page,
+ * head, slot; v_cache page, head, slot; index_cache page, slot; unit stride along D; cache rows 16-byte aligned.
+ * head_dim and index_dim: multiples of 16 up to 256 (status 2 otherwise). No two new tokens may share a slot,
+ * and in 8 bits no two sequences may append to one page. */
+int msa_cache_append(const void* k, const void* v, const void* index_k, int32_t dtype, int64_t kv_heads,
+                     int64_t head_dim, int64_t index_dim, const void* k_weight, const void* index_weight,
+                     int32_t weight_dtype, const float* cos_sin, int64_t table_rows, int64_t rotary_dim,
+                     double eps, void* k_cache, void* v_cache, void* index_cache, int32_t cache_is_fp8,
+                     float* k_scale, float* v_scale, const int64_t* strides, const int32_t* page_table,
+                     int64_t table_stride, int64_t pages_per_seq, int64_t num_pages, int64_t page_size,
+                     const int32_t* cu_seqlens, int64_t num_seqs, const int32_t* context_lens,
+                     int64_t total_tokens, void* stream);
+
 /* Testing hook; no counterpart in the reference. Overrides the byte budgets that size
  * the query-token chunks of the KV-major bf16 passes: msa_attn_fwd (default 2 GiB of
  * per-(token, head, slot) partial records per chunk), msa_attn_bwd (3 GiB) and

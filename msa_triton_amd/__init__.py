@@ -29,6 +29,12 @@ attention probabilities; student: the index token logits);
 norms the query and key heads and rotates them by their positions (``rope_table``), before the
 stages above, with gradients;
 
+    m3_cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, *, index_k=None, index_cache=None,
+                    k_scale=None, v_scale=None, k_weight=None, index_weight=None, cos_sin=None, eps=1e-6)
+
+writes new keys, values and index keys into a paged cache (16-bit, or 8-bit with a scale for each page and
+head), keys normed and rotated on the way;
+
     prepare_sequences(cu_seqlens, *, block_size=128) -> PackedSequences
 
 validates ``cu_seqlens`` once and returns immutable metadata with device copies;
@@ -87,6 +93,15 @@ def m3_qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, *, eps=1e-6, 
     return implementation(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps=eps, context_lens=context_lens)
 
 
+def m3_cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, *, index_k=None, index_cache=None,
+                    k_scale=None, v_scale=None, k_weight=None, index_weight=None, cos_sin=None, eps=1e-6):
+    from .cache_append import m3_cache_append as implementation
+
+    return implementation(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, index_k=index_k,
+                          index_cache=index_cache, k_scale=k_scale, v_scale=v_scale, k_weight=k_weight,
+                          index_weight=index_weight, cos_sin=cos_sin, eps=eps)
+
+
 def rope_table(num_positions, rotary_dim, *, base=10000.0, device=None):
     from .norm_rope import rope_table as implementation
 
@@ -100,4 +115,4 @@ def prepare_sequences(cu_seqlens, *, block_size=128):
 
 
 __all__ = ["m3_index_score", "m3_topk", "m3_sparse_attention", "m3_index_score_topk", "m3_indexer_kl",
-           "m3_qk_norm_rope", "rope_table", "prepare_sequences", "PackedSequences"]
+           "m3_qk_norm_rope", "m3_cache_append", "rope_table", "prepare_sequences", "PackedSequences"]

@@ -1,0 +1,105 @@
+"""New tokens into a paged cache: keys normed and rotated on the way, values as they are.
+
+The step between a layer's projections and its attention when a cache serves the tokens in front:
+``m3_qk_norm_rope`` prepares the queries, this call writes what the queries will read. The keys and values
+go to a cache of their own type or to an 8-bit one (e4m3 with a power-of-two scale for each page and
+head), the index keys to a 16-bit one (their scores decide which blocks are read, and equal scores have to stay
+equal). One launch (``msa_cache_append``); the caches are written in place.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .norm_rope import check_table, check_weight
+from .paged import FP8, check_cache, check_kv_caches, check_pages, page_args, sixteen_bit, unit_rows
+
+
+@torch.no_grad()
+def m3_cache_append(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    cu_seqlens,
+    context_lens: torch.Tensor,
+    *,
+    index_k: torch.Tensor | None = None,
+    index_cache: torch.Tensor | None = None,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    index_weight: torch.Tensor | None = None,
+    cos_sin: torch.Tensor | None = None,
+    eps: float = 1e-6,
+) -> None:
+    """Write ``k``, ``v`` (``[T,H,D]``) and ``index_k`` (``[T,1,Di]``) of new tokens into paged caches
+    ``[P,H,page,D]`` (``index_cache``: ``[P,1,page,Di]``), behind ``context_lens`` tokens of each sequence.
+
+    Keys are normed where ``k_weight`` is given and rotated where ``cos_sin`` (``rope_table``) is; index keys
+    likewise with ``index_weight``. In an 8-bit cache (``torch.float8_e4m3fn``) a value is its byte times
+    ``k_scale`` / ``v_scale`` ``[P,H]``, the smallest power of two that lets the page's largest magnitude fit; the
+    scale of a page that already holds tokens only grows, and they are then rounded again. A page whose
+    first new token is at slot 0 starts over. Values that are not finite are stored as NaN.
+
+    Tokens of missing pages (entries outside ``[0, P)``, or past the table) and of absent sequences
+    (negative ``context_lens``) are left out. No two new tokens may share a slot; in 8 bits no two
+    sequences may append to one page. D and Di: multiples of 16 up to 256. No gradients."""
+    if k.ndim != 3 or v.shape != k.shape or k.shape[1] < 1 or k.shape[2] < 1:
+        raise ValueError("expected k and v [T,H,D] of one shape with H, D > 0")
+    total, heads, dim = k.shape
+    sixteen_bit(k, "m3_cache_append")
+    if v.dtype != k.dtype or v.device != k.device:
+        raise ValueError("k and v must share dtype and device")
+    page = check_kv_caches(k_cache, v_cache, k_scale, v_scale, heads, dim, k.dtype, k.device)
+    if (index_k is None) != (index_cache is None):
+        raise ValueError("index_k and index_cache go together")
+    index_dim = 0
+    if index_k is not None:
+        if index_k.ndim != 3 or index_k.shape[:2] != (total, 1) or index_k.shape[2] < 1:
+            raise ValueError("expected index_k [T,1,Di] with Di > 0")
+        if index_k.dtype != k.dtype or index_k.device != k.device:
+            raise ValueError("index_k must share dtype and device with k")
+        index_dim = index_k.shape[2]
+        check_cache(index_cache, "index_cache", (k.dtype,), 1, index_dim, k.device)
+        if index_cache.shape[0] != k_cache.shape[0] or index_cache.shape[2] != page:
+            raise ValueError("index_cache must have the pages of k_cache")
+    weights = [w for w in (k_weight, index_weight) if w is not None]
+    if k_weight is not None:
+        check_weight(k_weight, k, "k_weight")
+    if index_weight is not None:
+        if index_k is None:
+            raise ValueError("index_weight without index_k")
+        check_weight(index_weight, index_k, "index_weight")
+    if len(weights) == 2 and k_weight.dtype != index_weight.dtype:
+        raise ValueError("k_weight and index_weight must share a dtype")
+    table, rows, rot = check_table(cos_sin, min(dim, index_dim) if index_k is not None else dim, k.device)
+    if not (isinstance(eps, (int, float)) and math.isfinite(eps) and eps >= 0):
+        raise ValueError("eps must be nonnegative and finite")
+    pages, cu, num_seqs, context = check_pages(page_table, cu_seqlens, context_lens, total, page, k.device)
+    if dim % 16 or dim > 256 or index_dim % 16 or index_dim > 256:
+        raise NotImplementedError("m3_cache_append takes head and index dims that are multiples of 16, up to 256")
+    _lib.require_gpu(k, "m3_cache_append")
+    if not total:
+        return
+    k, v = unit_rows(k), unit_rows(v)
+    ik = None if index_k is None else unit_rows(index_k)
+    wk = None if k_weight is None else k_weight.contiguous()
+    wi = None if index_weight is None else index_weight.contiguous()
+    strides = (ctypes.c_int64 * 13)(
+        k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0 if ik is None else ik.stride(0), *k_cache.stride()[:3],
+        *v_cache.stride()[:3], *((0, 0) if ik is None else (index_cache.stride(0), index_cache.stride(2))))
+    dtype = _lib.DTYPE_CODE[k.dtype]
+    with _lib.on_device(k.device):
+        status = _lib.lib().msa_cache_append(
+            k.data_ptr(), v.data_ptr(), _lib.ptr(ik), dtype, heads, dim, index_dim, _lib.ptr(wk), _lib.ptr(wi),
+            _lib.DTYPE_CODE[weights[0].dtype] if weights else dtype, _lib.ptr(table), rows, rot, eps,
+            k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(index_cache), k_cache.dtype == FP8, _lib.ptr(k_scale),
+            _lib.ptr(v_scale), strides, *page_args(pages, k_cache), cu.data_ptr(), num_seqs, context.data_ptr(), total,
+            _lib.stream_of(k.device))
+    _lib.check(status, "msa_cache_append")

@@ -1,0 +1,358 @@
+// New keys, values and index keys written into a paged cache, keys normed and rotated on the way.
+//
+// A key row passes y = rotate(x / sqrt(mean x^2 + eps) * w) (qk_norm_rope.hip; either part may be left
+// out), a value row is copied. A 16-bit cache takes y rounded once, with the bits that m3_qk_norm_rope
+// gives. An 8-bit cache (e4m3) takes y / s rounded once, with one scale s for each page and head: the
+// smallest power of two with 448 s >= max |y| over the page's new rows, joined by max with the scale of
+// the tokens that the page already holds. Where that makes the scale grow, the held tokens are rounded
+// again (exact for a power of two, except where they fall below e4m3's normal range). Values that are
+// not finite become NaN and do not enter the scale.
+//
+// y / s is formed in FP64 and rounded to e4m3 through round-to-odd fp32, so that the stored byte is
+// that of the exact y: a value an fp32 step away from a rounding border would be off by a whole e4m3 step
+// (2^-3) otherwise. The pass is bound by memory and, for single tokens, by its chain of loads
+// (sequence, page, row, scale), so the FP64 work is not seen.
+//
+// Work: 16-bit rows go to runs of LPR lanes, as in the norm. An 8-bit page, head and side is one
+// workgroup's, because its scale is needed before its first byte: one pass over the page's new rows for the
+// maximum, one to write them (from registers where they are few). Pages are numbered without a list of them:
+// sequence s gets the numbers from cu[s] / page + 2 s on, which leaves room for the two pages that n tokens can
+// touch beyond n / page; numbers without a page end at once.
+#include "norm_rope.hpp"
+#include "paged.hpp"
+
+namespace msa {
+namespace {
+
+struct AppendSide {
+  const void* x;
+  int64_t stride_t, stride_h;
+  const void* w;  // null: not normed
+  CacheView cache;
+  float* scale;  // [P][heads], 8-bit caches
+  int heads, dim;
+  bool turned;
+};
+
+struct AppendArgs {
+  AppendSide side[3];  // keys, values, index keys
+  int first[3];        // first workgroup of a side's rows
+  int page_blocks;     // workgroups of 8-bit pages, in front
+  bool w_f32;
+  RopeTable rope;
+  PageMap pages;
+  const int32_t* cu;
+  int nseq;
+  const int32_t* context;
+  int64_t tokens;
+  float eps;
+};
+
+template <int LPR>
+__device__ __forceinline__ double run_sum_f64(double v) {
+#pragma unroll
+  for (int o = 1; o < LPR; o <<= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+
+// The row's values y in FP64.
+template <int DT, int VEC, int C, int LPR>
+__device__ __forceinline__ void row_f64(const AppendArgs& A, const AppendSide& S, const RowLanes<DT, VEC, C, LPR>& lanes,
+                                        int64_t t, int head, int pos, bool live, double (&a)[C][VEC],
+                                        double (&b)[C][VEC]) {
+  float xa[C][VEC], xb[C][VEC];
+  lanes.load(S.x, t * S.stride_t + head * S.stride_h, live, xa, xb);
+  double ss = 0.0;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      a[c][j] = xa[c][j], b[c][j] = xb[c][j];
+      ss = fma(a[c][j], a[c][j], fma(b[c][j], b[c][j], ss));
+    }
+  if (S.w) {
+    const double r = 1.0 / sqrt(run_sum_f64<LPR>(ss) / S.dim + static_cast<double>(A.eps));
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) a[c][j] *= r * lanes.wa[c][j], b[c][j] *= r * lanes.wb[c][j];
+  }
+  if (S.turned && live) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float co[VEC], si[VEC];
+      load_turn<VEC>(A.rope, lanes.pc[c], pos, co, si);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const double u = a[c][j], v = b[c][j];
+        a[c][j] = u * co[j] - v * si[j];
+        b[c][j] = v * co[j] + u * si[j];
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float finite_size(double x) {
+  const float m = fabsf(f64_to_f32_odd(x));
+  return m < __builtin_inff() ? m : 0.f;  // (NaN: 0)
+}
+
+// x rounded once to the fp32 whose rounding to e4m3 is that of x; NaN for what is not finite.
+__device__ __forceinline__ float for_fp8(double x) {
+  return __builtin_isfinite(x) ? f64_to_f32_odd(x) : __builtin_nanf("");
+}
+
+__device__ __forceinline__ uint32_t pack4_fp8(float x0, float x1, float x2, float x3) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, w, true));
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_fp8(uint8_t* p, const double (&v)[VEC], double inv) {
+  if constexpr (VEC == 1) {
+    *p = static_cast<uint8_t>(pack4_fp8(for_fp8(v[0] * inv), 0.f, 0.f, 0.f));
+  } else {
+    uint2 w;
+    w.x = pack4_fp8(for_fp8(v[0] * inv), for_fp8(v[1] * inv), for_fp8(v[2] * inv), for_fp8(v[3] * inv));
+    w.y = pack4_fp8(for_fp8(v[4] * inv), for_fp8(v[5] * inv), for_fp8(v[6] * inv), for_fp8(v[7] * inv));
+    *reinterpret_cast<uint2*>(p) = w;
+  }
+}
+
+// The smallest power of two s >= 2^-100 with 448 s >= amax (448 = 1.75 x 2^8); 0 for 0.
+__device__ __forceinline__ float scale_for(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  if (u == 0u) return 0.f;
+  int k = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  k = k < -100 ? -100 : k;
+  return __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
+}
+
+// One 8-bit page, head and side.
+template <int DT, int VEC, int C, int LPR>
+__device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t unit, int head, float* amax_of_wave) {
+  using Lanes = RowLanes<DT, VEC, C, LPR>;
+  int lo = 0, hi = A.nseq;  // the last sequence whose numbers start at or below `unit`
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((A.cu[mid] >> A.pages.shift) + 2 * static_cast<int64_t>(mid) <= unit) lo = mid; else hi = mid;
+  }
+  const int s = lo;
+  const int64_t start = A.cu[s], n = A.cu[s + 1] - start, context = A.context[s];
+  if (context < 0 || n <= 0) return;
+  const int64_t p = (context >> A.pages.shift) + (unit - (start >> A.pages.shift) - 2 * static_cast<int64_t>(s));
+  const int64_t page_pos = p << A.pages.shift, page_end = page_pos + (int64_t{1} << A.pages.shift);
+  if (page_pos >= context + n) return;
+  const int page = A.pages.page_of(s, page_pos);
+  if (page < 0) return;
+  const int64_t first = context > page_pos ? context : page_pos;
+  const int kept = static_cast<int>(first - page_pos);  // tokens that the page holds already
+  const int rows = static_cast<int>((context + n < page_end ? context + n : page_end) - first);
+  const int64_t t0 = start + (first - context);
+  float* scale = S.scale + static_cast<int64_t>(page) * S.heads + head;
+  const float before = kept ? *scale : 0.f;
+  const Lanes lanes(S.w, A.w_f32, S.turned ? A.rope.half : 0, S.dim);
+  const int row = threadIdx.x / LPR;
+  double a[C][VEC], b[C][VEC];
+  float amax = 0.f;
+  for (int base = (rows - 1) / Lanes::kRows * Lanes::kRows; base >= 0; base -= Lanes::kRows) {  // the first rows stay
+    const int i = base + row;
+    row_f64<DT, VEC, C, LPR>(A, S, lanes, t0 + i, head, static_cast<int>(first + i), i < rows, a, b);
+    if (i < rows) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, fmaxf(finite_size(a[c][j]), finite_size(b[c][j])));
+    }
+  }
+  amax = wave_max_f32(amax);
+  if (threadIdx.x % kWave == 0) amax_of_wave[threadIdx.x / kWave] = amax;
+  __syncthreads();  // (also: every thread has read the old scale)
+  amax = fmaxf(fmaxf(amax_of_wave[0], amax_of_wave[1]), fmaxf(amax_of_wave[2], amax_of_wave[3]));
+  const float after = fmaxf(before, scale_for(amax));
+  const double inv = after > 0.f ? 1.0 / static_cast<double>(after) : 0.0;
+  uint8_t* dst = static_cast<uint8_t*>(S.cache.base) + page * S.cache.stride_page + head * S.cache.stride_head;
+  for (int base = 0; base < rows; base += Lanes::kRows) {
+    const int i = base + row;
+    if (base) row_f64<DT, VEC, C, LPR>(A, S, lanes, t0 + i, head, static_cast<int>(first + i), i < rows, a, b);
+    if (i < rows) {
+      uint8_t* to = dst + (kept + i) * S.cache.stride_slot;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if (lanes.pc[c].ok) store_fp8<VEC>(to + lanes.pc[c].a, a[c], inv);
+        if (lanes.pc[c].b_ok) store_fp8<VEC>(to + lanes.pc[c].b, b[c], inv);
+      }
+    }
+  }
+  if (kept && after != before) {  // round the held tokens again
+    const float ratio = static_cast<float>(static_cast<double>(before) * inv);
+    const int words = S.dim / 8;
+    for (int i = threadIdx.x; i < kept * words; i += kNormThreads) {
+      uint2* at = reinterpret_cast<uint2*>(dst + i / words * S.cache.stride_slot + i % words * 8);
+      uint2 w = *at;
+      auto again = [&](uint32_t x) {
+        const auto l = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x), false);
+        const auto h = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x), true);
+        return pack4_fp8(l[0] * ratio, l[1] * ratio, h[0] * ratio, h[1] * ratio);
+      };
+      w.x = again(w.x);
+      w.y = again(w.y);
+      *at = w;
+    }
+  }
+  if (threadIdx.x == 0) *scale = after;
+}
+
+// One batch of 16-bit rows.
+template <int DT, int VEC, int C, int LPR>
+__device__ void append_rows(const AppendArgs& A, const AppendSide& S, int64_t r0, int2* place) {
+  using Lanes = RowLanes<DT, VEC, C, LPR>;
+  const int64_t rows = A.tokens * S.heads, t0 = r0 / S.heads;
+  const int h0 = static_cast<int>(r0 - t0 * S.heads);
+  const int n = static_cast<int>(min(rows - r0, static_cast<int64_t>(Lanes::kRows)));
+  const int i = threadIdx.x / LPR;
+  const int tok = static_cast<int>(static_cast<uint32_t>(h0 + i) / static_cast<uint32_t>(S.heads));
+  const int head = h0 + i - tok * S.heads;
+  const Lanes lanes(S.w, A.w_f32, S.turned ? A.rope.half : 0, S.dim);
+  float a[C][VEC], b[C][VEC];
+  lanes.load(S.x, (t0 + tok) * S.stride_t + head * S.stride_h, i < n, a, b);
+  for (int k = threadIdx.x; k < (h0 + n - 1) / S.heads + 1; k += kNormThreads) {
+    const TokenPlace at = place_of(A.cu, A.nseq, A.context, t0 + k);
+    place[k] = make_int2(static_cast<int>(at.pos), at.pos < 0 ? -1 : A.pages.page_of(at.seq, at.pos));
+  }
+  __syncthreads();
+  float r = 1.f;
+  if (S.w) r = 1.f / sqrtf(run_sum<LPR>(sum_products(a, b, a, b)) / static_cast<float>(S.dim) + A.eps);
+  if (i >= n || place[tok].y < 0) return;
+  const int pos = place[tok].x;
+  const int slot = pos & ((1 << A.pages.shift) - 1);
+  const int64_t to = place[tok].y * S.cache.stride_page + head * S.cache.stride_head + slot * S.cache.stride_slot;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (S.w) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) a[c][j] = a[c][j] * r * lanes.wa[c][j], b[c][j] = b[c][j] * r * lanes.wb[c][j];
+    }
+    if (S.turned) {
+      float co[VEC], si[VEC];
+      load_turn<VEC>(A.rope, lanes.pc[c], pos, co, si);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float u = a[c][j], v = b[c][j];
+        a[c][j] = u * co[j] - v * si[j];
+        b[c][j] = v * co[j] + u * si[j];
+      }
+    }
+  }
+  lanes.store(S.cache.base, to, a, b);
+}
+
+template <int DT, bool FP8, int VEC, int C, int LPR>
+__global__ __launch_bounds__(kNormThreads) void cache_append_kernel(AppendArgs A) {
+  __shared__ int2 place[kNormThreads / LPR + 1];
+  const int block = static_cast<int>(blockIdx.x);
+  if constexpr (FP8) {
+    __shared__ float amax_of_wave[kNormThreads / kWave];
+    if (block < A.page_blocks) {
+      const int per_unit = A.side[0].heads + A.side[1].heads;
+      const int64_t unit = block / per_unit;
+      const int which = block % per_unit, second = which >= A.side[0].heads;
+      append_page<DT, VEC, C, LPR>(A, A.side[second], unit, which - (second ? A.side[0].heads : 0), amax_of_wave);
+      return;
+    }
+  }
+  const int side = block >= A.first[2] ? 2 : block >= A.first[1] ? 1 : 0;
+  append_rows<DT, VEC, C, LPR>(A, A.side[side], static_cast<int64_t>(block - A.first[side]) * (kNormThreads / LPR), place);
+}
+
+template <int DT, bool FP8>
+int append_launch(AppendArgs A, bool vectors, hipStream_t st) {
+  int chunks = 0;
+  for (const AppendSide& s : A.side)
+    if (s.heads && s.dim / 16 > chunks) chunks = s.dim / 16;
+  auto go = [&](auto kernel, int rows) {
+    int64_t blocks = 0;
+    if (FP8) {
+      const int64_t units = (A.tokens >> A.pages.shift) + 2 * static_cast<int64_t>(A.nseq);
+      blocks = units * (A.side[0].heads + A.side[1].heads);
+      if (blocks >= (int64_t{1} << 24)) return static_cast<int>(kErrUnsupported);
+      A.page_blocks = static_cast<int>(blocks);
+    }
+    for (int i = 0; i < 3; ++i) {
+      A.first[i] = static_cast<int>(blocks);
+      if (!FP8 || i == 2) blocks += (A.tokens * A.side[i].heads + rows - 1) / rows;
+      if (blocks >= (int64_t{1} << 24)) return static_cast<int>(kErrUnsupported);  // 2^32 threads of a launch
+    }
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kNormThreads), 0, st, A);
+    return static_cast<int>(status_from(hipGetLastError()));
+  };
+#define MSA_APPEND(VEC, C, LPR) return go(cache_append_kernel<DT, FP8, VEC, C, LPR>, kNormThreads / LPR)
+  if (!vectors) MSA_APPEND(1, 2, 64);
+  if (chunks <= 4) MSA_APPEND(8, 1, 4);
+  if (chunks <= 8) MSA_APPEND(8, 1, 8);
+  MSA_APPEND(8, 1, 16);
+#undef MSA_APPEND
+}
+
+bool rows_fit(const AppendSide& s, int half) {
+  return !s.heads || (aligned16(s.x) && aligned16(s.w) && s.stride_t % 8 == 0 && s.stride_h % 8 == 0 &&
+                      (!s.turned || half % 8 == 0));
+}
+
+}  // namespace
+}  // namespace msa
+
+using namespace msa;
+
+extern "C" int msa_cache_append(const void* k, const void* v, const void* index_k, int32_t dtype, int64_t kv_heads,
+                                int64_t head_dim, int64_t index_dim, const void* k_weight, const void* index_weight,
+                                int32_t weight_dtype, const float* cos_sin, int64_t table_rows, int64_t rotary_dim,
+                                double eps, void* k_cache, void* v_cache, void* index_cache, int32_t cache_is_fp8,
+                                float* k_scale, float* v_scale, const int64_t* strides, const int32_t* page_table,
+                                int64_t table_stride, int64_t pages_per_seq, int64_t num_pages, int64_t page_size,
+                                const int32_t* cu_seqlens, int64_t num_seqs, const int32_t* context_lens,
+                                int64_t total_tokens, void* stream) {
+  const bool with_index = index_k != nullptr;
+  if (!strides || !cu_seqlens || !context_lens || num_seqs <= 0 || num_seqs > 0x3fffffff || total_tokens < 0 ||
+      total_tokens > 0x7fffffff || !valid_pages(page_table, table_stride, pages_per_seq, num_pages, page_size) ||
+      (dtype != kBF16 && dtype != kF16) || (weight_dtype != dtype && weight_dtype != kF32) || !(eps >= 0.0) ||
+      rotary_dim < 0 || rotary_dim % 2 || (rotary_dim > 0 && (!cos_sin || table_rows < 0)))
+    return kErrInvalidArgument;
+  if (!k || !v || !k_cache || !v_cache || kv_heads <= 0 || kv_heads >= (1 << 20) || head_dim <= 0 ||
+      rotary_dim > head_dim || (cache_is_fp8 && (!k_scale || !v_scale)))
+    return kErrInvalidArgument;
+  if (with_index && (!index_cache || index_dim <= 0 || rotary_dim > index_dim)) return kErrInvalidArgument;
+  if (head_dim % 16 || head_dim > 256 || (with_index && (index_dim % 16 || index_dim > 256))) return kErrUnsupported;
+  if (total_tokens == 0) return kOk;
+  AppendArgs A{};
+  const int H = static_cast<int>(kv_heads), D = static_cast<int>(head_dim);
+  const bool turned = rotary_dim > 0;
+  A.side[0] = AppendSide{k, strides[0], strides[1], k_weight, CacheView{k_cache, strides[5], strides[6], strides[7]},
+                         k_scale, H, D, turned};
+  A.side[1] = AppendSide{v, strides[2], strides[3], nullptr, CacheView{v_cache, strides[8], strides[9], strides[10]},
+                         v_scale, H, D, false};
+  A.side[2] = AppendSide{index_k, strides[4], 0, index_weight, CacheView{index_cache, strides[11], 0, strides[12]},
+                         nullptr, with_index ? 1 : 0, static_cast<int>(index_dim), turned};
+  A.w_f32 = weight_dtype == kF32;
+  A.rope = RopeTable{cos_sin, table_rows, static_cast<int>(rotary_dim / 2)};
+  A.pages = page_map(page_table, table_stride, pages_per_seq, num_pages, page_size);
+  A.cu = cu_seqlens;
+  A.nseq = static_cast<int>(num_seqs);
+  A.context = context_lens;
+  A.tokens = total_tokens;
+  A.eps = static_cast<float>(eps);
+  // cache rows are written in 16-byte pieces (8-byte ones in 8 bits)
+  for (int i = 0; i < 3; ++i) {
+    const AppendSide& s = A.side[i];
+    const int unit = cache_is_fp8 && i < 2 ? 16 : 8;
+    if (s.heads && (!aligned16(s.cache.base) || s.cache.stride_page % unit || s.cache.stride_head % unit ||
+                    s.cache.stride_slot % unit))
+      return kErrInvalidArgument;
+  }
+  bool vectors = aligned16(cos_sin);
+  for (const AppendSide& s : A.side) vectors = vectors && rows_fit(s, A.rope.half);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == kBF16)
+    return cache_is_fp8 ? append_launch<kBF16, true>(A, vectors, st) : append_launch<kBF16, false>(A, vectors, st);
+  return cache_is_fp8 ? append_launch<kF16, true>(A, vectors, st) : append_launch<kF16, false>(A, vectors, st);
+}

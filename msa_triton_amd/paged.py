@@ -1,0 +1,97 @@
+"""What the paged operators share: the checks of a cache and of its page table.
+
+A cache is ``[P, H, page, D]`` (pages, heads, slots of a page, dims); ``page_table`` int32
+``[N, M]`` says where each sequence's tokens are: position ``j`` of sequence ``s`` is slot
+``j % page`` of page ``page_table[s, j // page]``. Entries outside ``[0, P)`` are pages that do not exist.
+New tokens come packed by ``cu_seqlens`` (as everywhere); ``context_lens`` int32 ``[N]`` holds the number of
+tokens that the cache has in front of them, so the new token at offset ``i`` of its sequence has
+position ``context_lens[s] + i``. A negative length marks a sequence that is not there, as in a batch padded to
+a fixed size. ``page_table`` and ``context_lens`` are read on the device only: a step captured in a
+graph replays with whatever they hold then.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .layout import context_of, packed_tokens
+
+CACHE_TYPES = (torch.bfloat16, torch.float16)
+FP8 = torch.float8_e4m3fn
+
+
+def check_cache(cache, name, dtypes, heads, dim, device):
+    """Shape, type, device and row alignment of a cache; returns its page size."""
+    if cache.ndim != 4 or cache.shape[1] != heads or cache.shape[3] != dim:
+        raise ValueError(f"{name} must be [pages, {heads}, page size, {dim}]")
+    if cache.dtype not in dtypes:
+        raise TypeError(f"{name} must have dtype {' or '.join(str(d) for d in dtypes)}")
+    if cache.device != device:
+        raise ValueError(f"{name} must be on the input device")
+    page = cache.shape[2]
+    if page < 16 or page > 256 or page & (page - 1):
+        raise ValueError("the page size must be a power of two from 16 to 256")
+    size = cache.element_size()
+    if cache.stride(3) != 1 or cache.data_ptr() % 16 or any(s * size % 16 for s in cache.stride()[:3]):
+        raise ValueError(f"{name} rows must be contiguous and 16-byte aligned")
+    return page
+
+
+def check_scale(scale, name, cache):
+    """The scales [P, H] that go with an 8-bit cache (and only with one)."""
+    if cache.dtype != FP8:
+        if scale is not None:
+            raise ValueError(f"{name} goes with an 8-bit cache")
+        return
+    if scale is None or scale.dtype != torch.float32 or scale.shape != cache.shape[:2] or not scale.is_contiguous():
+        raise ValueError(f"{name} must be contiguous fp32 [pages, heads]")
+    if scale.device != cache.device:
+        raise ValueError(f"{name} must be on the cache's device")
+
+
+def check_kv_caches(k_cache, v_cache, k_scale, v_scale, heads, dim, dtype, device):
+    """The key and value caches of one layer: of the input type, or both in 8 bits. Returns the page size."""
+    page = check_cache(k_cache, "k_cache", (dtype, FP8), heads, dim, device)
+    check_cache(v_cache, "v_cache", (k_cache.dtype,), heads, dim, device)
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have one shape")
+    check_scale(k_scale, "k_scale", k_cache)
+    check_scale(v_scale, "v_scale", v_cache)
+    return page
+
+
+def check_pages(page_table, cu_seqlens, context_lens, total, page, device):
+    """The sequences of a paged call: (page table, cu_seqlens, sequences, context lengths), on the device."""
+    cu, num_seqs = packed_tokens(cu_seqlens, total, device)
+    if context_lens is None:
+        raise TypeError("context_lens must be int32")
+    context = context_of(context_lens, num_seqs, device)
+    if not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32:
+        raise TypeError("page_table must be int32")
+    if page_table.ndim != 2 or page_table.shape[0] != num_seqs:
+        raise ValueError("page_table must be [sequences, pages]")
+    if page_table.device != device:
+        raise ValueError("page_table must be on the input device")
+    if page_table.shape[1] * page > 2147483647:
+        raise ValueError("positions must fit int32 metadata")
+    if page_table.stride(1) != 1:
+        page_table = page_table.contiguous()
+    return page_table, cu, num_seqs, context
+
+
+def page_args(page_table, cache):
+    """The page map's arguments of a C call."""
+    return page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cache.shape[0], cache.shape[2]
+
+
+def sixteen_bit(x, what):
+    if x.dtype == torch.float32:
+        raise NotImplementedError(f"{what} takes BF16 or FP16 inputs")
+    if x.dtype not in CACHE_TYPES:
+        raise TypeError(f"{what} takes BF16 or FP16 inputs")
+
+
+def unit_rows(x):
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
