@@ -284,6 +284,22 @@ int msa_cache_append(const void* k, const void* v, const void* index_k, int32_t 
                      const int32_t* cu_seqlens, int64_t num_seqs, const int32_t* context_lens,
                      int64_t total_tokens, void* stream);
 
+/* msa_index_score_topk for new tokens against the index keys of a paged cache (msa_cache_append): index_q
+ * [T,G,Di] contiguous, packed by cu_seqlens behind context_lens[s] cached tokens; index_cache
+ * [num_pages,1,page_size,Di] of the same dtype (bf16 or fp16) with page and slot strides, the new tokens'
+ * keys already in it. Scores [T,G,num_blocks] are those of the packed entry point (the exact block maxima over
+ * the keys up to the token's position; keys of missing pages do not exist), selections those of
+ * msa_topk at that position (topk_blocks 0: indices unread). Rows of a sequence with a negative context get
+ * scores of -inf and no block. index_dim: a multiple of 8 up to 256, block_size a multiple of 16 (status 2
+ * otherwise); cache rows and index_q 16-byte aligned. */
+int msa_index_score_topk_paged(const void* index_q, const void* index_cache, int32_t dtype,
+                               int64_t cache_stride_page, int64_t cache_stride_slot, const int32_t* page_table,
+                               int64_t table_stride, int64_t pages_per_seq, int64_t num_pages, int64_t page_size,
+                               const int32_t* cu_seqlens, int64_t num_seqs, const int32_t* context_lens,
+                               int64_t total_tokens, int64_t groups, int64_t index_dim, int64_t num_blocks,
+                               int64_t block_size, double scale, int64_t topk_blocks, int64_t local_blocks,
+                               float* scores, int32_t* indices, void* stream);
+
 /* Testing hook; no counterpart in the reference. Overrides the byte budgets that size
  * the query-token chunks of the KV-major bf16 passes: msa_attn_fwd (default 2 GiB of
  * per-(token, head, slot) partial records per chunk), msa_attn_bwd (3 GiB) and

@@ -35,6 +35,11 @@ stages above, with gradients;
 writes new keys, values and index keys into a paged cache (16-bit, or 8-bit with a scale for each page and
 head), keys normed and rotated on the way;
 
+    m3_index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, context_lens, max_seqlen, *,
+                              block_size=128, scale=1.0, topk_blocks=16, local_blocks=1) -> (scores, indices)
+
+scores new tokens against the cached index keys and selects their blocks;
+
     prepare_sequences(cu_seqlens, *, block_size=128) -> PackedSequences
 
 validates ``cu_seqlens`` once and returns immutable metadata with device copies;
@@ -102,6 +107,14 @@ def m3_cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens
                           index_weight=index_weight, cos_sin=cos_sin, eps=eps)
 
 
+def m3_index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, context_lens, max_seqlen, *,
+                              block_size=128, scale=1.0, topk_blocks=16, local_blocks=1):
+    from .paged_score import m3_index_score_topk_paged as implementation
+
+    return implementation(index_q, index_cache, page_table, cu_seqlens, context_lens, max_seqlen,
+                          block_size=block_size, scale=scale, topk_blocks=topk_blocks, local_blocks=local_blocks)
+
+
 def rope_table(num_positions, rotary_dim, *, base=10000.0, device=None):
     from .norm_rope import rope_table as implementation
 
@@ -115,4 +128,5 @@ def prepare_sequences(cu_seqlens, *, block_size=128):
 
 
 __all__ = ["m3_index_score", "m3_topk", "m3_sparse_attention", "m3_index_score_topk", "m3_indexer_kl",
-           "m3_qk_norm_rope", "m3_cache_append", "rope_table", "prepare_sequences", "PackedSequences"]
+           "m3_qk_norm_rope", "m3_cache_append",
+           "m3_index_score_topk_paged", "rope_table", "prepare_sequences", "PackedSequences"]

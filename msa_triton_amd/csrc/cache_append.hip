@@ -318,10 +318,11 @@ extern "C" int msa_cache_append(const void* k, const void* v, const void* index_
       (dtype != kBF16 && dtype != kF16) || (weight_dtype != dtype && weight_dtype != kF32) || !(eps >= 0.0) ||
       rotary_dim < 0 || rotary_dim % 2 || (rotary_dim > 0 && (!cos_sin || table_rows < 0)))
     return kErrInvalidArgument;
-  if (!k || !v || !k_cache || !v_cache || kv_heads <= 0 || kv_heads >= (1 << 20) || head_dim <= 0 ||
-      rotary_dim > head_dim || (cache_is_fp8 && (!k_scale || !v_scale)))
+  if (!k || !v || kv_heads <= 0 || kv_heads >= (1 << 20) || head_dim <= 0 || rotary_dim > head_dim)
     return kErrInvalidArgument;
-  if (with_index && (!index_cache || index_dim <= 0 || rotary_dim > index_dim)) return kErrInvalidArgument;
+  if (num_pages > 0 && (!k_cache || !v_cache || (with_index && !index_cache) || (cache_is_fp8 && (!k_scale || !v_scale))))
+    return kErrInvalidArgument;
+  if (with_index && (index_dim <= 0 || rotary_dim > index_dim)) return kErrInvalidArgument;
   if (head_dim % 16 || head_dim > 256 || (with_index && (index_dim % 16 || index_dim > 256))) return kErrUnsupported;
   if (total_tokens == 0) return kOk;
   AppendArgs A{};

@@ -22,47 +22,46 @@ namespace msa {
 // Sixteen lanes per row, four rows per wavefront (topk_row16). In these kernels the
 // workgroups take the rows from the last one back: a row's work grows with its
 // position in the sequence, so the heaviest rows start first.
-template <int VPL>
+template <int VPL, class Rows>
 __global__ __launch_bounds__(256) void topk_kernel(const float* __restrict__ scores,
-                                                   const int32_t* __restrict__ cu, int nseq,
-                                                   int64_t rows, int G, int NB, int B, int K, int L,
+                                                   Rows at, int64_t rows, int G, int NB, int B, int K, int L,
                                                    int32_t* __restrict__ out) {
-  topk_row16<VPL>(scores, cu, nseq, rows, G, NB, B, K, L, out,
+  topk_row16<VPL>(scores, at, rows, G, NB, B, K, L, out,
                   static_cast<int64_t>(gridDim.x - 1 - blockIdx.x) * 16 + (threadIdx.x >> 4), threadIdx.x & 15);
 }
 
 // Threshold and sort, 64 / CAP rows per wavefront: topk_threshold.
-template <int VPL, int CAP>
+template <int VPL, int CAP, class Rows>
 __global__ __launch_bounds__(256) void topk_select_kernel(const float* __restrict__ scores,
-                                                          const int32_t* __restrict__ cu, int nseq, int64_t rows,
+                                                          Rows at, int64_t rows,
                                                           int G, int NB, int B, int K, int L,
                                                           int32_t* __restrict__ out) {
   __shared__ uint2 cand[4][64];
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t wave = static_cast<int64_t>(gridDim.x - 1 - blockIdx.x) * 4 + wid;
   if (wave * (64 / CAP) >= rows) return;
-  topk_threshold<VPL, CAP>(scores, cu, nseq, rows, G, NB, B, K, L, out, wave, threadIdx.x & 63, cand[wid]);
+  topk_threshold<VPL, CAP>(scores, at, rows, G, NB, B, K, L, out, wave, threadIdx.x & 63, cand[wid]);
 }
 
 // One wavefront per row for long rows (more than 1024 blocks): topk_row64.
-template <int VPL>
+template <int VPL, class Rows>
 __global__ __launch_bounds__(256) void topk_wave_kernel(const float* __restrict__ scores,
-                                                        const int32_t* __restrict__ cu, int nseq,
-                                                        int64_t rows, int G, int NB, int B, int K, int L,
+                                                        Rows at, int64_t rows, int G, int NB, int B, int K, int L,
                                                         int32_t* __restrict__ out) {
   const int64_t row = static_cast<int64_t>(gridDim.x - 1 - blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
-  topk_row64<VPL>(scores, cu, nseq, G, NB, B, K, L, out, row, threadIdx.x & 63);
+  topk_row64<VPL>(scores, at, G, NB, B, K, L, out, row, threadIdx.x & 63);
 }
 
 // One wavefront per row, row streamed from memory (more than 4096 blocks): topk_row_stream.
+template <class Rows>
 __global__ __launch_bounds__(256) void topk_stream_kernel(const float* __restrict__ scores,
-                                                          const int32_t* __restrict__ cu, int nseq, int64_t rows,
+                                                          Rows at, int64_t rows,
                                                           int G, int NB, int B, int K, int L,
                                                           int32_t* __restrict__ out) {
   const int64_t row = static_cast<int64_t>(gridDim.x - 1 - blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
-  topk_row_stream(scores, cu, nseq, G, NB, B, K, L, out, row, threadIdx.x & 63);
+  topk_row_stream(scores, at, G, NB, B, K, L, out, row, threadIdx.x & 63);
 }
 
 }  // namespace msa
@@ -71,19 +70,20 @@ using namespace msa;
 
 namespace msa {
 
-int topk_launch(const float* scores, const int32_t* cu_seqlens, int nseq, int64_t rows, int G, int NB, int B, int K,
-                int L, int32_t* indices, hipStream_t st) {
+template <class Rows>
+static int topk_launch_rows(const float* scores, const Rows& at, int64_t rows, int G, int NB, int B, int K, int L,
+                            int32_t* indices, hipStream_t st) {
   if (rows == 0 || K == 0) return kOk;
   dim3 grid(grid_1d(rows, 16)), block(256);
 #define MSA_TOPK_LAUNCH(V) \
-  hipLaunchKernelGGL(topk_kernel<V>, grid, block, 0, st, scores, cu_seqlens, nseq, rows, G, NB, B, K, L, indices)
+  hipLaunchKernelGGL((topk_kernel<V, Rows>), grid, block, 0, st, scores, at, rows, G, NB, B, K, L, indices)
 #define MSA_TOPK_WAVE(V) \
-  hipLaunchKernelGGL(topk_wave_kernel<V>, dim3(grid_1d(rows, 4)), block, 0, st, scores, cu_seqlens, nseq, rows, G, NB, B, K, L, indices)
+  hipLaunchKernelGGL((topk_wave_kernel<V, Rows>), dim3(grid_1d(rows, 4)), block, 0, st, scores, at, rows, G, NB, B, K, L, indices)
 #define MSA_TOPK_SELECT(V)                                                                                              \
   if (K <= kSelectPairSlots)                                                                                          \
-    hipLaunchKernelGGL((topk_select_kernel<V, 32>), dim3(grid_1d(rows, 8)), block, 0, st, scores, cu_seqlens, nseq, rows, G, NB, B, K, L, indices); \
+    hipLaunchKernelGGL((topk_select_kernel<V, 32, Rows>), dim3(grid_1d(rows, 8)), block, 0, st, scores, at, rows, G, NB, B, K, L, indices); \
   else                                                                                                                \
-    hipLaunchKernelGGL((topk_select_kernel<V, 64>), dim3(grid_1d(rows, 4)), block, 0, st, scores, cu_seqlens, nseq, rows, G, NB, B, K, L, indices)
+    hipLaunchKernelGGL((topk_select_kernel<V, 64, Rows>), dim3(grid_1d(rows, 4)), block, 0, st, scores, at, rows, G, NB, B, K, L, indices)
   if (NB <= 16) MSA_TOPK_LAUNCH(1);
   else if (NB <= 32) MSA_TOPK_LAUNCH(2);
   else if (NB <= 64) MSA_TOPK_LAUNCH(4);
@@ -100,11 +100,18 @@ int topk_launch(const float* scores, const int32_t* cu_seqlens, int nseq, int64_
   else if (NB <= 1024) MSA_TOPK_LAUNCH(64);
   else if (NB <= 2048) MSA_TOPK_WAVE(32);
   else if (NB <= 4096) MSA_TOPK_WAVE(64);
-  else hipLaunchKernelGGL(topk_stream_kernel, dim3(grid_1d(rows, 4)), block, 0, st, scores, cu_seqlens, nseq, rows, G, NB, B, K, L, indices);
+  else hipLaunchKernelGGL(topk_stream_kernel<Rows>, dim3(grid_1d(rows, 4)), block, 0, st, scores, at, rows, G, NB, B, K, L, indices);
 #undef MSA_TOPK_LAUNCH
 #undef MSA_TOPK_SELECT
 #undef MSA_TOPK_WAVE
   return status_from(hipGetLastError());
+}
+
+int topk_launch(const float* scores, const int32_t* cu_seqlens, int nseq, int64_t rows, int G, int NB, int B, int K,
+                int L, int32_t* indices, hipStream_t st, const int32_t* context) {
+  if (context)
+    return topk_launch_rows(scores, CachedRows{cu_seqlens, nseq, context}, rows, G, NB, B, K, L, indices, st);
+  return topk_launch_rows(scores, PackedRows{cu_seqlens, nseq}, rows, G, NB, B, K, L, indices, st);
 }
 
 }  // namespace msa

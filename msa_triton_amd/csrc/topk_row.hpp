@@ -12,6 +12,25 @@
 
 namespace msa {
 
+// The query block of a token (its position / B): of a packed batch, or behind cached tokens (context[s] of
+// them; -1 for a sequence that is not there, whose rows then select nothing).
+struct PackedRows {
+  const int32_t* cu;
+  int nseq;
+  __device__ __forceinline__ int query_block(int32_t t, int B) const { return (t - cu[find_seq(cu, nseq, t)]) / B; }
+};
+struct CachedRows {
+  const int32_t* cu;
+  int nseq;
+  const int32_t* context;
+  __device__ __forceinline__ int query_block(int32_t t, int B) const {
+    const int s = find_seq(cu, nseq, t);
+    const int32_t c = context[s];
+    // (a sum past 2^31 has no block: the position does not fit a page table)
+    return c < 0 ? -1 : static_cast<int>(min((static_cast<int64_t>(c) + (t - cu[s])) / B, int64_t{0x7fffffff} - 1));
+  }
+};
+
 // Monotone map of float bits onto uint32 (+0 and -0 collapse to the same key). NaN of
 // either sign ranks above +inf, as in torch.topk (the reference's selection,
 // triton/topk.py:44-45); 0xfffffffe keeps the 64-bit key of block 0 below the scan's
@@ -88,15 +107,12 @@ struct TopN {
 // still take part in the DPP and shuffle steps). The selection key is the ordered
 // float bits << 32 | ~block, so one 64-bit comparison implements "larger value,
 // then smaller block id".
-template <int VPL>
-__device__ __forceinline__ void topk_row16(const float* __restrict__ scores, const int32_t* __restrict__ cu,
-                                           int nseq, int64_t rows, int G, int NB, int B, int K, int L,
+template <int VPL, class Rows>
+__device__ __forceinline__ void topk_row16(const float* __restrict__ scores, const Rows& at, int64_t rows, int G, int NB, int B, int K, int L,
                                            int32_t* __restrict__ out, int64_t row, int sub) {
   const bool live = row < rows;
   const int64_t rr = live ? row : rows - 1;
-  const int64_t t = rr / G;
-  const int s = find_seq(cu, nseq, t);
-  const int64_t qb = (t - cu[s]) / B;
+  const int64_t qb = at.query_block(static_cast<int32_t>(rr / G), B);
   const int n = static_cast<int>(qb + 1 < NB ? qb + 1 : NB);
   const int count = K < NB ? K : NB;
   const int sel = live ? (count < n ? count : n) : 0;
@@ -219,9 +235,8 @@ constexpr int kSelectMostSlots = 64, kSelectPairSlots = 24;
 // 100, 10 101 / 100; 16 384 rows: 128 blocks with 4 5.4 / 7.4, 10 7.6 / 7.6, 256 with 7 9.3 / 8.6; 257 blocks and
 // more: sort (320 blocks, one slot, 262 144 rows: 202 / 107).
 constexpr int kArgmaxSlots128 = 11, kArgmaxSlots256 = 7;
-template <int VPL, int CAP>
-__device__ __forceinline__ void topk_threshold(const float* __restrict__ scores, const int32_t* __restrict__ cu,
-                                               int nseq, int64_t rows, int G, int NB, int B, int K, int L,
+template <int VPL, int CAP, class Rows>
+__device__ __forceinline__ void topk_threshold(const float* __restrict__ scores, const Rows& rows_at, int64_t rows, int G, int NB, int B, int K, int L,
                                                int32_t* __restrict__ out, int64_t wave, int lane, uint2* cand) {
   constexpr int ROWS = 64 / CAP;
   cand[lane] = make_uint2(0u, 0u);  // below every real key
@@ -231,7 +246,7 @@ __device__ __forceinline__ void topk_threshold(const float* __restrict__ scores,
     if (row >= rows) break;  // wave-uniform
     const int32_t t = static_cast<int32_t>(rows <= 0x7fffffff ? static_cast<uint32_t>(row) / static_cast<uint32_t>(G)
                                                               : row / G);
-    const int32_t qb = (t - cu[find_seq(cu, nseq, t)]) / B;
+    const int32_t qb = rows_at.query_block(t, B);
     const int n = qb + 1 < NB ? qb + 1 : NB;
     const int sel = K < n ? K : n;  // slots to fill
     const int own0 = L > 0 && qb - L + 1 < n ? qb - L + 1 : n;  // the forced local blocks: own0 .. n - 1
@@ -324,18 +339,16 @@ __device__ __forceinline__ void topk_threshold(const float* __restrict__ scores,
 // Host launch of the stand-alone selection (topk.hip): 16-lane rows up to 64 blocks,
 // threshold and sort up to 1024 (16-lane rows there for more than 64 slots, and up to 256
 // blocks for few), one wavefront per row with the row in registers up to 4096, streamed above.
+// With `context` the rows are tokens behind that many cached ones of their sequence.
 int topk_launch(const float* scores, const int32_t* cu_seqlens, int nseq, int64_t rows, int G, int NB, int B, int K,
-                int L, int32_t* indices, hipStream_t st);
+                int L, int32_t* indices, hipStream_t st, const int32_t* context = nullptr);
 
 // One wavefront per row: lane j holds blocks j, j + 64, ... (VPL values); each pick
 // is a 64-lane max. All lanes of the wavefront call it for the same row.
-template <int VPL>
-__device__ __forceinline__ void topk_row64(const float* __restrict__ scores, const int32_t* __restrict__ cu,
-                                           int nseq, int G, int NB, int B, int K, int L,
+template <int VPL, class Rows>
+__device__ __forceinline__ void topk_row64(const float* __restrict__ scores, const Rows& at, int G, int NB, int B, int K, int L,
                                            int32_t* __restrict__ out, int64_t row, int lane) {
-  const int64_t t = row / G;
-  const int s = find_seq(cu, nseq, t);
-  const int64_t qb = (t - cu[s]) / B;
+  const int64_t qb = at.query_block(static_cast<int32_t>(row / G), B);
   const int n = static_cast<int>(qb + 1 < NB ? qb + 1 : NB);
   const int count = K < NB ? K : NB;
   const int sel = count < n ? count : n;
@@ -373,12 +386,10 @@ __device__ __forceinline__ void topk_row64(const float* __restrict__ scores, con
 // above 4096): lane j scans blocks j, j + 64, ... and keeps its eight largest keys
 // below its last pick (TopN<8>); it rescans its blocks only when that cache runs empty,
 // so a row is read about once. Picks, order and padding are those of topk_row64.
-__device__ __forceinline__ void topk_row_stream(const float* __restrict__ scores, const int32_t* __restrict__ cu,
-                                                int nseq, int G, int NB, int B, int K, int L,
+template <class Rows>
+__device__ __forceinline__ void topk_row_stream(const float* __restrict__ scores, const Rows& at, int G, int NB, int B, int K, int L,
                                                 int32_t* __restrict__ out, int64_t row, int lane) {
-  const int64_t t = row / G;
-  const int s = find_seq(cu, nseq, t);
-  const int64_t qb = (t - cu[s]) / B;
+  const int64_t qb = at.query_block(static_cast<int32_t>(row / G), B);
   const int n = static_cast<int>(qb + 1 < NB ? qb + 1 : NB);
   const int count = K < NB ? K : NB;
   const int sel = count < n ? count : n;
