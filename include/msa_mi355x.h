@@ -300,6 +300,26 @@ int msa_index_score_topk_paged(const void* index_q, const void* index_cache, int
                                int64_t block_size, double scale, int64_t topk_blocks, int64_t local_blocks,
                                float* scores, int32_t* indices, void* stream);
 
+/* msa_attn_paged's workspace in bytes (0: none needed). */
+int64_t msa_attn_paged_workspace_bytes(int64_t total_tokens, int64_t q_heads, int64_t kv_groups, int64_t head_dim,
+                                       int64_t topk_slots, int64_t block_size);
+
+/* msa_attn_fwd for new tokens over a paged cache (msa_cache_append): q [T,Hq,D] contiguous, bf16 or fp16,
+ * packed by cu_seqlens behind context_lens[s] cached tokens; caches [num_pages,G,page_size,D] of `dtype`, or of
+ * e4m3 (cache_is_fp8) with fp32 scales [num_pages,G]; the new tokens' keys and values already in them. Attends to
+ * the keys up to the token's position of the blocks in indices [T,G,K] (ids outside the sequence and a second
+ * mention of a block are left out; so are keys of missing pages). out [T,Hq,D] in `dtype`, lse [T,Hq] natural log;
+ * rows without a key, and rows of a sequence with a negative context, get 0 and -inf. strides (host array,
+ * elements): k_cache page, head, slot; v_cache page, head, slot. head_dim: a multiple of 16 up to 256,
+ * block_size a multiple of 16 (status 2 otherwise); cache rows and q 16-byte aligned. Deterministic. */
+int msa_attn_paged(const void* q, const void* k_cache, const void* v_cache, int32_t dtype, int32_t cache_is_fp8,
+                   const float* k_scale, const float* v_scale, const int64_t* strides, const int32_t* indices,
+                   const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq, int64_t num_pages,
+                   int64_t page_size, const int32_t* cu_seqlens, int64_t num_seqs, const int32_t* context_lens,
+                   int64_t total_tokens, int64_t q_heads, int64_t kv_groups, int64_t head_dim, int64_t topk_slots,
+                   int64_t block_size, double scale, void* workspace, int64_t workspace_bytes, void* out,
+                   float* lse, void* stream);
+
 /* Testing hook; no counterpart in the reference. Overrides the byte budgets that size
  * the query-token chunks of the KV-major bf16 passes: msa_attn_fwd (default 2 GiB of
  * per-(token, head, slot) partial records per chunk), msa_attn_bwd (3 GiB) and

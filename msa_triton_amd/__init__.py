@@ -40,6 +40,11 @@ head), keys normed and rotated on the way;
 
 scores new tokens against the cached index keys and selects their blocks;
 
+    m3_sparse_attention_paged(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, *,
+                              block_size=128, scale=None, k_scale=None, v_scale=None, return_lse=False)
+
+is the attention of new tokens over the selected blocks of the cache;
+
     prepare_sequences(cu_seqlens, *, block_size=128) -> PackedSequences
 
 validates ``cu_seqlens`` once and returns immutable metadata with device copies;
@@ -115,6 +120,14 @@ def m3_index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, cont
                           block_size=block_size, scale=scale, topk_blocks=topk_blocks, local_blocks=local_blocks)
 
 
+def m3_sparse_attention_paged(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, *,
+                              block_size=128, scale=None, k_scale=None, v_scale=None, return_lse=False):
+    from .paged_attention import m3_sparse_attention_paged as implementation
+
+    return implementation(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, block_size=block_size,
+                          scale=scale, k_scale=k_scale, v_scale=v_scale, return_lse=return_lse)
+
+
 def rope_table(num_positions, rotary_dim, *, base=10000.0, device=None):
     from .norm_rope import rope_table as implementation
 
@@ -129,4 +142,5 @@ def prepare_sequences(cu_seqlens, *, block_size=128):
 
 __all__ = ["m3_index_score", "m3_topk", "m3_sparse_attention", "m3_index_score_topk", "m3_indexer_kl",
            "m3_qk_norm_rope", "m3_cache_append",
-           "m3_index_score_topk_paged", "rope_table", "prepare_sequences", "PackedSequences"]
+           "m3_index_score_topk_paged", "m3_sparse_attention_paged", "rope_table",
+           "prepare_sequences", "PackedSequences"]

@@ -63,6 +63,9 @@ SIGNATURES = {
                                 _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp]),
     "msa_index_score_topk_paged": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64,
                                           _i64, _i64, _i64, _i64, _f64, _i64, _i64, _vp, _vp, _vp]),
+    "msa_attn_paged_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "msa_attn_paged": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64,
+                              _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f64, _vp, _i64, _vp, _vp, _vp]),
     "msa_set_chunk_budgets": (_i32, [_i64, _i64, _i64]),
     "msa_set_item_order": (_i32, [_i32]),
     "msa_profile_begin": (_i32, []),

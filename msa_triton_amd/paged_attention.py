@@ -1,0 +1,86 @@
+"""Sparse attention of new tokens over the selected blocks of a paged cache.
+
+``m3_sparse_attention`` for serving: a token attends to the keys up to its position of the blocks that its
+group selected (``m3_index_score_topk_paged``), read from a 16-bit cache or an 8-bit one with a scale for
+each page and head. One C call (``msa_attn_paged``: a launch that reads the selected keys and values, and, for
+few rows, a second one that joins the parts of a row). The new tokens are in the cache already
+(``m3_cache_append``). Made for the few tokens of a decoding step; a prompt goes through the packed operators. No
+gradients.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .paged import FP8, check_kv_caches, check_pages, page_args, sixteen_bit
+
+
+@torch.no_grad()
+def m3_sparse_attention_paged(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    indices: torch.Tensor,
+    page_table: torch.Tensor,
+    cu_seqlens,
+    context_lens: torch.Tensor,
+    *,
+    block_size: int = 128,
+    scale: float | None = None,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+    return_lse: bool = False,
+):
+    """Attend ``q[T,Hq,D]`` to the selected blocks of paged caches ``[P,G,page,D]``: ``out[T,Hq,D]``.
+
+    ``indices[T,G,K]`` (int32) holds sequence-local block ids with ``-1`` padding, as the selection gives them; ids
+    behind the token and repeated ids count for nothing. Each contiguous group of ``Hq / G`` query heads shares a
+    selection. 8-bit caches (``torch.float8_e4m3fn``) come with ``k_scale`` and ``v_scale`` (fp32 ``[P,G]``). Keys in
+    missing pages do not exist; rows without keys, and those of an absent sequence (negative ``context_lens``),
+    give zero output and an LSE of -inf. ``block_size`` and ``D`` are multiples of 16, ``D`` at most 256."""
+    if q.ndim != 3 or q.shape[1] < 1 or q.shape[2] < 1:
+        raise ValueError("expected q[T,Hq,D] with Hq, D > 0")
+    total, heads, dim = q.shape
+    sixteen_bit(q, "m3_sparse_attention_paged")
+    if indices.ndim != 3 or indices.shape[0] != total or indices.shape[1] < 1 or indices.dtype != torch.int32:
+        raise ValueError("indices must be int32 [T,G,K]")
+    groups, slots = indices.shape[1:]
+    if heads % groups:
+        raise ValueError("Hq must be a positive multiple of G")
+    if indices.device != q.device:
+        raise ValueError("indices must be on the input device")
+    page = check_kv_caches(k_cache, v_cache, k_scale, v_scale, groups, dim, q.dtype, q.device)
+    if not isinstance(block_size, int) or block_size <= 0:
+        raise ValueError("block_size must be a positive integer")
+    if block_size > 2147483647:
+        raise ValueError("block_size must fit int32 metadata")
+    effective_scale = dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(effective_scale):
+        raise ValueError("scale must be finite")
+    pages, cu, num_seqs, context = check_pages(page_table, cu_seqlens, context_lens, total, page, q.device)
+    if block_size % 16 or dim % 16 or dim > 256:
+        raise NotImplementedError("m3_sparse_attention_paged takes block sizes and head dims that are multiples of 16, "
+                                  "head dims up to 256")
+    _lib.require_gpu(q, "m3_sparse_attention_paged")
+    q, indices = q.contiguous(), indices.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((total, heads), dtype=torch.float32, device=q.device)
+    if total:
+        lib = _lib.lib()
+        size = lib.msa_attn_paged_workspace_bytes(total, heads, groups, dim, slots, block_size)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        strides = (ctypes.c_int64 * 6)(*k_cache.stride()[:3], *v_cache.stride()[:3])
+        with _lib.on_device(q.device):
+            status = lib.msa_attn_paged(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.DTYPE_CODE[q.dtype], k_cache.dtype == FP8,
+                _lib.ptr(k_scale), _lib.ptr(v_scale), strides, indices.data_ptr(), *page_args(pages, k_cache),
+                cu.data_ptr(), num_seqs, context.data_ptr(), total, heads, groups, dim, slots, block_size,
+                effective_scale, _lib.ptr(workspace), size, out.data_ptr(), lse.data_ptr(), _lib.stream_of(q.device))
+        _lib.check(status, "msa_attn_paged")
+    return (out, lse) if return_lse else out
