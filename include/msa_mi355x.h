@@ -308,7 +308,7 @@ int64_t msa_attn_paged_workspace_bytes(int64_t total_tokens, int64_t q_heads, in
  * packed by cu_seqlens behind context_lens[s] cached tokens; caches [num_pages,G,page_size,D] of `dtype`, or of
  * e4m3 (cache_is_fp8) with fp32 scales [num_pages,G]; the new tokens' keys and values already in them. Attends to
  * the keys up to the token's position of the blocks in indices [T,G,K] (ids outside the sequence and a second
- * mention of a block are left out; so are keys of missing pages). out [T,Hq,D] in `dtype`, lse [T,Hq] natural log;
+ * mention of a block are left out; so are keys of missing pages). out [T,Hq,D] in `dtype`, lse [T,Hq] (NULL: none) natural log;
  * rows without a key, and rows of a sequence with a negative context, get 0 and -inf. strides (host array,
  * elements): k_cache page, head, slot; v_cache page, head, slot. head_dim: a multiple of 16 up to 256,
  * block_size a multiple of 16 (status 2 otherwise); cache rows and q 16-byte aligned. Deterministic. */

@@ -18,8 +18,9 @@ from . import _lib
 from .norm_rope import check_table, check_weight
 from .paged import FP8, check_cache, check_kv_caches, check_pages, page_args, sixteen_bit, unit_rows
 
+_Strides = ctypes.c_int64 * 13
 
-@torch.no_grad()
+
 def m3_cache_append(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -56,17 +57,17 @@ def m3_cache_append(
     sixteen_bit(k, "m3_cache_append")
     if v.dtype != k.dtype or v.device != k.device:
         raise ValueError("k and v must share dtype and device")
-    page = check_kv_caches(k_cache, v_cache, k_scale, v_scale, heads, dim, k.dtype, k.device)
+    page, of_kv = check_kv_caches(k_cache, v_cache, k_scale, v_scale, heads, dim, k.dtype, k.device)
     if (index_k is None) != (index_cache is None):
         raise ValueError("index_k and index_cache go together")
-    index_dim = 0
+    index_dim, of_index = 0, (0, 0, 0)
     if index_k is not None:
         if index_k.ndim != 3 or index_k.shape[:2] != (total, 1) or index_k.shape[2] < 1:
             raise ValueError("expected index_k [T,1,Di] with Di > 0")
         if index_k.dtype != k.dtype or index_k.device != k.device:
             raise ValueError("index_k must share dtype and device with k")
         index_dim = index_k.shape[2]
-        check_cache(index_cache, "index_cache", (k.dtype,), 1, index_dim, k.device)
+        _, of_index = check_cache(index_cache, "index_cache", (k.dtype,), 1, index_dim, k.device)
         if index_cache.shape[0] != k_cache.shape[0] or index_cache.shape[2] != page:
             raise ValueError("index_cache must have the pages of k_cache")
     weights = [w for w in (k_weight, index_weight) if w is not None]
@@ -91,9 +92,8 @@ def m3_cache_append(
     ik = None if index_k is None else unit_rows(index_k)
     wk = None if k_weight is None else k_weight.contiguous()
     wi = None if index_weight is None else index_weight.contiguous()
-    strides = (ctypes.c_int64 * 13)(
-        k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0 if ik is None else ik.stride(0), *k_cache.stride()[:3],
-        *v_cache.stride()[:3], *((0, 0) if ik is None else (index_cache.stride(0), index_cache.stride(2))))
+    strides = _Strides(*k.stride()[:2], *v.stride()[:2], 0 if ik is None else ik.stride(0), *of_kv, of_index[0],
+                       of_index[2])
     dtype = _lib.DTYPE_CODE[k.dtype]
     with _lib.on_device(k.device):
         status = _lib.lib().msa_cache_append(

@@ -25,7 +25,8 @@
 namespace msa {
 namespace {
 
-constexpr int kList = 256;  // steps listed at once: one a thread
+constexpr int kList = 256;       // steps listed at once: one a thread
+constexpr int kMostSplits = 64;  // of one row: a lane of the joining wave each
 
 struct PagedAttnArgs {
   const uint16_t* q;  // [T][Hq][D]
@@ -41,7 +42,7 @@ struct PagedAttnArgs {
   int head_tiles, splits;
   float scale_log2;  // scale * log2(e)
   uint16_t* out;     // [T][Hq][D]
-  float* lse;        // [T][Hq]
+  float* lse;        // [T][Hq], or null
   float* part;       // [items][splits][16][D]
   float* stats;      // [items][splits][2][16]: maximum (log2), sum
 };
@@ -78,8 +79,8 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   const int64_t tg = item / A.head_tiles, t = tg / A.G;
   const int g = static_cast<int>(tg % A.G);
   const int ratio = A.Hq / A.G, head = 16 * ht + c;
-  const TokenPlace at = place_of(A.cu, A.nseq, A.context, t);
-  const int pos = at.pos > 0x7fffffff ? 0x7fffffff : static_cast<int>(at.pos);
+  const int32_t* ids = A.indices + tg * A.K;
+  const int32_t wave_id = lane < A.K ? ids[lane] : -1;  // the first 64 ids, one a lane
   const bool full = A.D == DP;
 
   // dims of a lane in step kk of the first product (any order, the same for keys and queries)
@@ -92,10 +93,11 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
       qf[kk] = head < ratio && dim_of(kk) < A.D ? load_frag(row + dim_of(kk)) : zero_frag();
   }
 
+  const TokenPlace at = wave_place_of(A.cu, A.nseq, A.context, t);
+  const int pos = at.pos > 0x7fffffff ? 0x7fffffff : static_cast<int>(at.pos);
   const int per_block = (A.B + 31) / 32;
-  const int64_t steps = static_cast<int64_t>(A.K) * per_block, per_split = (steps + A.splits - 1) / A.splits;
-  const int64_t n0 = split * per_split, n1 = min(steps, n0 + per_split);
-  const int32_t* ids = A.indices + tg * A.K;
+  // this workgroup's steps: every splits-th (the blocks that exist come first in a selection)
+  const int64_t steps = static_cast<int64_t>(A.K) * per_block;
 
   float m = -__builtin_inff(), l = 0.f;  // of head c: the maximum over all quarters, the sum over this one
   f32x4 acc[ND];
@@ -140,17 +142,19 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
     }
   };
 
-  for (int64_t base = n0; base < n1; base += kList) {
+  for (int64_t base = split; base < steps; base += static_cast<int64_t>(kList) * A.splits) {
     // ---- the steps of this stretch that hold visible keys, in order
-    const int64_t n = base + threadIdx.x;
+    const int64_t n = base + static_cast<int64_t>(threadIdx.x) * A.splits;
     int key = -1, a = -1, b = -1;
-    if (n < n1) {
-      const int slot = static_cast<int>(n / per_block), step = static_cast<int>(n - static_cast<int64_t>(slot) * per_block);
-      const int id = ids[slot];
+    const int slot = static_cast<int>(min(n, steps - 1) / per_block);
+    const int id = A.K <= 64 ? __shfl(wave_id, slot, kWave) : ids[slot];
+    bool again = false;  // an id that an earlier slot holds
+    for (int i = 0; i < min(A.K, 64); ++i) again |= i < slot && __builtin_amdgcn_readlane(wave_id, i) == id;
+    for (int i = 64; i < slot; ++i) again |= ids[i] == id;
+    if (n < steps) {
+      const int step = static_cast<int>(n - static_cast<int64_t>(slot) * per_block);
       const int64_t first = static_cast<int64_t>(id) * A.B + 32 * step;
       if (id >= 0 && first <= pos) {
-        bool again = false;  // an id that an earlier slot holds
-        for (int i = 0; i < slot; ++i) again |= ids[i] == id;
         if (!again) {
           a = A.pages.page_of(at.seq, first);
           b = 32 * step + 16 < A.B && first + 16 <= pos ? A.pages.page_of(at.seq, first + 16) : -1;
@@ -282,7 +286,8 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   const bool whole = A.splits == 1;
   const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
   float* part = whole ? nullptr : A.part + ((item * A.splits + split) * 16 + row) * A.D;
-  for (int d = 4 * col; d < A.D; d += 64) {
+  const bool none = !whole && top == -__builtin_inff();  // (the joining launch does not look at it)
+  for (int d = 4 * col; d < A.D && !none; d += 64) {
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -301,7 +306,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   }
   if (col == 0) {
     if (whole) {
-      A.lse[out_row] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
+      if (A.lse) A.lse[out_row] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
     } else {
       float* st = A.stats + (item * A.splits + split) * 32;
       st[row] = top;
@@ -310,48 +315,60 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   }
 }
 
-// The splits of a row joined: 16 lanes a head, 4 dims each at a time.
+// The splits of a row joined, a wave for each head's row: lane z weighs split z (at most kMostSplits = 64), and
+// the lanes take two dims each of all of them, eight splits' loads in flight at a time.
 template <int DT>
 __global__ __launch_bounds__(256) void attn_paged_join(PagedAttnArgs A) {
-  const int64_t item = blockIdx.x;
-  const int ht = static_cast<int>(item % A.head_tiles);
-  const int64_t tg = item / A.head_tiles, t = tg / A.G;
-  const int g = static_cast<int>(tg % A.G), ratio = A.Hq / A.G;
-  const int row = threadIdx.x >> 4, col = threadIdx.x & 15, h = 16 * ht + row;
-  if (h >= ratio) return;
-  const float* st = A.stats + item * A.splits * 32 + row;
-  float top = -__builtin_inff(), sum = 0.f;
-  for (int z = 0; z < A.splits; ++z) top = fmaxf(top, st[z * 32]);
-  const float shift = top == -__builtin_inff() ? 0.f : top;
-  for (int z = 0; z < A.splits; ++z) sum = fmaf(__builtin_amdgcn_exp2f(st[z * 32] - shift), st[z * 32 + 16], sum);
+  const int lane = threadIdx.x & 63;
+  const int64_t out_row = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (out_row >= A.tokens * A.Hq) return;
+  const int64_t t = out_row / A.Hq;
+  const int ratio = A.Hq / A.G, hq = static_cast<int>(out_row - t * A.Hq), g = hq / ratio, h = hq - g * ratio;
+  const int64_t item = (t * A.G + g) * A.head_tiles + (h >> 4);
+  const int row = h & 15;
+  const float* st = A.stats + (item * A.splits + lane) * 32 + row;
+  const bool live = lane < A.splits;
+  const float top_z = live ? st[0] : -__builtin_inff(), sum_z = live ? st[16] : 0.f;
+  const float top = wave_max_f32(top_z);
+  const float weight = top_z == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(top_z - top);
+  const float sum = wave_sum_f32(weight * sum_z);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t out_row = t * A.Hq + g * ratio + h;
   const float* part = A.part + (item * A.splits * 16 + row) * A.D;
-  for (int d = 4 * col; d < A.D; d += 64) {
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int z = 0; z < A.splits; ++z) {
-      const float f = __builtin_amdgcn_exp2f(st[z * 32] - shift);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(z) * 16 * A.D + d);
+  for (int d = 2 * lane; d < A.D; d += 128) {
+    float o0 = 0.f, o1 = 0.f;
+    for (int z0 = 0; z0 < A.splits; z0 += 8) {
+      float2 x[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = fmaf(f, x[i], o[i]);
+      for (int i = 0; i < 8; ++i)  // (past the last split: that one again, with a weight of 0)
+        x[i] = *reinterpret_cast<const float2*>(part + static_cast<int64_t>(min(z0 + i, A.splits - 1)) * 16 * A.D + d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), z0 + i));
+        o0 = f == 0.f ? o0 : fmaf(f, x[i].x, o0);  // (a split without keys wrote nothing)
+        o1 = f == 0.f ? o1 : fmaf(f, x[i].y, o1);
+      }
     }
-    o *= inv;
-    const uint2 r = DT == kF16 ? make_uint2(cvt_pk_f16(o[0], o[1]), cvt_pk_f16(o[2], o[3]))
-                               : make_uint2(cvt_pk_bf16(o[0], o[1]), cvt_pk_bf16(o[2], o[3]));
-    *reinterpret_cast<uint2*>(A.out + out_row * A.D + d) = r;
+    reinterpret_cast<uint32_t*>(A.out)[(out_row * A.D + d) >> 1] =
+        DT == kF16 ? cvt_pk_f16(o0 * inv, o1 * inv) : cvt_pk_bf16(o0 * inv, o1 * inv);
   }
-  if (col == 0) A.lse[out_row] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
+  if (lane == 0 && A.lse) A.lse[out_row] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
 }
 
 int64_t head_tiles_of(int64_t heads, int64_t groups) { return (heads / groups + 15) / 16; }
 
-// Workgroups that share one row's steps: about 1024 workgroups in all, each wave with a step at least.
+// Workgroups that share one row's steps. 512 of them (two a CU) run at once and draw what HBM gives (64 rows of 16
+// blocks over 4 groups: 256 items of 128 dims in bf16 take 52 us, 5.1 TB/s, as 512 workgroups, 58 as 768 and 55 as 1024;
+// e4m3 33, 34 and 38); a workgroup costs about four steps of its waves before the first and after the last one. So:
+// the number with the fewest steps, rounds of 512 times the steps of a wave and those four. 328 items of 128 steps as
+// 328, 656 and 984 workgroups: 112, 115 and 98 us; 4 items of 64 steps: one step a wave, 64 workgroups, 13 us.
 int64_t split_count(int64_t items, int64_t slots, int64_t block_size) {
   const int64_t steps = slots * ((block_size + 31) / 32);
-  int64_t n = (1024 + items - 1) / items;
-  const int64_t most = (steps + 3) / 4;
-  n = n < most ? n : most;
-  return n < 1 ? 1 : n;
+  int64_t best = 1, cost = -1;
+  for (int64_t n = 1; n == 1 || (n <= (steps + 3) / 4 && n <= kMostSplits); ++n) {
+    const int64_t x = ((items * n + 511) / 512) * ((steps + 4 * n - 1) / (4 * n) + 4);
+    if (cost < 0 || x < cost) best = n, cost = x;
+  }
+  return best;
 }
 
 }  // namespace
@@ -376,7 +393,7 @@ extern "C" int msa_attn_paged(const void* q, const void* k_cache, const void* v_
                               int64_t num_seqs, const int32_t* context_lens, int64_t total_tokens, int64_t q_heads,
                               int64_t kv_groups, int64_t head_dim, int64_t topk_slots, int64_t block_size, double scale,
                               void* workspace, int64_t workspace_bytes, void* out, float* lse, void* stream) {
-  if (!q || !out || !lse || !strides || !cu_seqlens || !context_lens || num_seqs <= 0 || num_seqs > 0x3fffffff ||
+  if (!q || !out || !strides || !cu_seqlens || !context_lens || num_seqs <= 0 || num_seqs > 0x3fffffff ||
       total_tokens < 0 || total_tokens > 0x7fffffff || q_heads <= 0 || kv_groups <= 0 || q_heads % kv_groups ||
       q_heads >= (1 << 20) || head_dim <= 0 || topk_slots < 0 || topk_slots > 0x7fffffff || (topk_slots > 0 && !indices) ||
       block_size <= 0 || block_size > 0x7fffffff || !__builtin_isfinite(scale) || (dtype != kBF16 && dtype != kF16) ||
@@ -440,7 +457,8 @@ extern "C" int msa_attn_paged(const void* q, const void* k_cache, const void* v_
 #undef MSA_ATTN_PAGED
   const int rc = status_from(hipGetLastError());
   if (rc != kOk || A.splits == 1) return rc;
-  if (dtype == kBF16) hipLaunchKernelGGL(attn_paged_join<kBF16>, dim3(static_cast<unsigned>(items)), block, 0, st, A);
-  else hipLaunchKernelGGL(attn_paged_join<kF16>, dim3(static_cast<unsigned>(items)), block, 0, st, A);
+  const dim3 rows(grid_1d(total_tokens * q_heads, 4));
+  if (dtype == kBF16) hipLaunchKernelGGL(attn_paged_join<kBF16>, rows, block, 0, st, A);
+  else hipLaunchKernelGGL(attn_paged_join<kF16>, rows, block, 0, st, A);
   return status_from(hipGetLastError());
 }

@@ -36,9 +36,42 @@ struct TokenPlace {
   int seq;
   int64_t pos;
 };
+
+// The last s in [0, n) with first(s) <= x, for nondecreasing first with first(0) <= x; x the same in all lanes of the
+// wave, which all call it. 64 entries are compared at a time, so that a batch of up to 64 sequences costs one load's
+// latency (a bisection: one for every halving) and one of 4096 two.
+template <class First>
+__device__ __forceinline__ int wave_upper_index(int n, int64_t x, First first) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  for (int64_t step = 1;; step = 1) {
+    while (n - lo > 64 * step) step *= 64;
+    const int64_t i = lo + lane * step;
+    const uint64_t at_most = __ballot(i < n && first(static_cast<int>(i)) <= x);
+    lo += static_cast<int>((__popcll(at_most) - 1) * step);
+    if (step == 1) return lo;
+    n = static_cast<int>(min(static_cast<int64_t>(n), lo + step));
+  }
+}
 __device__ __forceinline__ TokenPlace place_of(const int32_t* __restrict__ cu, int nseq,
                                                const int32_t* __restrict__ context, int64_t t) {
   const int s = find_seq(cu, nseq, t);
+  const int32_t c = context[s];
+  return TokenPlace{s, c < 0 ? -1 : c + (t - cu[s])};
+}
+
+// place_of for a token that is the same in all lanes of a wave, which all call it.
+__device__ __forceinline__ TokenPlace wave_place_of(const int32_t* __restrict__ cu, int nseq,
+                                                    const int32_t* __restrict__ context, int64_t t) {
+  const auto start_of = [&](int i) { return static_cast<int64_t>(cu[i]); };
+  if (nseq <= 64) {  // both loads at once
+    const int lane = threadIdx.x & 63, i = lane < nseq ? lane : nseq - 1;
+    const int32_t start = cu[i], c_own = context[i];
+    const int s = __popcll(__ballot(lane < nseq && start <= t)) - 1;
+    const int32_t c = __builtin_amdgcn_readlane(c_own, s);
+    return TokenPlace{s, c < 0 ? -1 : c + (t - __builtin_amdgcn_readlane(start, s))};
+  }
+  const int s = wave_upper_index(nseq, t, start_of);
   const int32_t c = context[s];
   return TokenPlace{s, c < 0 ? -1 : c + (t - cu[s])};
 }

@@ -65,63 +65,71 @@ def _unit_rows(x):
     return x if x is None or x.stride(2) == 1 else x.contiguous()
 
 
-def _forward(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps):
-    side = [(x.data_ptr(), x.stride(0), x.stride(1), x.shape[1]) if x is not None else (None, 0, 0, 0) for x in (q, k)]
-    out = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if x is not None else None for x in (q, k)]
+def _call_args(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps):
+    """The arguments that both C calls begin with."""
+    total, heads, dim = q.shape
+    return (q.data_ptr(), *q.stride()[:2], heads, *((None, 0, 0, 0) if k is None else
+                                                    (k.data_ptr(), *k.stride()[:2], k.shape[1])),
+            _lib.DTYPE_CODE[q.dtype], wq.data_ptr(), None if wk is None else wk.data_ptr(), _lib.DTYPE_CODE[wq.dtype],
+            None if table is None else table.data_ptr(), rows, rot, cu.data_ptr(), num_seqs,
+            None if context is None else context.data_ptr(), total, dim, eps)
+
+
+def _forward(q, k, call):
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format, requires_grad=False)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format, requires_grad=False)
     if q.shape[0]:
         with _lib.on_device(q.device):
-            status = _lib.lib().msa_qk_norm_rope(
-                *side[0], *side[1], _lib.DTYPE_CODE[q.dtype], wq.data_ptr(), _lib.ptr(wk),
-                _lib.DTYPE_CODE[wq.dtype], _lib.ptr(table), rows, rot, cu.data_ptr(), num_seqs, _lib.ptr(context),
-                q.shape[0], q.shape[2], eps, out[0].data_ptr(), _lib.ptr(out[1]), _lib.stream_of(q.device))
+            status = _lib.lib().msa_qk_norm_rope(*call, q_out.data_ptr(), None if k is None else k_out.data_ptr(),
+                                                 _lib.stream_of(q.device))
         _lib.check(status, "msa_qk_norm_rope")
-    return out
+    return q_out, k_out
 
 
-def _backward(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps, dq_out, dk_out, need):
+def _side_gradients(x, w, g, need_x, need_w):
+    """(incoming gradient, dx, dw, heads) of one side, as the backward call takes them: 0 heads where nothing of it is
+    needed or no gradient came in."""
+    if x is None or g is None or not (need_x or need_w):
+        return None, None, None, 0
+    if g.dtype != x.dtype or not g.is_contiguous():
+        g = g.to(x.dtype).contiguous()
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+    dw = (torch.empty_like if x.shape[0] else torch.zeros_like)(w) if need_w else None
+    return g, dx, dw, x.shape[1]
+
+
+def _backward(q, k, wq, wk, call, dq_out, dk_out, need):
     """Gradients (q, k, q_weight, k_weight), None where not needed or no gradient came in."""
+    gq, dq, dwq, hq = _side_gradients(q, wq, dq_out, need[0], need[2])
+    gk, dk, dwk, hk = _side_gradients(k, wk, dk_out, need[1], need[3])
     total, _, dim = q.shape
-    xs, ws, gs = (q, k), (wq, wk), (dq_out, dk_out)
-    side, dx, dw, heads = [], [], [], []
-    gs = tuple(None if g is None else g.to(x.dtype).contiguous() for g, x in zip(gs, xs))
-    for x, w, g, need_x, need_w in zip(xs, ws, gs, need[:2], need[2:]):
-        on = x is not None and g is not None
-        dx.append(torch.empty(x.shape, dtype=x.dtype, device=x.device) if on and need_x else None)
-        dw.append(torch.zeros_like(w) if on and need_w and not total else
-                  torch.empty_like(w) if on and need_w else None)
-        heads.append(x.shape[1] if dx[-1] is not None or dw[-1] is not None else 0)
-        side.append((x.data_ptr(), x.stride(0), x.stride(1), x.shape[1]) if x is not None else (None, 0, 0, 0))
-    if total and any(heads):
+    if total and (hq or hk):
         lib = _lib.lib()
-        size = lib.msa_qk_norm_rope_bwd_workspace_bytes(total, heads[0], heads[1], dim) if any(
-            w is not None for w in dw) else 0
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        size, workspace = 0, None
+        if dwq is not None or dwk is not None:
+            size = lib.msa_qk_norm_rope_bwd_workspace_bytes(total, hq, hk, dim)
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
         with _lib.on_device(q.device):
             status = lib.msa_qk_norm_rope_bwd(
-                *side[0], *side[1], _lib.DTYPE_CODE[q.dtype], wq.data_ptr(), _lib.ptr(wk),
-                _lib.DTYPE_CODE[wq.dtype], _lib.ptr(table), rows, rot, cu.data_ptr(), num_seqs, _lib.ptr(context),
-                total, dim, eps, _lib.ptr(gs[0]), _lib.ptr(gs[1]), _lib.ptr(dx[0]), _lib.ptr(dx[1]), _lib.ptr(dw[0]),
-                _lib.ptr(dw[1]), _lib.ptr(workspace), size, _lib.stream_of(q.device))
+                *call, *[None if x is None else x.data_ptr() for x in (gq, gk, dq, dk, dwq, dwk, workspace)], size,
+                _lib.stream_of(q.device))
         _lib.check(status, "msa_qk_norm_rope_bwd")
-    return dx[0], dx[1], dw[0], dw[1]
+    return dq, dk, dwq, dwk
 
 
 class _NormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps):
+    def forward(ctx, q, k, wq, wk, table, cu, context, call):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, wq, wk, table, cu, context)
-        ctx.args = (rows, rot, num_seqs, eps)
-        return tuple(_forward(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps))
+        ctx.save_for_backward(q, k, wq, wk, table, cu, context)  # (all that `call` points into)
+        ctx.call = call
+        return _forward(q, k, call)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
-        q, k, wq, wk, table, cu, context = ctx.saved_tensors
-        rows, rot, num_seqs, eps = ctx.args
-        grads = _backward(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps, dq_out, dk_out,
-                          ctx.needs_input_grad[:4])
-        return (*grads, None, None, None, None, None, None, None)
+        q, k, wq, wk, _, _, _ = ctx.saved_tensors
+        return (*_backward(q, k, wq, wk, ctx.call, dq_out, dk_out, ctx.needs_input_grad), None, None, None, None)
 
 
 def _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps, context_lens):
@@ -174,7 +182,10 @@ def m3_qk_norm_rope(
     packed sequence plus ``context_lens`` of that sequence (int32 ``[N]`` on the device, default 0); where the
     table has no row for it, the rotated dims are NaN. Token and head strides of ``q`` and ``k`` are free
     (slices of a fused projection are read in place). The index heads go through the same call."""
-    args = _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps, context_lens)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in args[:4]):
-        return _NormRope.apply(*args)
-    return tuple(_forward(*args))
+    q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps = _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens,
+                                                                           eps, context_lens)
+    call = _call_args(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps)
+    if torch.is_grad_enabled() and (q.requires_grad or wq.requires_grad or
+                                    (k is not None and (k.requires_grad or wk.requires_grad))):
+        return _NormRope.apply(q, k, wq, wk, table, cu, context, call)
+    return _forward(q, k, call)

@@ -21,20 +21,21 @@ FP8 = torch.float8_e4m3fn
 
 
 def check_cache(cache, name, dtypes, heads, dim, device):
-    """Shape, type, device and row alignment of a cache; returns its page size."""
-    if cache.ndim != 4 or cache.shape[1] != heads or cache.shape[3] != dim:
+    """Shape, type, device and row alignment of a cache; returns its page size and its (page, head, slot) strides."""
+    shape = cache.shape
+    if len(shape) != 4 or shape[1] != heads or shape[3] != dim:
         raise ValueError(f"{name} must be [pages, {heads}, page size, {dim}]")
     if cache.dtype not in dtypes:
         raise TypeError(f"{name} must have dtype {' or '.join(str(d) for d in dtypes)}")
     if cache.device != device:
         raise ValueError(f"{name} must be on the input device")
-    page = cache.shape[2]
+    page = shape[2]
     if page < 16 or page > 256 or page & (page - 1):
         raise ValueError("the page size must be a power of two from 16 to 256")
-    size = cache.element_size()
-    if cache.stride(3) != 1 or cache.data_ptr() % 16 or any(s * size % 16 for s in cache.stride()[:3]):
+    of_page, of_head, of_slot, of_dim = cache.stride()
+    if of_dim != 1 or (cache.data_ptr() | (of_page | of_head | of_slot) * cache.element_size()) & 15:
         raise ValueError(f"{name} rows must be contiguous and 16-byte aligned")
-    return page
+    return page, (of_page, of_head, of_slot)
 
 
 def check_scale(scale, name, cache):
@@ -50,14 +51,15 @@ def check_scale(scale, name, cache):
 
 
 def check_kv_caches(k_cache, v_cache, k_scale, v_scale, heads, dim, dtype, device):
-    """The key and value caches of one layer: of the input type, or both in 8 bits. Returns the page size."""
-    page = check_cache(k_cache, "k_cache", (dtype, FP8), heads, dim, device)
-    check_cache(v_cache, "v_cache", (k_cache.dtype,), heads, dim, device)
+    """The key and value caches of one layer: of the input type, or both in 8 bits. Returns the page size and the
+    strides of both."""
+    page, of_k = check_cache(k_cache, "k_cache", (dtype, FP8), heads, dim, device)
+    _, of_v = check_cache(v_cache, "v_cache", (k_cache.dtype,), heads, dim, device)
     if k_cache.shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have one shape")
     check_scale(k_scale, "k_scale", k_cache)
     check_scale(v_scale, "v_scale", v_cache)
-    return page
+    return page, of_k + of_v
 
 
 def check_pages(page_table, cu_seqlens, context_lens, total, page, device):

@@ -18,8 +18,9 @@ import torch
 from . import _lib
 from .paged import FP8, check_kv_caches, check_pages, page_args, sixteen_bit
 
+_Strides = ctypes.c_int64 * 6
 
-@torch.no_grad()
+
 def m3_sparse_attention_paged(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -53,7 +54,7 @@ def m3_sparse_attention_paged(
         raise ValueError("Hq must be a positive multiple of G")
     if indices.device != q.device:
         raise ValueError("indices must be on the input device")
-    page = check_kv_caches(k_cache, v_cache, k_scale, v_scale, groups, dim, q.dtype, q.device)
+    page, strides = check_kv_caches(k_cache, v_cache, k_scale, v_scale, groups, dim, q.dtype, q.device)
     if not isinstance(block_size, int) or block_size <= 0:
         raise ValueError("block_size must be a positive integer")
     if block_size > 2147483647:
@@ -69,18 +70,17 @@ def m3_sparse_attention_paged(
     q, indices = q.contiguous(), indices.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((total, heads), dtype=torch.float32, device=q.device)
+    out = torch.empty_like(q, requires_grad=False)
+    lse = torch.empty((total, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if total:
         lib = _lib.lib()
         size = lib.msa_attn_paged_workspace_bytes(total, heads, groups, dim, slots, block_size)
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        strides = (ctypes.c_int64 * 6)(*k_cache.stride()[:3], *v_cache.stride()[:3])
         with _lib.on_device(q.device):
             status = lib.msa_attn_paged(
                 q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.DTYPE_CODE[q.dtype], k_cache.dtype == FP8,
-                _lib.ptr(k_scale), _lib.ptr(v_scale), strides, indices.data_ptr(), *page_args(pages, k_cache),
+                _lib.ptr(k_scale), _lib.ptr(v_scale), _Strides(*strides), indices.data_ptr(), *page_args(pages, k_cache),
                 cu.data_ptr(), num_seqs, context.data_ptr(), total, heads, groups, dim, slots, block_size,
-                effective_scale, _lib.ptr(workspace), size, out.data_ptr(), lse.data_ptr(), _lib.stream_of(q.device))
+                effective_scale, _lib.ptr(workspace), size, out.data_ptr(), _lib.ptr(lse), _lib.stream_of(q.device))
         _lib.check(status, "msa_attn_paged")
     return (out, lse) if return_lse else out

@@ -17,7 +17,6 @@ from . import _lib
 from .paged import check_cache, check_pages, page_args, sixteen_bit
 
 
-@torch.no_grad()
 def m3_index_score_topk_paged(
     index_q: torch.Tensor,
     index_cache: torch.Tensor,
@@ -42,7 +41,7 @@ def m3_index_score_topk_paged(
         raise ValueError("expected index_q[T,G,Di] with G, Di > 0")
     total, groups, dim = index_q.shape
     sixteen_bit(index_q, "m3_index_score_topk_paged")
-    page = check_cache(index_cache, "index_cache", (index_q.dtype,), 1, dim, index_q.device)
+    page, strides = check_cache(index_cache, "index_cache", (index_q.dtype,), 1, dim, index_q.device)
     if not isinstance(block_size, int) or block_size <= 0:
         raise ValueError("block_size must be a positive integer")
     if not isinstance(max_seqlen, int) or max_seqlen <= 0:
@@ -69,8 +68,8 @@ def m3_index_score_topk_paged(
     if total:
         with _lib.on_device(q.device):
             status = _lib.lib().msa_index_score_topk_paged(
-                q.data_ptr(), index_cache.data_ptr(), _lib.DTYPE_CODE[q.dtype], index_cache.stride(0),
-                index_cache.stride(2), *page_args(pages, index_cache), cu.data_ptr(), num_seqs, context.data_ptr(),
+                q.data_ptr(), index_cache.data_ptr(), _lib.DTYPE_CODE[q.dtype], strides[0],
+                strides[2], *page_args(pages, index_cache), cu.data_ptr(), num_seqs, context.data_ptr(),
                 total, groups, dim, blocks, block_size, scale, topk_blocks, local_blocks, scores.data_ptr(),
                 indices.data_ptr(), _lib.stream_of(q.device))
         _lib.check(status, "msa_index_score_topk_paged")
