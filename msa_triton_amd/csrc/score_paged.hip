@@ -16,17 +16,20 @@
 //
 // Bound by reading the index keys once from HBM (256 bytes a key for 128 dims): a wave takes one key
 // block for 16 query rows (tokens x groups of a sequence), its key fragments straight from memory in the
-// operand layout (lane c a key, 64 contiguous bytes of it for each 32 dims and four lanes). Query rows are
-// numbered without a list of tiles: sequence s gets the tiles from cu[s] G / 16 + s on, which leaves room
-// for its partly filled last one.
+// operand layout (lane c a key, 64 contiguous bytes of it for each 32 dims and four lanes), the next group of
+// them in flight during the products of one. Sequences of a batch differ in length by orders, so the (tile,
+// block) pairs of all of them are counted in front and shared out evenly over the waves.
 #include "mfma_util.hpp"
 #include "paged.hpp"
 #include "score_mfma.hpp"
 #include "topk_row.hpp"
-#include <stdlib.h>
 
 namespace msa {
 namespace {
+
+// Workgroups of a call: two a CU, as many as run at once (us with 256 / 512 / 768, top-k included: 32 requests of
+// 0.5 to 30K tokens 27.6 / 25.7 / 30.0, 64 of 16K 58.0 / 58.5 / 61.9, 256 of 4K 63.9 / 62.2 / 64.9).
+constexpr int64_t kBlocks = 512;
 
 struct PagedScoreArgs {
   const uint16_t* iq;  // [T][G][Di]
@@ -37,10 +40,28 @@ struct PagedScoreArgs {
   const int32_t* context;
   int64_t tokens;
   int G, Di, NB, B;
-  int parts;         // workgroups of a tile: four blocks each at a time
   float sign, scale; // of the logits: direction and magnitude
   float* scores;     // [T][G][NB]
 };
+
+// A sequence of the call: its first token and its tokens, the cached ones in front, its tiles of 16 query rows and the key
+// blocks they go through (one for a sequence that is not there).
+struct SeqWork {
+  int32_t start, count, context;
+  int tiles, blocks;
+  __device__ __forceinline__ int64_t items() const { return static_cast<int64_t>(tiles) * blocks; }
+};
+__device__ __forceinline__ SeqWork seq_work(const PagedScoreArgs& A, int32_t start, int32_t end, int32_t context) {
+  // (unsigned: a context that no page table holds may bring the sum past 2^31)
+  const uint32_t n = end - start, blocks = context < 0 || n == 0 ? 1u : (context + n - 1) / static_cast<uint32_t>(A.B) + 1;
+  return SeqWork{start, end - start, context, static_cast<int>((n * A.G + 15) / 16),
+                 static_cast<int>(min(blocks, static_cast<uint32_t>(A.NB)))};
+}
+
+// a / b, in 32 bits where a fits (a 64-bit division is some 100 instructions)
+__device__ __forceinline__ int64_t quotient(int64_t a, uint32_t b) {
+  return a >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / b);
+}
 
 template <int NK>
 struct QueryFrags {
@@ -72,32 +93,25 @@ __device__ __forceinline__ double fma_words(bf16x8 a, bf16x8 b, double acc) {
   return acc;
 }
 
+// Blocks [block0, block1) of one tile of a sequence, by a wave; what its tokens do not see, up to block `fill`, gets -inf.
 // FULL: Di is 32 NK, and a lane's pieces of a key row are at constant offsets.
 template <int DT, int NK, bool FULL>
-__global__ __launch_bounds__(256, NK == 8 ? 1 : 2) void score_paged_kernel(PagedScoreArgs A) {
+__device__ __forceinline__ void score_run(const PagedScoreArgs& A, const SeqWork& W, int s, int tile, int block0,
+                                          int block1, int fill) {
   const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tile = blockIdx.x / A.parts;
-  const int part = static_cast<int>(blockIdx.x % A.parts);
-  // the last sequence whose tiles start at or below `tile`
-  const int s = wave_upper_index(A.nseq, tile, [&](int i) { return ((A.cu[i] * static_cast<int64_t>(A.G)) >> 4) + i; });
-  const int64_t start = A.cu[s], rows = (A.cu[s + 1] - start) * A.G;
-  const int32_t context = A.context[s];
-  const int64_t r0 = (tile - ((start * A.G) >> 4) - s) * 16;
-  if (r0 >= rows) return;
+  const int64_t start = W.start, rows = static_cast<int64_t>(W.count) * A.G, r0 = static_cast<int64_t>(tile) * 16;
+  const int32_t context = W.context;
   const int64_t row = r0 + c;
   const bool live = row < rows;
-  const int32_t i = static_cast<int32_t>((live ? row : rows - 1) / A.G);  // token of the sequence
+  const int32_t i = static_cast<uint32_t>(live ? row : rows - 1) / static_cast<uint32_t>(A.G);  // token of the sequence
   const int64_t pos = context < 0 ? -1 : static_cast<int64_t>(context) + i;
-  const int64_t last = context < 0 ? -1 : static_cast<int64_t>(context) + (min(r0 + 16, rows) - 1) / A.G;
+  const int64_t last = context < 0 ? -1 : static_cast<int64_t>(context) + static_cast<uint32_t>(min(r0 + 16, rows) - 1) / static_cast<uint32_t>(A.G);
   float* out = A.scores + (start * A.G + (live ? row : rows - 1)) * A.NB;
-  const int seen_blocks = A.pages.num_pages > 0 ? static_cast<int>(min((last + A.B) / A.B, static_cast<int64_t>(A.NB))) : 0;
-
-  // blocks behind the tile's tokens: four lanes a row, this workgroup's share
-  for (int b = seen_blocks + 16 * part + 4 * wave + q4; b < A.NB; b += 16 * A.parts)
+  const int seen_blocks = A.pages.num_pages == 0 || last < 0 ? 0 : static_cast<int>(min(static_cast<uint32_t>(last) / A.B + 1, static_cast<uint32_t>(A.NB)));
+  const int stop = min(block1, seen_blocks);
+  for (int b = max(block0, seen_blocks) + q4; b < fill; b += 4)
     if (live) out[b] = -__builtin_inff();
-
-  if (4 * part + wave >= seen_blocks) return;
+  if (block0 >= stop) return;
   const uint16_t* qrow = A.iq + (start * A.G + (live ? row : rows - 1)) * A.Di;
   QueryFrags<NK> Q;
   float most = 0.f, tiny = 0.f;
@@ -145,7 +159,7 @@ __global__ __launch_bounds__(256, NK == 8 ? 1 : 2) void score_paged_kernel(Paged
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  int block = 4 * part + wave;
+  int block = block0;
   int64_t kc = static_cast<int64_t>(block) * A.B, k1 = min(kc + A.B, last + 1);
   int own_page = pages_of(kc, k1);
   bf16x8 f0[GT][NK], f1[GT][NK];
@@ -155,8 +169,8 @@ __global__ __launch_bounds__(256, NK == 8 ? 1 : 2) void score_paged_kernel(Paged
   while (true) {
     // the chunk behind this one: of this block, or the first of this wave's next one
     const bool block_ends = kc + 16 * kTiles >= k1;
-    const int next_block = block_ends ? block + 4 * A.parts : block;
-    const bool more = next_block < seen_blocks;
+    const int next_block = block_ends ? block + 1 : block;
+    const bool more = next_block < stop;
     const int64_t next_kc = block_ends ? static_cast<int64_t>(next_block) * A.B : kc + 16 * kTiles;
     const int64_t next_k1 = block_ends ? min(next_kc + A.B, last + 1) : k1;
     const int next_page = more ? pages_of(next_kc, next_k1) : -1;
@@ -236,12 +250,79 @@ __global__ __launch_bounds__(256, NK == 8 ? 1 : 2) void score_paged_kernel(Paged
   }
 }
 
-int part_count(int64_t tiles, int64_t blocks) {
-  const char* e = getenv("MSA_PARTS");
-  int64_t n = ((e ? atoi(e) : 1024) + tiles - 1) / tiles;
-  const int64_t most = (blocks + 3) / 4;
-  n = n < most ? n : most;
-  return static_cast<int>(n < 1 ? 1 : n);
+template <int DT, int NK, bool FULL>
+__global__ __launch_bounds__(256, 2) void score_paged_kernel(PagedScoreArgs A) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // The batch's work is its (tile, block) pairs, numbered sequence by sequence: counted here, a sequence a lane where
+  // there are up to 64 (no LDS, no barrier: 2 us of the 10 us of one long sequence's call), otherwise `per` a thread.
+  __shared__ int64_t first_item[257];  // of the sequences that thread i counts
+  __shared__ int64_t wave_items[4];
+  const bool few = A.nseq <= 64;
+  const int per = (A.nseq + 255) / 256;
+  SeqWork mine{};
+  int64_t upto = 0, items;
+  if (few) {
+    if (lane < A.nseq) mine = seq_work(A, A.cu[lane], A.cu[lane + 1], A.context[lane]);
+    upto = mine.items();
+  } else {
+    for (int s = threadIdx.x * per; s < min(A.nseq, (static_cast<int>(threadIdx.x) + 1) * per); ++s)
+      upto += seq_work(A, A.cu[s], A.cu[s + 1], A.context[s]).items();
+  }
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int64_t x = __shfl_up(upto, o, kWave);
+    if (lane >= o) upto += x;
+  }
+  if (few) {
+    items = __shfl(upto, 63, kWave);
+  } else {
+    if (lane == 63) wave_items[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += wave_items[w];
+    first_item[threadIdx.x + 1] = upto;
+    if (threadIdx.x == 0) first_item[0] = 0;
+    __syncthreads();
+    items = first_item[256];
+  }
+  // a wave takes a stretch of them as long as the others', to one
+  const uint32_t waves = gridDim.x * 4, own = blockIdx.x * 4 + wave;
+  const int64_t share = quotient(items, waves), extra = items - share * waves;
+  int64_t item = own * share + min(static_cast<int64_t>(own), extra);
+  const int64_t end_item = item + share + (own < extra ? 1 : 0);
+  while (item < end_item) {
+    int s;
+    int64_t rest;
+    SeqWork work;
+    if (few) {
+      s = __builtin_ctzll(__ballot(upto > item));
+      work.start = __builtin_amdgcn_readlane(mine.start, s);
+      work.count = __builtin_amdgcn_readlane(mine.count, s);
+      work.context = __builtin_amdgcn_readlane(mine.context, s);
+      work.tiles = __builtin_amdgcn_readlane(mine.tiles, s);
+      work.blocks = __builtin_amdgcn_readlane(mine.blocks, s);
+      rest = item - (__shfl(upto, s, kWave) - work.items());
+    } else {
+      int lo = 0, hi = 256;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first_item[mid] <= item) lo = mid; else hi = mid;
+      }
+      s = __builtin_amdgcn_readfirstlane(lo * per);
+      rest = item - first_item[lo];
+      work = seq_work(A, A.cu[s], A.cu[s + 1], A.context[s]);
+      while (rest >= work.items()) {
+        rest -= work.items();
+        ++s;
+        work = seq_work(A, A.cu[s], A.cu[s + 1], A.context[s]);
+      }
+    }
+    const int tile = static_cast<int>(quotient(rest, work.blocks));
+    const int block0 = static_cast<int>(rest - static_cast<int64_t>(tile) * work.blocks);
+    const int block1 = static_cast<int>(min(static_cast<int64_t>(work.blocks), block0 + (end_item - item)));
+    item += block1 - block0;
+    score_run<DT, NK, FULL>(A, work, s, tile, block0, block1, block1 == work.blocks ? A.NB : block1);
+  }
 }
 
 }  // namespace
@@ -267,7 +348,7 @@ extern "C" int msa_index_score_topk_paged(const void* index_q, const void* index
   if (reinterpret_cast<uintptr_t>(index_cache) % 16 || reinterpret_cast<uintptr_t>(index_q) % 16 ||
       cache_stride_page % 8 || cache_stride_slot % 8)
     return kErrInvalidArgument;
-  if (index_dim % 8 || index_dim > 256 || block_size % 16) return kErrUnsupported;
+  if (index_dim % 8 || index_dim > 256 || block_size % 16 || total_tokens * groups > 0x7fffffff) return kErrUnsupported;
   if (total_tokens == 0) return kOk;
   PagedScoreArgs A{};
   A.iq = static_cast<const uint16_t*>(index_q);
@@ -284,11 +365,9 @@ extern "C" int msa_index_score_topk_paged(const void* index_q, const void* index
   A.sign = scale > 0.0 ? 1.f : scale < 0.0 ? -1.f : 0.f;
   A.scale = static_cast<float>(scale < 0.0 ? -scale : scale);
   A.scores = scores;
-  const int64_t tiles = total_tokens * groups / 16 + num_seqs;
-  A.parts = part_count(tiles, A.NB);
-  if (tiles >= (int64_t{1} << 24) / A.parts) return kErrUnsupported;  // 2^32 threads of a launch
+  const int64_t items = (total_tokens * groups / 16 + num_seqs) * num_blocks;  // at most
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(tiles * A.parts)), block(256);
+  const dim3 grid(static_cast<unsigned>(items < 4 * kBlocks ? (items + 3) / 4 : kBlocks)), block(256);
 #define MSA_SCORE_PAGED(NK)                                                                               \
   if (dtype == kBF16 && index_dim == 32 * NK)                                                             \
     hipLaunchKernelGGL((score_paged_kernel<kBF16, NK, true>), grid, block, 0, st, A);                     \

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void topk_select_kernel(const float* __restric
   topk_threshold<VPL, CAP>(scores, at, rows, G, NB, B, K, L, out, wave, threadIdx.x & 63, cand[wid]);
 }
 
-// One wavefront per row for long rows (more than 1024 blocks): topk_row64.
+// One wavefront per row for long rows with more than 64 slots (1025 to 4096 blocks): topk_row64.
 template <int VPL, class Rows>
 __global__ __launch_bounds__(256) void topk_wave_kernel(const float* __restrict__ scores,
                                                         Rows at, int64_t rows, int G, int NB, int B, int K, int L,
@@ -87,12 +87,14 @@ static int topk_launch_rows(const float* scores, const Rows& at, int64_t rows, i
   if (NB <= 16) MSA_TOPK_LAUNCH(1);
   else if (NB <= 32) MSA_TOPK_LAUNCH(2);
   else if (NB <= 64) MSA_TOPK_LAUNCH(4);
-  else if (K <= kSelectMostSlots && NB <= 1024 && K > (NB <= 128 ? kArgmaxSlots128 : NB <= 256 ? kArgmaxSlots256 : 0) &&
+  else if (K <= kSelectMostSlots && NB <= 4096 && K > (NB <= 128 ? kArgmaxSlots128 : NB <= 256 ? kArgmaxSlots256 : 0) &&
            rows < (int64_t{1} << 32) / kWave) {  // (a launch holds fewer than 2^32 threads: up to a wave per row here)
     if (NB <= 128) { MSA_TOPK_SELECT(2); }
     else if (NB <= 256) { MSA_TOPK_SELECT(4); }
     else if (NB <= 512) { MSA_TOPK_SELECT(8); }
-    else { MSA_TOPK_SELECT(16); }
+    else if (NB <= 1024) { MSA_TOPK_SELECT(16); }
+    else if (NB <= 2048) { MSA_TOPK_SELECT(32); }
+    else { MSA_TOPK_SELECT(64); }
   }
   else if (NB <= 128) MSA_TOPK_LAUNCH(8);
   else if (NB <= 256) MSA_TOPK_LAUNCH(16);

@@ -8,7 +8,7 @@
 // torch.topk). Ties (equal values, e.g. several +inf local blocks, or NaNs) are
 // emitted in ascending block order.
 #pragma once
-#include "common.hpp"
+#include "paged.hpp"
 
 namespace msa {
 
@@ -18,16 +18,22 @@ struct PackedRows {
   const int32_t* cu;
   int nseq;
   __device__ __forceinline__ int query_block(int32_t t, int B) const { return (t - cu[find_seq(cu, nseq, t)]) / B; }
+  __device__ __forceinline__ int wave_query_block(int32_t t, int B) const { return query_block(t, B); }
 };
 struct CachedRows {
   const int32_t* cu;
   int nseq;
   const int32_t* context;
   __device__ __forceinline__ int query_block(int32_t t, int B) const {
-    const int s = find_seq(cu, nseq, t);
-    const int32_t c = context[s];
-    // (a sum past 2^31 has no block: the position does not fit a page table)
-    return c < 0 ? -1 : static_cast<int>(min((static_cast<int64_t>(c) + (t - cu[s])) / B, int64_t{0x7fffffff} - 1));
+    return block_at(place_of(cu, nseq, context, t).pos, B);
+  }
+  // for a token that is the same in all lanes of a wave, which all call it
+  __device__ __forceinline__ int wave_query_block(int32_t t, int B) const {
+    return block_at(wave_place_of(cu, nseq, context, t).pos, B);
+  }
+  // (a position past 2^31 has no block: it does not fit a page table)
+  static __device__ __forceinline__ int block_at(int64_t pos, int B) {
+    return pos < 0 ? -1 : static_cast<int>(min(pos / B, int64_t{0x7fffffff} - 1));
   }
 };
 
@@ -218,7 +224,7 @@ __device__ __forceinline__ uint32_t bitonic_sort_u32(uint32_t x) {
   else return r;
 }
 
-// The selection of rows of 65 to 1024 blocks with up to 64 slots, by threshold and sort:
+// The selection of rows of 65 to 4096 blocks with up to 64 slots, by threshold and sort:
 // the row's ordered keys sit in the wave's registers (lane j: blocks j, j + 64, ...), the
 // sel-th largest of the lane maxima (one bitonic sort over lanes), or a bisection on ballot
 // counts from there, gives a key that between `sel` and CAP values reach; those go to LDS and
@@ -227,7 +233,9 @@ __device__ __forceinline__ uint32_t bitonic_sort_u32(uint32_t x) {
 // scalar counts (threshold by bisection alone: 410 us where the lane maxima give 325, and 538
 // with 32 slots in CAP = 32). Measured against the iterated argmax of topk_row16, a 16-lane
 // 64-bit maximum per slot: 65 536 tokens x 8 groups, 512 blocks, 32 slots 757 -> 325 us;
-// 32 768 x 4, 256 blocks, 16 slots 71 -> 52 us.
+// 32 768 x 4, 256 blocks, 16 slots 71 -> 52 us. Rows of more than 1024 blocks against topk_row64's pick by
+// pick: 8192 rows, 2048 blocks, 16 slots 66 -> 15 us; 65 536 rows, 4096 blocks, 32 slots 1707 -> 186, 1500 blocks, one slot
+// 111 -> 63; 4400 rows, 1100 blocks, 16 slots 45 -> 11.
 constexpr int kSelectMostSlots = 64, kSelectPairSlots = 24;
 // A row's threshold and two sorts cost the same for one slot as for 24, the argmax of topk_row16 by
 // the slot: rows of up to 128 (256) blocks take that one up to these many slots. Argmax / sort, us,
@@ -246,7 +254,7 @@ __device__ __forceinline__ void topk_threshold(const float* __restrict__ scores,
     if (row >= rows) break;  // wave-uniform
     const int32_t t = static_cast<int32_t>(rows <= 0x7fffffff ? static_cast<uint32_t>(row) / static_cast<uint32_t>(G)
                                                               : row / G);
-    const int32_t qb = rows_at.query_block(t, B);
+    const int32_t qb = rows_at.wave_query_block(t, B);
     const int n = qb + 1 < NB ? qb + 1 : NB;
     const int sel = K < n ? K : n;  // slots to fill
     const int own0 = L > 0 && qb - L + 1 < n ? qb - L + 1 : n;  // the forced local blocks: own0 .. n - 1
@@ -337,8 +345,8 @@ __device__ __forceinline__ void topk_threshold(const float* __restrict__ scores,
 }
 
 // Host launch of the stand-alone selection (topk.hip): 16-lane rows up to 64 blocks,
-// threshold and sort up to 1024 (16-lane rows there for more than 64 slots, and up to 256
-// blocks for few), one wavefront per row with the row in registers up to 4096, streamed above.
+// threshold and sort up to 4096 (for more than 64 slots 16-lane rows up to 1024 blocks and one wavefront per row
+// with the row in registers above; for few slots 16-lane rows up to 256 blocks), streamed above.
 // With `context` the rows are tokens behind that many cached ones of their sequence.
 int topk_launch(const float* scores, const int32_t* cu_seqlens, int nseq, int64_t rows, int G, int NB, int B, int K,
                 int L, int32_t* indices, hipStream_t st, const int32_t* context = nullptr);
@@ -348,7 +356,7 @@ int topk_launch(const float* scores, const int32_t* cu_seqlens, int nseq, int64_
 template <int VPL, class Rows>
 __device__ __forceinline__ void topk_row64(const float* __restrict__ scores, const Rows& at, int G, int NB, int B, int K, int L,
                                            int32_t* __restrict__ out, int64_t row, int lane) {
-  const int64_t qb = at.query_block(static_cast<int32_t>(row / G), B);
+  const int64_t qb = at.wave_query_block(static_cast<int32_t>(row / G), B);
   const int n = static_cast<int>(qb + 1 < NB ? qb + 1 : NB);
   const int count = K < NB ? K : NB;
   const int sel = count < n ? count : n;
@@ -389,7 +397,7 @@ __device__ __forceinline__ void topk_row64(const float* __restrict__ scores, con
 template <class Rows>
 __device__ __forceinline__ void topk_row_stream(const float* __restrict__ scores, const Rows& at, int G, int NB, int B, int K, int L,
                                                 int32_t* __restrict__ out, int64_t row, int lane) {
-  const int64_t qb = at.query_block(static_cast<int32_t>(row / G), B);
+  const int64_t qb = at.wave_query_block(static_cast<int32_t>(row / G), B);
   const int n = static_cast<int>(qb + 1 < NB ? qb + 1 : NB);
   const int count = K < NB ? K : NB;
   const int sel = count < n ? count : n;
