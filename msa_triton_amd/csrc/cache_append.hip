@@ -8,14 +8,13 @@
 // again (exact for a power of two, except where they fall below e4m3's normal range). Values that are
 // not finite become NaN and do not enter the scale.
 //
-// y / s is formed in FP64 and rounded to e4m3 through round-to-odd fp32, so that the stored byte is
-// that of the exact y: a value an fp32 step away from a rounding border would be off by a whole e4m3 step
-// (2^-3) otherwise. The pass is bound by memory and, for single tokens, by its chain of loads
-// (sequence, page, row, scale), so the FP64 work is not seen.
+// y / s is formed in FP64 and rounded to e4m3 once, so that the stored byte is that of the exact y: a value an
+// fp32 step away from a rounding border would be off by a whole e4m3 step (2^-3) otherwise. The scale needs the
+// page's maximum only, which fp32 gives except next to a border (append_page).
 //
 // Work: 16-bit rows go to runs of LPR lanes, as in the norm. An 8-bit page, head and side is one
 // workgroup's, because its scale is needed before its first byte: one pass over the page's new rows for the
-// maximum, one to write them (from registers where they are few). Pages are numbered without a list of them:
+// maximum, one to write them (from registers where they are few, from the caches otherwise). Pages are numbered without a list of them:
 // sequence s gets the numbers from cu[s] / page + 2 s on, which leaves room for the two pages that n tokens can
 // touch beyond n / page; numbers without a page end at once.
 #include "norm_rope.hpp"
@@ -48,75 +47,87 @@ struct AppendArgs {
   float eps;
 };
 
+// Sum over runs of LPR lanes.
 template <int LPR>
 __device__ __forceinline__ double run_sum_f64(double v) {
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) v += __shfl_xor(v, o, kWave);
+#define MSA_DPP_ADD64(CTRL)                                                                                    \
+  {                                                                                                            \
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));                                         \
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(u), CTRL, 0xF, 0xF, false);       \
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0u, static_cast<uint32_t>(u >> 32), CTRL, 0xF, 0xF, false); \
+    v += __longlong_as_double(static_cast<long long>((static_cast<uint64_t>(hi) << 32) | lo));                  \
+  }
+  if constexpr (LPR >= 2) MSA_DPP_ADD64(0xB1)    // quad_perm [1, 0, 3, 2]
+  if constexpr (LPR >= 4) MSA_DPP_ADD64(0x4E)    // quad_perm [2, 3, 0, 1]
+  if constexpr (LPR >= 8) MSA_DPP_ADD64(0x141)   // row_half_mirror
+  if constexpr (LPR >= 16) MSA_DPP_ADD64(0x140)  // row_mirror
+#undef MSA_DPP_ADD64
+  if constexpr (LPR >= 32) v += __shfl_xor(v, 16, kWave);
+  if constexpr (LPR >= 64) v += __shfl_xor(v, 32, kWave);
   return v;
 }
 
-// The row's values y in FP64.
-template <int DT, int VEC, int C, int LPR>
-__device__ __forceinline__ void row_f64(const AppendArgs& A, const AppendSide& S, const RowLanes<DT, VEC, C, LPR>& lanes,
-                                        int64_t t, int head, int pos, bool live, double (&a)[C][VEC],
-                                        double (&b)[C][VEC]) {
-  float xa[C][VEC], xb[C][VEC];
-  lanes.load(S.x, t * S.stride_t + head * S.stride_h, live, xa, xb);
-  double ss = 0.0;
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      a[c][j] = xa[c][j], b[c][j] = xb[c][j];
-      ss = fma(a[c][j], a[c][j], fma(b[c][j], b[c][j], ss));
-    }
+// A loaded row's values y in FP64, in place.
+template <int VEC, int C, int LPR, class Lanes>
+__device__ __forceinline__ void norm_turn(const AppendArgs& A, const AppendSide& S, const Lanes& lanes,
+                                          const float (&co)[C][VEC], const float (&si)[C][VEC], double (&a)[C][VEC],
+                                          double (&b)[C][VEC]) {
   if (S.w) {
-    const double r = 1.0 / sqrt(run_sum_f64<LPR>(ss) / S.dim + static_cast<double>(A.eps));
+    double ss = 0.0;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) ss = fma(a[c][j], a[c][j], fma(b[c][j], b[c][j], ss));
+    const double r = rsqrt(run_sum_f64<LPR>(ss) / S.dim + static_cast<double>(A.eps));
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) a[c][j] *= r * lanes.wa[c][j], b[c][j] *= r * lanes.wb[c][j];
   }
-  if (S.turned && live) {
+  if (S.turned) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float co[VEC], si[VEC];
-      load_turn<VEC>(A.rope, lanes.pc[c], pos, co, si);
+    for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const double u = a[c][j], v = b[c][j];
-        a[c][j] = u * co[j] - v * si[j];
-        b[c][j] = v * co[j] + u * si[j];
+        a[c][j] = u * co[c][j] - v * si[c][j];
+        b[c][j] = v * co[c][j] + u * si[c][j];
       }
-    }
   }
 }
 
-__device__ __forceinline__ float finite_size(double x) {
-  const float m = fabsf(f64_to_f32_odd(x));
+__device__ __forceinline__ float finite_size(float x) {
+  const float m = fabsf(x);
   return m < __builtin_inff() ? m : 0.f;  // (NaN: 0)
 }
 
-// x rounded once to the fp32 whose rounding to e4m3 is that of x; NaN for what is not finite.
+// An fp32 value whose rounding to e4m3 is that of x, and that is above 448 x 2^k where x is: x cut to 21 significant
+// bits with what was cut off folded into the last one (e4m3 has 4, 448 has 3).
 __device__ __forceinline__ float for_fp8(double x) {
-  return __builtin_isfinite(x) ? f64_to_f32_odd(x) : __builtin_nanf("");
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x));
+  const uint32_t high = static_cast<uint32_t>(u >> 32) | (static_cast<uint32_t>(u) ? 1u : 0u);
+  return static_cast<float>(__longlong_as_double(static_cast<long long>(static_cast<uint64_t>(high) << 32)));
 }
+__device__ __forceinline__ float for_fp8(float x) { return x; }
 
 __device__ __forceinline__ uint32_t pack4_fp8(float x0, float x1, float x2, float x3) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, w, true));
 }
 
-template <int VEC>
-__device__ __forceinline__ void store_fp8(uint8_t* p, const double (&v)[VEC], double inv) {
-  if constexpr (VEC == 1) {
-    *p = static_cast<uint8_t>(pack4_fp8(for_fp8(v[0] * inv), 0.f, 0.f, 0.f));
-  } else {
-    uint2 w;
-    w.x = pack4_fp8(for_fp8(v[0] * inv), for_fp8(v[1] * inv), for_fp8(v[2] * inv), for_fp8(v[3] * inv));
-    w.y = pack4_fp8(for_fp8(v[4] * inv), for_fp8(v[5] * inv), for_fp8(v[6] * inv), for_fp8(v[7] * inv));
-    *reinterpret_cast<uint2*>(p) = w;
+// v * inv rounded to e4m3; NaN for what is not finite.
+template <int VEC, typename T>
+__device__ __forceinline__ void store_fp8(uint8_t* p, const T (&v)[VEC], T inv) {
+  float x[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    x[j] = for_fp8(v[j] * inv);
+    x[j] = fabsf(x[j]) < __builtin_inff() ? x[j] : __builtin_nanf("");
   }
+  if constexpr (VEC == 1)
+    *p = static_cast<uint8_t>(pack4_fp8(x[0], 0.f, 0.f, 0.f));
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack4_fp8(x[0], x[1], x[2], x[3]), pack4_fp8(x[4], x[5], x[6], x[7]));
 }
 
 // The smallest power of two s >= 2^-100 with 448 s >= amax (448 = 1.75 x 2^8); 0 for 0.
@@ -128,16 +139,28 @@ __device__ __forceinline__ float scale_for(float amax) {
   return __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
 }
 
+// The largest of three values over the workgroup (three floats of every wave in `lds`).
+__device__ __forceinline__ void block_max3(float& x, float& y, float& z, float* lds) {
+  x = wave_max_f32(x);
+  y = wave_max_f32(y);
+  z = wave_max_f32(z);
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) {
+    float* mine = lds + 3 * (threadIdx.x / kWave);
+    mine[0] = x, mine[1] = y, mine[2] = z;
+  }
+  __syncthreads();
+  x = fmaxf(fmaxf(lds[0], lds[3]), fmaxf(lds[6], lds[9]));
+  y = fmaxf(fmaxf(lds[1], lds[4]), fmaxf(lds[7], lds[10]));
+  z = fmaxf(fmaxf(lds[2], lds[5]), fmaxf(lds[8], lds[11]));
+}
+
 // One 8-bit page, head and side.
 template <int DT, int VEC, int C, int LPR>
-__device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t unit, int head, float* amax_of_wave) {
+__device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t unit, int head, float* lds) {
   using Lanes = RowLanes<DT, VEC, C, LPR>;
-  int lo = 0, hi = A.nseq;  // the last sequence whose numbers start at or below `unit`
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if ((A.cu[mid] >> A.pages.shift) + 2 * static_cast<int64_t>(mid) <= unit) lo = mid; else hi = mid;
-  }
-  const int s = lo;
+  // the last sequence whose numbers start at or below `unit`
+  const int s = wave_upper_index(A.nseq, unit, [&](int i) { return (A.cu[i] >> A.pages.shift) + 2 * static_cast<int64_t>(i); });
   const int64_t start = A.cu[s], n = A.cu[s + 1] - start, context = A.context[s];
   if (context < 0 || n <= 0) return;
   const int64_t p = (context >> A.pages.shift) + (unit - (start >> A.pages.shift) - 2 * static_cast<int64_t>(s));
@@ -152,35 +175,96 @@ __device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t un
   float* scale = S.scale + static_cast<int64_t>(page) * S.heads + head;
   const float before = kept ? *scale : 0.f;
   const Lanes lanes(S.w, A.w_f32, S.turned ? A.rope.half : 0, S.dim);
-  const int row = threadIdx.x / LPR;
-  double a[C][VEC], b[C][VEC];
-  float amax = 0.f;
-  for (int base = (rows - 1) / Lanes::kRows * Lanes::kRows; base >= 0; base -= Lanes::kRows) {  // the first rows stay
-    const int i = base + row;
-    row_f64<DT, VEC, C, LPR>(A, S, lanes, t0 + i, head, static_cast<int>(first + i), i < rows, a, b);
-    if (i < rows) {
+  const int row = threadIdx.x / LPR, last_batch = (rows - 1) / Lanes::kRows;
+  const bool exact = S.w || S.turned;  // (otherwise y is the input itself)
+  float a[C][VEC], b[C][VEC], co[C][VEC], si[C][VEC];
+  auto load = [&](int batch) {
+    const int i = batch * Lanes::kRows + row;
+    lanes.load(S.x, (t0 + i) * S.stride_t + head * S.stride_h, i < rows, a, b);
+    if (S.turned) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) load_turn<VEC>(A.rope, lanes.pc[c], i < rows ? static_cast<int>(first + i) : -1, co[c], si[c]);
+    }
+    return i;
+  };
+  // The maximum, in fp32: off by less than 2^-19 of the largest |u cos| + |v sin| (`size`; some 16 steps of 2^-24), which
+  // can matter only next to 448 x 2^k, or by more where fp32 has no range for the norm (`odd`; also what is not
+  // finite). Both are seen below, and the maximum is taken again in FP64.
+  float amax = 0.f, size = 0.f, odd = 0.f;
+  for (int batch = last_batch; batch >= 0; --batch) {  // the first rows last: they stay in registers
+    const int i = load(batch);
+    if (!exact) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, fmaxf(finite_size(a[c][j]), finite_size(b[c][j])));
+      continue;
+    }
+    float r = 1.f;
+    if (S.w) {
+      const float ms = run_sum<LPR>(sum_products(a, b, a, b)) / static_cast<float>(S.dim) + A.eps;
+      if (i < rows && !(ms < 0x1p100f && ms > 0x1p-60f)) odd = 1.f;
+      r = 1.f / sqrtf(ms);
+    }
+    if (i < rows) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float u = S.w ? a[c][j] * r * lanes.wa[c][j] : a[c][j], v = S.w ? b[c][j] * r * lanes.wb[c][j] : b[c][j];
+          const float cs = S.turned ? co[c][j] : 1.f, sn = S.turned ? si[c][j] : 0.f;
+          const float m = fmaxf(fabsf(u * cs - v * sn), fabsf(v * cs + u * sn));
+          if (!(m < __builtin_inff())) odd = 1.f;
+          amax = fmaxf(amax, m);
+          size = fmaxf(size, fmaxf(fabsf(u * cs) + fabsf(v * sn), fabsf(v * cs) + fabsf(u * sn)));
+        }
     }
   }
-  amax = wave_max_f32(amax);
-  if (threadIdx.x % kWave == 0) amax_of_wave[threadIdx.x / kWave] = amax;
-  __syncthreads();  // (also: every thread has read the old scale)
-  amax = fmaxf(fmaxf(amax_of_wave[0], amax_of_wave[1]), fmaxf(amax_of_wave[2], amax_of_wave[3]));
+  block_max3(amax, size, odd, lds);  // (every thread has read the old scale)
+  if (exact && (odd != 0.f || scale_for(fmaxf(amax - 0x1p-19f * size, 0.f)) != scale_for(amax + 0x1p-19f * size))) {
+    amax = 0.f;
+    for (int batch = last_batch; batch >= 0; --batch) {
+      const int i = load(batch);
+      double ya[C][VEC], yb[C][VEC];
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) ya[c][j] = a[c][j], yb[c][j] = b[c][j];
+      norm_turn<VEC, C, LPR>(A, S, lanes, co, si, ya, yb);
+      if (i < rows) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            amax = fmaxf(amax, fmaxf(finite_size(for_fp8(ya[c][j])), finite_size(for_fp8(yb[c][j]))));
+      }
+    }
+    block_max3(amax, size, odd, lds);
+  }
   const float after = fmaxf(before, scale_for(amax));
   const double inv = after > 0.f ? 1.0 / static_cast<double>(after) : 0.0;
   uint8_t* dst = static_cast<uint8_t*>(S.cache.base) + page * S.cache.stride_page + head * S.cache.stride_head;
-  for (int base = 0; base < rows; base += Lanes::kRows) {
-    const int i = base + row;
-    if (base) row_f64<DT, VEC, C, LPR>(A, S, lanes, t0 + i, head, static_cast<int>(first + i), i < rows, a, b);
+  for (int batch = 0; batch <= last_batch; ++batch) {
+    const int i = batch ? load(batch) : row;
+    double ya[C][VEC], yb[C][VEC];
+    if (exact) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) ya[c][j] = a[c][j], yb[c][j] = b[c][j];
+      norm_turn<VEC, C, LPR>(A, S, lanes, co, si, ya, yb);
+    }
     if (i < rows) {
       uint8_t* to = dst + (kept + i) * S.cache.stride_slot;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        if (lanes.pc[c].ok) store_fp8<VEC>(to + lanes.pc[c].a, a[c], inv);
-        if (lanes.pc[c].b_ok) store_fp8<VEC>(to + lanes.pc[c].b, b[c], inv);
+        if (exact) {
+          if (lanes.pc[c].ok) store_fp8<VEC>(to + lanes.pc[c].a, ya[c], inv);
+          if (lanes.pc[c].b_ok) store_fp8<VEC>(to + lanes.pc[c].b, yb[c], inv);
+        } else {  // (a 16-bit value times a power of two: exact)
+          if (lanes.pc[c].ok) store_fp8<VEC>(to + lanes.pc[c].a, a[c], static_cast<float>(inv));
+          if (lanes.pc[c].b_ok) store_fp8<VEC>(to + lanes.pc[c].b, b[c], static_cast<float>(inv));
+        }
       }
     }
   }
@@ -252,12 +336,12 @@ __global__ __launch_bounds__(kNormThreads) void cache_append_kernel(AppendArgs A
   __shared__ int2 place[kNormThreads / LPR + 1];
   const int block = static_cast<int>(blockIdx.x);
   if constexpr (FP8) {
-    __shared__ float amax_of_wave[kNormThreads / kWave];
+    __shared__ float lds[3 * kNormThreads / kWave];
     if (block < A.page_blocks) {
       const int per_unit = A.side[0].heads + A.side[1].heads;
       const int64_t unit = block / per_unit;
       const int which = block % per_unit, second = which >= A.side[0].heads;
-      append_page<DT, VEC, C, LPR>(A, A.side[second], unit, which - (second ? A.side[0].heads : 0), amax_of_wave);
+      append_page<DT, VEC, C, LPR>(A, A.side[second], unit, which - (second ? A.side[0].heads : 0), lds);
       return;
     }
   }
