@@ -96,11 +96,6 @@ __device__ __forceinline__ void norm_turn(const AppendArgs& A, const AppendSide&
   }
 }
 
-__device__ __forceinline__ float finite_size(float x) {
-  const float m = fabsf(x);
-  return m < __builtin_inff() ? m : 0.f;  // (NaN: 0)
-}
-
 // An fp32 value whose rounding to e4m3 is that of x, and that is above 448 x 2^k where x is: x cut to 21 significant
 // bits with what was cut off folded into the last one (e4m3 has 4, 448 has 3).
 __device__ __forceinline__ float for_fp8(double x) {
@@ -108,34 +103,62 @@ __device__ __forceinline__ float for_fp8(double x) {
   const uint32_t high = static_cast<uint32_t>(u >> 32) | (static_cast<uint32_t>(u) ? 1u : 0u);
   return static_cast<float>(__longlong_as_double(static_cast<long long>(static_cast<uint64_t>(high) << 32)));
 }
-__device__ __forceinline__ float for_fp8(float x) { return x; }
+
+// The magnitude of a finite value times 2^-16, as for_fp8 (products of 16-bit values may pass fp32's range); 0 otherwise.
+__device__ __forceinline__ float finite_size(double x) {
+  const float m = fabsf(for_fp8(x * 0x1p-16));
+  return m < __builtin_inff() ? m : 0.f;  // (NaN: 0)
+}
 
 __device__ __forceinline__ uint32_t pack4_fp8(float x0, float x1, float x2, float x3) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, w, true));
 }
 
-// v * inv rounded to e4m3; NaN for what is not finite.
-template <int VEC, typename T>
-__device__ __forceinline__ void store_fp8(uint8_t* p, const T (&v)[VEC], T inv) {
+// VEC values in e4m3.
+template <int VEC>
+struct Bytes {
+  uint32_t w[VEC == 8 ? 2 : 1];
+};
+template <int VEC>
+__device__ __forceinline__ Bytes<VEC> to_fp8(const float (&x)[VEC]) {
+  Bytes<VEC> r;
+  if constexpr (VEC == 1) {
+    r.w[0] = pack4_fp8(x[0], 0.f, 0.f, 0.f);
+  } else {
+    r.w[0] = pack4_fp8(x[0], x[1], x[2], x[3]);
+    r.w[1] = pack4_fp8(x[4], x[5], x[6], x[7]);
+  }
+  return r;
+}
+// v * inv rounded once; NaN for what is not finite, or not held by the largest scale.
+template <int VEC>
+__device__ __forceinline__ Bytes<VEC> to_fp8(const double (&v)[VEC], double inv) {
   float x[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
     x[j] = for_fp8(v[j] * inv);
-    x[j] = fabsf(x[j]) < __builtin_inff() ? x[j] : __builtin_nanf("");
+    x[j] = fabsf(x[j]) <= 449.f ? x[j] : __builtin_nanf("");
   }
-  if constexpr (VEC == 1)
-    *p = static_cast<uint8_t>(pack4_fp8(x[0], 0.f, 0.f, 0.f));
-  else
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack4_fp8(x[0], x[1], x[2], x[3]), pack4_fp8(x[4], x[5], x[6], x[7]));
+  return to_fp8(x);
+}
+template <int VEC>
+__device__ __forceinline__ bool same(const Bytes<VEC>& x, const Bytes<VEC>& y) {
+  if constexpr (VEC == 1) return x.w[0] == y.w[0];
+  else return x.w[0] == y.w[0] && x.w[1] == y.w[1];
+}
+template <int VEC>
+__device__ __forceinline__ void store_bytes(uint8_t* p, const Bytes<VEC>& x) {
+  if constexpr (VEC == 1) *p = static_cast<uint8_t>(x.w[0]);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(x.w[0], x.w[1]);
 }
 
-// The smallest power of two s >= 2^-100 with 448 s >= amax (448 = 1.75 x 2^8); 0 for 0.
-__device__ __forceinline__ float scale_for(float amax) {
+// The smallest power of two s in [2^-100, 2^127] with 448 s >= amax 2^shift (448 = 1.75 x 2^8); 0 for 0.
+__device__ __forceinline__ float scale_for(float amax, int shift = 0) {
   const uint32_t u = __float_as_uint(amax);
   if (u == 0u) return 0.f;
-  int k = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-  k = k < -100 ? -100 : k;
+  int k = static_cast<int>(u >> 23) - 127 - 8 + shift + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  k = k < -100 ? -100 : k > 127 ? 127 : k;
   return __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
 }
 
@@ -166,108 +189,161 @@ __device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t un
   const int64_t p = (context >> A.pages.shift) + (unit - (start >> A.pages.shift) - 2 * static_cast<int64_t>(s));
   const int64_t page_pos = p << A.pages.shift, page_end = page_pos + (int64_t{1} << A.pages.shift);
   if (page_pos >= context + n) return;
-  const int page = A.pages.page_of(s, page_pos);
-  if (page < 0) return;
   const int64_t first = context > page_pos ? context : page_pos;
   const int kept = static_cast<int>(first - page_pos);  // tokens that the page holds already
   const int rows = static_cast<int>((context + n < page_end ? context + n : page_end) - first);
   const int64_t t0 = start + (first - context);
-  float* scale = S.scale + static_cast<int64_t>(page) * S.heads + head;
-  const float before = kept ? *scale : 0.f;
   const Lanes lanes(S.w, A.w_f32, S.turned ? A.rope.half : 0, S.dim);
   const int row = threadIdx.x / LPR, last_batch = (rows - 1) / Lanes::kRows;
   const bool exact = S.w || S.turned;  // (otherwise y is the input itself)
-  float a[C][VEC], b[C][VEC], co[C][VEC], si[C][VEC];
-  auto load = [&](int batch) {
+  // The page's rows stay in registers as they came (pages of up to kHeld batches of kRows), all loads in flight at once.
+  constexpr int kHeld = 4;
+  auto fetch = [&](int batch) {
     const int i = batch * Lanes::kRows + row;
-    lanes.load(S.x, (t0 + i) * S.stride_t + head * S.stride_h, i < rows, a, b);
-    if (S.turned) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) load_turn<VEC>(A.rope, lanes.pc[c], i < rows ? static_cast<int>(first + i) : -1, co[c], si[c]);
-    }
-    return i;
+    return lanes.fetch(S.x, (t0 + i) * S.stride_t + head * S.stride_h, i < rows);
   };
-  // The maximum, in fp32: off by less than 2^-19 of the largest |u cos| + |v sin| (`size`; some 16 steps of 2^-24), which
-  // can matter only next to 448 x 2^k, or by more where fp32 has no range for the norm (`odd`; also what is not
-  // finite). Both are seen below, and the maximum is taken again in FP64.
+  typename Lanes::Raw held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (k <= last_batch) held[k] = fetch(k);
+  const int page = A.pages.page_of(s, page_pos);
+  if (page < 0) return;
+  float* scale = S.scale + static_cast<int64_t>(page) * S.heads + head;
+  const float before = kept ? *scale : 0.f;
+  auto each_batch = [&](auto&& body) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (k <= last_batch) body(k, held[k]);
+    for (int k = kHeld; k <= last_batch; ++k) body(k, fetch(k));
+  };
+  auto turn = [&](int i, float (&co)[C][VEC], float (&si)[C][VEC]) {  // (1, 0) where nothing is rotated
+#pragma unroll
+    for (int c = 0; c < C; ++c) load_turn<VEC>(A.rope, lanes.pc[c], i < rows ? static_cast<int>(first + i) : -1, co[c], si[c]);
+  };
+  // The maximum. Values that are the input itself: of their bits, two at a time. Others in fp32: off by less than 2^-19 of
+  // the pair's larger value times |cos| + |sin| (`size` is the largest of these; some 16 steps of 2^-24), which can
+  // matter only next to 448 x 2^k, or by more where fp32 has no range for the norm. That, and what is not finite, is seen
+  // below and done again with care: in FP64, over the finite values.
   float amax = 0.f, size = 0.f, odd = 0.f;
-  for (int batch = last_batch; batch >= 0; --batch) {  // the first rows last: they stay in registers
-    const int i = load(batch);
-    if (!exact) {
+  auto normed = [&](float (&a)[C][VEC], float (&b)[C][VEC]) {  // in fp32; false: out of its range
+    if (!S.w) return true;
+    const float ms = run_sum<LPR>(sum_products(a, b, a, b)) / static_cast<float>(S.dim) + A.eps;
+    const float r = 1.f / sqrtf(ms);
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, fmaxf(finite_size(a[c][j]), finite_size(b[c][j])));
-      continue;
-    }
-    float r = 1.f;
-    if (S.w) {
-      const float ms = run_sum<LPR>(sum_products(a, b, a, b)) / static_cast<float>(S.dim) + A.eps;
-      if (i < rows && !(ms < 0x1p100f && ms > 0x1p-60f)) odd = 1.f;
-      r = 1.f / sqrtf(ms);
-    }
-    if (i < rows) {
+      for (int j = 0; j < VEC; ++j) a[c][j] *= r * lanes.wa[c][j], b[c][j] *= r * lanes.wb[c][j];
+    return ms < 0x1p100f && ms > 0x1p-60f;
+  };
+  if (exact) {
+    each_batch([&](int batch, const typename Lanes::Raw& raw) {
+      const int i = batch * Lanes::kRows + row;
+      float a[C][VEC], b[C][VEC], co[C][VEC], si[C][VEC];
+      Lanes::unpack(raw, a, b);
+      if (!normed(a, b) && i < rows) odd = 1.f;
+      turn(i, co, si);
+      if (i < rows) {
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float u = S.w ? a[c][j] * r * lanes.wa[c][j] : a[c][j], v = S.w ? b[c][j] * r * lanes.wb[c][j] : b[c][j];
-          const float cs = S.turned ? co[c][j] : 1.f, sn = S.turned ? si[c][j] : 0.f;
-          const float m = fmaxf(fabsf(u * cs - v * sn), fabsf(v * cs + u * sn));
-          if (!(m < __builtin_inff())) odd = 1.f;
-          amax = fmaxf(amax, m);
-          size = fmaxf(size, fmaxf(fabsf(u * cs) + fabsf(v * sn), fabsf(v * cs) + fabsf(u * sn)));
-        }
-    }
+          for (int j = 0; j < VEC; ++j) {
+            const float u = a[c][j], v = b[c][j], cs = co[c][j], sn = si[c][j];
+            amax = fmaxf(amax, fmaxf(fabsf(u * cs - v * sn), fabsf(v * cs + u * sn)));
+            size = fmaxf(size, fmaxf(fabsf(u), fabsf(v)) * (fabsf(cs) + fabsf(sn)));
+          }
+      }
+    });
+  } else {
+    u16x2 most = {0, 0};
+    each_batch([&](int, const typename Lanes::Raw& raw) { most = __builtin_elementwise_max(most, Lanes::largest(raw)); });
+    amax = lo16_f32<DT>(most.x > most.y ? most.x : most.y);
+    if (!(amax < __builtin_inff())) odd = 1.f;  // (a NaN is no maximum)
   }
   block_max3(amax, size, odd, lds);  // (every thread has read the old scale)
-  if (exact && (odd != 0.f || scale_for(fmaxf(amax - 0x1p-19f * size, 0.f)) != scale_for(amax + 0x1p-19f * size))) {
+  if (amax == __builtin_inff() || odd != 0.f ||
+      (exact && scale_for(fmaxf(amax - 0x1p-19f * size, 0.f)) != scale_for(amax + 0x1p-19f * size))) {
     amax = 0.f;
-    for (int batch = last_batch; batch >= 0; --batch) {
-      const int i = load(batch);
+    odd = 1.f;
+    for (int batch = 0; batch <= last_batch; ++batch) {
+      const int i = batch * Lanes::kRows + row;
       double ya[C][VEC], yb[C][VEC];
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) ya[c][j] = a[c][j], yb[c][j] = b[c][j];
+      Lanes::unpack(fetch(batch), ya, yb);
+      float co[C][VEC], si[C][VEC];
+      turn(i, co, si);
       norm_turn<VEC, C, LPR>(A, S, lanes, co, si, ya, yb);
       if (i < rows) {
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
           for (int j = 0; j < VEC; ++j)
-            amax = fmaxf(amax, fmaxf(finite_size(for_fp8(ya[c][j])), finite_size(for_fp8(yb[c][j]))));
+            amax = fmaxf(amax, fmaxf(finite_size(ya[c][j]), finite_size(yb[c][j])));
       }
     }
     block_max3(amax, size, odd, lds);
   }
-  const float after = fmaxf(before, scale_for(amax));
+  const float after = fmaxf(before, scale_for(amax, odd != 0.f ? 16 : 0));
   const double inv = after > 0.f ? 1.0 / static_cast<double>(after) : 0.0;
   uint8_t* dst = static_cast<uint8_t*>(S.cache.base) + page * S.cache.stride_page + head * S.cache.stride_head;
-  for (int batch = 0; batch <= last_batch; ++batch) {
-    const int i = batch ? load(batch) : row;
-    double ya[C][VEC], yb[C][VEC];
-    if (exact) {
+  const float inv32 = static_cast<float>(inv);
+  // The bytes. An input times a power of two is exact. Normed and rotated values in fp32 first, with their error e:
+  // where y - e and y + e round to the same byte that byte is right (all but about 2^-14 of them), and a wave with a
+  // value where they do not does its rows in FP64.
+  each_batch([&](int batch, const typename Lanes::Raw& raw) {
+    const int i = batch * Lanes::kRows + row;
+    uint8_t* to = dst + (kept + i) * S.cache.stride_slot;
+    float a[C][VEC], b[C][VEC];
+    Lanes::unpack(raw, a, b);
+    if (odd == 0.f) {
+      bool sure = true;
+      Bytes<VEC> wa[C], wb[C];
+      if (!exact) {
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) ya[c][j] = a[c][j], yb[c][j] = b[c][j];
-      norm_turn<VEC, C, LPR>(A, S, lanes, co, si, ya, yb);
-    }
-    if (i < rows) {
-      uint8_t* to = dst + (kept + i) * S.cache.stride_slot;
+          for (int j = 0; j < VEC; ++j) a[c][j] *= inv32, b[c][j] *= inv32;
+          wa[c] = to_fp8(a[c]), wb[c] = to_fp8(b[c]);
+        }
+      } else {
+        float co[C][VEC], si[C][VEC];
+        normed(a, b);
+        turn(i, co, si);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (exact) {
-          if (lanes.pc[c].ok) store_fp8<VEC>(to + lanes.pc[c].a, ya[c], inv);
-          if (lanes.pc[c].b_ok) store_fp8<VEC>(to + lanes.pc[c].b, yb[c], inv);
-        } else {  // (a 16-bit value times a power of two: exact)
-          if (lanes.pc[c].ok) store_fp8<VEC>(to + lanes.pc[c].a, a[c], static_cast<float>(inv));
-          if (lanes.pc[c].b_ok) store_fp8<VEC>(to + lanes.pc[c].b, b[c], static_cast<float>(inv));
+        for (int c = 0; c < C; ++c) {
+          float al[VEC], bl[VEC];  // y - e; a and b become y + e
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float u = a[c][j], v = b[c][j], cs = co[c][j] * inv32, sn = si[c][j] * inv32;
+            const float e = 0x1p-19f * fmaxf(fabsf(u), fabsf(v)) * (fabsf(cs) + fabsf(sn));
+            const float ya = u * cs - v * sn, yb = v * cs + u * sn;
+            al[j] = ya - e, bl[j] = yb - e;
+            a[c][j] = ya + e, b[c][j] = yb + e;
+          }
+          wa[c] = to_fp8(al), wb[c] = to_fp8(bl);
+          sure = sure && same(wa[c], to_fp8(a[c])) && same(wb[c], to_fp8(b[c]));
         }
       }
+      if (!__any(!sure && i < rows)) {
+        if (i >= rows) return;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          if (lanes.pc[c].ok) store_bytes(to + lanes.pc[c].a, wa[c]);
+          if (lanes.pc[c].b_ok) store_bytes(to + lanes.pc[c].b, wb[c]);
+        }
+        return;
+      }
     }
-  }
+    double ya[C][VEC], yb[C][VEC];
+    Lanes::unpack(raw, ya, yb);
+    float co[C][VEC], si[C][VEC];
+    turn(i, co, si);
+    norm_turn<VEC, C, LPR>(A, S, lanes, co, si, ya, yb);
+    if (i >= rows) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (lanes.pc[c].ok) store_bytes(to + lanes.pc[c].a, to_fp8(ya[c], inv));
+      if (lanes.pc[c].b_ok) store_bytes(to + lanes.pc[c].b, to_fp8(yb[c], inv));
+    }
+  });
   if (kept && after != before) {  // round the held tokens again
     const float ratio = static_cast<float>(static_cast<double>(before) * inv);
     const int words = S.dim / 8;
@@ -340,7 +416,8 @@ __global__ __launch_bounds__(kNormThreads) void cache_append_kernel(AppendArgs A
     if (block < A.page_blocks) {
       const int per_unit = A.side[0].heads + A.side[1].heads;
       const int64_t unit = block / per_unit;
-      const int which = block % per_unit, second = which >= A.side[0].heads;
+      // (the heads turn with the page: eight in a row go to the eight XCDs, and keys cost more than values)
+      const int which = static_cast<int>((block + unit) % per_unit), second = which >= A.side[0].heads;
       append_page<DT, VEC, C, LPR>(A, A.side[second], unit, which - (second ? A.side[0].heads : 0), lds);
       return;
     }

@@ -8,6 +8,8 @@ namespace msa {
 
 constexpr int kNormThreads = 256;
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 struct RopeTable {
   const float* table;  // [rows][2 * half]: cosines, then sines
   int64_t rows;
@@ -110,6 +112,47 @@ struct RowLanes {
       } else {
         if (pc[c].ok) load_vec<DT, VEC>(w, pc[c].a, wa[c]);
         if (pc[c].b_ok) load_vec<DT, VEC>(w, pc[c].b, wb[c]);
+      }
+    }
+  }
+  // A row's pieces as they are in memory (16-bit types), and their values.
+  struct Raw {
+    uint4 a[C], b[C];
+  };
+  __device__ __forceinline__ Raw fetch(const void* p, int64_t at, bool live) const {
+    Raw r;
+    const uint16_t* s = static_cast<const uint16_t*>(p) + at;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      r.a[c] = r.b[c] = make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (VEC == 8) {
+        if (live && pc[c].ok) r.a[c] = *reinterpret_cast<const uint4*>(s + pc[c].a);
+        if (live && pc[c].b_ok) r.b[c] = *reinterpret_cast<const uint4*>(s + pc[c].b);
+      } else {
+        if (live && pc[c].ok) r.a[c].x = s[pc[c].a];
+        if (live && pc[c].b_ok) r.b[c].x = s[pc[c].b];
+      }
+    }
+    return r;
+  }
+  // The largest magnitudes' bits among the low and the high elements of the words (NaN above infinity above all).
+  static __device__ __forceinline__ u16x2 largest(const Raw& r) {
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      for (uint32_t w : {r.a[c].x, r.a[c].y, r.a[c].z, r.a[c].w, r.b[c].x, r.b[c].y, r.b[c].z, r.b[c].w})
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
+    return m;
+  }
+  template <typename T>
+  static __device__ __forceinline__ void unpack(const Raw& r, T (&a)[C][VEC], T (&b)[C][VEC]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const uint32_t u[4] = {r.a[c].x, r.a[c].y, r.a[c].z, r.a[c].w}, v[4] = {r.b[c].x, r.b[c].y, r.b[c].z, r.b[c].w};
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        a[c][j] = j & 1 ? hi16_f32<DT>(u[j >> 1]) : lo16_f32<DT>(u[j >> 1]);
+        b[c][j] = j & 1 ? hi16_f32<DT>(v[j >> 1]) : lo16_f32<DT>(v[j >> 1]);
       }
     }
   }

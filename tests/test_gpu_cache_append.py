@@ -213,6 +213,45 @@ def test_not_finite_and_largest_values(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("normed", [False, True])
+def test_keys_at_scale_borders_and_out_of_range(dtype, normed, device):
+    """Rotated keys whose largest value is 448 x 2^k to the last bit, or next to it; rows that are zero, huge, tiny, infinite
+    or NaN beside ordinary ones; a rotation that is none."""
+    page, heads, dim = 16, 5, 32
+    x = _setup([page], [0], heads, dim, 16, 0, page, dtype, True, device)
+    x["wk"] = torch.ones(dim, dtype=dtype, device=device) if normed else None
+    x["wi"] = x["ik"] = x["ic"] = None
+    gen = torch.Generator().manual_seed(5)
+    x["k"] = torch.randn(page, heads, dim, generator=gen).to(dtype).to(device)
+    step = 1 + torch.finfo(dtype).eps
+    x["k"][3, 0, 7] = 448.0 / 64
+    x["k"][3, 1, 20] = -448.0 / 64 * step
+    x["k"][2, 2], x["k"][5, 2] = 0, 1e-7
+    big = 60000.0 if dtype == torch.float16 else 3e38
+    x["k"][4, 3] = big
+    x["k"][6, 4, 0], x["k"][7, 4, 1], x["k"][8, 4, 2] = float("inf"), float("nan"), -float("inf")
+    for turn in ("none", "scaled", "real"):
+        if turn == "none":
+            rope = torch.cat([torch.ones(page, 8), torch.zeros(page, 8)], 1)
+        elif turn == "scaled":
+            rope = torch.randn(page, 16, generator=gen) * 5
+        else:
+            rope = msa.rope_table(page - 1, 16)  # and no row for the last position
+        x["rope"] = rope.to(device)
+        x["kc"].view(torch.uint8).fill_(0)
+        x["ks"].fill_(0.25)
+        _call(x)
+        rows = _turned(x["k"], x["wk"], x["rope"], list(range(page)), 1e-5)
+        with np.errstate(invalid="ignore", over="ignore"):
+            held, scale = _append_fp8(torch.zeros_like(x["kc"], device="cpu"), torch.full_like(x["ks"], 0.25, device="cpu"),
+                                      rows, x["table"], [page], [0])
+        p = int(x["table"][0, 0])
+        assert np.array_equal(x["ks"].double().cpu().numpy(), scale), turn
+        assert np.array_equal(x["kc"][p].float().double().cpu().numpy(), held[p], equal_nan=True), turn
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fp8", [False, True])
 def test_missing_pages_strided_caches_and_views(fp8, device):
     lengths, context = [40, 9], [3, 14]
