@@ -196,73 +196,93 @@ __device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t un
   const Lanes lanes(S.w, A.w_f32, S.turned ? A.rope.half : 0, S.dim);
   const int row = threadIdx.x / LPR, last_batch = (rows - 1) / Lanes::kRows;
   const bool exact = S.w || S.turned;  // (otherwise y is the input itself)
-  // The page's rows stay in registers as they came (pages of up to kHeld batches of kRows), all loads in flight at once.
-  constexpr int kHeld = 4;
   auto fetch = [&](int batch) {
     const int i = batch * Lanes::kRows + row;
     return lanes.fetch(S.x, (t0 + i) * S.stride_t + head * S.stride_h, i < rows);
   };
-  typename Lanes::Raw held[kHeld];
+  // The values y of up to kHeld batches of kRows rows stay in registers, their loads in flight at once; those of more rows
+  // are read and formed again for the bytes (19 700 prompt tokens, 4 heads of 128: 38, 36 and 40 us with 1, 2 and 4).
+  constexpr int kHeld = 2;
+  typename Lanes::Raw raw[kHeld];
 #pragma unroll
   for (int k = 0; k < kHeld; ++k)
-    if (k <= last_batch) held[k] = fetch(k);
+    if (k <= last_batch) raw[k] = fetch(k);
   const int page = A.pages.page_of(s, page_pos);
   if (page < 0) return;
   float* scale = S.scale + static_cast<int64_t>(page) * S.heads + head;
   const float before = kept ? *scale : 0.f;
-  auto each_batch = [&](auto&& body) {
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k)
-      if (k <= last_batch) body(k, held[k]);
-    for (int k = kHeld; k <= last_batch; ++k) body(k, fetch(k));
-  };
   auto turn = [&](int i, float (&co)[C][VEC], float (&si)[C][VEC]) {  // (1, 0) where nothing is rotated
 #pragma unroll
     for (int c = 0; c < C; ++c) load_turn<VEC>(A.rope, lanes.pc[c], i < rows ? static_cast<int>(first + i) : -1, co[c], si[c]);
   };
-  // The maximum. Values that are the input itself: of their bits, two at a time. Others in fp32: off by less than 2^-19 of
-  // the pair's larger value times |cos| + |sin| (`size` is the largest of these; some 16 steps of 2^-24), which can
-  // matter only next to 448 x 2^k, or by more where fp32 has no range for the norm. That, and what is not finite, is seen
-  // below and done again with care: in FP64, over the finite values.
-  float amax = 0.f, size = 0.f, odd = 0.f;
-  auto normed = [&](float (&a)[C][VEC], float (&b)[C][VEC]) {  // in fp32; false: out of its range
-    if (!S.w) return true;
-    const float ms = run_sum<LPR>(sum_products(a, b, a, b)) / static_cast<float>(S.dim) + A.eps;
-    const float r = 1.f / sqrtf(ms);
+  // The values in fp32, and their maximum. They are off by less than 2^-20 (16 steps of 2^-24: half of the 9 levels that
+  // the squares pass and of the mean's two, root and reciprocal, two products, the rotation's two, one for what is done with
+  // them) of the pair's larger value times |cos| + |sin|, `e`; an input taken as it is is exact. The maximum of e decides
+  // below whether the scale is sure. odd: fp32 has no range for the norm, or a value is not finite.
+  struct Values {
+    float a[C][VEC], b[C][VEC], e[C][VEC];
+  };
+  float amax = 0.f, most_e = 0.f, odd = 0.f;
+  auto values = [&](const typename Lanes::Raw& x, int batch, bool peak) {
+    const int i = batch * Lanes::kRows + row;
+    Values y;
+    Lanes::unpack(x, y.a, y.b);
+    if (!exact) {
+      if (!peak) return y;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, fmaxf(fabsf(y.a[c][j]), fabsf(y.b[c][j])));
+      if (Lanes::not_finite(x)) odd = 1.f;
+      return y;
+    }
+    float co[C][VEC], si[C][VEC];
+    turn(i, co, si);
+    if (S.w) {
+      float ss = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float sq[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sq[j] = fmaf(y.a[c][j], y.a[c][j], y.b[c][j] * y.b[c][j]);
+#pragma unroll
+        for (int n = VEC / 2; n > 0; n /= 2)
+#pragma unroll
+          for (int j = 0; j < n; ++j) sq[j] += sq[j + n];
+        ss += sq[0];
+      }
+      const float ms = run_sum<LPR>(ss) / static_cast<float>(S.dim) + A.eps;
+      if (peak && i < rows && !(ms < 0x1p100f && ms > 0x1p-60f)) odd = 1.f;
+      const float r = 1.f / sqrtf(ms);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y.a[c][j] *= r * lanes.wa[c][j], y.b[c][j] *= r * lanes.wb[c][j];
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) a[c][j] *= r * lanes.wa[c][j], b[c][j] *= r * lanes.wb[c][j];
-    return ms < 0x1p100f && ms > 0x1p-60f;
-  };
-  if (exact) {
-    each_batch([&](int batch, const typename Lanes::Raw& raw) {
-      const int i = batch * Lanes::kRows + row;
-      float a[C][VEC], b[C][VEC], co[C][VEC], si[C][VEC];
-      Lanes::unpack(raw, a, b);
-      if (!normed(a, b) && i < rows) odd = 1.f;
-      turn(i, co, si);
-      if (i < rows) {
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float u = a[c][j], v = b[c][j], cs = co[c][j], sn = si[c][j];
-            amax = fmaxf(amax, fmaxf(fabsf(u * cs - v * sn), fabsf(v * cs + u * sn)));
-            size = fmaxf(size, fmaxf(fabsf(u), fabsf(v)) * (fabsf(cs) + fabsf(sn)));
-          }
+      for (int j = 0; j < VEC; ++j) {
+        const float u = y.a[c][j], v = y.b[c][j], cs = co[c][j], sn = si[c][j];
+        y.a[c][j] = u * cs - v * sn;
+        y.b[c][j] = v * cs + u * sn;
+        y.e[c][j] = fmaxf(fabsf(u), fabsf(v)) * (fabsf(cs) + fabsf(sn));
+        if (peak && i < rows) {
+          amax = fmaxf(amax, fmaxf(fabsf(y.a[c][j]), fabsf(y.b[c][j])));
+          most_e = fmaxf(most_e, y.e[c][j]);
+        }
       }
-    });
-  } else {
-    u16x2 most = {0, 0};
-    each_batch([&](int, const typename Lanes::Raw& raw) { most = __builtin_elementwise_max(most, Lanes::largest(raw)); });
-    amax = lo16_f32<DT>(most.x > most.y ? most.x : most.y);
-    if (!(amax < __builtin_inff())) odd = 1.f;  // (a NaN is no maximum)
-  }
-  block_max3(amax, size, odd, lds);  // (every thread has read the old scale)
+    return y;
+  };
+  Values held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (k <= last_batch) held[k] = values(raw[k], k, true);
+  for (int k = kHeld; k <= last_batch; ++k) values(fetch(k), k, true);
+  block_max3(amax, most_e, odd, lds);  // (every thread has read the old scale)
   if (amax == __builtin_inff() || odd != 0.f ||
-      (exact && scale_for(fmaxf(amax - 0x1p-19f * size, 0.f)) != scale_for(amax + 0x1p-19f * size))) {
-    amax = 0.f;
+      (exact && scale_for(fmaxf(amax - 0x1p-20f * most_e, 0.f)) != scale_for(amax + 0x1p-20f * most_e))) {
+    amax = 0.f;  // again, in FP64 and over the finite values
     odd = 1.f;
     for (int batch = 0; batch <= last_batch; ++batch) {
       const int i = batch * Lanes::kRows + row;
@@ -279,47 +299,36 @@ __device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t un
             amax = fmaxf(amax, fmaxf(finite_size(ya[c][j]), finite_size(yb[c][j])));
       }
     }
-    block_max3(amax, size, odd, lds);
+    block_max3(amax, most_e, odd, lds);
   }
   const float after = fmaxf(before, scale_for(amax, odd != 0.f ? 16 : 0));
   const double inv = after > 0.f ? 1.0 / static_cast<double>(after) : 0.0;
   uint8_t* dst = static_cast<uint8_t*>(S.cache.base) + page * S.cache.stride_page + head * S.cache.stride_head;
   const float inv32 = static_cast<float>(inv);
-  // The bytes. An input times a power of two is exact. Normed and rotated values in fp32 first, with their error e:
-  // where y - e and y + e round to the same byte that byte is right (all but about 2^-14 of them), and a wave with a
-  // value where they do not does its rows in FP64.
-  each_batch([&](int batch, const typename Lanes::Raw& raw) {
+  // The bytes. An input times a power of two is exact. For other values y - e and y + e: where both round to one byte it is
+  // that of the exact value, and a wave with a value where they do not (one in some 2^12) does its rows in FP64.
+  auto write = [&](const Values& y, int batch) {
     const int i = batch * Lanes::kRows + row;
     uint8_t* to = dst + (kept + i) * S.cache.stride_slot;
-    float a[C][VEC], b[C][VEC];
-    Lanes::unpack(raw, a, b);
     if (odd == 0.f) {
       bool sure = true;
       Bytes<VEC> wa[C], wb[C];
-      if (!exact) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) a[c][j] *= inv32, b[c][j] *= inv32;
-          wa[c] = to_fp8(a[c]), wb[c] = to_fp8(b[c]);
-        }
-      } else {
-        float co[C][VEC], si[C][VEC];
-        normed(a, b);
-        turn(i, co, si);
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          float al[VEC], bl[VEC];  // y - e; a and b become y + e
+      for (int c = 0; c < C; ++c) {
+        float al[VEC], bl[VEC], ah[VEC], bh[VEC];
+        if (exact) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            const float u = a[c][j], v = b[c][j], cs = co[c][j] * inv32, sn = si[c][j] * inv32;
-            const float e = 0x1p-19f * fmaxf(fabsf(u), fabsf(v)) * (fabsf(cs) + fabsf(sn));
-            const float ya = u * cs - v * sn, yb = v * cs + u * sn;
-            al[j] = ya - e, bl[j] = yb - e;
-            a[c][j] = ya + e, b[c][j] = yb + e;
+            const float e = 0x1p-20f * inv32 * y.e[c][j];
+            al[j] = fmaf(y.a[c][j], inv32, -e), ah[j] = fmaf(y.a[c][j], inv32, e);
+            bl[j] = fmaf(y.b[c][j], inv32, -e), bh[j] = fmaf(y.b[c][j], inv32, e);
           }
           wa[c] = to_fp8(al), wb[c] = to_fp8(bl);
-          sure = sure && same(wa[c], to_fp8(a[c])) && same(wb[c], to_fp8(b[c]));
+          sure = sure && same(wa[c], to_fp8(ah)) && same(wb[c], to_fp8(bh));
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) al[j] = y.a[c][j] * inv32, bl[j] = y.b[c][j] * inv32;
+          wa[c] = to_fp8(al), wb[c] = to_fp8(bl);
         }
       }
       if (!__any(!sure && i < rows)) {
@@ -333,7 +342,7 @@ __device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t un
       }
     }
     double ya[C][VEC], yb[C][VEC];
-    Lanes::unpack(raw, ya, yb);
+    Lanes::unpack(fetch(batch), ya, yb);
     float co[C][VEC], si[C][VEC];
     turn(i, co, si);
     norm_turn<VEC, C, LPR>(A, S, lanes, co, si, ya, yb);
@@ -343,7 +352,11 @@ __device__ void append_page(const AppendArgs& A, const AppendSide& S, int64_t un
       if (lanes.pc[c].ok) store_bytes(to + lanes.pc[c].a, to_fp8(ya[c], inv));
       if (lanes.pc[c].b_ok) store_bytes(to + lanes.pc[c].b, to_fp8(yb[c], inv));
     }
-  });
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (k <= last_batch) write(held[k], k);
+  for (int k = kHeld; k <= last_batch; ++k) write(values(fetch(k), k, false), k);
   if (kept && after != before) {  // round the held tokens again
     const float ratio = static_cast<float>(static_cast<double>(before) * inv);
     const int words = S.dim / 8;
@@ -408,7 +421,7 @@ __device__ void append_rows(const AppendArgs& A, const AppendSide& S, int64_t r0
 }
 
 template <int DT, bool FP8, int VEC, int C, int LPR>
-__global__ __launch_bounds__(kNormThreads) void cache_append_kernel(AppendArgs A) {
+__global__ __launch_bounds__(kNormThreads, FP8 ? 3 : 4) void cache_append_kernel(AppendArgs A) {
   __shared__ int2 place[kNormThreads / LPR + 1];
   const int block = static_cast<int>(blockIdx.x);
   if constexpr (FP8) {

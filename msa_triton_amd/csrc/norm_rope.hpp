@@ -135,14 +135,14 @@ struct RowLanes {
     }
     return r;
   }
-  // The largest magnitudes' bits among the low and the high elements of the words (NaN above infinity above all).
-  static __device__ __forceinline__ u16x2 largest(const Raw& r) {
+  // Whether an element is an infinity or a NaN.
+  static __device__ __forceinline__ bool not_finite(const Raw& r) {
     u16x2 m = {0, 0};
 #pragma unroll
     for (int c = 0; c < C; ++c)
       for (uint32_t w : {r.a[c].x, r.a[c].y, r.a[c].z, r.a[c].w, r.b[c].x, r.b[c].y, r.b[c].z, r.b[c].w})
         m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
-    return m;
+    return (m.x > m.y ? m.x : m.y) >= (DT == kF16 ? 0x7c00 : 0x7f80);
   }
   template <typename T>
   static __device__ __forceinline__ void unpack(const Raw& r, T (&a)[C][VEC], T (&b)[C][VEC]) {
