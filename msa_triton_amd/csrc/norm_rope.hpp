@@ -115,46 +115,58 @@ struct RowLanes {
       }
     }
   }
-  // A row's pieces as they are in memory (16-bit types), and their values.
+  // A row's pieces as they are in memory, and their values.
+  static constexpr int kWords = VEC == 8 && DT == kF32 ? 2 : 1;  // 16-byte words of VEC values
   struct Raw {
-    uint4 a[C], b[C];
+    uint4 a[C][kWords], b[C][kWords];
   };
+  static __device__ __forceinline__ void fetch_vec(const void* p, int64_t i, bool live, uint4 (&w)[kWords]) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (!live) return;
+    if constexpr (VEC == 8) {
+      const uint4* s = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2));
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) w[k] = s[k];
+    } else if constexpr (DT == kF32) {
+      w[0].x = static_cast<const uint32_t*>(p)[i];
+    } else {
+      w[0].x = static_cast<const uint16_t*>(p)[i];
+    }
+  }
   __device__ __forceinline__ Raw fetch(const void* p, int64_t at, bool live) const {
     Raw r;
-    const uint16_t* s = static_cast<const uint16_t*>(p) + at;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      r.a[c] = r.b[c] = make_uint4(0u, 0u, 0u, 0u);
-      if constexpr (VEC == 8) {
-        if (live && pc[c].ok) r.a[c] = *reinterpret_cast<const uint4*>(s + pc[c].a);
-        if (live && pc[c].b_ok) r.b[c] = *reinterpret_cast<const uint4*>(s + pc[c].b);
-      } else {
-        if (live && pc[c].ok) r.a[c].x = s[pc[c].a];
-        if (live && pc[c].b_ok) r.b[c].x = s[pc[c].b];
-      }
+      fetch_vec(p, at + pc[c].a, live && pc[c].ok, r.a[c]);
+      fetch_vec(p, at + pc[c].b, live && pc[c].b_ok, r.b[c]);
     }
     return r;
   }
-  // Whether an element is an infinity or a NaN.
-  static __device__ __forceinline__ bool not_finite(const Raw& r) {
-    u16x2 m = {0, 0};
+  template <typename T>
+  static __device__ __forceinline__ void unpack_vec(const uint4 (&w)[kWords], T (&v)[VEC]) {
+    const uint4 x = w[0], y = w[kWords - 1];
+    const uint32_t u[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      for (uint32_t w : {r.a[c].x, r.a[c].y, r.a[c].z, r.a[c].w, r.b[c].x, r.b[c].y, r.b[c].z, r.b[c].w})
-        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
-    return (m.x > m.y ? m.x : m.y) >= (DT == kF16 ? 0x7c00 : 0x7f80);
+    for (int j = 0; j < VEC; ++j) {
+      if constexpr (DT == kF32) v[j] = __uint_as_float(u[j]);
+      else v[j] = j & 1 ? hi16_f32<DT>(u[j >> 1]) : lo16_f32<DT>(u[j >> 1]);
+    }
   }
   template <typename T>
   static __device__ __forceinline__ void unpack(const Raw& r, T (&a)[C][VEC], T (&b)[C][VEC]) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const uint32_t u[4] = {r.a[c].x, r.a[c].y, r.a[c].z, r.a[c].w}, v[4] = {r.b[c].x, r.b[c].y, r.b[c].z, r.b[c].w};
+    for (int c = 0; c < C; ++c) unpack_vec(r.a[c], a[c]), unpack_vec(r.b[c], b[c]);
+  }
+  // Whether an element is an infinity or a NaN (16-bit types).
+  static __device__ __forceinline__ bool not_finite(const Raw& r) {
+    u16x2 m = {0, 0};
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        a[c][j] = j & 1 ? hi16_f32<DT>(u[j >> 1]) : lo16_f32<DT>(u[j >> 1]);
-        b[c][j] = j & 1 ? hi16_f32<DT>(v[j >> 1]) : lo16_f32<DT>(v[j >> 1]);
-      }
-    }
+    for (int c = 0; c < C; ++c)
+      for (const uint4& x : {r.a[c][0], r.b[c][0]})
+        for (uint32_t w : {x.x, x.y, x.z, x.w})
+          m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
+    return (m.x > m.y ? m.x : m.y) >= (DT == kF16 ? 0x7c00 : 0x7f80);
   }
   __device__ __forceinline__ void load(const void* p, int64_t at, bool live, float (&a)[C][VEC], float (&b)[C][VEC]) const {
 #pragma unroll

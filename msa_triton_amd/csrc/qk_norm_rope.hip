@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kMostTokens = 1024;    // tokens of one workgroup: positions in LDS
 constexpr int kMostDim = 512;
-constexpr int kBwdBlocks = 2048;     // workgroups of one side's backward, unless rows need more
+constexpr int kBwdBlocks = 1022;     // workgroups of the backward, both sides, unless rows need more
 
 struct NormSide {
   const void* x;
@@ -61,52 +61,47 @@ __device__ __forceinline__ void load_positions(const NormArgs& A, int64_t t0, in
   __syncthreads();
 }
 
-// U rows per lane run at once: their loads are all in flight before the first is used.
-template <int DT, int VEC, int C, int LPR, int U>
+// One row a lane run: with many workgroups a CU more rows in flight each only cost registers (32K tokens x 36 heads of 128,
+// bf16: 122 us; 136 and 152 with two and four).
+template <int DT, int VEC, int C, int LPR>
 __global__ __launch_bounds__(kNormThreads) void norm_rope_fwd_kernel(NormArgs A) {
   using Lanes = RowLanes<DT, VEC, C, LPR>;
-  __shared__ int32_t pos[Lanes::kRows * U + 1];
+  __shared__ int32_t pos[Lanes::kRows + 1];
   const bool second = static_cast<int>(blockIdx.x) >= A.q_blocks;
   const NormSide& S = A.side[second];
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x - (second ? A.q_blocks : 0)) * (Lanes::kRows * U);
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x - (second ? A.q_blocks : 0)) * Lanes::kRows;
   const int64_t rows = A.tokens * S.heads, t0 = r0 / S.heads;
   const int h0 = static_cast<int>(r0 - t0 * S.heads);
-  const int n = static_cast<int>(min(rows - r0, static_cast<int64_t>(Lanes::kRows * U)));
+  const int n = static_cast<int>(min(rows - r0, static_cast<int64_t>(Lanes::kRows)));
   const Lanes lanes(S.w, A.w_f32, A.rope.half, A.dim);
-  float a[U][C][VEC], b[U][C][VEC];
-  int tok[U], head[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = u * Lanes::kRows + threadIdx.x / LPR;
-    tok[u] = static_cast<int>(static_cast<uint32_t>(h0 + i) / static_cast<uint32_t>(S.heads));
-    head[u] = h0 + i - tok[u] * S.heads;
-    lanes.load(S.x, (t0 + tok[u]) * S.stride_t + head[u] * S.stride_h, i < n, a[u], b[u]);
-  }
+  const int i = threadIdx.x / LPR;
+  const int tok = static_cast<int>(static_cast<uint32_t>(h0 + i) / static_cast<uint32_t>(S.heads));
+  const int head = h0 + i - tok * S.heads;
+  float a[C][VEC], b[C][VEC];
+  lanes.load(S.x, (t0 + tok) * S.stride_t + head * S.stride_h, i < n, a, b);
   load_positions(A, t0, (h0 + n - 1) / S.heads + 1, pos);
+  const float ss = run_sum<LPR>(sum_products(a, b, a, b));
+  if (i >= n) return;
+  const float r = 1.f / sqrtf(ss / static_cast<float>(A.dim) + A.eps);
+  const int p = pos[tok];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = u * Lanes::kRows + threadIdx.x / LPR;
-    const float ss = run_sum<LPR>(sum_products(a[u], b[u], a[u], b[u]));
-    if (i >= n) continue;
-    const float r = 1.f / sqrtf(ss / static_cast<float>(A.dim) + A.eps);
-    const int p = pos[tok[u]];
+  for (int c = 0; c < C; ++c) {
+    float co[VEC], si[VEC];
+    load_turn<VEC>(A.rope, lanes.pc[c], p, co, si);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float co[VEC], si[VEC];
-      load_turn<VEC>(A.rope, lanes.pc[c], p, co, si);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float ma = a[u][c][j] * r * lanes.wa[c][j], mb = b[u][c][j] * r * lanes.wb[c][j];
-        a[u][c][j] = ma * co[j] - mb * si[j];
-        b[u][c][j] = mb * co[j] + ma * si[j];
-      }
+    for (int j = 0; j < VEC; ++j) {
+      const float ma = a[c][j] * r * lanes.wa[c][j], mb = b[c][j] * r * lanes.wb[c][j];
+      a[c][j] = ma * co[j] - mb * si[j];
+      b[c][j] = mb * co[j] + ma * si[j];
     }
-    lanes.store(S.y, ((t0 + tok[u]) * S.heads + head[u]) * A.dim, a[u], b[u]);
   }
+  lanes.store(S.y, ((t0 + tok) * S.heads + head) * A.dim, a, b);
 }
 
-template <int DT, int VEC, int C, int LPR, int U>
-__global__ __launch_bounds__(kNormThreads) void norm_rope_bwd_kernel(NormArgs A) {
+// The row after this one is on its way while it is worked on (32K tokens x 36 heads of 128, bf16: 193 us, 4.7 TB/s; 211
+// without).
+template <int DT, int VEC, int C, int LPR>
+__global__ __launch_bounds__(kNormThreads, 4) void norm_rope_bwd_kernel(NormArgs A) {
   using Lanes = RowLanes<DT, VEC, C, LPR>;
   __shared__ int32_t pos[kMostTokens + 1];
   __shared__ float sums[kNormThreads / kWave][kMostDim];
@@ -118,60 +113,66 @@ __global__ __launch_bounds__(kNormThreads) void norm_rope_bwd_kernel(NormArgs A)
   const int h0 = static_cast<int>(r0 - t0 * S.heads);
   const int n = static_cast<int>(min(rows - r0, static_cast<int64_t>(A.rows_per_block)));
   const Lanes lanes(S.w, A.w_f32, A.rope.half, A.dim);
+  struct Row {
+    typename Lanes::Raw x, g;
+    int tok;
+    int64_t at;
+  };
+  auto fetch = [&](int i) {
+    Row r;
+    r.tok = static_cast<int>(static_cast<uint32_t>(h0 + i) / static_cast<uint32_t>(S.heads));
+    const int head = h0 + i - r.tok * S.heads;
+    r.at = ((t0 + r.tok) * S.heads + head) * A.dim;
+    r.x = lanes.fetch(S.x, (t0 + r.tok) * S.stride_t + head * S.stride_h, i < n);
+    r.g = lanes.fetch(S.g, r.at, i < n);
+    return r;
+  };
+  const int own = threadIdx.x / LPR;
+  Row next = fetch(own);
   load_positions(A, t0, (h0 + n - 1) / S.heads + 1, pos);
   float da[C][VEC], db[C][VEC];
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) da[c][j] = db[c][j] = 0.f;
-  for (int base = 0; base < n; base += Lanes::kRows * U) {  // (uniform: every lane takes part in the sums)
-    float a[U][C][VEC], b[U][C][VEC], ga[U][C][VEC], gb[U][C][VEC];
-    int tok[U];
-    int64_t at[U];
+  for (int base = 0; base < n; base += Lanes::kRows) {  // (uniform: every lane takes part in the sums)
+    const Row now = next;
+    const int i = base + own;
+    if (base + Lanes::kRows < n) next = fetch(i + Lanes::kRows);
+    float a[C][VEC], b[C][VEC], ga[C][VEC], gb[C][VEC];
+    Lanes::unpack(now.x, a, b);
+    Lanes::unpack(now.g, ga, gb);
+    const float ss = run_sum<LPR>(sum_products(a, b, a, b));
+    const float r = 1.f / sqrtf(ss / static_cast<float>(A.dim) + A.eps);
+    const int p = i < n ? pos[now.tok] : 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = base + u * Lanes::kRows + threadIdx.x / LPR;
-      tok[u] = static_cast<int>(static_cast<uint32_t>(h0 + i) / static_cast<uint32_t>(S.heads));
-      const int head = h0 + i - tok[u] * S.heads;
-      at[u] = ((t0 + tok[u]) * S.heads + head) * A.dim;
-      lanes.load(S.x, (t0 + tok[u]) * S.stride_t + head * S.stride_h, i < n, a[u], b[u]);
-      lanes.load(S.g, at[u], i < n, ga[u], gb[u]);
+    for (int c = 0; c < C; ++c) {
+      float co[VEC], si[VEC];
+      load_turn<VEC>(A.rope, lanes.pc[c], p, co, si);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float dma = ga[c][j] * co[j] + gb[c][j] * si[j];
+        const float dmb = gb[c][j] * co[j] - ga[c][j] * si[j];
+        a[c][j] *= r;  // n
+        b[c][j] *= r;
+        if (i < n) {
+          da[c][j] = fmaf(dma, a[c][j], da[c][j]);
+          db[c][j] = fmaf(dmb, b[c][j], db[c][j]);
+        }
+        ga[c][j] = dma * lanes.wa[c][j];
+        gb[c][j] = dmb * lanes.wb[c][j];
+      }
     }
+    const float mean = run_sum<LPR>(sum_products(ga, gb, a, b)) / static_cast<float>(A.dim);
+    if (S.y && i < n) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = base + u * Lanes::kRows + threadIdx.x / LPR;
-      const float ss = run_sum<LPR>(sum_products(a[u], b[u], a[u], b[u]));
-      const float r = 1.f / sqrtf(ss / static_cast<float>(A.dim) + A.eps);
-      const int p = i < n ? pos[tok[u]] : 0;
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float co[VEC], si[VEC];
-        load_turn<VEC>(A.rope, lanes.pc[c], p, co, si);
+      for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float dma = ga[u][c][j] * co[j] + gb[u][c][j] * si[j];
-          const float dmb = gb[u][c][j] * co[j] - ga[u][c][j] * si[j];
-          a[u][c][j] *= r;  // n
-          b[u][c][j] *= r;
-          if (i < n) {
-            da[c][j] = fmaf(dma, a[u][c][j], da[c][j]);
-            db[c][j] = fmaf(dmb, b[u][c][j], db[c][j]);
-          }
-          ga[u][c][j] = dma * lanes.wa[c][j];
-          gb[u][c][j] = dmb * lanes.wb[c][j];
+          ga[c][j] = r * (ga[c][j] - a[c][j] * mean);
+          gb[c][j] = r * (gb[c][j] - b[c][j] * mean);
         }
-      }
-      const float mean = run_sum<LPR>(sum_products(ga[u], gb[u], a[u], b[u])) / static_cast<float>(A.dim);
-      if (S.y && i < n) {
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            ga[u][c][j] = r * (ga[u][c][j] - a[u][c][j] * mean);
-            gb[u][c][j] = r * (gb[u][c][j] - b[u][c][j] * mean);
-          }
-        lanes.store(S.y, at[u], ga[u], gb[u]);
-      }
+      lanes.store(S.y, now.at, ga, gb);
     }
   }
   if (!S.dw_part) return;
@@ -226,12 +227,13 @@ __global__ __launch_bounds__(256) void norm_weight_grad_kernel(const float* __re
   }
 }
 
-// Rows of one backward workgroup, the same on both sides: kBwdBlocks workgroups for the side with
-// more heads, at least 64 rows, and no more tokens than the LDS positions hold (n rows touch at most
-// n / heads + 2 tokens).
+// Rows of one backward workgroup, the same on both sides: as many workgroups as run at once (four a CU; one each side is
+// the last, partly filled one), at least 64 rows, and no more tokens than the LDS positions hold (n rows touch
+// at most n / heads + 2 tokens). 32K tokens x 36 heads of 128, bf16, backward and weights' sums: 193 + 5 us, with twice as
+// many workgroups 195 + 10; before the next row was fetched ahead 211 + 5, with 1152 workgroups 279 + 5.
 int64_t bwd_rows(int64_t tokens, int64_t hq, int64_t hk) {
   const int64_t more = hq > hk ? hq : hk, fewer = hq > hk ? hk : hq, least = fewer ? fewer : more;
-  int64_t n = (tokens * more + kBwdBlocks - 1) / kBwdBlocks;
+  int64_t n = (tokens * (hq + hk) + kBwdBlocks - 1) / kBwdBlocks;
   n = n < 64 ? 64 : n;
   const int64_t most = (kMostTokens - 1) * least;
   return n < most ? n : most;
@@ -254,14 +256,14 @@ int norm_launch(NormArgs A, bool vectors, int64_t q_rows, int64_t k_rows, hipStr
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(nq + nk)), dim3(kNormThreads), 0, st, A);
     return static_cast<int>(status_from(hipGetLastError()));
   };
-#define MSA_NORM(VEC, C, LPR, U)                                                         \
-  if constexpr (BWD) return go(norm_rope_bwd_kernel<DT, VEC, C, LPR, U>, 0);             \
-  else return go(norm_rope_fwd_kernel<DT, VEC, C, LPR, U>, kNormThreads / LPR * U)
-  if (!vectors) { MSA_NORM(1, 4, 64, 1); }
-  if (chunks <= 4) { MSA_NORM(8, 1, 4, 1); }
-  if (chunks <= 8) { MSA_NORM(8, 1, 8, 1); }
-  if (chunks <= 16) { MSA_NORM(8, 1, 16, 1); }
-  MSA_NORM(8, 1, 32, 1);
+#define MSA_NORM(VEC, C, LPR)                                                 \
+  if constexpr (BWD) return go(norm_rope_bwd_kernel<DT, VEC, C, LPR>, 0);     \
+  else return go(norm_rope_fwd_kernel<DT, VEC, C, LPR>, kNormThreads / LPR)
+  if (!vectors) { MSA_NORM(1, 4, 64); }
+  if (chunks <= 4) { MSA_NORM(8, 1, 4); }
+  if (chunks <= 8) { MSA_NORM(8, 1, 8); }
+  if (chunks <= 16) { MSA_NORM(8, 1, 16); }
+  MSA_NORM(8, 1, 32);
 #undef MSA_NORM
 }
 
