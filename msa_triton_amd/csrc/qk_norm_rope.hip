@@ -101,7 +101,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_rope_fwd_kernel(NormArgs A)
 // The row after this one is on its way while it is worked on (32K tokens x 36 heads of 128, bf16: 193 us, 4.7 TB/s; 211
 // without).
 template <int DT, int VEC, int C, int LPR>
-__global__ __launch_bounds__(kNormThreads, 4) void norm_rope_bwd_kernel(NormArgs A) {
+__global__ __launch_bounds__(kNormThreads, DT == kF32 ? 3 : 4) void norm_rope_bwd_kernel(NormArgs A) {
   using Lanes = RowLanes<DT, VEC, C, LPR>;
   __shared__ int32_t pos[kMostTokens + 1];
   __shared__ float sums[kNormThreads / kWave][kMostDim];

@@ -1,4 +1,4 @@
-"""torch.library registration of the three operators, for torch.compile.
+"""torch.library registration of the operators, for torch.compile.
 
 The reference names this as follow-on work (docs/code_review.md:321-322; a
 ``torch.library`` custom op with fake/meta kernels). Here the HIP launches are
@@ -20,11 +20,23 @@ graph breaks and AOTAutograd differentiates it:
     msa_mi355x::indexer_kl(index_q, index_k, q, k, indices, cu_seqlens, max_seqlen, block_size, index_scale,
                            scale, need_q, need_k, teacher_lse) -> (loss, row_kl, d_iq, d_ik)
                                                d_iq / d_ik: fp32 gradients of loss, empty when not wanted
+    msa_mi355x::qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, context_lens, eps)
+        -> (q_out, k_out)                      k_out: empty without k
+    msa_mi355x::qk_norm_rope_backward(q, k, q_weight, k_weight, cos_sin, cu_seqlens, context_lens, eps, grad_q_out,
+                                      grad_k_out, need_q, need_k, need_q_weight, need_k_weight)
+        -> (dq, dk, dq_weight, dk_weight)
+    msa_mi355x::cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, index_k, index_cache,
+                             k_scale, v_scale, k_weight, index_weight, cos_sin, eps) -> ()   caches and scales are written
+    msa_mi355x::index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, context_lens, max_seqlen,
+                                       block_size, scale, topk_blocks, local_blocks) -> (scores, indices)
+    msa_mi355x::sparse_attention_paged(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, block_size,
+                                       scale, k_scale, v_scale) -> (out, lse)
 
 A gradient that is not needed comes back as an empty tensor. ``m3_index_score``,
 ``m3_topk`` and ``m3_sparse_attention`` below keep the public signatures: their
 static checks (ranks, dtypes, devices) run in Python, the metadata checks that read
-``cu_seqlens`` run inside the ops when they execute, with the same messages.
+``cu_seqlens`` run inside the ops when they execute, with the same messages. The norm
+and the paged operators make all their checks when they execute.
 Importing this module registers the ops; it does not load the HIP library.
 """
 
@@ -37,9 +49,16 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from .cache_append import m3_cache_append as _eager_append
 from .index_score import _score_backward, _score_forward
 from .indexer_kl import _launch as _kl_launch
 from .layout import sequence_lengths, sequence_meta
+from .norm_rope import _backward as _norm_backward
+from .norm_rope import _call_args as _norm_args
+from .norm_rope import _validate as _norm_validate
+from .norm_rope import m3_qk_norm_rope as _eager_norm
+from .paged_attention import m3_sparse_attention_paged as _eager_attention_paged
+from .paged_score import m3_index_score_topk_paged as _eager_score_paged
 from .sparse_attention import _attn_backward, _attn_forward
 from .topk import m3_topk as _eager_topk
 
@@ -247,6 +266,108 @@ def _kl_grad(ctx, grad_loss, grad_rows, grad_diq, grad_dik):
 torch.library.register_autograd(f"{_NS}::indexer_kl", _kl_grad, setup_context=_kl_setup)
 
 
+# ---------------------------------------------------------------------------- norm and rotation
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope", mutates_args=())
+def _qk_norm_rope(q: Tensor, k: Optional[Tensor], q_weight: Tensor, k_weight: Optional[Tensor],
+                  cos_sin: Optional[Tensor], cu_seqlens: Tensor, context_lens: Optional[Tensor],
+                  eps: float) -> tuple[Tensor, Tensor]:
+    with torch.no_grad():
+        q_out, k_out = _eager_norm(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps=eps, context_lens=context_lens)
+    return q_out, k_out if k_out is not None else q.new_empty(0)
+
+
+@_qk_norm_rope.register_fake
+def _(q, k, q_weight, k_weight, cos_sin, cu_seqlens, context_lens, eps):
+    return q.new_empty(q.shape), q.new_empty(k.shape if k is not None else (0,))
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope_backward", mutates_args=())
+def _qk_norm_rope_backward(q: Tensor, k: Optional[Tensor], q_weight: Tensor, k_weight: Optional[Tensor],
+                           cos_sin: Optional[Tensor], cu_seqlens: Tensor, context_lens: Optional[Tensor], eps: float,
+                           grad_q_out: Tensor, grad_k_out: Tensor, need_q: bool, need_k: bool, need_q_weight: bool,
+                           need_k_weight: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    args = _norm_validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps, context_lens)
+    grads = _norm_backward(*args[:4], _norm_args(*args), grad_q_out, grad_k_out if k is not None else None,
+                           (need_q, need_k, need_q_weight, need_k_weight))
+    dq, dk, dwq, dwk = (g if g is not None else q.new_empty(0) for g in grads)
+    return dq, dk, dwq, dwk
+
+
+@_qk_norm_rope_backward.register_fake
+def _(q, k, q_weight, k_weight, cos_sin, cu_seqlens, context_lens, eps, grad_q_out, grad_k_out, need_q, need_k,
+      need_q_weight, need_k_weight):
+    return tuple(x.new_empty(x.shape) if x is not None and need else q.new_empty(0)
+                 for x, need in ((q, need_q), (k, need_k), (q_weight, need_q_weight), (k_weight, need_k_weight)))
+
+
+def _norm_setup(ctx, inputs, output):
+    *tensors, ctx.eps = inputs
+    ctx.save_for_backward(*tensors)
+
+
+def _norm_grad(ctx, grad_q_out, grad_k_out):
+    q, k = ctx.saved_tensors[:2]
+    need = [bool(x) for x in ctx.needs_input_grad[:4]]
+    grads = torch.ops.msa_mi355x.qk_norm_rope_backward(
+        *ctx.saved_tensors, ctx.eps, grad_q_out if grad_q_out is not None else torch.zeros_like(q),
+        grad_k_out if grad_k_out is not None else q.new_zeros(k.shape if k is not None else (0,)), *need)
+    return (*(g if n else None for g, n in zip(grads, need)), None, None, None, None)
+
+
+torch.library.register_autograd(f"{_NS}::qk_norm_rope", _norm_grad, setup_context=_norm_setup)
+
+
+# ---------------------------------------------------------------------------- paged cache
+
+@torch.library.custom_op(f"{_NS}::cache_append",
+                         mutates_args=("k_cache", "v_cache", "index_cache", "k_scale", "v_scale"))
+def _cache_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor, cu_seqlens: Tensor,
+                  context_lens: Tensor, index_k: Optional[Tensor], index_cache: Optional[Tensor],
+                  k_scale: Optional[Tensor], v_scale: Optional[Tensor], k_weight: Optional[Tensor],
+                  index_weight: Optional[Tensor], cos_sin: Optional[Tensor], eps: float) -> None:
+    _eager_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, index_k=index_k,
+                  index_cache=index_cache, k_scale=k_scale, v_scale=v_scale, k_weight=k_weight,
+                  index_weight=index_weight, cos_sin=cos_sin, eps=eps)
+
+
+@_cache_append.register_fake
+def _(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, index_k, index_cache, k_scale, v_scale, k_weight,
+      index_weight, cos_sin, eps):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::index_score_topk_paged", mutates_args=())
+def _index_score_topk_paged(index_q: Tensor, index_cache: Tensor, page_table: Tensor, cu_seqlens: Tensor,
+                            context_lens: Tensor, max_seqlen: int, block_size: int, scale: float, topk_blocks: int,
+                            local_blocks: int) -> tuple[Tensor, Tensor]:
+    return _eager_score_paged(index_q, index_cache, page_table, cu_seqlens, context_lens, max_seqlen,
+                              block_size=block_size, scale=scale, topk_blocks=topk_blocks, local_blocks=local_blocks)
+
+
+@_index_score_topk_paged.register_fake
+def _(index_q, index_cache, page_table, cu_seqlens, context_lens, max_seqlen, block_size, scale, topk_blocks,
+      local_blocks):
+    total, groups, _ = index_q.shape
+    blocks = (max_seqlen + block_size - 1) // block_size
+    return (index_q.new_empty((total, groups, blocks), dtype=torch.float32),
+            index_q.new_empty((total, groups, topk_blocks), dtype=torch.int32))
+
+
+@torch.library.custom_op(f"{_NS}::sparse_attention_paged", mutates_args=())
+def _sparse_attention_paged(q: Tensor, k_cache: Tensor, v_cache: Tensor, indices: Tensor, page_table: Tensor,
+                            cu_seqlens: Tensor, context_lens: Tensor, block_size: int, scale: float,
+                            k_scale: Optional[Tensor], v_scale: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    return _eager_attention_paged(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens,
+                                  block_size=block_size, scale=scale, k_scale=k_scale, v_scale=v_scale,
+                                  return_lse=True)
+
+
+@_sparse_attention_paged.register_fake
+def _(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, block_size, scale, k_scale, v_scale):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
 # ---------------------------------------------------------------------------- public wrappers
 
 def m3_index_score(index_q, index_k, cu_seqlens, max_seqlen, *, block_size=128, scale=1.0):
@@ -347,3 +468,33 @@ def m3_indexer_kl(index_q, index_k, q, k, indices, cu_seqlens, max_seqlen, *, bl
                                                        grad and index_q.requires_grad, grad and index_k.requires_grad,
                                                        None if teacher_lse is None else teacher_lse.detach())
     return (loss, rows) if return_rows else loss
+
+
+def m3_qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, *, eps=1e-6, context_lens=None):
+    """``msa_triton_amd.m3_qk_norm_rope`` through the registered op."""
+    q_out, k_out = torch.ops.msa_mi355x.qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, context_lens,
+                                                     float(eps))
+    return q_out, None if k is None else k_out
+
+
+def m3_cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, *, index_k=None, index_cache=None,
+                    k_scale=None, v_scale=None, k_weight=None, index_weight=None, cos_sin=None, eps=1e-6):
+    """``msa_triton_amd.m3_cache_append`` through the registered op."""
+    torch.ops.msa_mi355x.cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, index_k, index_cache,
+                                      k_scale, v_scale, k_weight, index_weight, cos_sin, float(eps))
+
+
+def m3_index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, context_lens, max_seqlen, *, block_size=128,
+                              scale=1.0, topk_blocks=16, local_blocks=1):
+    """``msa_triton_amd.m3_index_score_topk_paged`` through the registered op."""
+    return torch.ops.msa_mi355x.index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, context_lens,
+                                                       max_seqlen, block_size, float(scale), topk_blocks, local_blocks)
+
+
+def m3_sparse_attention_paged(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, *, block_size=128,
+                              scale=None, k_scale=None, v_scale=None, return_lse=False):
+    """``msa_triton_amd.m3_sparse_attention_paged`` through the registered op."""
+    out, lse = torch.ops.msa_mi355x.sparse_attention_paged(
+        q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, block_size,
+        q.shape[-1] ** -0.5 if scale is None else float(scale), k_scale, v_scale)
+    return (out, lse) if return_lse else out
