@@ -26,6 +26,7 @@ namespace msa {
 namespace {
 
 constexpr int kList = 256;       // steps listed at once: one a thread
+constexpr int kIds = 1024;       // ids kept in LDS where there are more than 64, to find repeated ones
 constexpr int kMostSplits = 64;  // of one row: a lane of the joining wave each
 
 struct PagedAttnArgs {
@@ -71,6 +72,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   __shared__ alignas(16) uint16_t vbuf[4][32 * RS];
   __shared__ int list_key[kList], list_p0[kList], list_p1[kList], listed[4];
   __shared__ float wave_max[4][16], wave_sum[4][16];
+  __shared__ int early_ids[kIds];
   const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t item = blockIdx.x / A.splits;
@@ -81,6 +83,10 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   const int ratio = A.Hq / A.G, head = 16 * ht + c;
   const int32_t* ids = A.indices + tg * A.K;
   const int32_t wave_id = lane < A.K ? ids[lane] : -1;  // the first 64 ids, one a lane
+  if (A.K > 64) {
+    for (int i = threadIdx.x; i < min(A.K, kIds); i += 256) early_ids[i] = ids[i];
+    __syncthreads();
+  }
   const bool full = A.D == DP;
 
   // dims of a lane in step kk of the first product (any order, the same for keys and queries)
@@ -94,10 +100,10 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   }
 
   const TokenPlace at = wave_place_of(A.cu, A.nseq, A.context, t);
-  const int pos = at.pos > 0x7fffffff ? 0x7fffffff : static_cast<int>(at.pos);
-  const int per_block = (A.B + 31) / 32;
+  const int pos = static_cast<int>(min(at.pos, A.pages.last_position()));
+  const int per_block = min((A.B - 1) / 32, pos / 32) + 1;  // steps of a block, of those up to the token
   // this workgroup's steps: every splits-th (the blocks that exist come first in a selection)
-  const int64_t steps = static_cast<int64_t>(A.K) * per_block;
+  const int64_t steps = pos < 0 ? 0 : static_cast<int64_t>(A.K) * per_block;
 
   float m = -__builtin_inff(), l = 0.f;  // of head c: the maximum over all quarters, the sum over this one
   f32x4 acc[ND];
@@ -150,7 +156,8 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
     const int id = A.K <= 64 ? __shfl(wave_id, slot, kWave) : ids[slot];
     bool again = false;  // an id that an earlier slot holds
     for (int i = 0; i < min(A.K, 64); ++i) again |= i < slot && __builtin_amdgcn_readlane(wave_id, i) == id;
-    for (int i = 64; i < slot; ++i) again |= ids[i] == id;
+    for (int i = 64; i < min(slot, kIds); ++i) again |= early_ids[i] == id;
+    for (int i = kIds; i < slot; ++i) again |= ids[i] == id;
     if (n < steps) {
       const int step = static_cast<int>(n - static_cast<int64_t>(slot) * per_block);
       const int64_t first = static_cast<int64_t>(id) * A.B + 32 * step;
@@ -362,7 +369,7 @@ int64_t head_tiles_of(int64_t heads, int64_t groups) { return (heads / groups + 
 // the number with the fewest steps, rounds of 512 times the steps of a wave and those four. 328 items of 128 steps as
 // 328, 656 and 984 workgroups: 112, 115 and 98 us; 4 items of 64 steps: one step a wave, 64 workgroups, 13 us.
 int64_t split_count(int64_t items, int64_t slots, int64_t block_size) {
-  const int64_t steps = slots * ((block_size + 31) / 32);
+  const int64_t steps = slots * ((block_size - 1) / 32 + 1);
   int64_t best = 1, cost = -1;
   for (int64_t n = 1; n == 1 || (n <= (steps + 3) / 4 && n <= kMostSplits); ++n) {
     const int64_t x = ((items * n + 511) / 512) * ((steps + 4 * n - 1) / (4 * n) + 4);

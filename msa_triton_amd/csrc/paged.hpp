@@ -22,6 +22,10 @@ struct PageMap {
   int num_pages;
   int shift;             // log2(page size)
 
+  // The last position that the table has an entry for (-1: none). Keys behind it do not exist, whatever a sequence's
+  // length says, and no loop goes there.
+  __device__ __forceinline__ int64_t last_position() const { return (static_cast<int64_t>(pages_per_seq) << shift) - 1; }
+
   // The page that holds position j of sequence s, or -1.
   __device__ __forceinline__ int page_of(int s, int64_t j) const {
     const int64_t m = j >> shift;

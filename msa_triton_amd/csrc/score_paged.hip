@@ -104,8 +104,10 @@ __device__ __forceinline__ void score_run(const PagedScoreArgs& A, const SeqWork
   const int64_t row = r0 + c;
   const bool live = row < rows;
   const int32_t i = static_cast<uint32_t>(live ? row : rows - 1) / static_cast<uint32_t>(A.G);  // token of the sequence
-  const int64_t pos = context < 0 ? -1 : static_cast<int64_t>(context) + i;
-  const int64_t last = context < 0 ? -1 : static_cast<int64_t>(context) + static_cast<uint32_t>(min(r0 + 16, rows) - 1) / static_cast<uint32_t>(A.G);
+  const int64_t end = A.pages.last_position();
+  const int64_t pos = context < 0 ? -1 : min(end, static_cast<int64_t>(context) + i);
+  const int64_t last = context < 0 ? -1 : min(end, static_cast<int64_t>(context) +
+                                                       static_cast<uint32_t>(min(r0 + 16, rows) - 1) / static_cast<uint32_t>(A.G));
   float* out = A.scores + (start * A.G + (live ? row : rows - 1)) * A.NB;
   const int seen_blocks = A.pages.num_pages == 0 || last < 0 ? 0 : static_cast<int>(min(static_cast<uint32_t>(last) / A.B + 1, static_cast<uint32_t>(A.NB)));
   const int stop = min(block1, seen_blocks);

@@ -22,7 +22,8 @@ def _turned(x, w, table, pos, eps):
     """Norm and rotation of rows [T, H, D] in float64 numpy."""
     x = x.double().cpu().numpy()
     if w is not None:
-        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + np.float64(np.float32(eps))) * w.double().cpu().numpy()
+        with np.errstate(invalid="ignore"):
+            x = x / np.sqrt((x * x).mean(-1, keepdims=True) + np.float64(np.float32(eps))) * w.double().cpu().numpy()
     if table is not None:
         t = table.double().cpu().numpy()
         half = t.shape[1] // 2
@@ -32,7 +33,8 @@ def _turned(x, w, table, pos, eps):
                 rows[i] = t[p]
         cos, sin = rows[:, None, :half], rows[:, None, half:]
         a, b = x[..., :half].copy(), x[..., half:2 * half].copy()
-        x[..., :half], x[..., half:2 * half] = a * cos - b * sin, b * cos + a * sin
+        with np.errstate(invalid="ignore"):
+            x[..., :half], x[..., half:2 * half] = a * cos - b * sin, b * cos + a * sin
     return x
 
 
@@ -119,6 +121,8 @@ CASES = [  # lengths, context, heads, D, Di, rot, page, dtype
     ([40, 3, 17], [-1, 13, -7], 2, 256, 128, 64, 16, torch.float16),
     ([21, 50], [9, 40], 2, 48, 16, 12, 32, torch.bfloat16),   # a rotation off 16-byte runs
     ([130], [60], 8, 64, 32, 0, 64, torch.bfloat16),          # no rotation
+    ([(i * 7) % 3 for i in range(150)], [(i * 37) % 50 - 5 for i in range(150)], 1, 32, 16, 16, 16,
+     torch.bfloat16),                                         # more sequences than lanes
 ]
 
 

@@ -134,6 +134,8 @@ CASES = [  # lengths, context, groups, ratio, D, page, slots, block, dtype
     ([70], [20], 2, 2, 48, 16, 2, 32, torch.float16),
     ([2], [9000], 1, 4, 128, 128, 5, 2048, torch.bfloat16),         # more steps than one list holds
     ([600], [0], 4, 8, 64, 64, 2, 64, torch.bfloat16),              # rows enough for one workgroup each
+    ([(i * 7) % 3 for i in range(300)], [(i * 37) % 150 - 5 for i in range(300)], 1, 2, 32, 16, 2, 32,
+     torch.float16),                                                # more sequences than lanes
 ]
 
 
@@ -170,6 +172,27 @@ def test_selections_pages_and_scale(fp8, device):
         empty.update(ks=x["ks"][:0], vs=x["vs"][:0])
     out, lse = _check(x, lengths, context, 64, **empty)
     assert (out == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_block_sizes_and_lengths_past_the_table(fp8, device):
+    """A block that holds every key there is, lengths that no table holds, and more slots than LDS keeps ids of."""
+    lengths, context = [1, 2], [150, 60]
+    x = _setup(lengths, context, 2, 4, 32, 16, 3, 16, torch.bfloat16, fp8, device)
+    ids = torch.full_like(x["ids"], -1)
+    ids[..., 1] = 0
+    _check(x, lengths, context, 2 ** 31 - 16, ids=ids)
+    table = x["table"][:, :4].clone()  # 64 positions
+    _check(x, lengths, context, 2 ** 30, ids=ids, table=table)
+    want = _call(x, 2 ** 30, ids=ids, table=table)
+    far = torch.tensor([2 ** 31 - 1, 2 ** 31 - 2], dtype=torch.int32, device=device)
+    got = _call(x, 2 ** 30, ids=ids, table=table, context=far)
+    assert torch.equal(got[0][0], want[0][0])  # (the second sequence's slots behind its tokens hold NaN)
+    many = torch.randint(-3, 12, (3, 2, 1500), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    many[:, :, :1400] = torch.where(many[:, :, :1400] > 5, -1, many[:, :, :1400])
+    _check(x, lengths, context, 16, ids=many.to(device))
+    _check(x, lengths, context, 16, ids=many[:, :, 1350:1450].to(device))
 
 
 @pytest.mark.gpu

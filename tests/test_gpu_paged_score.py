@@ -125,6 +125,33 @@ def test_missing_pages_and_short_tables(device):
 
 
 @pytest.mark.gpu
+def test_block_sizes_and_lengths_past_the_table(device):
+    """One block that holds every key, and a length that no table holds: what exists is scored, the own block selected."""
+    lengths, context = [2], [250]
+    x = _setup(lengths, context, 4, 64, 32, torch.bfloat16, device)
+    _check(x, lengths, context, 2 ** 31 - 16, 2, 1)
+    iq, cache, table, cu, _, _ = x
+    table = table[:, :6].to(device)  # 192 positions
+    far = torch.tensor([2 ** 31 - 40], dtype=torch.int32, device=device)
+    want, _ = msa.m3_index_score_topk_paged(iq[:1], cache, table, cu_tensor([1], device),
+                                            torch.tensor([191], dtype=torch.int32, device=device), 192, block_size=64)
+    got, ids = msa.m3_index_score_topk_paged(iq, cache, table, cu, far, 256, block_size=64, topk_blocks=5)
+    assert torch.equal(got[:1, :, :3], want) and torch.isinf(got[:, :, 3]).all()
+    assert (ids.sort(dim=2).values[..., 2:] == torch.tensor([0, 1, 2], device=device)).all()
+    got, _ = msa.m3_index_score_topk_paged(iq, cache, table, cu, far, 2 ** 31 - 1, block_size=2 ** 30, topk_blocks=1)
+    assert torch.equal(got[0, :, 0], want[0].amax(1)) and torch.isinf(got[:, :, 1]).all()
+
+
+@pytest.mark.gpu
+def test_more_sequences_than_lanes(device):
+    """65 and 600 sequences: the lookups that go through LDS and through several steps."""
+    for n in (65, 600):
+        lengths = [(i * 7) % 3 for i in range(n)]
+        context = [(i * 37) % 150 - 5 for i in range(n)]
+        _check(_setup(lengths, context, 2, 64, 16, torch.bfloat16, device), lengths, context, 32, 3, 1)
+
+
+@pytest.mark.gpu
 def test_equal_to_the_packed_operator(device):
     """A packed prompt scored whole, and its tail scored against a cache of it."""
     lengths, tails, block = [700, 333, 64], [3, 1, 64], 64
