@@ -119,17 +119,20 @@ def _backward(q, k, wq, wk, call, dq_out, dk_out, need):
 
 class _NormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, table, cu, context, call):
+    def forward(ctx, q, k, wq, wk, table, cu, context, sizes, eps):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, wq, wk, table, cu, context)  # (all that `call` points into)
-        ctx.call = call
-        return _forward(q, k, call)
+        ctx.save_for_backward(q, k, wq, wk, table, cu, context)
+        ctx.sizes, ctx.eps = sizes, eps
+        return _forward(q, k, _call_args(q, k, wq, wk, table, *sizes[:2], cu, sizes[2], context, eps))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
-        q, k, wq, wk, _, _, _ = ctx.saved_tensors
-        return (*_backward(q, k, wq, wk, ctx.call, dq_out, dk_out, ctx.needs_input_grad), None, None, None, None)
+        # (checkpointing and offloading hand back other tensors than the ones that were saved)
+        q, k, wq, wk, table, cu, context = ctx.saved_tensors
+        q, k = _unit_rows(q), _unit_rows(k)
+        call = _call_args(q, k, wq, wk, table, *ctx.sizes[:2], cu, ctx.sizes[2], context, ctx.eps)
+        return (*_backward(q, k, wq, wk, call, dq_out, dk_out, ctx.needs_input_grad), None, None, None, None, None)
 
 
 def _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps, context_lens):
@@ -184,8 +187,7 @@ def m3_qk_norm_rope(
     (slices of a fused projection are read in place). The index heads go through the same call."""
     q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps = _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens,
                                                                            eps, context_lens)
-    call = _call_args(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps)
     if torch.is_grad_enabled() and (q.requires_grad or wq.requires_grad or
                                     (k is not None and (k.requires_grad or wk.requires_grad))):
-        return _NormRope.apply(q, k, wq, wk, table, cu, context, call)
-    return _forward(q, k, call)
+        return _NormRope.apply(q, k, wq, wk, table, cu, context, (rows, rot, num_seqs), eps)
+    return _forward(q, k, _call_args(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps))

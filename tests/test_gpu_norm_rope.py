@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import msa_triton_amd as msa
 from tests.helpers import cu_tensor
@@ -227,6 +228,32 @@ def test_partial_gradients_and_determinism(device):
         outs = msa.m3_qk_norm_rope(*leaves, table, cu)
         (g,) = torch.autograd.grad(outs[0], leaves[0], dq.clone().requires_grad_(), create_graph=True)
         g.float().sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", ("checkpoint", "offload"))
+def test_saved_tensors_that_move(way, device):
+    """Checkpointing recomputes what the backward reads and offloading copies it: other tensors at other addresses."""
+    case = ([300, 211], "far", 8, 2, 128, 64, torch.bfloat16, None)
+    q, k, wq, wk, table, pos, ctx, dq, dk = _inputs(case, device)
+    cu = msa.prepare_sequences(cu_tensor(case[0], device))
+    leaves = [x.clone().requires_grad_() for x in (q, k, wq, wk)]
+
+    def layer(q, k, wq, wk):
+        # (weights and inputs that nothing but the saved state keeps; a transposed one comes back in another layout)
+        return msa.m3_qk_norm_rope(q * 2, (k * 2).transpose(1, 2).contiguous().transpose(1, 2), wq * 1.5, wk * 1.5, table,
+                                   cu, context_lens=ctx)
+
+    want = torch.autograd.grad(layer(*leaves), leaves, (dq, dk))
+    if way == "checkpoint":
+        outs = torch.utils.checkpoint.checkpoint(layer, *leaves, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            outs = layer(*leaves)
+    noise = [torch.full_like(q, float("nan")) for _ in range(4)]  # takes the place of what was freed
+    got = torch.autograd.grad(outs, leaves, (dq, dk))
+    del noise
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @pytest.mark.gpu
