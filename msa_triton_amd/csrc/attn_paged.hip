@@ -18,7 +18,8 @@
 //
 // Logits, statistics and outputs are fp32. A weight enters the second product as two 16-bit terms
 // (hi + lo, 2^-17 of it left out), so that the output's error stays that of its own rounding: one term would add 2^-9 of a
-// weight. Values of keys that are not visible are zeroed on their way to LDS: 0 x NaN is NaN.
+// weight. In fp16 they are the terms of the weight times 2^15 (fp16 ends at 2^-24; so weights down to 2^-22 keep that bound).
+// Values of keys that are not visible are zeroed on their way to LDS: 0 x NaN is NaN.
 #include "mfma_util.hpp"
 #include "paged.hpp"
 
@@ -68,6 +69,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   constexpr int VL = FP8 ? DP / 16 : DP / 8;    // lanes of one value row
   constexpr int NV = VL / 2, VR = 64 / VL;      // 16-byte pieces of 32 rows, rows of a piece
   constexpr int VD = FP8 ? 16 : 8;              // values of a piece
+  constexpr float kUp = PT == kF16 ? 0x1p15f : 1.f;  // of the weights in the second product
   constexpr int NKR = FP8 ? NK / 2 : NK;        // 16-byte pieces of a key row and lane
   __shared__ alignas(16) uint16_t vbuf[4][32 * RS];
   __shared__ int list_key[kList], list_p0[kList], list_p1[kList], listed[4];
@@ -242,6 +244,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
       for (int j = 0; j < 8; j += 2) {
         float y0 = __builtin_amdgcn_exp2f(x[j] - shift), y1 = __builtin_amdgcn_exp2f(x[j + 1] - shift);
         l += y0 + y1;
+        if constexpr (PT == kF16) y0 *= kUp, y1 *= kUp;
         if constexpr (FP8) y0 *= j < 4 ? vf0 : vf1, y1 *= j < 4 ? vf0 : vf1;
         if constexpr (PT == kF16) {
           hi[j >> 1] = cvt_pk_f16(y0, y1);
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   if (h >= ratio) return;
   const int64_t out_row = t * A.Hq + g * ratio + h;
   const bool whole = A.splits == 1;
-  const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+  const float inv = (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f) / kUp;
   float* part = whole ? nullptr : A.part + ((item * A.splits + split) * 16 + row) * A.D;
   const bool none = !whole && top == -__builtin_inff();  // (the joining launch does not look at it)
   for (int d = 4 * col; d < A.D && !none; d += 64) {
@@ -436,6 +439,7 @@ extern "C" int msa_attn_paged(const void* q, const void* k_cache, const void* v_
   const int64_t items = total_tokens * kv_groups * A.head_tiles;
   if (items >= (int64_t{1} << 24)) return kErrUnsupported;  // 2^32 threads of a launch
   A.splits = static_cast<int>(split_count(items, topk_slots, block_size));
+  if (items * A.splits >= (int64_t{1} << 24)) return kErrUnsupported;
   A.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   A.out = static_cast<uint16_t*>(out);
   A.lse = lse;

@@ -149,6 +149,34 @@ def test_attention(case, fp8, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fp8", (False, True))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_many_small_weights_count(dtype, fp8, device):
+    """64 keys of weight 1 (value 0) and thousands of weight 2^-26 (value 256): each is below half of fp16's smallest value,
+    together they are the output. The logits are products of one term, so a weight is off by 2 x 18 x 2^-23 (its logit, in
+    fp32) and 2^-22; its two 16-bit terms and the sums by 2^-14 together."""
+    n, block, tokens = 8192, 128, 520
+    x = _setup([tokens], [n - tokens], 1, 2, 16, 128, n // block, block, dtype, fp8, device)
+    x["kc"].copy_(torch.zeros((), dtype=torch.float32))
+    x["vc"].copy_(torch.full((), 256.0))
+    if fp8:
+        x["ks"].fill_(1.0)
+        x["vs"].fill_(1.0)
+    for page in x["table"][0, :16].tolist():  # at the head of each wave's keys, however they are shared out
+        x["kc"][page, 0, ::32, 0] = 18.0
+        x["vc"][page, 0, ::32] = 0.0
+    x["q"].zero_()
+    x["q"][..., 0] = 1.0
+    x["ids"].copy_(torch.arange(n // block, dtype=torch.int32))
+    got, _ = _call(x, block, scale=1.0)
+    count = torch.arange(n - tokens + 1, n + 1, dtype=torch.float64) - 64
+    want = 256 * count / (64 * np.exp(18.0) + count)
+    bound = torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -8) + 2.0 ** -14 + 36 * 2.0 ** -23 + 2.0 ** -22
+    err = (got.double().cpu() / want[:, None, None] - 1).abs()
+    assert (err <= bound).all(), float(err.max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fp8", [False, True])
 def test_selections_pages_and_scale(fp8, device):
     lengths, context = [2, 3], [250, 130]
