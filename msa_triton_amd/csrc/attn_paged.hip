@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
 }
 
 // The splits of a row joined, a wave for each head's row: lane z weighs split z (at most kMostSplits = 64), and
-// the lanes take two dims each of all of them, eight splits' loads in flight at a time.
+// the lanes take two dims each of all of them, eight splits' loads in flight at a time (4 us: a launch and two loads' latency).
 template <int DT>
 __global__ __launch_bounds__(256) void attn_paged_join(PagedAttnArgs A) {
   const int lane = threadIdx.x & 63;

@@ -62,7 +62,7 @@ __device__ __forceinline__ void load_positions(const NormArgs& A, int64_t t0, in
 }
 
 // One row a lane run: with many workgroups a CU more rows in flight each only cost registers (32K tokens x 36 heads of 128,
-// bf16: 122 us; 136 and 152 with two and four).
+// bf16: 122 us, 4.9 TB/s; 136 and 152 with two and four).
 template <int DT, int VEC, int C, int LPR>
 __global__ __launch_bounds__(kNormThreads) void norm_rope_fwd_kernel(NormArgs A) {
   using Lanes = RowLanes<DT, VEC, C, LPR>;

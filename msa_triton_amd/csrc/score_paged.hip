@@ -28,7 +28,9 @@ namespace msa {
 namespace {
 
 // Workgroups of a call: two a CU, as many as run at once (us with 256 / 512 / 768, top-k included: 32 requests of
-// 0.5 to 30K tokens 27.6 / 25.7 / 30.0, 64 of 16K 58.0 / 58.5 / 61.9, 256 of 4K 63.9 / 62.2 / 64.9).
+// 0.5 to 30K tokens 27.6 / 25.7 / 30.0, 64 of 16K 58.0 / 58.5 / 61.9, that is 4.6 TB/s, 256 of 4K 63.9 / 62.2 / 64.9). Their
+// stretches go block by block through one tile: all tiles of a few blocks first, for the keys to come from the L2 the second
+// time, gives 25.6 -> 24.4 us for 5 tokens of 4 groups behind 130 000, but 30.2 -> 36.7 for 16 requests of 16K with 5 each.
 constexpr int64_t kBlocks = 512;
 
 struct PagedScoreArgs {
