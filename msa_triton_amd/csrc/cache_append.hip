@@ -14,8 +14,8 @@
 //
 // Work: 16-bit rows go to runs of LPR lanes, as in the norm. An 8-bit page, head and side is one
 // workgroup's, because its scale is needed before its first byte: one pass over the page's new rows for the
-// maximum, one to write them (from registers where they are few, from the caches otherwise). Pages are numbered without a list of them:
-// sequence s gets the numbers from cu[s] / page + 2 s on, which leaves room for the two pages that n tokens can
+// maximum, one to write them (from registers where they are few, from the caches otherwise). Pages are
+// numbered without a list of them: sequence s gets the numbers from cu[s] / page + 2 s on, which leaves room for the two pages that n tokens can
 // touch beyond n / page; numbers without a page end at once.
 //
 // 16 bits: bound by memory (16 272 tokens, 4 heads of 128 and an index head: 19 us, 4.1 TB/s). 8 bits: by the vector work of

@@ -83,8 +83,8 @@ __device__ __forceinline__ TokenPlace wave_place_of(const int32_t* __restrict__ 
 // What every paged entry point checks about its page map.
 inline bool valid_pages(const int32_t* table, int64_t stride, int64_t pages_per_seq, int64_t num_pages,
                         int64_t page_size) {
-  return (table || pages_per_seq == 0) && stride >= 0 && num_pages >= 0 && num_pages <= 0x7fffffff && page_size >= 16 && page_size <= 256 &&
-         (page_size & (page_size - 1)) == 0 && pages_per_seq >= 0 && pages_per_seq <= 0x7fffffff / page_size;
+  return (table || pages_per_seq == 0) && stride >= 0 && num_pages >= 0 && num_pages <= 0x7fffffff && page_size >= 16 &&
+         page_size <= 256 && (page_size & (page_size - 1)) == 0 && pages_per_seq >= 0 && pages_per_seq <= 0x7fffffff / page_size;
 }
 
 inline PageMap page_map(const int32_t* table, int64_t stride, int64_t pages_per_seq, int64_t num_pages,

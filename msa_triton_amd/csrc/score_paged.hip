@@ -10,9 +10,10 @@
 // fp32, and DP additions of partial sums below S are off by at most a step of 2^-23 S each (also if the unit
 // truncates), plus what falls below fp32's range: below 2^-126 for a product, and below 2^-126 |q| for a bf16 key
 // value that the unit may take as zero (a query with such values is settled in FP64 throughout). A key can hold the
-// maximum only if s >= max s - 2 e, e = (DP + 16) (2^-23 max S + 2^-126 (1 + max |q|)); usually one key of a block does. Those keys' dots are formed in FP64 (four lanes a
-// row, each with the dims of its query fragment, two exchanges), and their maximum is the score. Rows with an
-// infinity or a NaN somewhere fail the comparison and are settled in FP64 as well.
+// maximum only if s >= max s - 2 e, e = (DP + 16) (2^-23 max S + 2^-126 (1 + max |q|)); usually one
+// key of a block does. Those keys' dots are formed in FP64 (four lanes a row, each with the dims of its query fragment, two
+// exchanges), and their maximum is the score. Rows with an infinity or a NaN somewhere fail the comparison and are
+// settled in FP64 as well.
 //
 // Bound by reading the index keys once from HBM (256 bytes a key for 128 dims): a wave takes one key
 // block for 16 query rows (tokens x groups of a sequence), its key fragments straight from memory in the
@@ -111,7 +112,9 @@ __device__ __forceinline__ void score_run(const PagedScoreArgs& A, const SeqWork
   const int64_t last = context < 0 ? -1 : min(end, static_cast<int64_t>(context) +
                                                        static_cast<uint32_t>(min(r0 + 16, rows) - 1) / static_cast<uint32_t>(A.G));
   float* out = A.scores + (start * A.G + (live ? row : rows - 1)) * A.NB;
-  const int seen_blocks = A.pages.num_pages == 0 || last < 0 ? 0 : static_cast<int>(min(static_cast<uint32_t>(last) / A.B + 1, static_cast<uint32_t>(A.NB)));
+  const int seen_blocks = A.pages.num_pages == 0 || last < 0
+                              ? 0
+                              : static_cast<int>(min(static_cast<uint32_t>(last) / A.B + 1, static_cast<uint32_t>(A.NB)));
   const int stop = min(block1, seen_blocks);
   for (int b = max(block0, seen_blocks) + q4; b < fill; b += 4)
     if (live) out[b] = -__builtin_inff();
