@@ -9,16 +9,16 @@ equal). One launch (``msa_cache_append``); the caches are written in place.
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 
 from . import _lib
 from .norm_rope import check_table, check_weight
-from .paged import FP8, check_cache, check_kv_caches, check_pages, page_args, sixteen_bit, unit_rows
+from .paged import check_cache, check_kv_caches, check_pages, sixteen_bit, unit_rows
 
-_Strides = ctypes.c_int64 * 13
+_pack_strides = struct.Struct("13q").pack
 
 
 def m3_cache_append(
@@ -55,34 +55,35 @@ def m3_cache_append(
         raise ValueError("expected k and v [T,H,D] of one shape with H, D > 0")
     total, heads, dim = k.shape
     sixteen_bit(k, "m3_cache_append")
-    if v.dtype != k.dtype or v.device != k.device:
+    dtype, device = k.dtype, k.device
+    if v.dtype != dtype or v.device != device:
         raise ValueError("k and v must share dtype and device")
-    page, of_kv = check_kv_caches(k_cache, v_cache, k_scale, v_scale, heads, dim, k.dtype, k.device)
+    page, of_kv, fp8 = check_kv_caches(k_cache, v_cache, k_scale, v_scale, heads, dim, dtype, device)
     if (index_k is None) != (index_cache is None):
         raise ValueError("index_k and index_cache go together")
     index_dim, of_index = 0, (0, 0, 0)
     if index_k is not None:
-        if index_k.ndim != 3 or index_k.shape[:2] != (total, 1) or index_k.shape[2] < 1:
+        index_dim = index_k.shape[-1] if index_k.ndim else 0
+        if index_k.shape != (total, 1, index_dim) or index_dim < 1:
             raise ValueError("expected index_k [T,1,Di] with Di > 0")
-        if index_k.dtype != k.dtype or index_k.device != k.device:
+        if index_k.dtype != dtype or index_k.device != device:
             raise ValueError("index_k must share dtype and device with k")
-        index_dim = index_k.shape[2]
-        _, of_index = check_cache(index_cache, "index_cache", (k.dtype,), 1, index_dim, k.device)
+        _, of_index = check_cache(index_cache, "index_cache", (dtype,), 1, index_dim, device)
         if index_cache.shape[0] != k_cache.shape[0] or index_cache.shape[2] != page:
             raise ValueError("index_cache must have the pages of k_cache")
     weights = [w for w in (k_weight, index_weight) if w is not None]
     if k_weight is not None:
-        check_weight(k_weight, k, "k_weight")
+        check_weight(k_weight, "k_weight", dim, dtype, device)
     if index_weight is not None:
         if index_k is None:
             raise ValueError("index_weight without index_k")
-        check_weight(index_weight, index_k, "index_weight")
+        check_weight(index_weight, "index_weight", index_dim, dtype, device)
     if len(weights) == 2 and k_weight.dtype != index_weight.dtype:
         raise ValueError("k_weight and index_weight must share a dtype")
-    table, rows, rot = check_table(cos_sin, min(dim, index_dim) if index_k is not None else dim, k.device)
+    table, rows, rot = check_table(cos_sin, min(dim, index_dim) if index_k is not None else dim, device)
     if not (isinstance(eps, (int, float)) and math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be nonnegative and finite")
-    pages, cu, num_seqs, context = check_pages(page_table, cu_seqlens, context_lens, total, page, k.device)
+    pages, cu, num_seqs, context, page_map = check_pages(page_table, cu_seqlens, context_lens, total, page, k_cache, device)
     if dim % 16 or dim > 256 or index_dim % 16 or index_dim > 256:
         raise NotImplementedError("m3_cache_append takes head and index dims that are multiples of 16, up to 256")
     _lib.require_gpu(k, "m3_cache_append")
@@ -92,14 +93,14 @@ def m3_cache_append(
     ik = None if index_k is None else unit_rows(index_k)
     wk = None if k_weight is None else k_weight.contiguous()
     wi = None if index_weight is None else index_weight.contiguous()
-    strides = _Strides(*k.stride()[:2], *v.stride()[:2], 0 if ik is None else ik.stride(0), *of_kv, of_index[0],
-                       of_index[2])
-    dtype = _lib.DTYPE_CODE[k.dtype]
-    with _lib.on_device(k.device):
+    strides = _pack_strides(*k.stride()[:2], *v.stride()[:2], 0 if ik is None else ik.stride(0), *of_kv, of_index[0],
+                            of_index[2])
+    code = _lib.DTYPE_CODE[dtype]
+    with _lib.on_device(device):
         status = _lib.lib().msa_cache_append(
-            k.data_ptr(), v.data_ptr(), _lib.ptr(ik), dtype, heads, dim, index_dim, _lib.ptr(wk), _lib.ptr(wi),
-            _lib.DTYPE_CODE[weights[0].dtype] if weights else dtype, _lib.ptr(table), rows, rot, eps,
-            k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(index_cache), k_cache.dtype == FP8, _lib.ptr(k_scale),
-            _lib.ptr(v_scale), strides, *page_args(pages, k_cache), cu.data_ptr(), num_seqs, context.data_ptr(), total,
-            _lib.stream_of(k.device))
+            k.data_ptr(), v.data_ptr(), _lib.ptr(ik), code, heads, dim, index_dim, _lib.ptr(wk), _lib.ptr(wi),
+            _lib.DTYPE_CODE[weights[0].dtype] if weights else code, _lib.ptr(table), rows, rot, eps,
+            k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(index_cache), fp8, _lib.ptr(k_scale),
+            _lib.ptr(v_scale), strides, *page_map, cu.data_ptr(), num_seqs, context.data_ptr(), total,
+            _lib.stream_of(device))
     _lib.check(status, "msa_cache_append")

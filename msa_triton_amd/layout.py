@@ -211,8 +211,12 @@ def packed_tokens(cu_seqlens: torch.Tensor | PackedSequences, total_tokens: int,
     """``cu_seqlens`` of an operator that needs token bounds only (any block size): the checked device tensor and
     the number of sequences. A tensor is read on the host, ``PackedSequences`` are not."""
     if isinstance(cu_seqlens, PackedSequences):
-        prepared_for(cu_seqlens, block_size=cu_seqlens.block_size, total_tokens=total_tokens, device=device)
-        return cu_seqlens.cu_seqlens, cu_seqlens.meta.num_seqs
+        bounds, cu = cu_seqlens.meta.bounds, cu_seqlens.cu_seqlens
+        if bounds[-1] != total_tokens:
+            raise ValueError("cu_seqlens must start at zero and end at total_tokens")
+        if cu.device != device:
+            raise ValueError("prepared sequences must be on the input device")
+        return cu, len(bounds) - 1
     if not isinstance(cu_seqlens, torch.Tensor):
         raise TypeError("cu_seqlens must be a tensor or PackedSequences")
     lengths = sequence_lengths(cu_seqlens, total_tokens)

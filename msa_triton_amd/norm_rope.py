@@ -45,19 +45,21 @@ def check_table(cos_sin, head_dim, device):
     """The rotation table's checks: (contiguous table or None, rows, rotary dim)."""
     if cos_sin is None:
         return None, 0, 0
-    if cos_sin.ndim != 2 or cos_sin.dtype != torch.float32 or cos_sin.shape[1] % 2:
+    shape = cos_sin.shape
+    if len(shape) != 2 or cos_sin.dtype != torch.float32 or shape[1] % 2:
         raise ValueError("cos_sin must be fp32 [positions, rotary_dim] with an even rotary_dim")
-    if cos_sin.shape[1] > head_dim:
+    rows, rot = shape
+    if rot > head_dim:
         raise ValueError("rotary_dim must not exceed the head dimension")
     if cos_sin.device != device:
         raise ValueError("cos_sin must be on the input device")
-    return cos_sin.contiguous(), cos_sin.shape[0], cos_sin.shape[1]
+    return cos_sin.contiguous(), rows, rot
 
 
-def check_weight(weight, x, name):
-    if weight is None or weight.shape != x.shape[-1:] or weight.dtype not in (x.dtype, torch.float32):
+def check_weight(weight, name, dim, dtype, device):
+    if weight is None or weight.shape != (dim,) or (weight.dtype != dtype and weight.dtype != torch.float32):
         raise ValueError(f"{name} must be [head dim], of the input dtype or fp32")
-    if weight.device != x.device:
+    if weight.device != device:
         raise ValueError(f"{name} must be on the input device")
 
 
@@ -142,23 +144,24 @@ def _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens, eps, context_lens):
     total, heads, dim = q.shape
     if heads < 1 or dim < 1 or (k is not None and (k.shape[0] != total or k.shape[1] < 1 or k.shape[2] != dim)):
         raise ValueError("expected q[T,Hq,D] and k[T,Hkv,D] with positive heads and D")
-    if q.dtype not in _TYPES:
+    dtype, device = q.dtype, q.device
+    if dtype not in _TYPES:
         raise TypeError("q must have BF16, FP16, or FP32 dtype")
-    if k is not None and (k.dtype != q.dtype or k.device != q.device):
+    if k is not None and (k.dtype != dtype or k.device != device):
         raise ValueError("q and k must share dtype and device")
-    check_weight(q_weight, q, "q_weight")
+    check_weight(q_weight, "q_weight", dim, dtype, device)
     if k is None:
         if k_weight is not None:
             raise ValueError("k_weight without k")
     else:
-        check_weight(k_weight, k, "k_weight")
+        check_weight(k_weight, "k_weight", dim, dtype, device)
         if k_weight.dtype != q_weight.dtype:
             raise ValueError("q_weight and k_weight must share a dtype")
-    table, rows, rot = check_table(cos_sin, dim, q.device)
+    table, rows, rot = check_table(cos_sin, dim, device)
     if not (isinstance(eps, (int, float)) and math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be nonnegative and finite")
-    cu, num_seqs = packed_tokens(cu_seqlens, total, q.device)
-    context = context_of(context_lens, num_seqs, q.device)
+    cu, num_seqs = packed_tokens(cu_seqlens, total, device)
+    context = context_of(context_lens, num_seqs, device)
     if dim > MAX_HEAD_DIM:
         raise NotImplementedError(f"m3_qk_norm_rope takes head dims up to {MAX_HEAD_DIM}")
     _lib.require_gpu(q, "m3_qk_norm_rope")

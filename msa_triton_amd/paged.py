@@ -38,52 +38,54 @@ def check_cache(cache, name, dtypes, heads, dim, device):
     return page, (of_page, of_head, of_slot)
 
 
-def check_scale(scale, name, cache):
+def check_scale(scale, name, fp8, shape, device):
     """The scales [P, H] that go with an 8-bit cache (and only with one)."""
-    if cache.dtype != FP8:
+    if not fp8:
         if scale is not None:
             raise ValueError(f"{name} goes with an 8-bit cache")
         return
-    if scale is None or scale.dtype != torch.float32 or scale.shape != cache.shape[:2] or not scale.is_contiguous():
+    if scale is None or scale.dtype != torch.float32 or scale.shape != shape or not scale.is_contiguous():
         raise ValueError(f"{name} must be contiguous fp32 [pages, heads]")
-    if scale.device != cache.device:
+    if scale.device != device:
         raise ValueError(f"{name} must be on the cache's device")
 
 
 def check_kv_caches(k_cache, v_cache, k_scale, v_scale, heads, dim, dtype, device):
-    """The key and value caches of one layer: of the input type, or both in 8 bits. Returns the page size and the
-    strides of both."""
+    """The key and value caches of one layer: of the input type, or both in 8 bits. Returns the page size, the
+    strides of both and whether they hold 8 bits."""
     page, of_k = check_cache(k_cache, "k_cache", (dtype, FP8), heads, dim, device)
-    _, of_v = check_cache(v_cache, "v_cache", (k_cache.dtype,), heads, dim, device)
-    if k_cache.shape != v_cache.shape:
+    held = k_cache.dtype
+    _, of_v = check_cache(v_cache, "v_cache", (held,), heads, dim, device)
+    shape = k_cache.shape
+    if shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have one shape")
-    check_scale(k_scale, "k_scale", k_cache)
-    check_scale(v_scale, "v_scale", v_cache)
-    return page, of_k + of_v
+    fp8 = held == FP8
+    check_scale(k_scale, "k_scale", fp8, shape[:2], device)
+    check_scale(v_scale, "v_scale", fp8, shape[:2], device)
+    return page, of_k + of_v, fp8
 
 
-def check_pages(page_table, cu_seqlens, context_lens, total, page, device):
-    """The sequences of a paged call: (page table, cu_seqlens, sequences, context lengths), on the device."""
+def check_pages(page_table, cu_seqlens, context_lens, total, page, cache, device):
+    """The sequences of a paged call: the page table, cu_seqlens, the sequences, the context lengths (on the device), and
+    the page map's arguments of a C call."""
     cu, num_seqs = packed_tokens(cu_seqlens, total, device)
     if context_lens is None:
         raise TypeError("context_lens must be int32")
     context = context_of(context_lens, num_seqs, device)
     if not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32:
         raise TypeError("page_table must be int32")
-    if page_table.ndim != 2 or page_table.shape[0] != num_seqs:
+    shape = page_table.shape
+    if len(shape) != 2 or shape[0] != num_seqs:
         raise ValueError("page_table must be [sequences, pages]")
     if page_table.device != device:
         raise ValueError("page_table must be on the input device")
-    if page_table.shape[1] * page > 2147483647:
+    if shape[1] * page > 2147483647:
         raise ValueError("positions must fit int32 metadata")
-    if page_table.stride(1) != 1:
+    of_seq, of_page = page_table.stride()
+    if of_page != 1:
         page_table = page_table.contiguous()
-    return page_table, cu, num_seqs, context
-
-
-def page_args(page_table, cache):
-    """The page map's arguments of a C call."""
-    return page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cache.shape[0], cache.shape[2]
+        of_seq = page_table.stride(0)
+    return page_table, cu, num_seqs, context, (page_table.data_ptr(), of_seq, shape[1], cache.shape[0], page)
 
 
 def sixteen_bit(x, what):
@@ -95,5 +97,3 @@ def sixteen_bit(x, what):
 
 def unit_rows(x):
     return x if x.stride(-1) == 1 else x.contiguous()
-
-

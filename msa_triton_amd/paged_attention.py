@@ -10,15 +10,15 @@ gradients.
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 
 from . import _lib
-from .paged import FP8, check_kv_caches, check_pages, page_args, sixteen_bit
+from .paged import check_kv_caches, check_pages, sixteen_bit
 
-_Strides = ctypes.c_int64 * 6
+_pack_strides = struct.Struct("6q").pack
 
 
 def m3_sparse_attention_paged(
@@ -47,14 +47,15 @@ def m3_sparse_attention_paged(
         raise ValueError("expected q[T,Hq,D] with Hq, D > 0")
     total, heads, dim = q.shape
     sixteen_bit(q, "m3_sparse_attention_paged")
+    dtype, device = q.dtype, q.device
     if indices.ndim != 3 or indices.shape[0] != total or indices.shape[1] < 1 or indices.dtype != torch.int32:
         raise ValueError("indices must be int32 [T,G,K]")
-    groups, slots = indices.shape[1:]
+    _, groups, slots = indices.shape
     if heads % groups:
         raise ValueError("Hq must be a positive multiple of G")
-    if indices.device != q.device:
+    if indices.device != device:
         raise ValueError("indices must be on the input device")
-    page, strides = check_kv_caches(k_cache, v_cache, k_scale, v_scale, groups, dim, q.dtype, q.device)
+    page, strides, fp8 = check_kv_caches(k_cache, v_cache, k_scale, v_scale, groups, dim, dtype, device)
     if not isinstance(block_size, int) or block_size <= 0:
         raise ValueError("block_size must be a positive integer")
     if block_size > 2147483647:
@@ -62,7 +63,7 @@ def m3_sparse_attention_paged(
     effective_scale = dim ** -0.5 if scale is None else float(scale)
     if not math.isfinite(effective_scale):
         raise ValueError("scale must be finite")
-    pages, cu, num_seqs, context = check_pages(page_table, cu_seqlens, context_lens, total, page, q.device)
+    pages, cu, num_seqs, context, page_map = check_pages(page_table, cu_seqlens, context_lens, total, page, k_cache, device)
     if block_size % 16 or dim % 16 or dim > 256:
         raise NotImplementedError("m3_sparse_attention_paged takes block sizes and head dims that are multiples of 16, "
                                   "head dims up to 256")
@@ -71,16 +72,16 @@ def m3_sparse_attention_paged(
     if q.data_ptr() % 16:
         q = q.clone()
     out = torch.empty_like(q, requires_grad=False)
-    lse = torch.empty((total, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.empty((total, heads), dtype=torch.float32, device=device) if return_lse else None
     if total:
         lib = _lib.lib()
         size = lib.msa_attn_paged_workspace_bytes(total, heads, groups, dim, slots, block_size)
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        with _lib.on_device(q.device):
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        with _lib.on_device(device):
             status = lib.msa_attn_paged(
-                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.DTYPE_CODE[q.dtype], k_cache.dtype == FP8,
-                _lib.ptr(k_scale), _lib.ptr(v_scale), _Strides(*strides), indices.data_ptr(), *page_args(pages, k_cache),
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.DTYPE_CODE[dtype], fp8,
+                _lib.ptr(k_scale), _lib.ptr(v_scale), _pack_strides(*strides), indices.data_ptr(), *page_map,
                 cu.data_ptr(), num_seqs, context.data_ptr(), total, heads, groups, dim, slots, block_size,
-                effective_scale, _lib.ptr(workspace), size, out.data_ptr(), _lib.ptr(lse), _lib.stream_of(q.device))
+                effective_scale, _lib.ptr(workspace), size, out.data_ptr(), _lib.ptr(lse), _lib.stream_of(device))
         _lib.check(status, "msa_attn_paged")
     return (out, lse) if return_lse else out

@@ -14,7 +14,7 @@ import math
 import torch
 
 from . import _lib
-from .paged import check_cache, check_pages, page_args, sixteen_bit
+from .paged import check_cache, check_pages, sixteen_bit
 
 
 def m3_index_score_topk_paged(
@@ -41,7 +41,8 @@ def m3_index_score_topk_paged(
         raise ValueError("expected index_q[T,G,Di] with G, Di > 0")
     total, groups, dim = index_q.shape
     sixteen_bit(index_q, "m3_index_score_topk_paged")
-    page, strides = check_cache(index_cache, "index_cache", (index_q.dtype,), 1, dim, index_q.device)
+    dtype, device = index_q.dtype, index_q.device
+    page, strides = check_cache(index_cache, "index_cache", (dtype,), 1, dim, device)
     if not isinstance(block_size, int) or block_size <= 0:
         raise ValueError("block_size must be a positive integer")
     if not isinstance(max_seqlen, int) or max_seqlen <= 0:
@@ -54,7 +55,8 @@ def m3_index_score_topk_paged(
         raise ValueError("local_blocks must satisfy 0 <= local_blocks <= topk_blocks")
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    pages, cu, num_seqs, context = check_pages(page_table, cu_seqlens, context_lens, total, page, index_q.device)
+    pages, cu, num_seqs, context, page_map = check_pages(page_table, cu_seqlens, context_lens, total, page, index_cache,
+                                                         device)
     if block_size % 16 or dim % 8 or dim > 256:
         raise NotImplementedError(
             "m3_index_score_topk_paged takes blocks of a multiple of 16 keys and index dims of a multiple of 8 up to 256")
@@ -63,14 +65,14 @@ def m3_index_score_topk_paged(
     if q.data_ptr() % 16:
         q = q.clone()
     blocks = (max_seqlen + block_size - 1) // block_size
-    scores = torch.empty((total, groups, blocks), dtype=torch.float32, device=q.device)
-    indices = torch.empty((total, groups, topk_blocks), dtype=torch.int32, device=q.device)
+    scores = torch.empty((total, groups, blocks), dtype=torch.float32, device=device)
+    indices = torch.empty((total, groups, topk_blocks), dtype=torch.int32, device=device)
     if total:
-        with _lib.on_device(q.device):
+        with _lib.on_device(device):
             status = _lib.lib().msa_index_score_topk_paged(
-                q.data_ptr(), index_cache.data_ptr(), _lib.DTYPE_CODE[q.dtype], strides[0],
-                strides[2], *page_args(pages, index_cache), cu.data_ptr(), num_seqs, context.data_ptr(),
+                q.data_ptr(), index_cache.data_ptr(), _lib.DTYPE_CODE[dtype], strides[0],
+                strides[2], *page_map, cu.data_ptr(), num_seqs, context.data_ptr(),
                 total, groups, dim, blocks, block_size, scale, topk_blocks, local_blocks, scores.data_ptr(),
-                indices.data_ptr(), _lib.stream_of(q.device))
+                indices.data_ptr(), _lib.stream_of(device))
         _lib.check(status, "msa_index_score_topk_paged")
     return scores, indices
