@@ -42,7 +42,8 @@ def m3_sparse_attention_paged(
     behind the token and repeated ids count for nothing. Each contiguous group of ``Hq / G`` query heads shares a
     selection. 8-bit caches (``torch.float8_e4m3fn``) come with ``k_scale`` and ``v_scale`` (fp32 ``[P,G]``). Keys in
     missing pages do not exist; rows without keys, and those of an absent sequence (negative ``context_lens``),
-    give zero output and an LSE of -inf. ``block_size`` and ``D`` are multiples of 16, ``D`` at most 256."""
+    give zero output and an LSE of -inf. A value of a visible key that is not finite makes its rows NaN in that dim
+    (also an infinity, which enters as two terms). ``block_size`` and ``D`` are multiples of 16, ``D`` at most 256."""
     if q.ndim != 3 or q.shape[1] < 1 or q.shape[2] < 1:
         raise ValueError("expected q[T,Hq,D] with Hq, D > 0")
     total, heads, dim = q.shape
