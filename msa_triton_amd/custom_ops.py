@@ -50,6 +50,7 @@ from torch import Tensor
 
 from . import _lib
 from .cache_append import m3_cache_append as _eager_append
+from .derivatives import refuse_tangents
 from .index_score import _score_backward, _score_forward
 from .indexer_kl import _launch as _kl_launch
 from .layout import sequence_lengths, sequence_meta
@@ -472,6 +473,7 @@ def m3_indexer_kl(index_q, index_k, q, k, indices, cu_seqlens, max_seqlen, *, bl
 
 def m3_qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, *, eps=1e-6, context_lens=None):
     """``msa_triton_amd.m3_qk_norm_rope`` through the registered op."""
+    refuse_tangents("m3_qk_norm_rope", q, k, q_weight, k_weight)
     q_out, k_out = torch.ops.msa_mi355x.qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, context_lens,
                                                      float(eps))
     return q_out, None if k is None else k_out

@@ -19,6 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .derivatives import wanted
 from .layout import context_of, packed_tokens
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -190,7 +191,6 @@ def m3_qk_norm_rope(
     (slices of a fused projection are read in place). The index heads go through the same call."""
     q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps = _validate(q, k, q_weight, k_weight, cos_sin, cu_seqlens,
                                                                            eps, context_lens)
-    if torch.is_grad_enabled() and (q.requires_grad or wq.requires_grad or
-                                    (k is not None and (k.requires_grad or wk.requires_grad))):
+    if wanted(q, k, wq, wk):
         return _NormRope.apply(q, k, wq, wk, table, cu, context, (rows, rot, num_seqs), eps)
     return _forward(q, k, _call_args(q, k, wq, wk, table, rows, rot, cu, num_seqs, context, eps))

@@ -1,0 +1,45 @@
+"""No operator returns outputs whose derivative was asked for and silently left out. On the CPU, with C calls that do
+nothing: what is tested is the path that a call takes."""
+
+from __future__ import annotations
+
+import contextlib
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import msa_triton_amd as msa
+from msa_triton_amd import _lib, custom_ops
+
+
+class _Calls:
+    """Every C entry point: workspaces of 0 bytes, status 0."""
+
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+@pytest.fixture
+def no_kernels(monkeypatch):
+    monkeypatch.setattr(_lib, "lib", _Calls)
+    monkeypatch.setattr(_lib, "require_gpu", lambda tensor, what: None)
+    monkeypatch.setattr(_lib, "stream_of", lambda device: 0)
+    monkeypatch.setattr(_lib, "on_device", lambda device: contextlib.nullcontext())
+
+
+def _norm_inputs():
+    x = [torch.randn(3, 4, 16), torch.randn(3, 2, 16), torch.ones(16), torch.ones(16)]
+    return x, (msa.rope_table(8, 16), torch.tensor([0, 3], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("grad", (False, True))
+@pytest.mark.parametrize("ops", (msa, custom_ops), ids=("eager", "library"))
+def test_norm_in_forward_mode(ops, which, grad, no_kernels):
+    x, rest = _norm_inputs()
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        ops.m3_qk_norm_rope(*x, *rest)  # (no tangent: as outside)
+        x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            ops.m3_qk_norm_rope(*x, *rest)
