@@ -392,6 +392,7 @@ def m3_index_score(index_q, index_k, cu_seqlens, max_seqlen, *, block_size=128, 
         raise ValueError("max_seqlen must be a positive integer")
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
+    refuse_tangents("m3_index_score", index_q, index_k)
     save_state = torch.is_grad_enabled() and (index_q.requires_grad or index_k.requires_grad)
     scores, _ = torch.ops.msa_mi355x.index_score(index_q, index_k, cu_seqlens, max_seqlen, block_size,
                                                  float(scale), save_state)
@@ -434,6 +435,7 @@ def m3_sparse_attention(q, k, v, indices, cu_seqlens, max_seqlen, *, block_size=
     effective_scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if not math.isfinite(effective_scale):
         raise ValueError("scale must be finite.")
+    refuse_tangents("m3_sparse_attention", q, k, v)
     save_state = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     out, lse, _, _ = torch.ops.msa_mi355x.sparse_attention(q, k, v, indices, cu_seqlens, max_seqlen, block_size,
                                                            effective_scale, save_state)
@@ -463,6 +465,7 @@ def m3_indexer_kl(index_q, index_k, q, k, indices, cu_seqlens, max_seqlen, *, bl
     effective_scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if not math.isfinite(effective_scale) or not math.isfinite(index_scale):
         raise ValueError("scale and index_scale must be finite")
+    refuse_tangents("m3_indexer_kl", index_q, index_k)
     grad = torch.is_grad_enabled()
     loss, rows, _, _ = torch.ops.msa_mi355x.indexer_kl(index_q, index_k, q.detach(), k.detach(), indices, cu_seqlens,
                                                        max_seqlen, block_size, float(index_scale), effective_scale,

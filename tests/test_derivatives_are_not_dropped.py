@@ -43,3 +43,19 @@ def test_norm_in_forward_mode(ops, which, grad, no_kernels):
         x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
         with pytest.raises(NotImplementedError, match="jvp"):
             ops.m3_qk_norm_rope(*x, *rest)
+
+
+@pytest.mark.parametrize("name,which", [("score", 0), ("score", 1), ("attention", 0), ("attention", 1), ("attention", 2),
+                                        ("kl", 0), ("kl", 1)])
+def test_library_ops_in_forward_mode(name, which, no_kernels):
+    """The registered operators would run below autograd and leave the tangent out."""
+    cu, ids = torch.tensor([0, 3], dtype=torch.int32), torch.zeros(3, 2, 1, dtype=torch.int32)
+    q, k = torch.randn(3, 4, 16), torch.randn(3, 2, 16)
+    x = [q[:, :2], k[:, :1]] if name != "attention" else [q, k, k.clone()]
+    call = dict(score=lambda a, b: custom_ops.m3_index_score(a, b, cu, 3),
+                attention=lambda a, b, c: custom_ops.m3_sparse_attention(a, b, c, ids, cu, 3),
+                kl=lambda a, b: custom_ops.m3_indexer_kl(a, b, q, k, ids, cu, 3))[name]
+    with forward_ad.dual_level(), torch.no_grad():
+        x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            call(*x)
