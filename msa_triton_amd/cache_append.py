@@ -15,6 +15,7 @@ import struct
 import torch
 
 from . import _lib
+from .derivatives import refuse_gradients, wanted
 from .norm_rope import check_table, check_weight
 from .paged import check_cache, check_kv_caches, check_pages, sixteen_bit, unit_rows
 
@@ -50,7 +51,11 @@ def m3_cache_append(
 
     Tokens of missing pages (entries outside ``[0, P)``, or past the table) and of absent sequences
     (negative ``context_lens``) are left out. No two new tokens may share a slot; in 8 bits no two
-    sequences may append to one page. D and Di: multiples of 16 up to 256. No gradients."""
+    sequences may append to one page. D and Di: multiples of 16 up to 256. No gradients: the caches are
+    written outside the graph, so a call whose inputs require grad is refused in grad mode (``torch.no_grad()`` or
+    detached inputs)."""
+    if wanted(k, v, index_k, k_weight, index_weight, k_cache, v_cache, index_cache):
+        refuse_gradients("m3_cache_append", k, v, index_k, k_weight, index_weight, k_cache, v_cache, index_cache)
     if k.ndim != 3 or v.shape != k.shape or k.shape[1] < 1 or k.shape[2] < 1:
         raise ValueError("expected k and v [T,H,D] of one shape with H, D > 0")
     total, heads, dim = k.shape

@@ -50,7 +50,7 @@ from torch import Tensor
 
 from . import _lib
 from .cache_append import m3_cache_append as _eager_append
-from .derivatives import refuse_tangents
+from .derivatives import refuse_gradients, refuse_tangents
 from .index_score import _score_backward, _score_forward
 from .indexer_kl import _launch as _kl_launch
 from .layout import sequence_lengths, sequence_meta
@@ -485,6 +485,7 @@ def m3_qk_norm_rope(q, k, q_weight, k_weight, cos_sin, cu_seqlens, *, eps=1e-6, 
 def m3_cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, *, index_k=None, index_cache=None,
                     k_scale=None, v_scale=None, k_weight=None, index_weight=None, cos_sin=None, eps=1e-6):
     """``msa_triton_amd.m3_cache_append`` through the registered op."""
+    refuse_gradients("m3_cache_append", k, v, index_k, k_weight, index_weight, k_cache, v_cache, index_cache)
     torch.ops.msa_mi355x.cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens, index_k, index_cache,
                                       k_scale, v_scale, k_weight, index_weight, cos_sin, float(eps))
 
@@ -492,6 +493,7 @@ def m3_cache_append(k, v, k_cache, v_cache, page_table, cu_seqlens, context_lens
 def m3_index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, context_lens, max_seqlen, *, block_size=128,
                               scale=1.0, topk_blocks=16, local_blocks=1):
     """``msa_triton_amd.m3_index_score_topk_paged`` through the registered op."""
+    refuse_tangents("m3_index_score_topk_paged", index_q, index_cache)
     return torch.ops.msa_mi355x.index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, context_lens,
                                                        max_seqlen, block_size, float(scale), topk_blocks, local_blocks)
 
@@ -499,6 +501,7 @@ def m3_index_score_topk_paged(index_q, index_cache, page_table, cu_seqlens, cont
 def m3_sparse_attention_paged(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, *, block_size=128,
                               scale=None, k_scale=None, v_scale=None, return_lse=False):
     """``msa_triton_amd.m3_sparse_attention_paged`` through the registered op."""
+    refuse_tangents("m3_sparse_attention_paged", q, k_cache, v_cache, k_scale, v_scale)
     out, lse = torch.ops.msa_mi355x.sparse_attention_paged(
         q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, block_size,
         q.shape[-1] ** -0.5 if scale is None else float(scale), k_scale, v_scale)

@@ -5,7 +5,7 @@ group selected (``m3_index_score_topk_paged``), read from a 16-bit cache or an 8
 each page and head. One C call (``msa_attn_paged``: a launch that reads the selected keys and values, and, for
 few rows, a second one that joins the parts of a row). The new tokens are in the cache already
 (``m3_cache_append``). Made for the few tokens of a decoding step; a prompt goes through the packed operators. No
-gradients.
+gradients: differentiating the outputs raises.
 """
 
 from __future__ import annotations
@@ -16,6 +16,7 @@ import struct
 import torch
 
 from . import _lib
+from .derivatives import NoBackward, wanted
 from .paged import check_kv_caches, check_pages, sixteen_bit
 
 _pack_strides = struct.Struct("6q").pack
@@ -85,4 +86,6 @@ def m3_sparse_attention_paged(
                 cu.data_ptr(), num_seqs, context.data_ptr(), total, heads, groups, dim, slots, block_size,
                 effective_scale, _lib.ptr(workspace), size, out.data_ptr(), _lib.ptr(lse), _lib.stream_of(device))
         _lib.check(status, "msa_attn_paged")
+    if wanted(q, k_cache, v_cache, k_scale, v_scale):
+        out, lse = NoBackward.apply("m3_sparse_attention_paged", (out, lse), q, k_cache, v_cache, k_scale, v_scale)
     return (out, lse) if return_lse else out

@@ -4,7 +4,7 @@
 the same selection, with the keys in pages and the queries at positions behind ``context_lens`` cached
 tokens. One C call (``msa_index_score_topk_paged``: a score launch that reads each cached index key once for 16 query
 rows of its sequence, and the top-k launch). The new tokens' index keys are in the cache already
-(``m3_cache_append``). No gradients.
+(``m3_cache_append``). No gradients: differentiating the scores raises.
 """
 
 from __future__ import annotations
@@ -14,6 +14,7 @@ import math
 import torch
 
 from . import _lib
+from .derivatives import NoBackward, wanted
 from .paged import check_cache, check_pages, sixteen_bit
 
 
@@ -75,4 +76,6 @@ def m3_index_score_topk_paged(
                 total, groups, dim, blocks, block_size, scale, topk_blocks, local_blocks, scores.data_ptr(),
                 indices.data_ptr(), _lib.stream_of(device))
         _lib.check(status, "msa_index_score_topk_paged")
+    if wanted(index_q, index_cache):
+        return NoBackward.apply("m3_index_score_topk_paged", (scores, indices), index_q, index_cache)
     return scores, indices

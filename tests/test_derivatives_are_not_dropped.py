@@ -59,3 +59,52 @@ def test_library_ops_in_forward_mode(name, which, no_kernels):
         x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
         with pytest.raises(NotImplementedError, match="jvp"):
             call(*x)
+
+
+def _paged(name, ops):
+    """(tensors that may be differentiated, a call of them) of a paged operator."""
+    cu, ctx = torch.tensor([0, 3], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    table, ids = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(3, 2, 1, dtype=torch.int32)
+    kc, vc, ic = (torch.zeros(2, h, 16, 16, dtype=torch.bfloat16) for h in (2, 2, 1))
+    q, k, v, ik = (torch.ones(3, h, 16, dtype=torch.bfloat16) for h in (4, 2, 2, 1))
+    w = torch.ones(16, dtype=torch.bfloat16)
+    if name == "append":
+        return [k, v, ik, w, w.clone(), kc], lambda k, v, ik, wk, wi, kc: ops.m3_cache_append(
+            k, v, kc, vc, table, cu, ctx, index_k=ik, index_cache=ic, k_weight=wk, index_weight=wi)
+    if name == "score":
+        return [q[:, :2].clone(), ic], lambda iq, ic: ops.m3_index_score_topk_paged(iq, ic, table, cu, ctx, 16, topk_blocks=1)
+    return [q, kc, vc], lambda q, kc, vc: ops.m3_sparse_attention_paged(q, kc, vc, ids, table, cu, ctx, return_lse=True)
+
+
+PAGED = [(name, i) for name, n in (("append", 6), ("score", 2), ("attention", 3)) for i in range(n)]
+
+
+@pytest.mark.parametrize("name,which", PAGED)
+@pytest.mark.parametrize("ops", (msa, custom_ops), ids=("eager", "library"))
+def test_paged_operators_and_gradients(ops, name, which, no_kernels):
+    x, call = _paged(name, ops)
+    plain = call(*x)
+    assert name == "append" or not any(y.requires_grad for y in plain)
+    x[which].requires_grad_()
+    with torch.no_grad():
+        call(*x)
+    if name == "append":
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call(*x)
+        call(*(y.detach() for y in x))
+        return
+    outs = call(*x)
+    assert outs[0].requires_grad and [y.shape for y in outs] == [y.shape for y in plain]
+    with pytest.raises(RuntimeError, match="no gradients|no autograd formula"):
+        outs[0].float().sum().backward()
+
+
+@pytest.mark.parametrize("name,which", PAGED)
+@pytest.mark.parametrize("ops", (msa, custom_ops), ids=("eager", "library"))
+def test_paged_operators_in_forward_mode(ops, name, which, no_kernels):
+    x, call = _paged(name, ops)
+    with forward_ad.dual_level(), torch.no_grad():
+        call(*x)
+        x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            call(*x)
