@@ -50,6 +50,8 @@ struct PagedAttnArgs {
 };
 
 constexpr float kLn2 = 0.69314718055994531f;
+// The least maximum of keys that exist (all of their logits may be -inf); -inf stands for no key.
+constexpr float kLeastMax = -3.402823466e38f;
 
 // Eight e4m3 values as a fragment of bf16 (or fp16): exact.
 template <bool F16>
@@ -108,6 +110,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   const int64_t steps = pos < 0 ? 0 : static_cast<int64_t>(A.K) * per_block;
 
   float m = -__builtin_inff(), l = 0.f;  // of head c: the maximum over all quarters, the sum over this one
+  bool had_keys = false;                 // this wave
   f32x4 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
     count = __builtin_amdgcn_readfirstlane(count);
 
     // ---- this wave's steps
-    if (wave < count) load_step(wave);
+    if (wave < count) load_step(wave), had_keys = true;
     for (int e = wave; e < count; e += 4) {
       const int k_now = key0, a_now = p0, b_now = p1;
       f32x4 s[2];
@@ -272,7 +275,9 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
     __syncthreads();  // the list and the tiles are free again
   }
 
-  // ---- the four waves joined: maxima and sums, then the outputs through LDS
+  // ---- the four waves joined: maxima and sums, then the outputs through LDS. A part with keys enters also with a factor of
+  // 0, so that a value that is not finite counts wherever its key lies.
+  if (had_keys) m = fmaxf(m, kLeastMax);
   l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
   if (q4 == 0) wave_max[wave][c] = m, wave_sum[wave][c] = l;
@@ -296,14 +301,14 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   const bool whole = A.splits == 1;
   const float inv = (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f) / kUp;
   float* part = whole ? nullptr : A.part + ((item * A.splits + split) * 16 + row) * A.D;
-  const bool none = !whole && top == -__builtin_inff();  // (the joining launch does not look at it)
+  const bool none = !whole && top == -__builtin_inff();  // no keys: the joining launch does not look at it
   for (int d = 4 * col; d < A.D && !none; d += 64) {
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(vbuf[w]) + row * OS + d);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = f[w] == 0.f ? o[i] : fmaf(f[w], x[i], o[i]);
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(f[w], x[i], o[i]);
     }
     o *= inv;
     if (whole) {
@@ -343,6 +348,7 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedAttnArgs A) {
   const float weight = top_z == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(top_z - top);
   const float sum = wave_sum_f32(weight * sum_z);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const uint64_t written = __ballot(top_z != -__builtin_inff());  // (a split without keys wrote nothing)
   const float* part = A.part + (item * A.splits * 16 + row) * A.D;
   for (int d = 2 * lane; d < A.D; d += 128) {
     float o0 = 0.f, o1 = 0.f;
@@ -354,8 +360,9 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedAttnArgs A) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), z0 + i));
-        o0 = f == 0.f ? o0 : fmaf(f, x[i].x, o0);  // (a split without keys wrote nothing)
-        o1 = f == 0.f ? o1 : fmaf(f, x[i].y, o1);
+        const bool there = written >> (z0 + i) & 1u;
+        o0 = there ? fmaf(f, x[i].x, o0) : o0;
+        o1 = there ? fmaf(f, x[i].y, o1) : o1;
       }
     }
     reinterpret_cast<uint32_t*>(A.out)[(out_row * A.D + d) >> 1] =

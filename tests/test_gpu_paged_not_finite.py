@@ -1,0 +1,146 @@
+"""m3_sparse_attention_paged where queries, keys or values are not finite: against the formula in float64, at one
+workgroup a row and at several."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import msa_triton_amd as msa
+from msa_triton_amd import _lib
+from msa_triton_amd.paged import FP8
+from tests.helpers import cu_tensor
+
+PAGE, BLOCK, SLOTS, GROUPS, RATIO, DIM = 32, 64, 6, 2, 3, 64
+KEYS = BLOCK * SLOTS  # every key of a sequence is selected
+
+
+def _inputs(tokens, dtype, fp8, device, seed=5):
+    """One sequence of KEYS + tokens - 1 positions: its last `tokens` ones attend to all blocks in front."""
+    gen = torch.Generator().manual_seed(seed)
+    pages = -(-(KEYS + tokens) // PAGE)
+    x = dict(q=torch.randn(tokens, GROUPS * RATIO, DIM, generator=gen).to(dtype).to(device))
+    for name in ("k", "v"):
+        c = torch.randn(pages, GROUPS, PAGE, DIM, generator=gen).to(dtype)
+        x[name + "c"] = (c.float() * 16).clamp(-400, 400).to(FP8).to(device) if fp8 else c.to(device)
+        x[name + "s"] = torch.full((pages, GROUPS), 2.0 ** -4, device=device) if fp8 else None
+    x["table"] = torch.randperm(pages, generator=gen, dtype=torch.int32)[None].to(device)
+    x["ids"] = torch.arange(SLOTS, dtype=torch.int32, device=device).expand(tokens, GROUPS, SLOTS).contiguous()
+    x["cu"] = cu_tensor([tokens], device)
+    x["ctx"] = torch.tensor([KEYS - 1], dtype=torch.int32, device=device)
+    return x
+
+
+def _at(x, j):
+    """(page, slot) of position j."""
+    return int(x["table"][0, j // PAGE]), j % PAGE
+
+
+def _call(x):
+    return msa.m3_sparse_attention_paged(x["q"], x["kc"], x["vc"], x["ids"], x["table"], x["cu"], x["ctx"], block_size=BLOCK,
+                                         k_scale=x["ks"], v_scale=x["vs"], return_lse=True)
+
+
+def _rows(x, name):
+    """The sequence's KEYS first rows [G, KEYS, D] in float64."""
+    c, s = x[name + "c"].float().double().cpu(), x[name + "s"]
+    if s is not None:
+        c = c * s.double().cpu()[:, :, None, None]
+    return np.stack([c[_at(x, j)[0], :, _at(x, j)[1]].numpy() for j in range(KEYS)], 1)
+
+
+def _formula(x):
+    q = x["q"].double().cpu().numpy()
+    k, v = _rows(x, "k"), _rows(x, "v")
+    out, lse = np.zeros(q.shape), np.zeros(q.shape[:2])
+    with np.errstate(all="ignore"):
+        for t in range(q.shape[0]):
+            for h in range(q.shape[1]):
+                logit = k[h // RATIO] @ q[t, h] * DIM ** -0.5
+                m = logit.max()  # (NaN if one is)
+                w = np.exp(logit - m)
+                lse[t, h] = m + np.log(w.sum())
+                out[t, h] = (w[:, None] * v[h // RATIO]).sum(0) / w.sum()
+    return out, lse
+
+
+def _splits(tokens):
+    size = _lib.lib().msa_attn_paged_workspace_bytes(tokens, GROUPS * RATIO, GROUPS, DIM, SLOTS, BLOCK)
+    return "several" if size else "one"
+
+
+# tokens of a call whose rows one workgroup each takes, and of one with several a row
+WAYS = [(600, "one"), (2, "several")]
+TYPES = [(torch.bfloat16, False), (torch.float16, False), (torch.bfloat16, True)]
+
+
+def _compare(x, rows, exact=True):
+    """The rows given against the formula: NaN and infinities where it has them (`exact`; otherwise not finite there), the
+    rest as near as fp32 logits, two-term weights and one rounding give (2^-7 of the largest value covers all)."""
+    out, lse = (y.double().cpu().numpy() for y in _call(x))
+    few = dict(x, q=x["q"][rows])
+    want, want_lse = _formula(few)
+    out, lse = out[rows], lse[rows]
+    odd = ~np.isfinite(want)
+    if exact:
+        wrong = np.argwhere(odd & (out != want) & ~(np.isnan(out) & np.isnan(want)))
+        assert not len(wrong), wrong[:5].tolist()
+    wrong = np.argwhere(~np.isfinite(out) != odd)
+    assert not len(wrong), wrong[:5].tolist()
+    assert np.abs(out[~odd] - want[~odd]).max(initial=0.0) <= 2 ** -7 * 6
+    assert np.array_equal(np.isnan(lse), np.isnan(want_lse))
+    ok = np.isfinite(want_lse)
+    assert np.abs(lse[ok] - want_lse[ok]).max(initial=0.0) <= 2 ** -10
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,fp8", TYPES)
+@pytest.mark.parametrize("tokens,ways", WAYS)
+def test_nan_logits_give_nan(tokens, ways, dtype, fp8, device):
+    """A query with a NaN, and the rows that see a key with one: NaN, whichever wave or workgroup has the key (positions 0, 40
+    and 300 lie with different ones)."""
+    assert _splits(tokens) == ways
+    x = _inputs(tokens, dtype, fp8, device)
+    x["q"][1, 2, 7] = float("nan")
+    _compare(x, [0, 1])
+    for j in (0, 40, 300):
+        x = _inputs(tokens, dtype, fp8, device)
+        page, slot = _at(x, j)
+        x["kc"][page, 1, slot, 3] = float("nan")
+        _compare(x, [0, 1])
+    x["kc"][x["table"][0].long(), 0] = float("nan")  # nothing else in one group
+    _compare(x, [0, 1])
+
+
+def _one_key_takes_all(x, winner, j, minus_inf):
+    """The key at `winner` leaves the others weights of e^-250 or less (or e^-inf); the one at `j` has values that are not
+    finite in some dims."""
+    x["q"][..., 0] = 8.0
+    fp8 = x["ks"] is not None
+    if minus_inf:
+        x["kc"][..., 0] = -float("inf")
+    for g in range(GROUPS):
+        page, slot = _at(x, winner)
+        x["kc"][page, g, slot] = torch.zeros(DIM).to(x["kc"].dtype)
+        x["kc"][page, g, slot, 0] = 448.0 if fp8 else 300.0
+        if fp8:
+            x["ks"][page, g] = 2.0
+        page, slot = _at(x, j)
+        x["vc"][page, g, slot, 1] = float("nan" if fp8 else "inf")
+        x["vc"][page, g, slot, 17] = float("nan" if fp8 else "-inf")
+        x["vc"][page, g, slot, 40] = float("nan")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,fp8", TYPES)
+@pytest.mark.parametrize("tokens,ways", WAYS)
+@pytest.mark.parametrize("minus_inf", (False, True))
+def test_values_of_keys_without_weight(minus_inf, tokens, ways, dtype, fp8, device):
+    """They count wherever the key lies: what a row gives does not depend on which wave or workgroup has its step."""
+    if minus_inf and fp8:
+        pytest.skip("e4m3 has no infinity")
+    for j in (0, 33, 77, 150, 200, KEYS - 1):
+        x = _inputs(tokens, dtype, fp8, device)
+        _one_key_takes_all(x, 170, j, minus_inf)
+        _compare(x, [0, 1], exact=False)
