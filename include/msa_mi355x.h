@@ -309,7 +309,8 @@ int64_t msa_attn_paged_workspace_bytes(int64_t total_tokens, int64_t q_heads, in
  * e4m3 (cache_is_fp8) with fp32 scales [num_pages,G]; the new tokens' keys and values already in them. Attends to
  * the keys up to the token's position of the blocks in indices [T,G,K] (ids outside the sequence and a second
  * mention of a block are left out; so are keys of missing pages). out [T,Hq,D] in `dtype`, lse [T,Hq] (NULL: none) natural log;
- * rows without a key, and rows of a sequence with a negative context, get 0 and -inf. strides (host array,
+ * rows without a key, and rows of a sequence with a negative context, get 0 and -inf. An infinity in a visible key's value is
+ * the row's in that dim whatever the key's weight (NaN where both signs meet or its logit is -inf). strides (host array,
  * elements): k_cache page, head, slot; v_cache page, head, slot. head_dim: a multiple of 16 up to 256,
  * block_size a multiple of 16 (status 2 otherwise); cache rows and q 16-byte aligned. Deterministic. */
 int msa_attn_paged(const void* q, const void* k_cache, const void* v_cache, int32_t dtype, int32_t cache_is_fp8,

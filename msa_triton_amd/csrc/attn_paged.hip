@@ -64,6 +64,19 @@ __device__ __forceinline__ uint4 widen_fp8(uint32_t a, uint32_t b) {
   return make_uint4(two(a, false), two(a, true), two(b, false), two(b, true));
 }
 
+// Four values of a 16-bit or e4m3 row.
+template <int DT, bool FP8>
+__device__ __forceinline__ void load4(const char* p, float (&x)[4]) {
+  if constexpr (FP8) {
+    const int w = *reinterpret_cast<const int*>(p);
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1];
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    x[0] = lo16_f32<DT>(w.x), x[1] = hi16_f32<DT>(w.x), x[2] = lo16_f32<DT>(w.y), x[3] = hi16_f32<DT>(w.y);
+  }
+}
+
 template <int DT, bool FP8, int NK>
 __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kernel(PagedAttnArgs A) {
   constexpr int DP = 32 * NK, RS = DP + 16, ND = DP / 16;
@@ -276,7 +289,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   }
 
   // ---- the four waves joined: maxima and sums, then the outputs through LDS. A part with keys enters also with a factor of
-  // 0, so that a value that is not finite counts wherever its key lies.
+  // 0, and a dim that is not finite in any part is looked at again (odd_values).
   if (had_keys) m = fmaxf(m, kLeastMax);
   l += __shfl_xor(l, 16, kWave);
   l += __shfl_xor(l, 32, kWave);
@@ -298,18 +311,55 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   const int h = 16 * ht + row;
   if (h >= ratio) return;
   const int64_t out_row = t * A.Hq + g * ratio + h;
+  // The values of dims d .. d + 3 that are not finite, added up over this workgroup's keys; 0 where there are none. A weight is
+  // positive, so an infinity stays itself whatever its weight and NaN comes of both signs; under a logit of -inf (weight 0) it
+  // is NaN. The matrix product cannot tell: a weight's two terms are 0 or negative as well. Rare, so a thread reads all keys.
+  auto odd_values = [&](int d) {
+    f32x4 odd = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int64_t n = split; n < steps; n += A.splits) {
+      const int64_t slot = n / per_block;  // (repeated ids add nothing new)
+      const int id = ids[slot], step = static_cast<int>(n - slot * per_block);
+      for (int half = 0; half < 2; ++half) {
+        const int64_t first = static_cast<int64_t>(id) * A.B + 32 * step + 16 * half;
+        if (id < 0 || first > pos || 32 * step + 16 * half >= A.B) break;
+        const int64_t page = A.pages.page_of(at.seq, first);
+        if (page < 0) continue;
+        const int64_t slot0 = first & slot_mask;
+        const char* vp = vbase + (page * A.v.stride_page + slot0 * A.v.stride_slot + d) * ES;
+        const char* kp = kbase + (page * A.k.stride_page + slot0 * A.k.stride_slot) * ES;
+        const float vs = FP8 ? A.v_scale[page * A.G + g] : 1.f, ks = FP8 ? A.k_scale[page * A.G + g] : 1.f;
+        const int keys = static_cast<int>(min(pos - first, int64_t{15})) + 1;
+#pragma unroll 4
+        for (int r = 0; r < keys; ++r) {
+          float x[4];
+          load4<DT, FP8>(vp + r * A.v.stride_slot * ES, x);
+          bool some = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] *= vs, some |= !(fabsf(x[i]) < __builtin_inff());
+          if (!some) continue;
+          const uint16_t* qrow = A.q + (t * A.Hq + g * ratio + h) * A.D;
+          float dot = 0.f;
+          for (int e = 0; e < A.D; e += 4) {
+            float y[4], z[4];
+            load4<DT, false>(reinterpret_cast<const char*>(qrow + e), y);
+            load4<DT, FP8>(kp + (r * A.k.stride_slot + e) * ES, z);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot = fmaf(y[i], z[i], dot);
+          }
+          const bool none = dot * (A.scale_log2 * ks) == -__builtin_inff();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(fabsf(x[i]) < __builtin_inff())) odd[i] += none ? __builtin_nanf("") : x[i];
+        }
+      }
+    }
+    return odd;
+  };
   const bool whole = A.splits == 1;
   const float inv = (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f) / kUp;
   float* part = whole ? nullptr : A.part + ((item * A.splits + split) * 16 + row) * A.D;
   const bool none = !whole && top == -__builtin_inff();  // no keys: the joining launch does not look at it
-  for (int d = 4 * col; d < A.D && !none; d += 64) {
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(vbuf[w]) + row * OS + d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = fmaf(f[w], x[i], o[i]);
-    }
+  auto store = [&](int d, f32x4 o) {
     o *= inv;
     if (whole) {
       const uint2 r = DT == kF16 ? make_uint2(cvt_pk_f16(o[0], o[1]), cvt_pk_f16(o[2], o[3]))
@@ -318,6 +368,18 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
     } else {
       *reinterpret_cast<f32x4*>(part + d) = o;
     }
+  };
+  float all = 0.f;  // not finite if an output is not, or a part with a factor of 0
+  for (int d = 4 * col; d < A.D && !none; d += 64) {
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(vbuf[w]) + row * OS + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(f[w], x[i], o[i]);
+    }
+    all += (o[0] + o[1]) + (o[2] + o[3]);
+    store(d, o);
   }
   if (col == 0) {
     if (whole) {
@@ -328,6 +390,27 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
       st[16 + row] = sum;
     }
   }
+  if (__builtin_expect(fabsf(all) < __builtin_inff() || sum != sum, 1)) return;  // (a sum of NaN makes the row NaN)
+  for (int d = 4 * col; d < A.D && !none; d += 64) {
+    const f32x4 odd = odd_values(d);
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < 4; ++w) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(vbuf[w]) + row * OS + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = f[w] == 0.f ? o[i] : fmaf(f[w], x[i], o[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (odd[i] != 0.f) o[i] = odd[i];
+      else if (!whole && fabsf(o[i]) == __builtin_inff()) o[i] = copysignf(-kLeastMax, o[i]);  // (a sum past fp32's range)
+    }
+    store(d, o);
+  }
+}
+
+// o + f x, with x itself where it is not finite: such a value counts whatever its weight, also 0.
+__device__ __forceinline__ float add_part(float f, float x, float o) {
+  return fabsf(x) < __builtin_inff() ? fmaf(f, x, o) : o + x;
 }
 
 // The splits of a row joined, a wave for each head's row: lane z weighs split z (at most kMostSplits = 64), and
@@ -355,7 +438,7 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedAttnArgs A) {
     for (int z0 = 0; z0 < A.splits; z0 += 8) {
       float2 x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)  // (past the last split: that one again, with a weight of 0)
+      for (int i = 0; i < 8; ++i)  // (past the last split: that one again, as a split that wrote nothing)
         x[i] = *reinterpret_cast<const float2*>(part + static_cast<int64_t>(min(z0 + i, A.splits - 1)) * 16 * A.D + d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -363,6 +446,16 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedAttnArgs A) {
         const bool there = written >> (z0 + i) & 1u;
         o0 = there ? fmaf(f, x[i].x, o0) : o0;
         o1 = there ? fmaf(f, x[i].y, o1) : o1;
+      }
+    }
+    if (__builtin_expect(!(fabsf(o0 + o1) < __builtin_inff()), 0)) {
+      o0 = o1 = 0.f;
+      for (int z = 0; z < A.splits; ++z) {
+        if (!(written >> z & 1u)) continue;
+        const float2 x = *reinterpret_cast<const float2*>(part + static_cast<int64_t>(z) * 16 * A.D + d);
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), z));
+        o0 = add_part(f, x.x, o0);
+        o1 = add_part(f, x.y, o1);
       }
     }
     reinterpret_cast<uint32_t*>(A.out)[(out_row * A.D + d) >> 1] =

@@ -43,8 +43,9 @@ def m3_sparse_attention_paged(
     behind the token and repeated ids count for nothing. Each contiguous group of ``Hq / G`` query heads shares a
     selection. 8-bit caches (``torch.float8_e4m3fn``) come with ``k_scale`` and ``v_scale`` (fp32 ``[P,G]``). Keys in
     missing pages do not exist; rows without keys, and those of an absent sequence (negative ``context_lens``),
-    give zero output and an LSE of -inf. A value of a visible key that is not finite makes its rows NaN in that dim
-    (also an infinity, which enters as two terms). ``block_size`` and ``D`` are multiples of 16, ``D`` at most 256."""
+    give zero output and an LSE of -inf. Values that are not finite give what the formula gives: an
+    infinity in a visible key's value is the row's in that dim whatever the key's weight (NaN where both signs meet, or the
+    weight is 0, of a logit of -inf), a NaN is NaN. ``block_size`` and ``D`` are multiples of 16, ``D`` at most 256."""
     if q.ndim != 3 or q.shape[1] < 1 or q.shape[2] < 1:
         raise ValueError("expected q[T,Hq,D] with Hq, D > 0")
     total, heads, dim = q.shape

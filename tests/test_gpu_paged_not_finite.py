@@ -144,3 +144,68 @@ def test_values_of_keys_without_weight(minus_inf, tokens, ways, dtype, fp8, devi
         x = _inputs(tokens, dtype, fp8, device)
         _one_key_takes_all(x, 170, j, minus_inf)
         _compare(x, [0, 1], exact=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,fp8", TYPES)
+@pytest.mark.parametrize("tokens,ways", WAYS)
+@pytest.mark.parametrize("weights", ("usual", "none", "minus_inf"))
+def test_infinite_values_are_the_formulas(weights, tokens, ways, dtype, fp8, device):
+    """Infinities stay themselves beside finite values, NaN comes of both signs, of a NaN and under a logit of -inf; dims
+    without any are as ever."""
+    if weights == "minus_inf" and fp8:
+        pytest.skip("e4m3 has no infinity")
+    for j, other in ((0, 1), (33, 300), (200, 40), (KEYS - 1, 0)):
+        x = _inputs(tokens, dtype, fp8, device)
+        if weights != "usual":
+            _one_key_takes_all(x, 170, j, weights == "minus_inf")
+        if not fp8:
+            page, slot = _at(x, j)
+            x["vc"][page, 0, slot, 3:6] = torch.tensor([float("inf"), -float("inf"), float("inf")])
+            page, slot = _at(x, other)
+            x["vc"][page, 0, slot, 5:8] = torch.tensor([-float("inf"), float("nan"), float("inf")])
+            page, slot = _at(x, 170)
+            x["vc"][page, 1, slot, 63] = float("inf")  # (of the key with the weight, where one has it)
+            x["vc"][page, 1, slot, 62] = -float("inf")
+        else:
+            page, slot = _at(x, j)
+            x["vc"][page, 0, slot, 3] = float("nan")
+            x["vs"][_at(x, other)[0], 1] = float("inf")  # a scale is a factor like any other (0 x inf: NaN)
+        _compare(x, [0, 1])
+
+
+@pytest.mark.gpu
+def test_infinite_values_of_keys_not_seen(device):
+    """Behind a token, in blocks that it did not select, and in pages that are not there."""
+    x = _inputs(2, torch.bfloat16, False, device)
+    want = _call(x)
+    page, slot = _at(x, KEYS)  # the second token's own position: behind the first one, in a block no one selected
+    x["vc"][page, :, slot] = float("inf")
+    got = _call(x)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    x["vc"][_at(x, 100)[0], :, 5] = float("inf")
+    x["ids"][1] = torch.where(x["ids"][1] == 100 // BLOCK, -1, x["ids"][1])
+    got = _call(x)
+    assert torch.isinf(got[0][0]).all() and torch.isfinite(got[0][1]).all()
+    x["table"][0, 100 // PAGE] = -1
+    assert torch.isfinite(_call(x)[0]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_one_infinity_at_other_dims_and_head_counts(dtype, device):
+    """More head tiles than one, dims that fill no tile, steps of half a block."""
+    gen = torch.Generator().manual_seed(9)
+    dim, page, block, ratio, keys = 80, 16, 48, 20, 150
+    pages = 10
+    q = torch.randn(1, ratio, dim, generator=gen).to(dtype).to(device)
+    kc, vc = (torch.randn(pages, 1, page, dim, generator=gen).to(dtype).to(device) for _ in range(2))
+    table = torch.randperm(pages, generator=gen, dtype=torch.int32)[None].to(device)
+    vc[int(table[0, 3]), 0, 1, 77] = float("inf")  # position 49
+    vc[int(table[0, 9]), 0, 5, 2] = -float("inf")  # position 149, the token's own
+    ids = torch.tensor([[[3, 1, 0, 1]]], dtype=torch.int32, device=device)
+    out = msa.m3_sparse_attention_paged(q, kc, vc, ids, table, cu_tensor([1], device),
+                                        torch.tensor([keys - 1], dtype=torch.int32, device=device), block_size=block)
+    assert (out[:, :, 77] == float("inf")).all() and (out[:, :, 2] == -float("inf")).all()
+    out[:, :, 77] = out[:, :, 2] = 0
+    assert torch.isfinite(out).all()
