@@ -93,6 +93,34 @@ __device__ __forceinline__ void load_turn(const RopeTable& R, const PairChunk& p
   }
 }
 
+__device__ __forceinline__ float fused(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return fma(a, b, c); }
+
+// A pair chunk rotated in place, or back. Dims past rot stay as they are: a product with a sine of 0 would carry a value
+// that is not finite over to the dim beside it. (The multiply-adds are written out: every kernel gives the same bits.)
+template <int VEC, typename T>
+__device__ __forceinline__ void turn(const PairChunk& pc, const float (&co)[VEC], const float (&si)[VEC], T (&a)[VEC],
+                                     T (&b)[VEC]) {
+  if (!pc.turned) return;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const T u = a[j], v = b[j];
+    a[j] = fused(u, T(co[j]), -(v * si[j]));
+    b[j] = fused(u, T(si[j]), v * co[j]);
+  }
+}
+template <int VEC, typename T>
+__device__ __forceinline__ void turn_back(const PairChunk& pc, const float (&co)[VEC], const float (&si)[VEC], T (&a)[VEC],
+                                          T (&b)[VEC]) {
+  if (!pc.turned) return;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const T u = a[j], v = b[j];
+    a[j] = fused(u, T(co[j]), v * si[j]);
+    b[j] = fused(v, T(co[j]), -(u * si[j]));
+  }
+}
+
 template <int DT, int VEC, int C, int LPR>
 struct RowLanes {
   static constexpr int kRows = kNormThreads / LPR;  // rows a workgroup holds at once

@@ -89,11 +89,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_rope_fwd_kernel(NormArgs A)
     float co[VEC], si[VEC];
     load_turn<VEC>(A.rope, lanes.pc[c], p, co, si);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float ma = a[c][j] * r * lanes.wa[c][j], mb = b[c][j] * r * lanes.wb[c][j];
-      a[c][j] = ma * co[j] - mb * si[j];
-      b[c][j] = mb * co[j] + ma * si[j];
-    }
+    for (int j = 0; j < VEC; ++j) a[c][j] = a[c][j] * r * lanes.wa[c][j], b[c][j] = b[c][j] * r * lanes.wb[c][j];
+    turn<VEC>(lanes.pc[c], co, si, a[c], b[c]);
   }
   lanes.store(S.y, ((t0 + tok) * S.heads + head) * A.dim, a, b);
 }
@@ -149,10 +146,10 @@ __global__ __launch_bounds__(kNormThreads, DT == kF32 ? 3 : 4) void norm_rope_bw
     for (int c = 0; c < C; ++c) {
       float co[VEC], si[VEC];
       load_turn<VEC>(A.rope, lanes.pc[c], p, co, si);
+      turn_back<VEC>(lanes.pc[c], co, si, ga[c], gb[c]);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float dma = ga[c][j] * co[j] + gb[c][j] * si[j];
-        const float dmb = gb[c][j] * co[j] - ga[c][j] * si[j];
+        const float dma = ga[c][j], dmb = gb[c][j];
         a[c][j] *= r;  // n
         b[c][j] *= r;
         if (i < n) {
