@@ -273,8 +273,8 @@ int msa_qk_norm_rope_bwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
  * the new ones (its first new token at slot 0 starts it over); where it grows they are rounded again. What is not
  * finite becomes NaN. strides (host array, elements): k token, head; v token, head; index_k token; k_cache page,
  * head, slot; v_cache page, head, slot; index_cache page, slot; unit stride along D; cache rows 16-byte aligned.
- * head_dim and index_dim: multiples of 16 up to 256 (status 2 otherwise). No two new tokens may share a slot,
- * and in 8 bits no two sequences may append to one page. */
+ * head_dim and index_dim: multiples of 16 up to 256 (status 2 otherwise, and from 2^31 workgroups on: one for each page and
+ * head, or for 4 rows at least). No two new tokens may share a slot, and in 8 bits no two sequences may append to one page. */
 int msa_cache_append(const void* k, const void* v, const void* index_k, int32_t dtype, int64_t kv_heads,
                      int64_t head_dim, int64_t index_dim, const void* k_weight, const void* index_weight,
                      int32_t weight_dtype, const float* cos_sin, int64_t table_rows, int64_t rotary_dim,
@@ -290,8 +290,8 @@ int msa_cache_append(const void* k, const void* v, const void* index_k, int32_t 
  * keys already in it. Scores [T,G,num_blocks] are those of the packed entry point (the exact block maxima over
  * the keys up to the token's position; keys of missing pages do not exist), selections those of
  * msa_topk at that position (topk_blocks 0: indices unread). Rows of a sequence with a negative context get
- * scores of -inf and no block. index_dim: a multiple of 8 up to 256, block_size a multiple of 16 (status 2
- * otherwise); cache rows and index_q 16-byte aligned. */
+ * scores of -inf and no block. index_dim: a multiple of 8 up to 256, block_size a multiple of 16, total_tokens * groups
+ * below 2^28 (2^31 without a selection; status 2 otherwise); cache rows and index_q 16-byte aligned. */
 int msa_index_score_topk_paged(const void* index_q, const void* index_cache, int32_t dtype,
                                int64_t cache_stride_page, int64_t cache_stride_slot, const int32_t* page_table,
                                int64_t table_stride, int64_t pages_per_seq, int64_t num_pages, int64_t page_size,

@@ -42,6 +42,7 @@ struct PagedAttnArgs {
   int64_t tokens;
   int Hq, G, D, K, B;
   int head_tiles, splits;
+  int64_t first;     // item (joining launch: workgroup) of this launch's first workgroup
   float scale_log2;  // scale * log2(e)
   uint16_t* out;     // [T][Hq][D]
   float* lse;        // [T][Hq], or null
@@ -92,8 +93,8 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
   __shared__ int early_ids[kIds];
   const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t item = blockIdx.x / A.splits;
-  const int split = static_cast<int>(blockIdx.x % A.splits);
+  const int64_t item = A.first + blockIdx.x / static_cast<unsigned>(A.splits);
+  const int split = static_cast<int>(blockIdx.x % static_cast<unsigned>(A.splits));
   const int ht = static_cast<int>(item % A.head_tiles);
   const int64_t tg = item / A.head_tiles, t = tg / A.G;
   const int g = static_cast<int>(tg % A.G);
@@ -418,7 +419,7 @@ __device__ __forceinline__ float add_part(float f, float x, float o) {
 template <int DT>
 __global__ __launch_bounds__(256) void attn_paged_join(PagedAttnArgs A) {
   const int lane = threadIdx.x & 63;
-  const int64_t out_row = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t out_row = (A.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (out_row >= A.tokens * A.Hq) return;
   const int64_t t = out_row / A.Hq;
   const int ratio = A.Hq / A.G, hq = static_cast<int>(out_row - t * A.Hq), g = hq / ratio, h = hq - g * ratio;
@@ -537,9 +538,7 @@ extern "C" int msa_attn_paged(const void* q, const void* k_cache, const void* v_
   A.B = static_cast<int>(block_size);
   A.head_tiles = static_cast<int>(head_tiles_of(q_heads, kv_groups));
   const int64_t items = total_tokens * kv_groups * A.head_tiles;
-  if (items >= (int64_t{1} << 24)) return kErrUnsupported;  // 2^32 threads of a launch
   A.splits = static_cast<int>(split_count(items, topk_slots, block_size));
-  if (items * A.splits >= (int64_t{1} << 24)) return kErrUnsupported;
   A.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   A.out = static_cast<uint16_t*>(out);
   A.lse = lse;
@@ -551,8 +550,16 @@ extern "C" int msa_attn_paged(const void* q, const void* k_cache, const void* v_
     A.stats = A.part + items * A.splits * 16 * head_dim;
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(items * A.splits)), block(256);
-#define MSA_ATTN_PAGED(DT, F8, NK) hipLaunchKernelGGL((attn_paged_kernel<DT, F8, NK>), grid, block, 0, st, A)
+  const dim3 block(256);
+  int rc = kOk;
+#define MSA_ATTN_PAGED(DT, F8, NK)                                                                              \
+  rc = launch_parts(                                                                                            \
+      items,                                                                                                    \
+      [&](int64_t first, unsigned count) {                                                                      \
+        A.first = first;                                                                                        \
+        hipLaunchKernelGGL((attn_paged_kernel<DT, F8, NK>), dim3(count * A.splits), block, 0, st, A);           \
+      },                                                                                                        \
+      A.splits)
 #define MSA_ATTN_PAGED_DIM(DT, F8)                \
   if (head_dim <= 64) MSA_ATTN_PAGED(DT, F8, 2);  \
   else if (head_dim <= 128) MSA_ATTN_PAGED(DT, F8, 4); \
@@ -566,10 +573,10 @@ extern "C" int msa_attn_paged(const void* q, const void* k_cache, const void* v_
   }
 #undef MSA_ATTN_PAGED_DIM
 #undef MSA_ATTN_PAGED
-  const int rc = status_from(hipGetLastError());
   if (rc != kOk || A.splits == 1) return rc;
-  const dim3 rows(grid_1d(total_tokens * q_heads, 4));
-  if (dtype == kBF16) hipLaunchKernelGGL(attn_paged_join<kBF16>, rows, block, 0, st, A);
-  else hipLaunchKernelGGL(attn_paged_join<kF16>, rows, block, 0, st, A);
-  return status_from(hipGetLastError());
+  return launch_parts((total_tokens * q_heads + 3) / 4, [&](int64_t first, unsigned count) {
+    A.first = first;
+    if (dtype == kBF16) hipLaunchKernelGGL(attn_paged_join<kBF16>, dim3(count), block, 0, st, A);
+    else hipLaunchKernelGGL(attn_paged_join<kF16>, dim3(count), block, 0, st, A);
+  });
 }

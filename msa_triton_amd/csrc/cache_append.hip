@@ -39,8 +39,9 @@ struct AppendSide {
 
 struct AppendArgs {
   AppendSide side[3];  // keys, values, index keys
-  int first[3];        // first workgroup of a side's rows
-  int page_blocks;     // workgroups of 8-bit pages, in front
+  uint32_t launch;       // workgroup of this launch's first one
+  uint32_t first[3];     // first workgroup of a side's rows
+  uint32_t page_blocks;  // workgroups of 8-bit pages, in front
   bool w_f32;
   RopeTable rope;
   PageMap pages;
@@ -415,12 +416,12 @@ __device__ void append_rows(const AppendArgs& A, const AppendSide& S, int64_t r0
 template <int DT, bool FP8, int VEC, int C, int LPR>
 __global__ __launch_bounds__(kNormThreads, FP8 ? 3 : 4) void cache_append_kernel(AppendArgs A) {
   __shared__ int2 place[kNormThreads / LPR + 1];
-  const int block = static_cast<int>(blockIdx.x);
+  const uint32_t block = A.launch + blockIdx.x;
   if constexpr (FP8) {
     __shared__ float lds[3 * kNormThreads / kWave];
     if (block < A.page_blocks) {
-      const int per_unit = A.side[0].heads + A.side[1].heads;
-      const int64_t unit = block / per_unit;
+      const uint32_t per_unit = A.side[0].heads + A.side[1].heads;
+      const uint32_t unit = block / per_unit;
       // (the heads turn with the page: eight in a row go to the eight XCDs, and keys cost more than values)
       const int which = static_cast<int>((block + unit) % per_unit), second = which >= A.side[0].heads;
       append_page<DT, VEC, C, LPR>(A, A.side[second], unit, which - (second ? A.side[0].heads : 0), lds);
@@ -436,21 +437,22 @@ int append_launch(AppendArgs A, bool vectors, hipStream_t st) {
   int chunks = 0;
   for (const AppendSide& s : A.side)
     if (s.heads && s.dim / 16 > chunks) chunks = s.dim / 16;
-  auto go = [&](auto kernel, int rows) {
+  auto go = [&](auto kernel, int rows) -> int {
     int64_t blocks = 0;
     if (FP8) {
       const int64_t units = (A.tokens >> A.pages.shift) + 2 * static_cast<int64_t>(A.nseq);
       blocks = units * (A.side[0].heads + A.side[1].heads);
-      if (blocks >= (int64_t{1} << 24)) return static_cast<int>(kErrUnsupported);
-      A.page_blocks = static_cast<int>(blocks);
+      A.page_blocks = static_cast<uint32_t>(blocks);
     }
     for (int i = 0; i < 3; ++i) {
-      A.first[i] = static_cast<int>(blocks);
+      A.first[i] = static_cast<uint32_t>(blocks);
       if (!FP8 || i == 2) blocks += (A.tokens * A.side[i].heads + rows - 1) / rows;
-      if (blocks >= (int64_t{1} << 24)) return static_cast<int>(kErrUnsupported);  // 2^32 threads of a launch
     }
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kNormThreads), 0, st, A);
-    return static_cast<int>(status_from(hipGetLastError()));
+    if (blocks >> 31) return static_cast<int>(kErrUnsupported);  // (inputs or caches of that many pass the memory)
+    return launch_parts(blocks, [&](int64_t first, unsigned count) {
+      A.launch = static_cast<uint32_t>(first);
+      hipLaunchKernelGGL(kernel, dim3(count), dim3(kNormThreads), 0, st, A);
+    });
   };
 #define MSA_APPEND(VEC, C, LPR) return go(cache_append_kernel<DT, FP8, VEC, C, LPR>, kNormThreads / LPR)
   if (!vectors) MSA_APPEND(1, 2, 64);

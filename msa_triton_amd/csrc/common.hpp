@@ -172,6 +172,19 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 
 inline int status_from(hipError_t e) { return e == hipSuccess ? kOk : kErrLaunch; }
 
+// A launch holds fewer than 2^32 threads: `units` of `per_unit` workgroups of up to 256 threads as launches of at most 2^23
+// workgroups, in order, each launch(first unit, number of units).
+template <class Launch>
+int launch_parts(int64_t units, Launch launch, int64_t per_unit = 1) {
+  const int64_t most = (int64_t{1} << 23) / per_unit;
+  for (int64_t first = 0; first < units; first += most) {
+    launch(first, static_cast<unsigned>(units - first < most ? units - first : most));
+    const int rc = status_from(hipGetLastError());
+    if (rc != kOk) return rc;
+  }
+  return kOk;
+}
+
 inline unsigned grid_1d(int64_t work, int per_block) {
   int64_t g = (work + per_block - 1) / per_block;
   return static_cast<unsigned>(g < 1 ? 1 : g);

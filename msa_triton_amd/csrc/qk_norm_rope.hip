@@ -38,7 +38,8 @@ struct NormSide {
 
 struct NormArgs {
   NormSide side[2];
-  int q_blocks;        // workgroups of side 0
+  int64_t first;       // workgroup of this launch's first one
+  int64_t q_blocks;    // workgroups of side 0
   int rows_per_block;
   bool w_f32;
   RopeTable rope;
@@ -67,9 +68,10 @@ template <int DT, int VEC, int C, int LPR>
 __global__ __launch_bounds__(kNormThreads) void norm_rope_fwd_kernel(NormArgs A) {
   using Lanes = RowLanes<DT, VEC, C, LPR>;
   __shared__ int32_t pos[Lanes::kRows + 1];
-  const bool second = static_cast<int>(blockIdx.x) >= A.q_blocks;
+  const int64_t at = A.first + blockIdx.x;
+  const bool second = at >= A.q_blocks;
   const NormSide& S = A.side[second];
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x - (second ? A.q_blocks : 0)) * Lanes::kRows;
+  const int64_t r0 = (at - (second ? A.q_blocks : 0)) * Lanes::kRows;
   const int64_t rows = A.tokens * S.heads, t0 = r0 / S.heads;
   const int h0 = static_cast<int>(r0 - t0 * S.heads);
   const int n = static_cast<int>(min(rows - r0, static_cast<int64_t>(Lanes::kRows)));
@@ -102,9 +104,10 @@ __global__ __launch_bounds__(kNormThreads, DT == kF32 ? 3 : 4) void norm_rope_bw
   using Lanes = RowLanes<DT, VEC, C, LPR>;
   __shared__ int32_t pos[kMostTokens + 1];
   __shared__ float sums[kNormThreads / kWave][kMostDim];
-  const bool second = static_cast<int>(blockIdx.x) >= A.q_blocks;
+  const int64_t at = A.first + blockIdx.x;
+  const bool second = at >= A.q_blocks;
   const NormSide& S = A.side[second];
-  const int64_t block = blockIdx.x - (second ? A.q_blocks : 0);
+  const int64_t block = at - (second ? A.q_blocks : 0);
   const int64_t r0 = block * A.rows_per_block;
   const int64_t rows = A.tokens * S.heads, t0 = r0 / S.heads;
   const int h0 = static_cast<int>(r0 - t0 * S.heads);
@@ -245,13 +248,14 @@ bool side_fits_vectors(const NormSide& s, int esize, bool w_f32, int dim) {
 template <int DT, bool BWD>
 int norm_launch(NormArgs A, bool vectors, int64_t q_rows, int64_t k_rows, hipStream_t st) {
   const int chunks = A.rope.half / 8 + (A.dim - 2 * A.rope.half) / 16;
-  auto go = [&](auto kernel, int rows) {
+  auto go = [&](auto kernel, int rows) -> int {
     if (BWD) rows = A.rows_per_block;
     const int64_t nq = (q_rows + rows - 1) / rows, nk = (k_rows + rows - 1) / rows;
-    if (nq + nk >= (int64_t{1} << 24)) return static_cast<int>(kErrUnsupported);  // 2^32 threads of a launch
-    A.q_blocks = static_cast<int>(nq);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(nq + nk)), dim3(kNormThreads), 0, st, A);
-    return static_cast<int>(status_from(hipGetLastError()));
+    A.q_blocks = nq;
+    return launch_parts(nq + nk, [&](int64_t first, unsigned count) {
+      A.first = first;
+      hipLaunchKernelGGL(kernel, dim3(count), dim3(kNormThreads), 0, st, A);
+    });
   };
 #define MSA_NORM(VEC, C, LPR)                                                 \
   if constexpr (BWD) return go(norm_rope_bwd_kernel<DT, VEC, C, LPR>, 0);     \

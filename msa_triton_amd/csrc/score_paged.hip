@@ -355,7 +355,10 @@ extern "C" int msa_index_score_topk_paged(const void* index_q, const void* index
   if (reinterpret_cast<uintptr_t>(index_cache) % 16 || reinterpret_cast<uintptr_t>(index_q) % 16 ||
       cache_stride_page % 8 || cache_stride_slot % 8)
     return kErrInvalidArgument;
-  if (index_dim % 8 || index_dim > 256 || block_size % 16 || total_tokens * groups > 0x7fffffff) return kErrUnsupported;
+  // (a selection's launch takes 16 rows a workgroup, of fewer than 2^24)
+  if (index_dim % 8 || index_dim > 256 || block_size % 16 || total_tokens * groups > 0x7fffffff ||
+      (topk_blocks > 0 && total_tokens * groups >= int64_t{1} << 28))
+    return kErrUnsupported;
   if (total_tokens == 0) return kOk;
   PagedScoreArgs A{};
   A.iq = static_cast<const uint16_t*>(index_q);

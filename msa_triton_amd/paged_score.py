@@ -37,7 +37,7 @@ def m3_index_score_topk_paged(
     ``m3_index_score_topk`` gives them for the whole sequences; ``max_seqlen`` bounds a sequence with its new tokens
     (blocks behind it are neither scored nor selected). Keys in missing pages do not exist; rows of an absent
     sequence (negative ``context_lens``) get -inf and -1. ``block_size`` is a multiple of 16, ``Di`` a multiple
-    of 8 up to 256. Inputs must be finite."""
+    of 8 up to 256, ``T * G`` below 2^28 (2^31 without a selection). Inputs must be finite."""
     if index_q.ndim != 3 or index_q.shape[1] < 1 or index_q.shape[2] < 1:
         raise ValueError("expected index_q[T,G,Di] with G, Di > 0")
     total, groups, dim = index_q.shape
