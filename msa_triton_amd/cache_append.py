@@ -15,11 +15,12 @@ import struct
 import torch
 
 from . import _lib
-from .derivatives import refuse_gradients, wanted
+from .derivatives import forward_mode, refuse_gradients
 from .norm_rope import check_table, check_weight
 from .paged import check_cache, check_kv_caches, check_pages, sixteen_bit, unit_rows
 
 _pack_strides = struct.Struct("13q").pack
+_increment_version = torch.autograd.graph.increment_version
 
 
 def m3_cache_append(
@@ -54,7 +55,9 @@ def m3_cache_append(
     sequences may append to one page. D and Di: multiples of 16 up to 256. No gradients: the caches are
     written outside the graph, so a call whose inputs require grad is refused in grad mode (``torch.no_grad()`` or
     detached inputs)."""
-    if wanted(k, v, index_k, k_weight, index_weight, k_cache, v_cache, index_cache):
+    if (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad or forward_mode() or
+            (index_k is not None and (index_k.requires_grad or index_cache is not None and index_cache.requires_grad)) or
+            (k_weight is not None and k_weight.requires_grad) or (index_weight is not None and index_weight.requires_grad)):
         refuse_gradients("m3_cache_append", k, v, index_k, k_weight, index_weight, k_cache, v_cache, index_cache)
     if k.ndim != 3 or v.shape != k.shape or k.shape[1] < 1 or k.shape[2] < 1:
         raise ValueError("expected k and v [T,H,D] of one shape with H, D > 0")
@@ -76,15 +79,17 @@ def m3_cache_append(
         _, of_index = check_cache(index_cache, "index_cache", (dtype,), 1, index_dim, device)
         if index_cache.shape[0] != k_cache.shape[0] or index_cache.shape[2] != page:
             raise ValueError("index_cache must have the pages of k_cache")
-    weights = [w for w in (k_weight, index_weight) if w is not None]
+    weight_type = dtype
     if k_weight is not None:
         check_weight(k_weight, "k_weight", dim, dtype, device)
+        weight_type = k_weight.dtype
     if index_weight is not None:
         if index_k is None:
             raise ValueError("index_weight without index_k")
         check_weight(index_weight, "index_weight", index_dim, dtype, device)
-    if len(weights) == 2 and k_weight.dtype != index_weight.dtype:
-        raise ValueError("k_weight and index_weight must share a dtype")
+        if k_weight is not None and weight_type != index_weight.dtype:
+            raise ValueError("k_weight and index_weight must share a dtype")
+        weight_type = index_weight.dtype
     table, rows, rot = check_table(cos_sin, min(dim, index_dim) if index_k is not None else dim, device)
     if not (isinstance(eps, (int, float)) and math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be nonnegative and finite")
@@ -94,18 +99,34 @@ def m3_cache_append(
     _lib.require_gpu(k, "m3_cache_append")
     if not total:
         return
-    k, v = unit_rows(k), unit_rows(v)
-    ik = None if index_k is None else unit_rows(index_k)
-    wk = None if k_weight is None else k_weight.contiguous()
-    wi = None if index_weight is None else index_weight.contiguous()
-    strides = _pack_strides(*k.stride()[:2], *v.stride()[:2], 0 if ik is None else ik.stride(0), *of_kv, of_index[0],
+    k, of_new_k = unit_rows(k)
+    v, of_new_v = unit_rows(v)
+    written = [k_cache, v_cache]
+    at_ik = at_ic = at_ks = at_vs = at_wk = at_wi = at_table = None
+    of_new_index = 0
+    if index_k is not None:
+        ik, (of_new_index, _, _) = unit_rows(index_k)
+        at_ik, at_ic = ik.data_ptr(), index_cache.data_ptr()
+        written.append(index_cache)
+    if fp8:
+        at_ks, at_vs = k_scale.data_ptr(), v_scale.data_ptr()
+        written += (k_scale, v_scale)
+    if k_weight is not None:
+        wk = k_weight.contiguous()
+        at_wk = wk.data_ptr()
+    if index_weight is not None:
+        wi = index_weight.contiguous()
+        at_wi = wi.data_ptr()
+    if table is not None:
+        at_table = table.data_ptr()
+    strides = _pack_strides(of_new_k[0], of_new_k[1], of_new_v[0], of_new_v[1], of_new_index, *of_kv, of_index[0],
                             of_index[2])
-    code = _lib.DTYPE_CODE[dtype]
+    codes = _lib.DTYPE_CODE
     with _lib.on_device(device):
         status = _lib.lib().msa_cache_append(
-            k.data_ptr(), v.data_ptr(), _lib.ptr(ik), code, heads, dim, index_dim, _lib.ptr(wk), _lib.ptr(wi),
-            _lib.DTYPE_CODE[weights[0].dtype] if weights else code, _lib.ptr(table), rows, rot, eps,
-            k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(index_cache), fp8, _lib.ptr(k_scale),
-            _lib.ptr(v_scale), strides, *page_map, cu.data_ptr(), num_seqs, context.data_ptr(), total,
-            _lib.stream_of(device))
+            k.data_ptr(), v.data_ptr(), at_ik, codes[dtype], heads, dim, index_dim, at_wk, at_wi, codes[weight_type],
+            at_table, rows, rot, eps, k_cache.data_ptr(), v_cache.data_ptr(), at_ic, fp8, at_ks, at_vs, strides, *page_map,
+            cu.data_ptr(), num_seqs, context.data_ptr(), total, _lib.stream_of(device))
     _lib.check(status, "msa_cache_append")
+    # (a backward pass that saved a cache before this write has to notice it, as after torch's own in-place operators)
+    _increment_version(written)

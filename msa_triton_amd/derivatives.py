@@ -7,6 +7,9 @@ import torch
 from torch.autograd import forward_ad
 
 
+_grad_enabled = torch.is_grad_enabled
+
+
 def forward_mode() -> bool:
     """Inside ``forward_ad.dual_level``: a tensor may carry a tangent, which ``requires_grad`` does not tell and grad
     mode does not stop. (Nowhere else has one a tangent.)"""
@@ -16,13 +19,10 @@ def forward_mode() -> bool:
 def wanted(*tensors: torch.Tensor | None) -> bool:
     """Whether the call goes through its autograd function: a gradient will be asked for, or a tangent may be there
     (the functions have no forward-mode rule and raise at one)."""
-    if forward_ad._current_level >= 0:
-        return True
-    if torch.is_grad_enabled():
-        for x in tensors:
-            if x is not None and x.requires_grad:
-                return True
-    return False
+    for x in tensors:
+        if x is not None and x.requires_grad:
+            return _grad_enabled() or forward_ad._current_level >= 0
+    return forward_ad._current_level >= 0
 
 
 def _has_tangent(x: torch.Tensor) -> bool:

@@ -96,4 +96,9 @@ def sixteen_bit(x, what):
 
 
 def unit_rows(x):
-    return x if x.stride(-1) == 1 else x.contiguous()
+    """A rank-3 tensor with unit stride along its rows, and its strides."""
+    strides = x.stride()
+    if strides[2] == 1:
+        return x, strides
+    x = x.contiguous()
+    return x, x.stride()

@@ -83,10 +83,12 @@ def m3_sparse_attention_paged(
         with _lib.on_device(device):
             status = lib.msa_attn_paged(
                 q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.DTYPE_CODE[dtype], fp8,
-                _lib.ptr(k_scale), _lib.ptr(v_scale), _pack_strides(*strides), indices.data_ptr(), *page_map,
+                k_scale.data_ptr() if fp8 else None, v_scale.data_ptr() if fp8 else None, _pack_strides(*strides),
+                indices.data_ptr(), *page_map,
                 cu.data_ptr(), num_seqs, context.data_ptr(), total, heads, groups, dim, slots, block_size,
-                effective_scale, _lib.ptr(workspace), size, out.data_ptr(), _lib.ptr(lse), _lib.stream_of(device))
+                effective_scale, workspace.data_ptr() if size else None, size, out.data_ptr(),
+                lse.data_ptr() if return_lse else None, _lib.stream_of(device))
         _lib.check(status, "msa_attn_paged")
-    if wanted(q, k_cache, v_cache, k_scale, v_scale):
+    if wanted(q, k_cache, v_cache) or fp8 and wanted(k_scale, v_scale):
         out, lse = NoBackward.apply("m3_sparse_attention_paged", (out, lse), q, k_cache, v_cache, k_scale, v_scale)
     return (out, lse) if return_lse else out

@@ -108,3 +108,24 @@ def test_paged_operators_in_forward_mode(ops, name, which, no_kernels):
         x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
         with pytest.raises(NotImplementedError, match="jvp"):
             call(*x)
+
+
+@pytest.mark.parametrize("ops", (msa, custom_ops), ids=("eager", "library"))
+def test_a_backward_pass_notices_an_append(ops, no_kernels):
+    """Caches and scales that a graph has saved and an append then wrote."""
+    cu, ctx = torch.tensor([0, 1], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    table = torch.zeros(1, 2, dtype=torch.int32)
+    k, ik = torch.ones(1, 2, 16, dtype=torch.bfloat16), torch.ones(1, 1, 16, dtype=torch.bfloat16)
+    kc, vc = (torch.zeros(2, 2, 16, 16, dtype=torch.bfloat16).to(torch.float8_e4m3fn) for _ in range(2))
+    ic, ks, vs = torch.zeros(2, 1, 16, 16, dtype=torch.bfloat16), torch.ones(2, 2), torch.ones(2, 2)
+    q = torch.ones(16, dtype=torch.bfloat16, requires_grad=True)
+    uses = [(q * ic).sum(), (q[:2] * ks).sum(), (q[:2] * vs).sum()]
+    before = [x._version for x in (kc, vc)]
+    ops.m3_cache_append(k, k, kc, vc, table, cu, ctx, index_k=ik, index_cache=ic, k_scale=ks, v_scale=vs)
+    for y in uses:
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.backward()
+    assert all(x._version > b for x, b in zip((kc, vc), before))
+    with torch.inference_mode():
+        ops.m3_cache_append(k, k, kc.clone(), vc.clone(), table, cu, ctx, index_k=ik, index_cache=ic.clone(), k_scale=ks.clone(),
+                            v_scale=vs.clone())
