@@ -18,8 +18,8 @@
 // numbered without a list of them: sequence s gets the numbers from cu[s] / page + 2 s on, which leaves room for the two pages that n tokens can
 // touch beyond n / page; numbers without a page end at once.
 //
-// 16 bits: bound by memory (16 272 tokens, 4 heads of 128 and an index head: 19 us, 4.1 TB/s). 8 bits: by the vector work of
-// norm, rotation and two roundings (19 700 tokens: 34 us, 2.4 TB/s), and for single tokens by its chain of loads,
+// 16 bits: bound by memory (16 272 tokens, 4 heads of 128 and an index head: 20 us, 4.0 TB/s). 8 bits: by the vector work of
+// norm, rotation and two roundings (19 700 tokens: 36 us, 2.3 TB/s), and for single tokens by its chain of loads,
 // sequence, page, scale (64 tokens: 11 us).
 #include "norm_rope.hpp"
 #include "paged.hpp"

@@ -63,7 +63,7 @@ __device__ __forceinline__ void load_positions(const NormArgs& A, int64_t t0, in
 }
 
 // One row a lane run: with many workgroups a CU more rows in flight each only cost registers (32K tokens x 36 heads of 128,
-// bf16: 122 us, 4.9 TB/s; 136 and 152 with two and four).
+// bf16: 132 us, 4.6 TB/s; two and four rows took 11 and 25 % longer).
 template <int DT, int VEC, int C, int LPR>
 __global__ __launch_bounds__(kNormThreads) void norm_rope_fwd_kernel(NormArgs A) {
   using Lanes = RowLanes<DT, VEC, C, LPR>;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_rope_fwd_kernel(NormArgs A)
   lanes.store(S.y, ((t0 + tok) * S.heads + head) * A.dim, a, b);
 }
 
-// The row after this one is on its way while it is worked on (32K tokens x 36 heads of 128, bf16: 193 us, 4.7 TB/s; 211
+// The row after this one is on its way while it is worked on (32K tokens x 36 heads of 128, bf16: 194 us, 4.7 TB/s; 211
 // without).
 template <int DT, int VEC, int C, int LPR>
 __global__ __launch_bounds__(kNormThreads, DT == kF32 ? 3 : 4) void norm_rope_bwd_kernel(NormArgs A) {

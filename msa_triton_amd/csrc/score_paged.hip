@@ -41,7 +41,6 @@ struct PagedScoreArgs {
   const int32_t* cu;
   int nseq;
   const int32_t* context;
-  int64_t tokens;
   int G, Di, NB, B;
   float sign, scale; // of the logits: direction and magnitude
   float* scores;     // [T][G][NB]
@@ -367,7 +366,6 @@ extern "C" int msa_index_score_topk_paged(const void* index_q, const void* index
   A.cu = cu_seqlens;
   A.nseq = static_cast<int>(num_seqs);
   A.context = context_lens;
-  A.tokens = total_tokens;
   A.G = static_cast<int>(groups);
   A.Di = static_cast<int>(index_dim);
   A.NB = static_cast<int>(num_blocks);

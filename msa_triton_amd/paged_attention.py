@@ -4,8 +4,9 @@
 group selected (``m3_index_score_topk_paged``), read from a 16-bit cache or an 8-bit one with a scale for
 each page and head. One C call (``msa_attn_paged``: a launch that reads the selected keys and values, and, for
 few rows, a second one that joins the parts of a row). The new tokens are in the cache already
-(``m3_cache_append``). Made for the few tokens of a decoding step; a prompt goes through the packed operators. No
-gradients: differentiating the outputs raises.
+(``m3_cache_append``). Made for the few tokens of a decoding step: a prompt goes through the packed operators, and
+one behind a cached prefix through this call, where each token reads its blocks on its own (512 tokens behind 8192, 32
+heads, 16 blocks: 169 us). No gradients: differentiating the outputs raises.
 """
 
 from __future__ import annotations
