@@ -401,10 +401,7 @@ __global__ __launch_bounds__(256, NK == 8 && !FP8 ? 1 : 2) void attn_paged_kerne
       for (int i = 0; i < 4; ++i) o[i] = f[w] == 0.f ? o[i] : fmaf(f[w], x[i], o[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (odd[i] != 0.f) o[i] = odd[i];
-      else if (!whole && fabsf(o[i]) == __builtin_inff()) o[i] = copysignf(-kLeastMax, o[i]);  // (a sum past fp32's range)
-    }
+    for (int i = 0; i < 4; ++i) o[i] = odd[i] != 0.f ? odd[i] : o[i];  // (a sum past fp32's range stays one)
     store(d, o);
   }
 }

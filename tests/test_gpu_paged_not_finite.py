@@ -209,3 +209,17 @@ def test_one_infinity_at_other_dims_and_head_counts(dtype, device):
     assert (out[:, :, 77] == float("inf")).all() and (out[:, :, 2] == -float("inf")).all()
     out[:, :, 77] = out[:, :, 2] = 0
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,ways", WAYS)
+def test_sums_past_the_range_give_no_wrong_number(tokens, ways, device):
+    """bf16 values whose weighted sum leaves fp32's range before it is divided: the mean of them, or an infinity."""
+    for value in (3e38, 2e37, 1e35):
+        x = _inputs(tokens, torch.bfloat16, False, device)
+        x["vc"].fill_(value)
+        out, _ = _call(x)
+        want = float(torch.tensor(value).bfloat16())
+        near = (out.double() - want).abs() <= 2 ** -8 * want
+        assert (near | (out == float("inf"))).all()
+    assert near.all()  # 384 x 1e35 is in range
