@@ -321,6 +321,32 @@ int msa_attn_paged(const void* q, const void* k_cache, const void* v_cache, int3
                    int64_t block_size, double scale, void* workspace, int64_t workspace_bytes, void* out,
                    float* lse, void* stream);
 
+/* Causal attention of packed sequences with a sliding window; no reference kernel (the reference has the block-sparse
+ * attention alone). q [T,Hq,D], k and v [T,G,D], fp32, fp16 or bf16; token i of a sequence sees the keys j <= i with
+ * i - j < window (0: all) or j < sinks. out [T,Hq,D] in `dtype`, out_lo (NULL: not wanted; fp32: unread) what its
+ * rounding left out, rounded to `dtype` as well; lse [T,Hq] (NULL: none) natural log. strides (host array, elements):
+ * q token, head; k token, head; v token, head; unit stride along D, rows 16-byte aligned. head_dim: rows of
+ * multiples of 16 bytes, up to 256; T * Hq / G below 0x7fff0000 (status 2 otherwise). One launch. */
+int msa_window_attn_fwd(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
+                        const int32_t* cu_seqlens, int64_t num_seqs, int64_t total_tokens, int64_t q_heads,
+                        int64_t kv_groups, int64_t head_dim, int64_t window, int64_t sinks, double scale, void* out,
+                        void* out_lo, float* lse, void* stream);
+
+/* msa_window_attn_bwd's workspace in bytes. longest: at least the tokens of the longest sequence. */
+int64_t msa_window_attn_bwd_workspace_bytes(int32_t dtype, int64_t total_tokens, int64_t num_seqs, int64_t longest,
+                                            int64_t q_heads, int64_t kv_groups, int64_t head_dim, int64_t window,
+                                            int64_t sinks);
+
+/* Gradients of msa_window_attn_fwd from its out, out_lo (NULL: taken as 0) and lse; grad_out in `dtype`.
+ * strides: the forward's six, then grad_out token, head. grad_q [T,Hq,D], grad_k and grad_v [T,G,D] in `dtype`,
+ * contiguous; NULL: not wanted. Deterministic (sums in fixed orders). Limits as in the forward. */
+int msa_window_attn_bwd(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
+                        const int32_t* cu_seqlens, int64_t num_seqs, int64_t longest, int64_t total_tokens,
+                        int64_t q_heads, int64_t kv_groups, int64_t head_dim, int64_t window, int64_t sinks,
+                        double scale, const void* out, const void* out_lo, const float* lse, const void* grad_out,
+                        void* grad_q, void* grad_k, void* grad_v, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
 /* Testing hook; no counterpart in the reference. Overrides the byte budgets that size
  * the query-token chunks of the KV-major bf16 passes: msa_attn_fwd (default 2 GiB of
  * per-(token, head, slot) partial records per chunk), msa_attn_bwd (3 GiB) and

@@ -45,6 +45,12 @@ scores new tokens against the cached index keys and selects their blocks;
 
 is the attention of new tokens over the selected blocks of the cache;
 
+    m3_window_attention(q, k, v, cu_seqlens, max_seqlen, *, window_size, sink_tokens=0, scale=None,
+                        return_lse=False)
+
+is causal attention with a sliding window and a few first tokens that stay visible (or without a window), for the
+layers beside the block-sparse ones, with gradients;
+
     prepare_sequences(cu_seqlens, *, block_size=128) -> PackedSequences
 
 validates ``cu_seqlens`` once and returns immutable metadata with device copies;
@@ -105,6 +111,7 @@ _OPERATORS = {
     "m3_cache_append": "cache_append",
     "m3_index_score_topk_paged": "paged_score",
     "m3_sparse_attention_paged": "paged_attention",
+    "m3_window_attention": "window_attention",
 }
 
 
@@ -129,5 +136,5 @@ def prepare_sequences(cu_seqlens, *, block_size=128):
 
 __all__ = ["m3_index_score", "m3_topk", "m3_sparse_attention", "m3_index_score_topk", "m3_indexer_kl",
            "m3_qk_norm_rope", "m3_cache_append",
-           "m3_index_score_topk_paged", "m3_sparse_attention_paged", "rope_table",
+           "m3_index_score_topk_paged", "m3_sparse_attention_paged", "rope_table", "m3_window_attention",
            "prepare_sequences", "PackedSequences"]

@@ -1,0 +1,309 @@
+// Causal attention of packed sequences with a sliding window and a few first tokens that stay visible: forward.
+//
+//   out[i, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[i, h] . k_j - max),
+// over the keys that token i sees (window.hpp), one pass over them with the running maximum and sum of each row.
+//
+// Bound by the matrix products (4 D flops a pair, against 2 R bytes of keys and values from L2 for R rows). A
+// workgroup has R = 64 MT rows of one key head, 16 MT a wave; keys and values of a step go to LDS, two steps'
+// worth, the next one's loads in flight during this one's products. S^T = K Q^T puts a row into a lane's column, so that
+// maximum and sum need two exchanges, and the weights P^T leave that product in the operand layout of
+// O^T = V^T P^T (values by transposed reads with the keys in that same order).
+//
+// Logits, statistics and outputs are fp32. The weights enter the second product rounded once to the input type (half a step
+// of 2^-8 in bf16, of the size of the output's own rounding and averaged over the keys; in fp16 times 2^15, so that weights
+// down to 2^-29 keep their bits). The sum of the weights is that of the unrounded ones.
+#include "window.hpp"
+
+namespace msa {
+namespace {
+
+struct WindowFwdArgs {
+  PackedView q, k, v;
+  const int32_t* cu;
+  int nseq, ratio, G, D;
+  Visible seen;
+  float scale_log2;  // scale * log2(e)
+  int64_t first;     // workgroup of this launch's first
+  void* out;         // [T][Hq][D]
+  void* out_lo;      // what the rounding of out left out, or null
+  float* lse;        // [T][Hq], or null
+};
+
+// The row of a token and head, key by key, by a wave: where a value that is not finite met the products of a tile,
+// which multiply the keys that a row does not see by 0. Such values count whatever their weight above 0; a weight of 0 under
+// a logit of -inf makes NaN of them. x2 = logit * log2(e); the weight is exp2(x2 + shift).
+template <int DT>
+__device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, int g, int tok, int head, float shift,
+                                            float inv) {
+  using E = typename Fragment<DT>::Element;
+  const int lane = threadIdx.x & 63;
+  const E* q = static_cast<const E*>(A.q.base) + (start + static_cast<int64_t>(tok)) * A.q.token + head * A.q.head;
+  const E* k = static_cast<const E*>(A.k.base) + start * A.k.token + g * A.k.head;
+  const E* v = static_cast<const E*>(A.v.base) + start * A.v.token + g * A.v.head;
+  const int low = A.seen.low(tok);
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+  auto keys = [&](int from, int to) {
+    for (int base = from; base < to; base += kWave) {
+      const int j = min(base + lane, to - 1), count = min(kWave, to - base);
+      float x = 0.f;
+      for (int d = 0; d < A.D; ++d) x = fmaf(value_at<DT>(q, d), value_at<DT>(k + j * A.k.token, d), x);
+      x *= A.scale_log2;
+      const float p = __builtin_amdgcn_exp2f(x + shift);
+      for (int i = 0; i < count; ++i) {
+        const float p_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), i));
+        const float x_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int d = lane + u * kWave;
+          if (d >= A.D) break;
+          const float y = value_at<DT>(v + (base + i) * A.v.token, d);
+          if (finite(y)) o[u] = fmaf(p_i, y, o[u]);
+          else odd[u] += x_i == -__builtin_inff() ? __builtin_nanf("") : y;
+        }
+      }
+    }
+  };
+  keys(0, min(A.seen.sinks, low));
+  keys(low, tok + 1);
+  const int64_t at = ((start + static_cast<int64_t>(tok)) * (A.G * A.ratio) + head) * A.D;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int d = lane + u * kWave;
+    if (d >= A.D) break;
+    const float y = odd[u] != 0.f ? odd[u] : o[u] * inv;
+    store_from_f32<DT>(A.out, at + d, y);
+    if (DT != kF32 && A.out_lo) {
+      const float lo = y - load_as_f32<DT>(A.out, at + d);
+      store_from_f32<DT>(A.out_lo, at + d, lo == lo ? lo : 0.f);
+    }
+  }
+}
+
+template <int DT, int NK, int MT, int KS>
+__global__ __launch_bounds__(256, 1) void window_fwd_kernel(WindowFwdArgs A) {
+  using E = typename Fragment<DT>::Element;
+  constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
+  constexpr float kUp = DT == kF16 ? 15.f : 0.f;
+  __shared__ alignas(16) E kbuf[2][KS * RS], vbuf[2][KS * RS];
+  const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t item = A.first + blockIdx.x;
+  const int g = static_cast<int>(item % A.G);
+  const TilePlace at = tile_place<R>(A.cu, A.nseq, item / A.G, A.ratio);
+  const int64_t rows = static_cast<int64_t>(at.n) * A.ratio, r0 = static_cast<int64_t>(at.tile) * R;
+  if (r0 >= rows) return;
+  const int live = static_cast<int>(min(rows - r0, int64_t{R}));
+  const int t0 = static_cast<int>(r0 / A.ratio), t1 = static_cast<int>((r0 + live - 1) / A.ratio);
+  const int off = static_cast<int>(r0 - static_cast<int64_t>(t0) * A.ratio);  // head of the first row
+  auto token_of = [&](int r) { return t0 + (off + r) / A.ratio; };
+
+  const E* kbase = static_cast<const E*>(A.k.base) + at.start * A.k.token + g * A.k.head;
+  const E* vbase = static_cast<const E*>(A.v.base) + at.start * A.v.token + g * A.v.head;
+  int tok[MT];
+  Fragment<DT> qf[MT][NK];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = min(16 * (MT * wave + m) + c, live - 1);
+    tok[m] = token_of(r);
+    const E* row = static_cast<const E*>(A.q.base) + (at.start + static_cast<int64_t>(tok[m])) * A.q.token +
+                   (g * A.ratio + (off + r) % A.ratio) * A.q.head;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk)
+      qf[m][kk] = 32 * kk + 8 * q4 < A.D && A.scale_log2 != 0.f ? fragment_at<DT>(row + 32 * kk + 8 * q4) : no_fragment<DT>();
+  }
+  // keys of this workgroup: sinks in front of the first row's window, then from there to the last row
+  const int low = A.seen.low(t0), sinks = min(A.seen.sinks, low);
+  const int sink_steps = (sinks + KS - 1) / KS, steps = sink_steps + (t1 - low) / KS + 1;
+  auto first_key = [&](int e) { return e < sink_steps ? e * KS : low + (e - sink_steps) * KS; };
+  // tokens of this wave's rows (none: first above last)
+  const bool has_rows = 16 * MT * wave < live;
+  const int w0 = token_of(min(16 * MT * wave, live - 1)), w1 = token_of(min(16 * MT * (wave + 1), live) - 1);
+
+  TileLoad<DT, DP, KS> kload, vload;
+  auto load_step = [&](int e) {
+    const int j0 = first_key(e);
+    kload.load(A.D, [&](int r) { return kbase + min(j0 + r, t1) * A.k.token; });
+    vload.load(A.D, [&](int r) { return vbase + min(j0 + r, t1) * A.v.token; });
+  };
+  auto store_step = [&](int e) {
+    kload.store(kbuf[e & 1], RS, A.D);
+    vload.store(vbuf[e & 1], RS, A.D);
+  };
+
+  // A maximum is kept of the raw dots, whose sign is turned where the scale's is negative.
+  const float turn = A.scale_log2 < 0.f ? -1.f : 1.f, scale = fabsf(A.scale_log2);
+  float top[MT], l[MT];
+  f32x4 acc[MT][ND];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    top[m] = -__builtin_inff(), l[m] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  load_step(0);
+  store_step(0);
+  for (int e = 0; e < steps; ++e) {
+    __syncthreads();
+    if (e + 1 < steps) load_step(e + 1);
+    const int j0 = first_key(e);
+    const bool of_sinks = e < sink_steps;
+    const E *kt_ = kbuf[e & 1], *vt_ = vbuf[e & 1];
+    if (has_rows && (of_sinks || (j0 <= w1 && (j0 + KS > A.seen.low(w0) || j0 < A.seen.sinks)))) {
+      f32x4 s[MT][KT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) s[m][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          const Fragment<DT> kf = fragment_at<DT>(kt_ + (16 * kt + c) * RS + 32 * kk + 8 * q4);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) s[m][kt] = product<DT>(kf, qf[m][kk], s[m][kt]);
+        }
+      }
+      if (turn < 0.f) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) s[m][kt] = -s[m][kt];
+      }
+      const bool whole = of_sinks ? j0 + KS <= sinks : j0 + KS - 1 <= w0 && (w1 - j0 < A.seen.window || j0 + KS <= A.seen.sinks);
+      if (!whole) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = j0 + 16 * kt + 4 * q4 + i;
+              const bool seen = of_sinks ? j < sinks : A.seen(tok[m], j);
+              s[m][kt][i] = seen ? s[m][kt][i] : -__builtin_inff();
+            }
+      }
+      Fragment<DT> pf[MT][KT / 2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float high = s[m][0][0];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) high = fmaxf(high, s[m][kt][i]);
+        high = quad_max(high);
+        if (__any(high > top[m])) {
+          const float next = fmaxf(top[m], high);
+          const float keep = top[m] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((top[m] - next) * scale);
+          top[m] = next;
+          l[m] *= keep;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) acc[m][d] *= keep;
+        }
+        // (masked logits stay -inf under a scale of 0, which has zero queries and a factor of 1 instead)
+        const float factor = A.scale_log2 == 0.f ? 1.f : scale;
+        const float shift = kUp - (top[m] == -__builtin_inff() ? 0.f : top[m] * factor);
+#pragma unroll
+        for (int u = 0; u < KT / 2; ++u) {
+          float p[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[m][2 * u + (i >> 2)][i & 3], factor, shift));
+            l[m] += p[i];
+          }
+          pf[m][u] = pack_fragment<DT>(p);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int u = 0; u < KT / 2; ++u) {
+          const Fragment<DT> vf = column_fragment<DT>(vt_, RS, 32 * u, 16 * d, c, q4);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m][d] = product<DT>(vf, pf[m][u], acc[m][d]);
+        }
+    }
+    if (e + 1 < steps) store_step(e + 1);
+  }
+
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = 16 * (MT * wave + m) + c;
+    const bool mine = r < live;
+    l[m] += __shfl_xor(l[m], 16, kWave);
+    l[m] += __shfl_xor(l[m], 32, kWave);
+    const float inv = l[m] == 0.f ? 0.f : 1.f / l[m];
+    const int head = g * A.ratio + (off + (mine ? r : 0)) % A.ratio;
+    const int64_t at_row = (at.start + static_cast<int64_t>(tok[m])) * (A.G * A.ratio) + head;
+    E* out = static_cast<E*>(A.out) + at_row * A.D;
+    E* lo = static_cast<E*>(A.out_lo) + at_row * A.D;
+    float all = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const f32x4 o = acc[m][d] * inv;
+      all += (o[0] + o[1]) + (o[2] + o[3]);
+      if (mine && 16 * d + 4 * q4 < A.D) {
+        store4<DT>(out + 16 * d + 4 * q4, o);
+        if constexpr (DT != kF32)
+          if (A.out_lo) store4<DT>(lo + 16 * d + 4 * q4, left_out<DT>(o));
+      }
+    }
+    const float factor = A.scale_log2 == 0.f ? 1.f : scale;
+    const float level = top[m] == -__builtin_inff() ? 0.f : top[m] * factor;
+    if (mine && q4 == 0 && A.lse)
+      A.lse[at_row] = l[m] == 0.f ? -__builtin_inff() : (level - kUp + __log2f(l[m])) * kLn2Window;
+    // (a sum of NaN makes the row NaN)
+    uint64_t odd = __ballot(mine && !finite(all) && l[m] == l[m]);
+    odd |= odd >> 32, odd |= odd >> 16;
+    for (uint32_t left = odd & 0xffffu; left; left &= left - 1) {
+      const int from = __builtin_ctz(left);
+      careful_row<DT>(A, at.start, g, __builtin_amdgcn_readlane(tok[m], from), __builtin_amdgcn_readlane(head, from),
+                      kUp - __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(level), from)),
+                      __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(inv), from)));
+    }
+  }
+}
+
+}  // namespace
+}  // namespace msa
+
+using namespace msa;
+
+extern "C" int msa_window_attn_fwd(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
+                                   const int32_t* cu_seqlens, int64_t num_seqs, int64_t total_tokens, int64_t q_heads,
+                                   int64_t kv_groups, int64_t head_dim, int64_t window, int64_t sinks, double scale, void* out,
+                                   void* out_lo, float* lse, void* stream) {
+  if (!valid_window_call(q, k, v, dtype, strides, cu_seqlens, num_seqs, total_tokens, q_heads, kv_groups, head_dim, window,
+                         sinks, scale) ||
+      !out)
+    return kErrInvalidArgument;
+  if (!window_supported(dtype, head_dim, total_tokens, q_heads / kv_groups)) return kErrUnsupported;
+  if (total_tokens == 0) return kOk;
+  WindowFwdArgs A{};
+  A.q = PackedView{q, strides[0], strides[1]};
+  A.k = PackedView{k, strides[2], strides[3]};
+  A.v = PackedView{v, strides[4], strides[5]};
+  A.cu = cu_seqlens;
+  A.nseq = static_cast<int>(num_seqs);
+  A.ratio = static_cast<int>(q_heads / kv_groups);
+  A.G = static_cast<int>(kv_groups);
+  A.D = static_cast<int>(head_dim);
+  A.seen = visible_of(window, sinks);
+  A.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  A.out = out;
+  A.out_lo = out_lo;
+  A.lse = lse;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define MSA_WINDOW_FWD(DT, NK, MT, KS)                                                                                 \
+  return launch_parts(tile_numbers(total_tokens, num_seqs, A.ratio, 64 * MT) * kv_groups, [&](int64_t first, unsigned count) { \
+    A.first = first;                                                                                                   \
+    hipLaunchKernelGGL((window_fwd_kernel<DT, NK, MT, KS>), dim3(count), dim3(256), 0, st, A);                         \
+  })
+#define MSA_WINDOW_FWD_DIM(DT, S2, S4, S8)         \
+  if (head_dim <= 64) MSA_WINDOW_FWD(DT, 2, 2, S2); \
+  if (head_dim <= 128) MSA_WINDOW_FWD(DT, 4, 2, S4); \
+  MSA_WINDOW_FWD(DT, 8, 1, S8)
+  if (dtype == kBF16) { MSA_WINDOW_FWD_DIM(kBF16, 64, 64, 32); }
+  if (dtype == kF16) { MSA_WINDOW_FWD_DIM(kF16, 64, 64, 32); }
+  MSA_WINDOW_FWD_DIM(kF32, 32, 32, 32);
+#undef MSA_WINDOW_FWD_DIM
+#undef MSA_WINDOW_FWD
+}
