@@ -347,6 +347,29 @@ int msa_window_attn_bwd(const void* q, const void* k, const void* v, int32_t dty
                         void* grad_q, void* grad_k, void* grad_v, void* workspace, int64_t workspace_bytes,
                         void* stream);
 
+/* msa_window_attn_paged's workspace in bytes. longest: the new tokens of the longest sequence. */
+int64_t msa_window_attn_paged_workspace_bytes(int64_t total_tokens, int64_t num_seqs, int64_t longest, int64_t q_heads,
+                                              int64_t kv_groups, int64_t head_dim, int64_t pages_per_seq,
+                                              int64_t page_size, int64_t window, int64_t sinks);
+
+/* msa_window_attn_fwd for new tokens over a paged cache (msa_cache_append): q [T,Hq,D] contiguous, bf16 or fp16,
+ * packed by cu_seqlens behind context_lens[s] cached tokens; caches and their scales as in msa_attn_paged, the new tokens'
+ * keys and values already in them. With parents (NULL: none) the new tokens of a sequence are the nodes of a tree, each
+ * parent in front of its children: parents[t] is the parent's place among the sequence's new tokens, and anything outside
+ * [0, own place) stands for the context itself. A node lies in slot context + place, has position context + depth
+ * and sees the cached tokens and, of the new ones, itself and its ancestors, both by their positions: the last `window` (0:
+ * all) and the first `sinks`. Keys of missing pages do not exist; rows without a key, and rows of a sequence with a
+ * negative context, get 0 and an lse of -inf. What is not finite: as in msa_attn_paged. strides (host array, elements):
+ * k_cache page, head, slot; v_cache page, head, slot. head_dim: a multiple of 16 up to 256, T * Hq / G below 0x7fff0000,
+ * longest up to 1024 with parents (status 2 otherwise); cache rows, q and workspace 16-byte aligned. Deterministic. */
+int msa_window_attn_paged(const void* q, const void* k_cache, const void* v_cache, int32_t dtype, int32_t cache_is_fp8,
+                          const float* k_scale, const float* v_scale, const int64_t* strides, const int32_t* parents,
+                          const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq, int64_t num_pages,
+                          int64_t page_size, const int32_t* cu_seqlens, int64_t num_seqs, int64_t longest,
+                          const int32_t* context_lens, int64_t total_tokens, int64_t q_heads, int64_t kv_groups,
+                          int64_t head_dim, int64_t window, int64_t sinks, double scale, void* workspace,
+                          int64_t workspace_bytes, void* out, float* lse, void* stream);
+
 /* Testing hook; no counterpart in the reference. Overrides the byte budgets that size
  * the query-token chunks of the KV-major bf16 passes: msa_attn_fwd (default 2 GiB of
  * per-(token, head, slot) partial records per chunk), msa_attn_bwd (3 GiB) and

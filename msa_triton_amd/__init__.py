@@ -51,6 +51,16 @@ is the attention of new tokens over the selected blocks of the cache;
 is causal attention with a sliding window and a few first tokens that stay visible (or without a window), for the
 layers beside the block-sparse ones, with gradients;
 
+    m3_window_attention_paged(q, k_cache, v_cache, page_table, cu_seqlens, context_lens, *, window_size, sink_tokens=0,
+                              scale=None, k_scale=None, v_scale=None, return_lse=False)
+
+is the same of new tokens over a paged cache, and
+
+    m3_tree_attention_paged(q, k_cache, v_cache, page_table, cu_seqlens, context_lens, parents, *, window_size=None,
+                            sink_tokens=0, scale=None, k_scale=None, v_scale=None, return_lse=False)
+
+that of a tree of drafted tokens, each of which sees the cached ones and its ancestors;
+
     prepare_sequences(cu_seqlens, *, block_size=128) -> PackedSequences
 
 validates ``cu_seqlens`` once and returns immutable metadata with device copies;
@@ -112,6 +122,8 @@ _OPERATORS = {
     "m3_index_score_topk_paged": "paged_score",
     "m3_sparse_attention_paged": "paged_attention",
     "m3_window_attention": "window_attention",
+    "m3_window_attention_paged": "window_paged",
+    "m3_tree_attention_paged": "window_paged",
 }
 
 
@@ -137,4 +149,5 @@ def prepare_sequences(cu_seqlens, *, block_size=128):
 __all__ = ["m3_index_score", "m3_topk", "m3_sparse_attention", "m3_index_score_topk", "m3_indexer_kl",
            "m3_qk_norm_rope", "m3_cache_append",
            "m3_index_score_topk_paged", "m3_sparse_attention_paged", "rope_table", "m3_window_attention",
+           "m3_window_attention_paged", "m3_tree_attention_paged",
            "prepare_sequences", "PackedSequences"]

@@ -71,6 +71,9 @@ SIGNATURES = {
     "msa_window_attn_bwd_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "msa_window_attn_bwd": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f64, _vp,
                                    _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "msa_window_attn_paged_workspace_bytes": (_i64, [_i64] * 10),
+    "msa_window_attn_paged": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64,
+                                     _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f64, _vp, _i64, _vp, _vp, _vp]),
     "msa_set_chunk_budgets": (_i32, [_i64, _i64, _i64]),
     "msa_set_item_order": (_i32, [_i32]),
     "msa_profile_begin": (_i32, []),

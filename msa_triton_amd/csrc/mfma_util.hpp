@@ -184,6 +184,30 @@ __device__ __forceinline__ bf16x8 frag_tr_at(const uint16_t* lo_p, const uint16_
   return __builtin_bit_cast(bf16x8, make_uint4(lo.x, lo.y, hi.x, hi.y));
 }
 
+// Eight e4m3 values as a fragment of bf16 (or fp16): exact.
+template <bool F16>
+__device__ __forceinline__ uint4 widen_fp8(uint32_t a, uint32_t b) {
+  auto two = [](uint32_t w, bool high) {
+    const auto x = high ? __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true)
+                        : __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
+    return F16 ? cvt_pk_f16(x[0], x[1]) : pack_hi16(__float_as_uint(x[0]), __float_as_uint(x[1]));
+  };
+  return make_uint4(two(a, false), two(a, true), two(b, false), two(b, true));
+}
+
+// Four values of a 16-bit or e4m3 row.
+template <int DT, bool FP8>
+__device__ __forceinline__ void load4(const char* p, float (&x)[4]) {
+  if constexpr (FP8) {
+    const int w = *reinterpret_cast<const int*>(p);
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1];
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    x[0] = lo16_f32<DT>(w.x), x[1] = hi16_f32<DT>(w.x), x[2] = lo16_f32<DT>(w.y), x[3] = hi16_f32<DT>(w.y);
+  }
+}
+
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, kWave));
   return fmaxf(v, __shfl_xor(v, 32, kWave));

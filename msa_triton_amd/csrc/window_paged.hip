@@ -1,0 +1,779 @@
+// Window and tree attention of new tokens over a paged cache (16-bit or e4m3 with a scale for each page and head).
+//
+//   out[t, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[t, h] . k_j - max),
+// over the keys that token t sees: those up to its own slot in its window, the first `sinks` ones, and in a tree of
+// drafted tokens, of the new ones, itself and its ancestors. Node i of a tree lies in slot context + i and has position
+// context + depth(i); windows and sinks go by positions.
+//
+// Bound by reading the visible keys and values once from HBM for few rows, by the matrix products for many. Rows of a key head
+// are (token, query head) pairs in tiles of R = 16 MT; a tile goes through its keys in steps of 32. All steps of the batch
+// are counted in front and shared out evenly over the workgroups, whatever the lengths (a request of 30 000 tokens next to
+// one of 60): a workgroup takes a stretch of them, its four waves every fourth step of a tile each on their own, as in
+// the block-sparse form: key fragments straight from memory, S^T = K Q^T, weights as they come out of it, values through
+// the wave's LDS tile. A tile that lies in one stretch is finished there; the parts of the others, maxima, sums and fp32
+// outputs, are joined by a second launch in a fixed order.
+//
+// Logits, statistics and outputs are fp32. With one tile of 16 rows, where the products are not the bound, a weight
+// enters the second product as two 16-bit terms (2^-17 of it left out); with more it is rounded once, as in the packed
+// form. In fp16 both are of the weight times 2^15. Bytes of an 8-bit page are exact in bf16; its scales go into logits
+// and weights.
+#include "window.hpp"
+
+namespace msa {
+namespace {
+
+constexpr int kMostParts = 128;     // workgroups that share a tile
+constexpr int kTreeNodes = 1024;    // most new tokens of a tree
+constexpr float kLowest = -3.402823466e38f;  // the least maximum of keys that exist
+
+struct PagedPlan {
+  int64_t items, share;  // steps of the batch, of a workgroup
+};
+
+struct PagedWindowArgs {
+  const uint16_t* q;  // [T][Hq][D]
+  CacheView k, v;
+  const float *k_scale, *v_scale;  // [P][G]
+  PageMap pages;
+  const int32_t* cu;
+  int nseq;
+  const int32_t* context;
+  const int32_t* parents;  // [T], or null: no tree
+  Divisor ratio;
+  int G, D;
+  Visible seen;
+  float scale_log2;  // scale * log2(e)
+  int64_t tokens;
+  uint16_t* out;  // [T][Hq][D]
+  float* lse;     // [T][Hq], or null
+  PagedPlan* plan;
+  int64_t* first_item;  // [N]
+  float* part;    // [workgroups][2][R][D]: of a tile that it does not begin, of one that it does not end
+  float* stats;   // [workgroups][2][2][R]: maximum (log2), sum
+};
+
+// The keys that a tile of rows goes through: [0, sinks) in steps of 32, then [low, hi] in steps of 32, low a multiple of it.
+struct TileKeys {
+  int a, b;  // first and last token
+  int low, hi, sinks, sink_steps, steps;
+  __device__ __forceinline__ int first(int e) const { return e < sink_steps ? 32 * e : low + 32 * (e - sink_steps); }
+};
+
+// A sequence of the call: its tiles, and the steps that each of them is given (those behind a tile's last do nothing).
+struct SeqPlan {
+  int n, context, tiles, steps;
+  __device__ __forceinline__ int64_t items(int groups) const { return static_cast<int64_t>(tiles) * groups * steps; }
+};
+
+template <int R>
+__device__ __forceinline__ TileKeys tile_keys(const PagedWindowArgs& A, int n, int context, int tile) {
+  TileKeys K;
+  const int r0 = tile * R;
+  K.a = A.ratio(r0);
+  K.b = A.ratio(min(r0 + R, n * A.ratio.d) - 1);
+  const int64_t last = A.pages.last_position(), c = context;
+  K.hi = context < 0 ? -1 : static_cast<int>(min(c + K.b, last));
+  const int64_t low = max(int64_t{0}, c + (A.parents ? 0 : K.a) - A.seen.window + 1);
+  K.low = static_cast<int>(min(low, static_cast<int64_t>(K.hi) + 32)) & ~31;  // (past hi: none)
+  if (context < 0) K.low = 0;
+  K.sinks = min(A.seen.sinks, min(K.low, K.hi + 1));
+  K.sink_steps = (K.sinks + 31) >> 5;
+  K.steps = K.sink_steps + (K.hi >= K.low ? (K.hi >> 5) - (K.low >> 5) + 1 : 0);
+  return K;
+}
+
+template <int R>
+__device__ __forceinline__ SeqPlan seq_plan(const PagedWindowArgs& A, int start, int end, int context) {
+  SeqPlan P;
+  P.n = end - start;
+  P.context = context;
+  P.tiles = (P.n * A.ratio.d + R - 1) / R;
+  P.steps = 1;
+  if (P.tiles == 0 || context < 0) return P;
+  const TileKeys K = tile_keys<R>(A, P.n, context, P.tiles - 1);
+  if (P.tiles == 1) {
+    P.steps = max(1, K.steps);
+  } else {  // at least those of any tile
+    const int64_t span = static_cast<int64_t>(A.seen.window) + (A.parents ? P.n : R / A.ratio.d + 1);
+    const int64_t by_window = (static_cast<int64_t>(A.seen.sinks) + 31) / 32 + span / 32 + 2;
+    P.steps = static_cast<int>(max(int64_t{1}, min(by_window, static_cast<int64_t>(K.hi >= 0 ? (K.hi >> 5) + 1 : 1))));
+  }
+  return P;
+}
+
+// a / b, in 32 bits where a fits
+__device__ __forceinline__ int64_t quotient(int64_t a, uint32_t b) {
+  return a >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / b);
+}
+
+// The parent of node i among its sequence's new tokens, or -1: anything that is not in front of it is none.
+__device__ __forceinline__ int parent_of(int p, int i) { return p >= 0 && p < i ? p : -1; }
+
+// One row, key by key, by a wave: where a value that is not finite met the products of a tile, which multiply the keys that
+// a row does not see by 0. Such values count whatever their weight above 0; a weight of 0 under a logit of -inf
+// makes NaN of them. The weight is exp2(logit * log2(e) - top).
+template <int DT, bool FP8>
+__device__ __forceinline__ void careful_row(const PagedWindowArgs& A, int s, int start, int context, int tok, int g, int head,
+                                            float top, float inv) {
+  constexpr int ES = FP8 ? 1 : 2;
+  const int lane = threadIdx.x & 63, slot_mask = (1 << A.pages.shift) - 1;
+  const int64_t row = (start + static_cast<int64_t>(tok)) * (A.G * A.ratio.d) + head;
+  const uint16_t* q = A.q + row * A.D;
+  const char* kbase = static_cast<const char*>(A.k.base) + g * A.k.stride_head * ES;
+  const char* vbase = static_cast<const char*>(A.v.base) + g * A.v.stride_head * ES;
+  const int32_t* parents = A.parents ? A.parents + start : nullptr;
+  int64_t pos = context + static_cast<int64_t>(tok);
+  if (parents) {
+    pos = context;
+    for (int i = parent_of(parents[tok], tok); i >= 0; i = parent_of(parents[i], i)) ++pos;
+  }
+  const int64_t hi = min(context + static_cast<int64_t>(tok), A.pages.last_position()), low = max(int64_t{0}, pos - A.seen.window + 1);
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+  auto keys = [&](int64_t from, int64_t to) {  // both below 2^31; cached tokens and new ones never in one go
+    for (int64_t base = from; base < to; base += kWave) {
+      const int64_t j = min(base + lane, to - 1);
+      bool seen = base + lane < to;
+      if (parents && base >= context) {  // new tokens on the way up
+        const int mine = static_cast<int>(j - context);
+        bool on_path = false;
+        int64_t place = pos;
+        for (int i = tok; i >= 0; i = parent_of(parents[i], i), --place)
+          on_path |= i == mine && (pos - place < A.seen.window || place < A.seen.sinks);
+        seen &= on_path;
+      }
+      const int page = A.pages.page_of(s, j);
+      seen &= page >= 0;
+      const int64_t p0 = page < 0 ? 0 : page, slot = j & slot_mask;
+      const char* kp = kbase + (p0 * A.k.stride_page + slot * A.k.stride_slot) * ES;
+      float x = 0.f;
+      for (int d = 0; d < A.D; d += 4) {
+        float y[4], z[4];
+        load4<DT, false>(reinterpret_cast<const char*>(q + d), y);
+        load4<DT, FP8>(kp + d * ES, z);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x = fmaf(y[i], z[i], x);
+      }
+      x *= A.scale_log2 * (FP8 ? A.k_scale[p0 * A.G + g] : 1.f);
+      const float p = __builtin_amdgcn_exp2f(x - top);
+      uint64_t left = __ballot(seen);
+      for (; left; left &= left - 1) {
+        const int i = __builtin_ctzll(left);
+        const float p_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), i));
+        const float x_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i));
+        const int64_t page_i = __builtin_amdgcn_readlane(page, i);
+        const char* vp = vbase + (page_i * A.v.stride_page + ((base + i) & slot_mask) * A.v.stride_slot) * ES;
+        const float vs = FP8 ? A.v_scale[page_i * A.G + g] : 1.f;
+        const int d = 4 * lane;  // (at most 256 dims)
+        if (d < A.D) {
+          float y[4];
+          load4<DT, FP8>(vp + d * ES, y);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            y[u] *= vs;
+            if (finite(y[u])) o[u] = fmaf(p_i, y[u], o[u]);
+            else odd[u] += x_i == -__builtin_inff() ? __builtin_nanf("") : y[u];
+          }
+        }
+      }
+    }
+  };
+  if (context >= 0 && A.pages.num_pages > 0) {
+    const int64_t cached = parents ? min(static_cast<int64_t>(context), hi + 1) : hi + 1;
+    keys(0, min(static_cast<int64_t>(A.seen.sinks), min(low, cached)));
+    keys(min(low, cached), cached);
+    if (parents) keys(context, hi + 1);
+  }
+  const int d = 4 * lane;
+  if (d >= A.D) return;
+  f32x4 y;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) y[u] = odd[u] != 0.f ? odd[u] : o[u] * inv;
+  store4<DT>(A.out + row * A.D + d, y);
+}
+
+template <int DT, bool FP8, int NK, int MT>
+__global__ __launch_bounds__(256, MT == 1 && !(NK == 8 && !FP8) ? 2 : 1) void window_paged_kernel(PagedWindowArgs A) {
+  constexpr int R = 16 * MT, DP = 32 * NK, RS = DP + 16, ND = DP / 16, ES = FP8 ? 1 : 2;
+  constexpr int PT = FP8 ? kBF16 : DT;          // type of the second product
+  constexpr bool kTwo = MT == 1;                // terms of a weight
+  constexpr float kUp = PT == kF16 ? 15.f : 0.f;
+  constexpr int VL = FP8 ? DP / 16 : DP / 8, NV = VL / 2, VR = 64 / VL, VD = FP8 ? 16 : 8;
+  constexpr int NKR = FP8 ? NK / 2 : NK;
+  constexpr int OS = DP + 4;
+  static_assert(16 * OS * 4 <= 32 * RS * 2, "a wave's output fits its value tile");
+  __shared__ alignas(16) uint16_t vbuf[4][32 * RS];
+  __shared__ float wave_max[4][R], wave_sum[4][R];
+  __shared__ int64_t first_item[257], wave_items[4];  // of the sequences that thread i counts
+  __shared__ int wave_most[4];
+  __shared__ int parent[kTreeNodes], depth[R + 1];
+  __shared__ uint32_t path[(R + 1) * (kTreeNodes / 32)];
+  __shared__ uint32_t odd_rows[MT];
+  __shared__ float row_top[R], row_inv[R];
+  const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ratio = A.ratio.d;
+
+  // ---- the batch's steps, sequence by sequence: a sequence a lane where there are up to 64, otherwise `per` a thread
+  const bool few = A.nseq <= 64;
+  const int per = (A.nseq + 255) / 256;
+  SeqPlan mine{};
+  int64_t upto = 0, items;
+  int most = 1;
+  if (few) {
+    if (lane < A.nseq) {
+      mine = seq_plan<R>(A, A.cu[lane], A.cu[lane + 1], A.context[lane]);
+      upto = mine.items(A.G), most = mine.steps;
+    }
+  } else {
+    for (int s = threadIdx.x * per; s < min(A.nseq, (static_cast<int>(threadIdx.x) + 1) * per); ++s) {
+      const SeqPlan P = seq_plan<R>(A, A.cu[s], A.cu[s + 1], A.context[s]);
+      upto += P.items(A.G), most = max(most, P.steps);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int64_t x = __shfl_up(upto, o, kWave);
+    if (lane >= o) upto += x;
+    most = max(most, __shfl_xor(most, o, kWave));
+  }
+  if (few) {
+    items = __shfl(upto, 63, kWave);
+  } else {
+    if (lane == 63) wave_items[wave] = upto, wave_most[wave] = most;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += wave_items[w];
+    for (int w = 0; w < 4; ++w) most = max(most, wave_most[w]);
+    first_item[threadIdx.x + 1] = upto;
+    if (threadIdx.x == 0) first_item[0] = 0;
+    __syncthreads();
+    items = first_item[256];
+  }
+  most = __builtin_amdgcn_readfirstlane(most);
+  // a step for each wave at least, and no tile in more than kMostParts stretches
+  const int64_t share = max(max(int64_t{4}, quotient(items + gridDim.x - 1, gridDim.x)),
+                            static_cast<int64_t>((most + kMostParts - 2) / (kMostParts - 1)));
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) *A.plan = PagedPlan{items, share};
+    if (few) {
+      if (wave == 0 && lane < A.nseq) A.first_item[lane] = upto - mine.items(A.G);
+    } else {
+      int64_t at = first_item[threadIdx.x];
+      for (int s = threadIdx.x * per; s < min(A.nseq, (static_cast<int>(threadIdx.x) + 1) * per); ++s) {
+        A.first_item[s] = at;
+        at += seq_plan<R>(A, A.cu[s], A.cu[s + 1], A.context[s]).items(A.G);
+      }
+    }
+  }
+
+  auto dim_of = [&](int kk) { return FP8 ? 64 * (kk >> 1) + 16 * q4 + 8 * (kk & 1) : 32 * kk + 8 * q4; };
+  const bool full = A.D == DP;
+  const int slot_mask = (1 << A.pages.shift) - 1;
+  int64_t item = blockIdx.x * share;
+  const int64_t end_item = min(item + share, items);
+  while (item < end_item) {
+    // ---- the tile of this step, and how many of its steps are this workgroup's: [e0, e1)
+    int s;
+    int64_t rest;
+    SeqPlan P;
+    if (few) {
+      s = __builtin_ctzll(__ballot(upto > item));
+      P.n = __builtin_amdgcn_readlane(mine.n, s);
+      P.context = __builtin_amdgcn_readlane(mine.context, s);
+      P.tiles = __builtin_amdgcn_readlane(mine.tiles, s);
+      P.steps = __builtin_amdgcn_readlane(mine.steps, s);
+      rest = item - (__shfl(upto, s, kWave) - P.items(A.G));
+    } else {
+      int lo = 0, hi = 256;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first_item[mid] <= item) lo = mid; else hi = mid;
+      }
+      s = __builtin_amdgcn_readfirstlane(lo * per);
+      rest = item - first_item[lo];
+      P = seq_plan<R>(A, A.cu[s], A.cu[s + 1], A.context[s]);
+      while (rest >= P.items(A.G)) {
+        rest -= P.items(A.G);
+        ++s;
+        P = seq_plan<R>(A, A.cu[s], A.cu[s + 1], A.context[s]);
+      }
+    }
+    const int64_t tile_no = quotient(rest, P.steps);  // group by group
+    const int e0 = static_cast<int>(rest - tile_no * P.steps);
+    const int e1 = static_cast<int>(min(static_cast<int64_t>(P.steps), e0 + (end_item - item)));
+    item += e1 - e0;
+    const int g = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(tile_no, P.tiles)));
+    const int tile = __builtin_amdgcn_readfirstlane(static_cast<int>(tile_no - static_cast<int64_t>(g) * P.tiles));
+    const TileKeys K = tile_keys<R>(A, P.n, P.context, tile);
+    const int start = A.cu[s], r0 = tile * R, live = min(R, P.n * ratio - r0);
+
+    if (A.parents) {  // which new tokens each token of the tile sees: a bit each
+      for (int i = threadIdx.x; i <= K.b; i += 256) parent[i] = parent_of(A.parents[start + i], i);
+      __syncthreads();
+      const int t = threadIdx.x;
+      if (t <= K.b - K.a) {
+        uint32_t* bits = path + t * (kTreeNodes / 32);
+        for (int w = 0; w <= K.b >> 5; ++w) bits[w] = 0;
+        int deep = 0;
+        for (int i = parent[K.a + t]; i >= 0; i = parent[i]) ++deep;
+        depth[t] = deep;
+        int up = 0;
+        for (int i = K.a + t; i >= 0; i = parent[i], ++up)
+          if (up < A.seen.window || static_cast<int64_t>(P.context) + deep - up < A.seen.sinks) bits[i >> 5] |= 1u << (i & 31);
+      }
+      __syncthreads();
+    }
+    int low[MT], slot[MT], tree_row[MT];
+    bf16x8 qf[MT][NK];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = min(16 * m + c, live - 1), tok = A.ratio(r0 + r);
+      const uint16_t* row = A.q + ((start + static_cast<int64_t>(tok)) * (A.G * ratio) + g * ratio + r0 + r - tok * ratio) * A.D;
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) qf[m][kk] = dim_of(kk) < A.D ? load_frag(row + dim_of(kk)) : zero_frag();
+      tree_row[m] = (tok - K.a) * (kTreeNodes / 32);
+      const int64_t pos = static_cast<int64_t>(P.context) + (A.parents ? depth[tok - K.a] : tok);
+      low[m] = static_cast<int>(min(max(int64_t{0}, pos - A.seen.window + 1), int64_t{0x7fffffff}));
+      slot[m] = static_cast<int>(min(static_cast<int64_t>(P.context) + tok, static_cast<int64_t>(K.hi)));
+    }
+    // keys below `common` are in no row's future, and those from low_most on in every row's window
+    const int common = A.parents ? P.context : static_cast<int>(min(static_cast<int64_t>(P.context) + K.a, static_cast<int64_t>(K.hi))) + 1;
+    const int64_t low_most = static_cast<int64_t>(P.context) + K.b - A.seen.window + 1;
+
+    float top[MT], l[MT];
+    bool had_keys = false;
+    f32x4 acc[MT][ND];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      top[m] = -__builtin_inff(), l[m] = 0.f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const char* kbase = static_cast<const char*>(A.k.base) + g * A.k.stride_head * ES;
+    const char* vbase = static_cast<const char*>(A.v.base) + g * A.v.stride_head * ES;
+    uint4 kr[2][NKR], vr[NV];
+    int key0 = 0, p0 = -1, p1 = -1;
+    float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f;
+
+    // this wave's steps: pages of 32 at a time, a half step a lane; those with a page that exists are gone through
+    int batch = e0 + wave, own_page = -1;
+    uint64_t open = 0;
+    const int stop = min(e1, K.steps);
+    auto key_of = [&](int i) { return K.first(batch - 128 + 4 * (i >> 1)) + 16 * (i & 1); };
+    auto next_step = [&]() {  // false: none left
+      while (open == 0) {
+        if (batch >= stop) return false;
+        const int e = batch + 4 * (lane >> 1);
+        const int j = K.first(e) + 16 * (lane & 1);
+        own_page = e < stop && j <= (e < K.sink_steps ? K.sinks - 1 : K.hi) ? A.pages.page_of(s, j) : -1;
+        const uint64_t there = __ballot(own_page >= 0);
+        open = (there | there >> 1) & 0x5555555555555555ull;
+        batch += 128;
+      }
+      const int i = __builtin_ctzll(open);
+      open &= open - 1;
+      key0 = __builtin_amdgcn_readfirstlane(key_of(i));
+      p0 = __builtin_amdgcn_readlane(own_page, i);
+      p1 = __builtin_amdgcn_readlane(own_page, i + 1);
+      return true;
+    };
+    auto load_step = [&]() {
+      const int64_t s0 = p0 < 0 ? 0 : p0, s1 = p1 < 0 ? 0 : p1;  // (page 0 exists; its rows are masked)
+      const int slot0 = key0 & slot_mask, slot1 = (key0 + 16) & slot_mask;
+      const char* kp[2] = {kbase + (s0 * A.k.stride_page + (slot0 + c) * A.k.stride_slot) * ES,
+                           kbase + (s1 * A.k.stride_page + (slot1 + c) * A.k.stride_slot) * ES};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < NKR; ++i) {
+          const int d = FP8 ? 64 * i + 16 * q4 : 32 * i + 8 * q4;
+          kr[h][i] = *reinterpret_cast<const uint4*>(kp[h] + (d < A.D ? d : 0) * ES);
+        }
+      const int d = lane % VL * VD;
+      const char* v0 = vbase + (s0 * A.v.stride_page + (d < A.D ? d : 0)) * ES;
+      const char* v1 = vbase + (s1 * A.v.stride_page + (d < A.D ? d : 0)) * ES;
+#pragma unroll
+      for (int p = 0; p < NV; ++p) {
+        const int r = p * VR + lane / VL;
+        vr[p] = *reinterpret_cast<const uint4*>(
+            p < NV / 2 ? v0 + (slot0 + r) * A.v.stride_slot * ES : v1 + (slot1 + r - 16) * A.v.stride_slot * ES);
+      }
+      if constexpr (FP8) {
+        // (a page that is not there has weights of 0: its factor must be finite)
+        ks0 = p0 < 0 ? 0.f : A.k_scale[s0 * A.G + g], ks1 = p1 < 0 ? 0.f : A.k_scale[s1 * A.G + g];
+        vs0 = p0 < 0 ? 0.f : A.v_scale[s0 * A.G + g], vs1 = p1 < 0 ? 0.f : A.v_scale[s1 * A.G + g];
+      }
+    };
+
+    bool more = next_step();
+    if (more) load_step();
+    while (more) {
+      had_keys = true;
+      const int k_now = key0, a_now = p0, b_now = p1;
+      const bool of_sinks = k_now < K.low;
+      const int upto_key = of_sinks ? K.sinks - 1 : K.hi;  // of the tile
+      f32x4 sc[MT][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) sc[m][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          uint4 w;
+          if constexpr (FP8) {
+            const uint4 x = kr[h][kk >> 1];
+            w = kk & 1 ? widen_fp8<DT == kF16>(x.z, x.w) : widen_fp8<DT == kF16>(x.x, x.y);
+          } else {
+            w = kr[h][kk];
+          }
+          if (!full && dim_of(kk) >= A.D) w = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) sc[m][h] = mfma_t<DT>(__builtin_bit_cast(bf16x8, w), qf[m][kk], sc[m][h]);
+        }
+      }
+      uint16_t* vt = vbuf[wave];
+#pragma unroll
+      for (int p = 0; p < NV; ++p) {
+        const int r = p * VR + lane / VL;
+        const bool there = (p < NV / 2 ? a_now : b_now) >= 0 && k_now + r <= upto_key;  // (unwritten slots hold anything)
+        const uint4 x = there ? vr[p] : make_uint4(0u, 0u, 0u, 0u);
+        uint4* to = reinterpret_cast<uint4*>(vt + r * RS + lane % VL * VD);
+        if constexpr (FP8) {
+          to[0] = widen_fp8<false>(x.x, x.y);
+          to[1] = widen_fp8<false>(x.z, x.w);
+        } else {
+          to[0] = x;
+        }
+      }
+      const float kf0 = A.scale_log2 * ks0, kf1 = A.scale_log2 * ks1, vf0 = vs0, vf1 = vs1;
+      more = next_step();
+      if (more) load_step();
+      const bool whole = a_now >= 0 && b_now >= 0 && k_now + 31 < common && k_now + 31 <= upto_key &&
+                         (of_sinks || k_now >= low_most || k_now + 31 < A.seen.sinks);
+      bf16x8 ph[MT], pl[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float x[8], high = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = sc[m][j >> 2][j & 3] * (j >> 2 ? kf1 : kf0);
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int h = j >> 2, key = k_now + 16 * h + 4 * q4 + (j & 3);
+            bool seen = (h ? b_now : a_now) >= 0 && key <= upto_key && (key >= low[m] || key < A.seen.sinks);
+            if (A.parents) {
+              const int node = key - P.context;
+              if (node >= 0 && key <= upto_key) seen = (h ? b_now : a_now) >= 0 && (path[tree_row[m] + (node >> 5)] >> (node & 31) & 1u);
+            } else {
+              seen = seen && key <= slot[m];
+            }
+            x[j] = seen ? x[j] : -__builtin_inff();
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) high = fmaxf(high, x[j]);
+        high = quad_max(high);
+        if (__any(high > top[m])) {
+          const float next = fmaxf(top[m], high);
+          const float keep = top[m] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(top[m] - next);
+          top[m] = next;
+          l[m] *= keep;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) acc[m][d] *= keep;
+        }
+        const float shift = kUp - (top[m] == -__builtin_inff() ? 0.f : top[m]);  // (all logits -inf: weights 0)
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          float y0 = __builtin_amdgcn_exp2f(x[j] + shift), y1 = __builtin_amdgcn_exp2f(x[j + 1] + shift);
+          l[m] += y0 + y1;
+          if constexpr (FP8) y0 *= j < 4 ? vf0 : vf1, y1 *= j < 4 ? vf0 : vf1;
+          if constexpr (PT == kF16) {
+            hi[j >> 1] = cvt_pk_f16(y0, y1);
+            if constexpr (kTwo) lo[j >> 1] = cvt_pk_f16(sub_lo_half_f16(hi[j >> 1], y0), sub_hi_half_f16(hi[j >> 1], y1));
+          } else {
+            hi[j >> 1] = cvt_pk_bf16(y0, y1);
+            if constexpr (kTwo) lo[j >> 1] = cvt_pk_bf16(sub_lo_half(hi[j >> 1], y0), sub_hi_half(hi[j >> 1], y1));
+          }
+        }
+        ph[m] = __builtin_bit_cast(bf16x8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+        if constexpr (kTwo) pl[m] = __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const bf16x8 f = frag_tr(vt, RS, 4 * q4, 16 + 4 * q4, 16 * d, c);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          acc[m][d] = mfma_t<PT>(f, ph[m], acc[m][d]);
+          if constexpr (kTwo) acc[m][d] = mfma_t<PT>(f, pl[m], acc[m][d]);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+
+    // ---- the four waves joined, 16 rows at a time: maxima and sums, then the outputs through LDS
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (had_keys) top[m] = fmaxf(top[m], kLowest);
+      l[m] += __shfl_xor(l[m], 16, kWave);
+      l[m] += __shfl_xor(l[m], 32, kWave);
+      if (q4 == 0) wave_max[wave][16 * m + c] = top[m], wave_sum[wave][16 * m + c] = l[m];
+    }
+    if (threadIdx.x < MT) odd_rows[threadIdx.x] = 0;
+    const bool done = e0 == 0 && e1 == P.steps;
+    const int64_t place = static_cast<int64_t>(blockIdx.x) * 2 + (e0 > 0 ? 0 : 1);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float* own = reinterpret_cast<float*>(vbuf[wave]);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(own + c * OS + 16 * d + 4 * q4) = acc[m][d];
+      __syncthreads();
+      const int row = threadIdx.x >> 4, col = threadIdx.x & 15, r = 16 * m + row;  // 16 threads a row
+      const float high = fmaxf(fmaxf(wave_max[0][r], wave_max[1][r]), fmaxf(wave_max[2][r], wave_max[3][r]));
+      float f[4], sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        f[w] = wave_max[w][r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(wave_max[w][r] - high);
+        sum += f[w] * wave_sum[w][r];
+      }
+      if (r < live) {
+        const int tok = A.ratio(r0 + r);
+        const int64_t out_row = (start + static_cast<int64_t>(tok)) * (A.G * ratio) + g * ratio + r0 + r - tok * ratio;
+        const float inv = done ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+        float all = 0.f;
+        for (int d = 4 * col; d < A.D; d += 64) {
+          f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(vbuf[w]) + row * OS + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(f[w], x[i], o[i]);
+          }
+          o *= inv;
+          all += (o[0] + o[1]) + (o[2] + o[3]);
+          if (done) store4<DT>(A.out + out_row * A.D + d, o);
+          else *reinterpret_cast<f32x4*>(A.part + (place * R + r) * A.D + d) = o;
+        }
+        if (col == 0) {
+          if (!done) {
+            A.stats[(place * 2) * R + r] = high;
+            A.stats[(place * 2 + 1) * R + r] = sum;
+          } else if (A.lse) {
+            A.lse[out_row] = sum == 0.f ? -__builtin_inff() : (high - kUp + __log2f(sum)) * kLn2Window;
+          }
+          row_top[r] = high - kUp, row_inv[r] = inv;
+        }
+        // (a sum of NaN makes the row NaN)
+        if (done && !finite(all) && sum == sum) atomicOr(&odd_rows[m], 1u << row);
+      }
+      __syncthreads();
+    }
+#pragma unroll 1
+    for (int m = 0; m < MT; ++m) {
+      uint32_t left = __builtin_amdgcn_readfirstlane(odd_rows[m]);
+      for (int turn = 0; left; left &= left - 1, ++turn) {
+        if ((turn & 3) != wave) continue;
+        const int r = 16 * m + __builtin_ctz(left), tok = A.ratio(r0 + r);
+        careful_row<DT, FP8>(A, s, start, P.context, tok, g, g * ratio + r0 + r - tok * ratio, row_top[r], row_inv[r]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The parts of rows that several workgroups share, a workgroup a row: each of its waves takes every fourth part, eight of
+// them in flight, two dims a lane and pass; then the waves are added up.
+template <int DT, bool FP8, int MT>
+__global__ __launch_bounds__(256) void window_paged_join(PagedWindowArgs A, int64_t first) {
+  constexpr int R = 16 * MT;
+  constexpr float kUp = !FP8 && DT == kF16 ? 15.f : 0.f;
+  __shared__ float weight[kMostParts], sums[4][256];
+  const int lane = threadIdx.x & 63, ratio = A.ratio.d;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t out_row = first + blockIdx.x;
+  const int heads = A.G * ratio;
+  const int64_t t = out_row / heads;
+  const int hq = static_cast<int>(out_row - t * heads), g = A.ratio(hq);
+  const int s = wave_upper_index(A.nseq, t, [&](int i) { return static_cast<int64_t>(A.cu[i]); });
+  const int start = A.cu[s], context = A.context[s];
+  const SeqPlan P = seq_plan<R>(A, start, A.cu[s + 1], context);
+  const int tok = static_cast<int>(t - start), rr = tok * ratio + hq - g * ratio, tile = rr / R, r = rr - tile * R;
+  const PagedPlan plan = *A.plan;
+  const int64_t item = A.first_item[s] + (static_cast<int64_t>(g) * P.tiles + tile) * P.steps;
+  const int64_t w0 = item / plan.share, parts = (item + P.steps - 1) / plan.share - w0 + 1;
+  if (parts == 1) return;
+  auto place_of = [&](int64_t z) { return (w0 + z) * 2 + (z == 0 ? 1 : 0); };
+  // every wave weighs all of them (at most kMostParts = 128: two a lane)
+  float high[2], sum_z[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t z = lane + 64 * i, at = place_of(min(z, parts - 1)) * 2 * R + r;
+    high[i] = z < parts ? A.stats[at] : -__builtin_inff();
+    sum_z[i] = z < parts ? A.stats[at + R] : 0.f;
+  }
+  const float top = wave_max_f32(fmaxf(high[0], high[1]));
+  float w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = high[i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(high[i] - top);
+    if (wave == 0) weight[lane + 64 * i] = w[i];
+  }
+  const float sum = wave_sum_f32(w[0] * sum_z[0] + w[1] * sum_z[1]);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  __syncthreads();
+  float all = 0.f;
+  for (int d0 = 0; d0 < A.D; d0 += 128) {
+    const int d = min(d0 + 2 * lane, A.D - 2);
+    float o0 = 0.f, o1 = 0.f;
+    for (int64_t z0 = wave; z0 < parts; z0 += 32) {
+      float2 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = *reinterpret_cast<const float2*>(A.part + (place_of(min(z0 + 4 * i, parts - 1)) * R + r) * A.D + d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = z0 + 4 * i < parts ? weight[z0 + 4 * i] : 0.f;
+        o0 = fmaf(f, z0 + 4 * i < parts ? x[i].x : 0.f, o0);
+        o1 = fmaf(f, z0 + 4 * i < parts ? x[i].y : 0.f, o1);
+      }
+    }
+    sums[wave][2 * lane] = o0, sums[wave][2 * lane + 1] = o1;
+    __syncthreads();
+    const int e = threadIdx.x;
+    if (e < 128 && d0 + e < A.D) {
+      const float o = ((sums[0][e] + sums[1][e]) + (sums[2][e] + sums[3][e])) * inv;
+      all += o;
+      store_from_f32<DT>(A.out, out_row * A.D + d0 + e, o);
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && A.lse) A.lse[out_row] = sum == 0.f ? -__builtin_inff() : (top - kUp + __log2f(sum)) * kLn2Window;
+  if (__syncthreads_or(!finite(all)) && sum == sum && wave == 0)
+    careful_row<DT, FP8>(A, s, start, context, tok, g, hq, top - kUp, inv);
+}
+
+// Tiles of 16 rows where no sequence has more of them a key head, otherwise as many as a wave's registers hold.
+int row_tiles(int64_t longest, int64_t ratio, int64_t dim) { return longest * ratio <= 16 || dim > 128 ? 1 : dim <= 64 ? 4 : 2; }
+
+constexpr int64_t kWorkgroups = 512;
+
+struct PagedShape {
+  int row_tiles;
+  int64_t workgroups;
+};
+// keys: most that a sequence may have (its page table's entries)
+PagedShape paged_shape(int64_t tokens, int64_t nseq, int64_t longest, int64_t ratio, int64_t groups, int64_t dim, int64_t keys,
+                       int64_t window, int64_t sinks) {
+  PagedShape S{row_tiles(longest, ratio, dim), 0};
+  const int64_t rows = 16 * S.row_tiles, tiles = (tokens * ratio / rows + nseq) * groups;
+  int64_t steps = (keys + 31) / 32;
+  if (window) {
+    const int64_t seen = (window + longest) / 32 + 2 + (sinks + 31) / 32;
+    steps = steps < seen ? steps : seen;
+  }
+  const int64_t most = (tiles * (steps < 1 ? 1 : steps) + 3) / 4;
+  S.workgroups = most < kWorkgroups ? most : kWorkgroups;
+  return S;
+}
+
+}  // namespace
+}  // namespace msa
+
+using namespace msa;
+
+extern "C" int64_t msa_window_attn_paged_workspace_bytes(int64_t total_tokens, int64_t num_seqs, int64_t longest,
+                                                         int64_t q_heads, int64_t kv_groups, int64_t head_dim,
+                                                         int64_t pages_per_seq, int64_t page_size, int64_t window,
+                                                         int64_t sinks) {
+  if (total_tokens <= 0 || num_seqs <= 0 || longest <= 0 || q_heads <= 0 || kv_groups <= 0 || q_heads % kv_groups ||
+      head_dim <= 0 || pages_per_seq < 0 || page_size <= 0 || window < 0 || sinks < 0)
+    return 0;
+  const PagedShape S = paged_shape(total_tokens, num_seqs, longest, q_heads / kv_groups, kv_groups, head_dim,
+                                   pages_per_seq * page_size, window, sinks);
+  const int64_t rows = 2 * S.workgroups * 16 * S.row_tiles;
+  return static_cast<int64_t>(sizeof(PagedPlan)) + 8 * num_seqs + 4 * rows * (head_dim + 2);
+}
+
+extern "C" int msa_window_attn_paged(const void* q, const void* k_cache, const void* v_cache, int32_t dtype,
+                                     int32_t cache_is_fp8, const float* k_scale, const float* v_scale, const int64_t* strides,
+                                     const int32_t* parents, const int32_t* page_table, int64_t table_stride,
+                                     int64_t pages_per_seq, int64_t num_pages, int64_t page_size, const int32_t* cu_seqlens,
+                                     int64_t num_seqs, int64_t longest, const int32_t* context_lens, int64_t total_tokens,
+                                     int64_t q_heads, int64_t kv_groups, int64_t head_dim, int64_t window, int64_t sinks,
+                                     double scale, void* workspace, int64_t workspace_bytes, void* out, float* lse,
+                                     void* stream) {
+  if (!q || !out || !strides || !cu_seqlens || !context_lens || num_seqs <= 0 || num_seqs > 0x3fffffff || total_tokens < 0 ||
+      total_tokens > 0x7fffffff || longest < 0 || longest > total_tokens || q_heads <= 0 || kv_groups <= 0 ||
+      q_heads % kv_groups || q_heads >= (1 << 20) || head_dim <= 0 || window < 0 || sinks < 0 || !__builtin_isfinite(scale) ||
+      (dtype != kBF16 && dtype != kF16) || !valid_pages(page_table, table_stride, pages_per_seq, num_pages, page_size) ||
+      (num_pages > 0 && (!k_cache || !v_cache || (cache_is_fp8 && (!k_scale || !v_scale)))))
+    return kErrInvalidArgument;
+  const int unit = cache_is_fp8 ? 16 : 8;
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] % unit) return kErrInvalidArgument;
+  if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(k_cache) % 16 ||
+      reinterpret_cast<uintptr_t>(v_cache) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return kErrInvalidArgument;
+  const int64_t ratio = q_heads / kv_groups;
+  if (head_dim % 16 || head_dim > 256 || total_tokens * ratio >= 0x7fff0000 || (parents && longest > kTreeNodes))
+    return kErrUnsupported;
+  if (total_tokens == 0) return kOk;
+  if (longest == 0 || !workspace ||
+      workspace_bytes < msa_window_attn_paged_workspace_bytes(total_tokens, num_seqs, longest, q_heads, kv_groups, head_dim,
+                                                              pages_per_seq, page_size, window, sinks))
+    return kErrInvalidArgument;
+  const PagedShape S = paged_shape(total_tokens, num_seqs, longest, ratio, kv_groups, head_dim, pages_per_seq * page_size,
+                                   window, sinks);
+  PagedWindowArgs A{};
+  A.q = static_cast<const uint16_t*>(q);
+  A.k = CacheView{const_cast<void*>(k_cache), strides[0], strides[1], strides[2]};
+  A.v = CacheView{const_cast<void*>(v_cache), strides[3], strides[4], strides[5]};
+  A.k_scale = k_scale;
+  A.v_scale = v_scale;
+  A.pages = page_map(page_table, table_stride, pages_per_seq, num_pages, page_size);
+  A.cu = cu_seqlens;
+  A.nseq = static_cast<int>(num_seqs);
+  A.context = context_lens;
+  A.parents = parents;
+  A.ratio = divisor_of(ratio);
+  A.G = static_cast<int>(kv_groups);
+  A.D = static_cast<int>(head_dim);
+  A.seen = visible_of(window, sinks);
+  A.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  A.tokens = total_tokens;
+  A.out = static_cast<uint16_t*>(out);
+  A.lse = lse;
+  A.plan = static_cast<PagedPlan*>(workspace);
+  A.part = reinterpret_cast<float*>(A.plan + 1);
+  A.stats = A.part + 2 * S.workgroups * 16 * S.row_tiles * head_dim;
+  A.first_item = reinterpret_cast<int64_t*>(A.stats + 4 * S.workgroups * 16 * S.row_tiles);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(S.workgroups)), block(256);
+#define MSA_WINDOW_PAGED(DT, F8, NK, MT)                                                              \
+  {                                                                                                   \
+    hipLaunchKernelGGL((window_paged_kernel<DT, F8, NK, MT>), grid, block, 0, st, A);                 \
+    const int rc = status_from(hipGetLastError());                                                    \
+    if (rc != kOk) return rc;                                                                         \
+    return launch_parts(total_tokens * q_heads, [&](int64_t first, unsigned count) {                  \
+      hipLaunchKernelGGL((window_paged_join<DT, F8, MT>), dim3(count), block, 0, st, A, first);       \
+    });                                                                                               \
+  }
+#define MSA_WINDOW_PAGED_DIM(DT, F8)                                            \
+  if (head_dim > 128) MSA_WINDOW_PAGED(DT, F8, 8, 1)                            \
+  if (head_dim > 64 && S.row_tiles == 1) MSA_WINDOW_PAGED(DT, F8, 4, 1)         \
+  if (head_dim > 64) MSA_WINDOW_PAGED(DT, F8, 4, 2)                             \
+  if (S.row_tiles == 1) MSA_WINDOW_PAGED(DT, F8, 2, 1)                          \
+  MSA_WINDOW_PAGED(DT, F8, 2, 4)
+  if (dtype == kBF16) {
+    if (cache_is_fp8) { MSA_WINDOW_PAGED_DIM(kBF16, true) }
+    MSA_WINDOW_PAGED_DIM(kBF16, false)
+  }
+  if (cache_is_fp8) { MSA_WINDOW_PAGED_DIM(kF16, true) }
+  MSA_WINDOW_PAGED_DIM(kF16, false)
+#undef MSA_WINDOW_PAGED_DIM
+#undef MSA_WINDOW_PAGED
+}

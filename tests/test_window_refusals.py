@@ -61,3 +61,59 @@ def test_there_is_no_cpu_path():
     for window in (3, None, 1 << 40):
         with pytest.raises(RuntimeError, match="no CPU execution path"):
             _call(*_packed(), window_size=window, sink_tokens=1 << 40)
+
+
+def _paged(tokens=3, hq=4, g=2, d=16, page=16, pages=4, dtype=torch.bfloat16, cache=None, scales=False):
+    cache = cache or dtype
+    x = dict(q=torch.zeros(tokens, hq, d, dtype=dtype), k_cache=torch.zeros(pages, g, page, d).to(cache),
+             v_cache=torch.zeros(pages, g, page, d).to(cache), page_table=torch.zeros(2, 2, dtype=torch.int32),
+             cu_seqlens=cu_tensor([1, tokens - 1]), context_lens=torch.zeros(2, dtype=torch.int32), window_size=3)
+    if scales:
+        x |= dict(k_scale=torch.ones(pages, g), v_scale=torch.ones(pages, g))
+    return x
+
+
+def _serve(tree, **x):
+    if tree:
+        x.setdefault("parents", torch.full((x["q"].shape[0],), -1, dtype=torch.int32))
+    return (msa.m3_tree_attention_paged if tree else msa.m3_window_attention_paged)(**x)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_paged_arguments(tree):
+    x = _paged()
+    fp8 = torch.float8_e4m3fn
+    for change, error in [
+        (dict(window_size=0), ValueError), (dict(sink_tokens=-2), ValueError), (dict(scale=float("nan")), ValueError),
+        (dict(q=x["q"].float()), NotImplementedError), (dict(q=x["q"].double()), TypeError), (dict(q=x["q"][0]), ValueError),
+        (dict(q=x["q"][:, :3]), ValueError), (dict(q=x["q"][:2]), ValueError), (dict(q=x["q"].half()), TypeError),
+        (dict(k_cache=x["k_cache"][0]), ValueError), (dict(k_cache=x["k_cache"][:, :, :8]), ValueError),
+        (dict(v_cache=x["v_cache"][:3]), ValueError), (dict(k_cache=x["k_cache"].transpose(2, 3)), ValueError),
+        (dict(k_scale=torch.ones(4, 2)), ValueError), (dict(page_table=x["page_table"].long()), TypeError),
+        (dict(page_table=x["page_table"][:1]), ValueError), (dict(context_lens=None), TypeError),
+        (dict(context_lens=x["context_lens"].long()), TypeError), (dict(context_lens=x["context_lens"][:1]), ValueError),
+        (dict(cu_seqlens=cu_tensor([1, 3])), ValueError), (dict(cu_seqlens=torch.tensor([0, 1, 3])), TypeError),
+    ]:
+        with pytest.raises(error):
+            _serve(tree, **dict(x, **change))
+    for x in (_paged(cache=fp8), dict(_paged(cache=fp8, scales=True), k_scale=torch.ones(4, 2).half()),
+              dict(_paged(cache=fp8, scales=True), v_scale=torch.ones(4, 1))):
+        with pytest.raises(ValueError):
+            _serve(tree, **x)
+    for x in (_paged(d=24), _paged(d=272)):
+        with pytest.raises(NotImplementedError):
+            _serve(tree, **x)
+    with pytest.raises(RuntimeError, match="no CPU execution path"):
+        _serve(tree, **_paged(cache=fp8, scales=True))
+
+
+def test_parents():
+    x = _paged()
+    for parents, error in ((None, TypeError), ([-1, -1, 0], TypeError), (torch.zeros(3), TypeError),
+                           (torch.zeros(3, dtype=torch.int64), TypeError), (torch.zeros(2, dtype=torch.int32), ValueError),
+                           (torch.zeros(3, 1, dtype=torch.int32), ValueError),
+                           (torch.zeros(3, dtype=torch.int32, device="meta"), ValueError)):
+        with pytest.raises(error):
+            _serve(True, **x, parents=parents)
+    with pytest.raises(NotImplementedError, match="1024 nodes"):
+        _serve(True, **_paged(tokens=1026))
