@@ -10,11 +10,16 @@
 
 namespace msa {
 
-// A packed tensor [T, heads, D] with free strides over tokens and heads.
+// A packed tensor [T, heads, D] with free strides over tokens and heads, so small that 33 tokens and the heads of a key head lie
+// within 2^30 elements: a tile's rows are at 32-bit offsets from an address that the whole wave shares.
 struct PackedView {
   const void* base;
-  int64_t token, head;  // elements
+  int token, head;  // elements
+  __device__ __forceinline__ int64_t at(int64_t t, int h) const { return t * token + static_cast<int64_t>(h) * head; }
 };
+inline PackedView packed_view(const void* base, const int64_t* strides) {
+  return PackedView{base, static_cast<int>(strides[0]), static_cast<int>(strides[1])};
+}
 
 struct Visible {
   int window;  // 2^31 - 1: none
@@ -29,19 +34,20 @@ struct TilePlace {
   int seq, start, n, tile;
 };
 
-// Tiles of `size` units, `per_token` of them a token, sequence by sequence: sequence s has the numbers from
+// Tiles of 2^size_log2 units, `per_token` of them a token, sequence by sequence: sequence s has the numbers from
 // cu[s] per_token / size + s on, which leaves each of them at least as many as it has tiles (a number behind its last
 // tile stands for nothing), so that no prefix sum over the sequences is needed. tile_numbers() of them in all.
-template <int SIZE>
-__device__ __forceinline__ TilePlace tile_place(const int32_t* __restrict__ cu, int nseq, int64_t number, int per_token) {
-  const auto first = [&](int s) { return static_cast<int64_t>(static_cast<uint64_t>(cu[s]) * per_token / SIZE) + s; };
+__device__ __forceinline__ TilePlace tile_place(const int32_t* __restrict__ cu, int nseq, int64_t number, int per_token,
+                                                int size_log2) {
+  const auto first = [&](int s) { return (static_cast<int64_t>(cu[s]) * per_token >> size_log2) + s; };
   const int s = __builtin_amdgcn_readfirstlane(nseq == 1 ? 0 : wave_upper_index(nseq, number, first));
   const int start = cu[s];
   return TilePlace{s, start, cu[s + 1] - start, static_cast<int>(number - first(s))};
 }
-inline int64_t tile_numbers(int64_t tokens, int64_t nseq, int64_t per_token, int64_t size) {
-  return tokens * per_token / size + nseq;
+inline int64_t tile_numbers(int64_t tokens, int64_t nseq, int64_t per_token, int size_log2) {
+  return (tokens * per_token >> size_log2) + nseq;
 }
+constexpr int log2_of(int size) { return size <= 1 ? 0 : 1 + log2_of(size / 2); }
 
 // x / d for x < 2^31.
 struct Divisor {
@@ -137,30 +143,53 @@ __device__ __forceinline__ Fragment<DT> pack_fragment(const float (&x)[8]) {
   return f;
 }
 
+// The same in two halves: elements 4 half .. 4 half + 3 of f.
+template <int DT>
+__device__ __forceinline__ void pack_half(Fragment<DT>& f, int half, f32x4 x) {
+  if constexpr (DT == kF32) {
+    if (half == 0) f.a = x; else f.b = x;
+  } else {
+    auto two = [](float a, float b) { return DT == kF16 ? cvt_pk_f16(a, b) : cvt_pk_bf16(a, b); };
+    uint4 w = __builtin_bit_cast(uint4, f.v);
+    if (half == 0) w.x = two(x[0], x[1]), w.y = two(x[2], x[3]);
+    else w.z = two(x[0], x[1]), w.w = two(x[2], x[3]);
+    f.v = __builtin_bit_cast(bf16x8, w);
+  }
+}
+
 // Rows [0, ROWS) of a tile by a workgroup of 256: 16-byte pieces through registers, zeros past D.
 template <int DT, int DP, int ROWS>
 struct TileLoad {
   using E = typename Fragment<DT>::Element;
-  static constexpr int kPer = 16 / sizeof(E);        // values of a piece
-  static constexpr int kLanes = DP / kPer;           // lanes of a row
-  static constexpr int kRows = 256 / kLanes;         // rows at once
-  static constexpr int kPieces = ROWS / kRows;
-  static_assert(256 % kLanes == 0 && ROWS % kRows == 0, "whole rows");
+  static constexpr int kPer = 16 / sizeof(E);   // values of a piece
+  static constexpr int kLanes = DP / kPer;      // pieces of a row
+  static constexpr int kAll = ROWS * kLanes;
+  static constexpr int kPieces = (kAll + 255) / 256;
   uint4 r[kPieces];
-  static __device__ __forceinline__ int row(int p) { return p * kRows + threadIdx.x / kLanes; }
-  static __device__ __forceinline__ int dim() { return threadIdx.x % kLanes * kPer; }
+  static __device__ __forceinline__ int piece(int p) {
+    const int i = p * 256 + static_cast<int>(threadIdx.x);
+    return kAll % 256 == 0 ? i : min(i, kAll - 1);
+  }
+  static __device__ __forceinline__ int row(int p) { return piece(p) / kLanes; }
+  static __device__ __forceinline__ int dim(int p) { return piece(p) % kLanes * kPer; }
+  // offset(row): elements from base to the row (to any row that exists where it is not wanted)
+  template <class Offset>
+  __device__ __forceinline__ void load_near(int D, const E* base, Offset offset) {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+      r[p] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(base) +
+                                             static_cast<uint32_t>(offset(row(p)) + (dim(p) < D ? dim(p) : 0)) * uint32_t{sizeof(E)});
+  }
   // at(row): address of the row in memory (of any row that exists where it is not wanted)
   template <class At>
   __device__ __forceinline__ void load(int D, At at) {
-    const int d = dim() < D ? dim() : 0;
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) r[p] = *reinterpret_cast<const uint4*>(at(row(p)) + d);
+    for (int p = 0; p < kPieces; ++p) r[p] = *reinterpret_cast<const uint4*>(at(row(p)) + (dim(p) < D ? dim(p) : 0));
   }
   __device__ __forceinline__ void store(E* tile, int stride, int D) const {
-    const bool there = dim() < D;
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p)
-      *reinterpret_cast<uint4*>(tile + row(p) * stride + dim()) = there ? r[p] : make_uint4(0u, 0u, 0u, 0u);
+    for (int p = 0; p < kPieces; ++p)  // (a last piece that several threads hold is written by all of them alike)
+      *reinterpret_cast<uint4*>(tile + row(p) * stride + dim(p)) = dim(p) < D ? r[p] : make_uint4(0u, 0u, 0u, 0u);
   }
 };
 
@@ -194,7 +223,12 @@ __device__ __forceinline__ f32x4 left_out(f32x4 x) {
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 
-constexpr float kLn2Window = 0.69314718055994531f;
+constexpr float kLn2Window = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
+
+inline bool near_rows(const int64_t* strides, int64_t ratio) {
+  return strides[0] >= 0 && strides[1] >= 0 && strides[0] < (1 << 25) && strides[1] < (1 << 30) &&
+         33 * strides[0] + ratio * strides[1] < (1 << 30);
+}
 
 // What the packed entry points check. strides: token and head strides of q, k, v (elements).
 inline bool valid_window_call(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
@@ -207,6 +241,8 @@ inline bool valid_window_call(const void* q, const void* k, const void* v, int32
   const int unit = dtype == kF32 ? 4 : 8;  // 16 bytes
   for (int i = 0; i < 6; ++i)
     if (strides[i] % unit) return false;
+  for (int i = 0; i < 6; i += 2)
+    if (!near_rows(strides + i, q_heads / groups)) return false;
   return reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 &&
          reinterpret_cast<uintptr_t>(v) % 16 == 0;
 }

@@ -20,7 +20,7 @@
 namespace msa {
 namespace {
 
-constexpr int kChunk = 1024;  // tokens of a chunk of the rows that see first tokens from behind the window
+constexpr int kChunk = 256;  // tokens of a chunk of the rows that see first tokens from behind the window
 
 struct WindowBwdArgs {
   PackedView q, k, v, dout;
@@ -36,7 +36,10 @@ struct WindowBwdArgs {
   float* delta;               // [T][Hq]
   void *dq, *dk, *dv;         // [T][Hq][D], [T][G][D]; null: not wanted
   float* part;                // [chunk numbers][sink tiles][G][2][sink rows][D]
+  float* split;               // [splits][2][T][G][D]
+  int splits;                 // workgroups that share the rows of a tile of keys
   int sink_tiles, sink_rows;  // of a tile
+  int chunk_log2;             // tokens of a chunk of the rows that see first tokens from behind the window
 };
 
 // ---- delta: 16 lanes a row
@@ -90,6 +93,14 @@ struct Range {
   __device__ __forceinline__ float down() const { return up == 0.f ? 0.f : cap * 0x1p-15f; }
 };
 
+// The first four fp16 elements of f times a power of two (downwards).
+__device__ __forceinline__ void rescale_half(Fragment<kF16>& f, float factor) {
+  uint4 w = __builtin_bit_cast(uint4, f.v);
+  w.x = cvt_pk_f16(lo16_f32<kF16>(w.x) * factor, hi16_f32<kF16>(w.x) * factor);
+  w.y = cvt_pk_f16(lo16_f32<kF16>(w.y) * factor, hi16_f32<kF16>(w.y) * factor);
+  f.v = __builtin_bit_cast(bf16x8, w);
+}
+
 // ---- dQ
 
 // The gradient of one row, key by key, by a wave: where a value that is not finite met the products of a tile, which
@@ -99,11 +110,11 @@ __device__ __forceinline__ void careful_dq(const WindowBwdArgs& A, int start, in
   using E = typename Fragment<DT>::Element;
   const int lane = threadIdx.x & 63;
   const int64_t t = start + static_cast<int64_t>(tok), row = t * (A.G * A.ratio.d) + head;
-  const E* q = static_cast<const E*>(A.q.base) + t * A.q.token + head * A.q.head;
-  const E* dout = static_cast<const E*>(A.dout.base) + t * A.dout.token + head * A.dout.head;
-  const E* k = static_cast<const E*>(A.k.base) + start * A.k.token + g * A.k.head;
-  const E* v = static_cast<const E*>(A.v.base) + start * A.v.token + g * A.v.head;
-  const float lse = A.lse[row], shift = -lse / kLn2Window, delta = A.delta[row];
+  const E* q = static_cast<const E*>(A.q.base) + A.q.at(t, head);
+  const E* dout = static_cast<const E*>(A.dout.base) + A.dout.at(t, head);
+  const E* k = static_cast<const E*>(A.k.base) + A.k.at(start, g);
+  const E* v = static_cast<const E*>(A.v.base) + A.v.at(start, g);
+  const float lse = A.lse[row], shift = lse * -kLog2e, delta = A.delta[row];
   const int low = A.seen.low(tok);
   float o[4] = {0.f, 0.f, 0.f, 0.f};
   bool lost = false;  // a ds of NaN: no dim is left
@@ -112,8 +123,8 @@ __device__ __forceinline__ void careful_dq(const WindowBwdArgs& A, int start, in
       const int j = min(base + lane, to - 1), count = min(kWave, to - base);
       float x = 0.f, dp = 0.f;
       for (int d = 0; d < A.D; ++d) {
-        x = fmaf(value_at<DT>(q, d), value_at<DT>(k + j * A.k.token, d), x);
-        dp = fmaf(value_at<DT>(dout, d), value_at<DT>(v + j * A.v.token, d), dp);
+        x = fmaf(value_at<DT>(q, d), value_at<DT>(k + static_cast<int64_t>(j) * A.k.token, d), x);
+        dp = fmaf(value_at<DT>(dout, d), value_at<DT>(v + static_cast<int64_t>(j) * A.v.token, d), dp);
       }
       const float ds = __builtin_amdgcn_exp2f(fmaf(x, A.scale_log2, shift)) * (dp - delta);
       lost = __any(ds != ds);
@@ -122,7 +133,7 @@ __device__ __forceinline__ void careful_dq(const WindowBwdArgs& A, int start, in
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int d = lane + u * kWave;
-          if (d < A.D) o[u] = fmaf(ds_i, value_at<DT>(k + (base + i) * A.k.token, d), o[u]);
+          if (d < A.D) o[u] = fmaf(ds_i, value_at<DT>(k + static_cast<int64_t>(base + i) * A.k.token, d), o[u]);
         }
       }
     }
@@ -137,7 +148,7 @@ __device__ __forceinline__ void careful_dq(const WindowBwdArgs& A, int start, in
 }
 
 template <int DT, int NK, int MT, int KS>
-__global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowBwdArgs A) {
+__global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dq_kernel(WindowBwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
   __shared__ alignas(16) E kbuf[2][KS * RS], vbuf[2][KS * RS];
@@ -145,15 +156,15 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowBwdArgs A) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t item = A.first + blockIdx.x;
   const int g = static_cast<int>(item % A.G), ratio = A.ratio.d;
-  const TilePlace at = tile_place<R>(A.cu, A.nseq, item / A.G, ratio);
+  const TilePlace at = tile_place(A.cu, A.nseq, item / A.G, ratio, log2_of(R));
   const int64_t rows = static_cast<int64_t>(at.n) * ratio, r0 = static_cast<int64_t>(at.tile) * R;
   if (r0 >= rows) return;
   const int live = static_cast<int>(min(rows - r0, int64_t{R}));
   auto token_of = [&](int r) { return A.ratio(static_cast<int>(r0) + r); };
   const int t0 = token_of(0), t1 = token_of(live - 1);
 
-  const E* kbase = static_cast<const E*>(A.k.base) + at.start * A.k.token + g * A.k.head;
-  const E* vbase = static_cast<const E*>(A.v.base) + at.start * A.v.token + g * A.v.head;
+  const E* kbase = static_cast<const E*>(A.k.base) + A.k.at(at.start, g);
+  const E* vbase = static_cast<const E*>(A.v.base) + A.v.at(at.start, g);
   int tok[MT], head[MT];
   float shift[MT], delta[MT];
   Fragment<DT> qf[MT][NK], gf[MT][NK];
@@ -163,15 +174,15 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowBwdArgs A) {
     tok[m] = token_of(r);
     head[m] = g * ratio + static_cast<int>(r0) + r - tok[m] * ratio;
     const int64_t t = at.start + static_cast<int64_t>(tok[m]);
-    const E* q = static_cast<const E*>(A.q.base) + t * A.q.token + head[m] * A.q.head;
-    const E* dout = static_cast<const E*>(A.dout.base) + t * A.dout.token + head[m] * A.dout.head;
+    const E* q = static_cast<const E*>(A.q.base) + A.q.at(t, head[m]);
+    const E* dout = static_cast<const E*>(A.dout.base) + A.dout.at(t, head[m]);
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
       const int d = 32 * kk + 8 * q4;
       qf[m][kk] = d < A.D ? fragment_at<DT>(q + d) : no_fragment<DT>();
       gf[m][kk] = d < A.D ? fragment_at<DT>(dout + d) : no_fragment<DT>();
     }
-    shift[m] = -A.lse[t * (A.G * ratio) + head[m]] / kLn2Window;
+    shift[m] = A.lse[t * (A.G * ratio) + head[m]] * -kLog2e;
     delta[m] = A.delta[t * (A.G * ratio) + head[m]];
     if (shift[m] == __builtin_inff()) shift[m] = -__builtin_inff();  // (no weights)
   }
@@ -184,8 +195,8 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowBwdArgs A) {
   TileLoad<DT, DP, KS> kload, vload;
   auto load_step = [&](int e) {
     const int j0 = first_key(e);
-    kload.load(A.D, [&](int r) { return kbase + min(j0 + r, t1) * A.k.token; });
-    vload.load(A.D, [&](int r) { return vbase + min(j0 + r, t1) * A.v.token; });
+    kload.load_near(A.D, kbase + static_cast<int64_t>(j0) * A.k.token, [&](int r) { return min(r, t1 - j0) * A.k.token; });
+    vload.load_near(A.D, vbase + static_cast<int64_t>(j0) * A.v.token, [&](int r) { return min(r, t1 - j0) * A.v.token; });
   };
   auto store_step = [&](int e) {
     kload.store(kbuf[e & 1], RS, A.D);
@@ -310,8 +321,8 @@ __device__ __forceinline__ void careful_dkv(const WindowBwdArgs& A, int start, i
   using E = typename Fragment<DT>::Element;
   const int lane = threadIdx.x & 63, ratio = A.ratio.d;
   const int64_t t = start + static_cast<int64_t>(j);
-  const E* k = static_cast<const E*>(A.k.base) + t * A.k.token + g * A.k.head;
-  const E* v = static_cast<const E*>(A.v.base) + t * A.v.token + g * A.v.head;
+  const E* k = static_cast<const E*>(A.k.base) + A.k.at(t, g);
+  const E* v = static_cast<const E*>(A.v.base) + A.v.at(t, g);
   const int end = (j < A.seen.sinks || A.seen.window >= n - j ? n : j + A.seen.window) * ratio;
   float ok[4] = {0.f, 0.f, 0.f, 0.f}, ov[4] = {0.f, 0.f, 0.f, 0.f};
   bool lost_k = false, lost_v = false;  // a ds (a p) of NaN: no dim is left
@@ -319,15 +330,15 @@ __device__ __forceinline__ void careful_dkv(const WindowBwdArgs& A, int start, i
     const int r = min(base + lane, end - 1), count = min(kWave, end - base);
     const int64_t tr = start + static_cast<int64_t>(A.ratio(r));
     const int head = g * ratio + r - A.ratio(r) * ratio;
-    const E* q = static_cast<const E*>(A.q.base) + tr * A.q.token + head * A.q.head;
-    const E* dout = static_cast<const E*>(A.dout.base) + tr * A.dout.token + head * A.dout.head;
+    const E* q = static_cast<const E*>(A.q.base) + A.q.at(tr, head);
+    const E* dout = static_cast<const E*>(A.dout.base) + A.dout.at(tr, head);
     const float lse = A.lse[tr * (A.G * ratio) + head];
     float x = 0.f, dp = 0.f;
     for (int d = 0; d < A.D; ++d) {
       x = fmaf(value_at<DT>(q, d), value_at<DT>(k, d), x);
       dp = fmaf(value_at<DT>(dout, d), value_at<DT>(v, d), dp);
     }
-    const float p = lse == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(fmaf(x, A.scale_log2, -lse / kLn2Window));
+    const float p = lse == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(fmaf(x, A.scale_log2, lse * -kLog2e));
     const float ds = p * (dp - A.delta[tr * (A.G * ratio) + head]);
     lost_k |= __any(ds != ds) != 0;
     lost_v |= __any(p != p) != 0;
@@ -335,8 +346,8 @@ __device__ __forceinline__ void careful_dkv(const WindowBwdArgs& A, int start, i
       const float p_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), i));
       const float ds_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ds), i));
       const int ti = A.ratio(base + i), hi = g * ratio + base + i - ti * ratio;
-      const E* qi = static_cast<const E*>(A.q.base) + (start + static_cast<int64_t>(ti)) * A.q.token + hi * A.q.head;
-      const E* gi = static_cast<const E*>(A.dout.base) + (start + static_cast<int64_t>(ti)) * A.dout.token + hi * A.dout.head;
+      const E* qi = static_cast<const E*>(A.q.base) + A.q.at(start + static_cast<int64_t>(ti), hi);
+      const E* gi = static_cast<const E*>(A.dout.base) + A.dout.at(start + static_cast<int64_t>(ti), hi);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int d = lane + u * kWave;
@@ -355,15 +366,26 @@ __device__ __forceinline__ void careful_dkv(const WindowBwdArgs& A, int start, i
   }
 }
 
+// What the rows behind the window give for first tokens: floats of one chunk, and the part of a chunk, tile and key head.
+__device__ __forceinline__ int64_t sink_chunk_floats(const WindowBwdArgs& A) {
+  return int64_t{2} * A.sink_rows * A.D * A.G * A.sink_tiles;
+}
+__device__ __forceinline__ float* sink_part(const WindowBwdArgs& A, int start, int seq, int chunk, int tile, int g) {
+  const int64_t number = (static_cast<int64_t>(start) >> A.chunk_log2) + seq + chunk;
+  return A.part + ((number * A.sink_tiles + tile) * A.G + g) * 2 * A.sink_rows * A.D;
+}
+
 // SINKS: the rows of one chunk that see the first tokens from behind the window; their sums go to A.part.
 template <int DT, int NK, int KT, bool SINKS>
-__global__ __launch_bounds__(256, 1) void window_dkv_kernel(WindowBwdArgs A) {
+__global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dkv_kernel(WindowBwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, BK = 64 * KT, QS = 32;
   constexpr float kUp = DT == kF16 ? 15.f : 0.f;
-  __shared__ alignas(16) E qbuf[2][QS * RS], gbuf[2][QS * RS];
-  __shared__ alignas(16) float shift_of[2][QS], delta_of[2][QS];
-  __shared__ alignas(16) int token_at[2][QS];
+  constexpr int kBuffers = NK <= 4 || DT == kF32 ? 2 : 1;  // (of LDS for two workgroups a CU)
+  constexpr bool kValuesInLds = DT != kF32;  // (in registers with the keys they would leave room for one wave a SIMD)
+  __shared__ alignas(16) E qbuf[kBuffers][QS * RS], gbuf[kBuffers][QS * RS], values[kValuesInLds ? BK * RS : 8];
+  __shared__ alignas(16) float shift_of[kBuffers][QS], delta_of[kBuffers][QS];
+  __shared__ alignas(16) int token_at[kBuffers][QS];
   const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int64_t item = A.first + blockIdx.x;
@@ -372,41 +394,60 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(WindowBwdArgs A) {
   TilePlace at;
   int j0, from, to;  // first key; tokens of the rows
   int64_t number = item;
+  int z = 0;  // which split of them
   if constexpr (SINKS) {
     number = item / A.sink_tiles;
-    at = tile_place<kChunk>(A.cu, A.nseq, number, 1);
+    at = tile_place(A.cu, A.nseq, number, 1, A.chunk_log2);
     j0 = static_cast<int>(item - number * A.sink_tiles) * BK;
-    const int64_t behind = static_cast<int64_t>(j0) + BK - 1 + A.seen.window, start = static_cast<int64_t>(at.tile) * kChunk;
+    const int64_t behind = static_cast<int64_t>(j0) + BK - 1 + A.seen.window, start = static_cast<int64_t>(at.tile) << A.chunk_log2;
     if (max(behind, start) >= at.n) return;
     from = static_cast<int>(max(behind, start));
-    to = static_cast<int>(min(start + kChunk, static_cast<int64_t>(at.n)));
+    to = static_cast<int>(min(start + (1 << A.chunk_log2), static_cast<int64_t>(at.n)));
     if (from >= to) return;
   } else {
-    at = tile_place<BK>(A.cu, A.nseq, item, 1);
+    number = item / A.splits;
+    z = static_cast<int>(item - number * A.splits);
+    at = tile_place(A.cu, A.nseq, number, 1, log2_of(BK));
     if (static_cast<int64_t>(at.tile) * BK >= at.n) return;
     j0 = at.tile * BK;
     from = j0;
     to = static_cast<int>(min(static_cast<int64_t>(at.n), static_cast<int64_t>(j0) + BK - 1 + A.seen.window));
   }
-  const int rb = from * ratio, re = to * ratio;
+  int rb = from * ratio, re = to * ratio;
+  if (!SINKS && A.splits > 1) {
+    const int share = ((re - rb + A.splits - 1) / A.splits + QS - 1) / QS * QS;
+    rb = min(re, rb + z * share);
+    re = min(re, rb + share);
+  }
 
   // keys of this wave: [ka, kb], lane c one of each 16
   const int ka = j0 + 16 * KT * wave, last = SINKS ? min(at.n, A.seen.sinks) - 1 : at.n - 1;
   const int kb = min(ka + 16 * KT - 1, last);
   const bool has_keys = ka <= last;
-  Fragment<DT> kf[KT][NK], vf[KT][NK];
+  Fragment<DT> kf[KT][NK], vf[kValuesInLds ? 1 : KT][kValuesInLds ? 1 : NK];
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
     const int64_t t = at.start + static_cast<int64_t>(min(ka + 16 * kt + c, at.n - 1));
-    const E* k = static_cast<const E*>(A.k.base) + t * A.k.token + g * A.k.head;
-    const E* v = static_cast<const E*>(A.v.base) + t * A.v.token + g * A.v.head;
+    const E* k = static_cast<const E*>(A.k.base) + A.k.at(t, g);
+    const E* v = static_cast<const E*>(A.v.base) + A.v.at(t, g);
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
       const int d = 32 * kk + 8 * q4;
       kf[kt][kk] = d < A.D ? fragment_at<DT>(k + d) : no_fragment<DT>();
-      vf[kt][kk] = d < A.D ? fragment_at<DT>(v + d) : no_fragment<DT>();
+      if constexpr (!kValuesInLds) vf[kt][kk] = d < A.D ? fragment_at<DT>(v + d) : no_fragment<DT>();
     }
   }
+  if constexpr (kValuesInLds) {
+    TileLoad<DT, DP, BK> load;
+    load.load(A.D, [&](int r) {
+      return static_cast<const E*>(A.v.base) + (at.start + static_cast<int64_t>(min(j0 + r, at.n - 1))) * A.v.token + g * A.v.head;
+    });
+    load.store(values, RS, A.D);
+  }
+  auto value_fragment = [&](int kt, int kk) {
+    if constexpr (kValuesInLds) return fragment_at<DT>(values + (16 * (KT * wave + kt) + c) * RS + 32 * kk + 8 * q4);
+    else return vf[kt][kk];
+  };
   f32x4 dk[KT][ND], dv[KT][ND];
   Range range[KT];
 #pragma unroll
@@ -418,21 +459,24 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(WindowBwdArgs A) {
   float own_shift = 0.f, own_delta = 0.f;
   int own_token = -1;
   auto load_step = [&](int r0) {
-    auto row_of = [&](const PackedView& x, int r) {
-      r = min(r, re - 1);
-      const int t = A.ratio(r);
-      return static_cast<const E*>(x.base) + (at.start + static_cast<int64_t>(t)) * x.token +
-             (g * ratio + r - t * ratio) * x.head;
+    // (tokens and heads from those of the step's first row on)
+    const int t0 = A.ratio(r0), h0 = r0 - t0 * ratio, end = re - 1 - t0 * ratio;
+    auto token_of = [&](int r) { return A.ratio(min(h0 + r, end)); };
+    auto offset = [&](const PackedView& x, int r) {
+      const int t = token_of(r);
+      return t * x.token + (min(h0 + r, end) - t * ratio) * x.head;
     };
-    qload.load(A.D, [&](int r) { return row_of(A.q, r0 + r); });
-    gload.load(A.D, [&](int r) { return row_of(A.dout, r0 + r); });
+    const int64_t first = at.start + static_cast<int64_t>(t0);
+    qload.load_near(A.D, static_cast<const E*>(A.q.base) + A.q.at(first, g * ratio), [&](int r) { return offset(A.q, r); });
+    gload.load_near(A.D, static_cast<const E*>(A.dout.base) + A.dout.at(first, g * ratio), [&](int r) { return offset(A.dout, r); });
     if (threadIdx.x < QS) {
-      const int r = min(r0 + static_cast<int>(threadIdx.x), re - 1), t = A.ratio(r);
-      const int64_t row = (at.start + static_cast<int64_t>(t)) * (A.G * ratio) + g * ratio + r - t * ratio;
-      const float lse = A.lse[row];
-      own_shift = lse == -__builtin_inff() ? -__builtin_inff() : -lse / kLn2Window;
-      own_delta = A.delta[row];
-      own_token = r0 + static_cast<int>(threadIdx.x) < re ? t : -1;  // (no row: sees nothing)
+      const int r = min(h0 + static_cast<int>(threadIdx.x), end), t = A.ratio(r);
+      const int64_t row = first * (A.G * ratio) + g * ratio;
+      const uint32_t own = t * (A.G * ratio) + r - t * ratio;
+      const float lse = A.lse[row + own];
+      own_shift = lse == -__builtin_inff() ? -__builtin_inff() : lse * -kLog2e;
+      own_delta = A.delta[row + own];
+      own_token = h0 + static_cast<int>(threadIdx.x) <= end ? t0 + t : -1;  // (no row: sees nothing)
     }
   };
   auto store_step = [&](int b) {
@@ -442,72 +486,73 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(WindowBwdArgs A) {
       shift_of[b][threadIdx.x] = own_shift, delta_of[b][threadIdx.x] = own_delta, token_at[b][threadIdx.x] = own_token;
   };
 
-  load_step(rb);
-  store_step(0);
+  if (rb < re) {
+    load_step(rb);
+    store_step(0);
+  }
   int b = 0;
-  for (int r0 = rb; r0 < re; r0 += QS, b ^= 1) {
+  for (int r0 = rb; r0 < re; r0 += QS, b ^= kBuffers - 1) {
     __syncthreads();
     const bool more = r0 + QS < re;
     if (more) load_step(r0 + QS);
     const int ta = A.ratio(r0), tb = A.ratio(min(r0 + QS, re) - 1);
     if (has_keys && tb >= ka && (ta - kb < A.seen.window || ka < A.seen.sinks)) {
       const E *qt = qbuf[b], *gt = gbuf[b];
-      f32x4 s[2][KT], dp[2][KT];
+      const bool whole = r0 + QS <= re && ta >= kb && (tb - ka < A.seen.window || kb < A.seen.sinks);
+      Fragment<DT> pf[KT], df[KT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) pf[kt] = df[kt] = no_fragment<DT>();
+      // (16 rows after the other: both at once take more registers than two waves a SIMD have)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        f32x4 s[KT], dp[KT];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) s[h][kt] = dp[h][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int kt = 0; kt < KT; ++kt) s[kt] = dp[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
           const Fragment<DT> qf = fragment_at<DT>(qt + (16 * h + c) * RS + 32 * kk + 8 * q4);
           const Fragment<DT> gf = fragment_at<DT>(gt + (16 * h + c) * RS + 32 * kk + 8 * q4);
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) {
-            s[h][kt] = product<DT>(qf, kf[kt][kk], s[h][kt]);
-            dp[h][kt] = product<DT>(gf, vf[kt][kk], dp[h][kt]);
+            s[kt] = product<DT>(qf, kf[kt][kk], s[kt]);
+            dp[kt] = product<DT>(gf, value_fragment(kt, kk), dp[kt]);
           }
         }
-      }
-      const bool whole = r0 + QS <= re && ta >= kb && (tb - ka < A.seen.window || kb < A.seen.sinks);
-      Fragment<DT> pf[KT], df[KT];
-      f32x4 shift[2], delta[2];
+        const f32x4 shift = *reinterpret_cast<const f32x4*>(&shift_of[b][16 * h + 4 * q4]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_of[b][16 * h + 4 * q4]);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        shift[h] = *reinterpret_cast<const f32x4*>(&shift_of[b][16 * h + 4 * q4]);
-        delta[h] = *reinterpret_cast<const f32x4*>(&delta_of[b][16 * h + 4 * q4]);
-      }
+        for (int kt = 0; kt < KT; ++kt) {
+          f32x4 p, ds;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        float p[8], ds[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][kt][i & 3], A.scale_log2, shift[i >> 2][i & 3]));
-          ds[i] = p[i] * (dp[i >> 2][kt][i & 3] - delta[i >> 2][i & 3]);
-        }
-        if (!whole) {
-          const int j = ka + 16 * kt + c;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const bool seen = A.seen(token_at[b][16 * (i >> 2) + 4 * q4 + (i & 3)], j);
-            p[i] = seen ? p[i] : 0.f;
-            ds[i] = seen ? ds[i] : 0.f;
+          for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], A.scale_log2, shift[i]));
+            ds[i] = p[i] * (dp[kt][i] - delta[i]);
           }
-        }
-        if constexpr (DT == kF16) {
-          float big = 0.f;
+          if (!whole) {
+            const int j = ka + 16 * kt + c;
+            const int4 tok = *reinterpret_cast<const int4*>(&token_at[b][16 * h + 4 * q4]);
+            const int toks[4] = {tok.x, tok.y, tok.z, tok.w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(ds[i]));
-          big = quad_max(big);
-          if (__any(big >= range[kt].cap && big != 0.f)) {
-            const float factor = range[kt].widen(big);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) dk[kt][d] *= factor;
+            for (int i = 0; i < 4; ++i) {
+              const bool seen = A.seen(toks[i], j);
+              p[i] = seen ? p[i] : 0.f;
+              ds[i] = seen ? ds[i] : 0.f;
+            }
           }
+          if constexpr (DT == kF16) {
+            const float big = quad_max(fmaxf(fmaxf(fabsf(ds[0]), fabsf(ds[1])), fmaxf(fabsf(ds[2]), fabsf(ds[3]))));
+            if (__any(big >= range[kt].cap && big != 0.f)) {
+              const float factor = range[kt].widen(big);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ds[i] *= range[kt].up, p[i] *= 0x1p15f;
+              for (int d = 0; d < ND; ++d) dk[kt][d] *= factor;
+              if (h == 1) rescale_half(df[kt], factor);
+            }
+            ds *= range[kt].up, p *= 0x1p15f;
+          }
+          pack_half<DT>(pf[kt], h, p);
+          pack_half<DT>(df[kt], h, ds);
         }
-        pf[kt] = pack_fragment<DT>(p);
-        df[kt] = pack_fragment<DT>(ds);
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
@@ -520,51 +565,48 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(WindowBwdArgs A) {
         }
       }
     }
-    if (more) store_step(b ^ 1);
+    if (kBuffers == 1) __syncthreads();
+    if (more) store_step(b ^ (kBuffers - 1));
   }
 
-  const int64_t tile_floats = int64_t{2} * A.sink_rows * A.D;  // of one chunk, tile of first tokens and key head
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
-    const int j = ka + 16 * kt + c, local = j - j0;
+    const int j = ka + 16 * kt + c;
+    const bool mine = j <= last;
     const float down_k = DT == kF16 ? A.scale * range[kt].down() : A.scale, down_v = kUp == 0.f ? 1.f : 0x1p-15f;
+    const int64_t row = (at.start + static_cast<int64_t>(mine ? j : 0)) * A.G + g;
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[kt][d] *= down_k, dv[kt][d] *= down_v;
-    if constexpr (SINKS) {
-      if (j > last) continue;
-      float* part = A.part + (item * A.G + g) * tile_floats + static_cast<int64_t>(local) * A.D;
+    if (SINKS || A.splits > 1) {  // parts of a sum
+      float* part = SINKS ? A.part + ((item * A.G + g) * 2 * A.sink_rows + j - j0) * A.D : A.split + (z * 2 * A.tokens * A.G + row) * A.D;
+      float* part_v = part + (SINKS ? A.sink_rows : A.tokens * A.G) * A.D;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
-        if (16 * d + 4 * q4 < A.D) {
+        if (mine && 16 * d + 4 * q4 < A.D) {
           *reinterpret_cast<f32x4*>(part + 16 * d + 4 * q4) = dk[kt][d];
-          *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(A.sink_rows) * A.D + 16 * d + 4 * q4) = dv[kt][d];
+          *reinterpret_cast<f32x4*>(part_v + 16 * d + 4 * q4) = dv[kt][d];
         }
     } else {
-      const bool mine = j < at.n;
-      if (mine && j < A.seen.sinks && to < at.n) {  // what the chunks of later rows gave
-        const int64_t chunk0 = static_cast<int64_t>(at.start) / kChunk + at.seq;
-        for (int ch = to / kChunk; ch <= (at.n - 1) / kChunk; ++ch) {
-          const float* part = A.part + (((chunk0 + ch) * A.sink_tiles + at.tile) * A.G + g) * tile_floats +
-                              static_cast<int64_t>(local) * A.D;
+      if (mine && j < A.seen.sinks && to < at.n) {
+        const float* part = sink_part(A, at.start, at.seq, to >> A.chunk_log2, at.tile, g) + static_cast<int64_t>(j - j0) * A.D + 4 * q4;
 #pragma unroll
-          for (int d = 0; d < ND; ++d)
-            if (16 * d + 4 * q4 < A.D) {
-              dk[kt][d] += *reinterpret_cast<const f32x4*>(part + 16 * d + 4 * q4);
-              dv[kt][d] += *reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(A.sink_rows) * A.D + 16 * d + 4 * q4);
-            }
-        }
+        for (int d = 0; d < ND; ++d)
+          if (16 * d + 4 * q4 < A.D) {
+            dk[kt][d] += *reinterpret_cast<const f32x4*>(part + 16 * d);
+            dv[kt][d] += *reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(A.sink_rows) * A.D + 16 * d);
+          }
       }
-      const int64_t row = (at.start + static_cast<int64_t>(mine ? j : 0)) * A.G + g;
       float all = 0.f;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
+      for (int d = 0; d < ND; ++d)
         all += ((dk[kt][d][0] + dk[kt][d][1]) + (dk[kt][d][2] + dk[kt][d][3])) +
                ((dv[kt][d][0] + dv[kt][d][1]) + (dv[kt][d][2] + dv[kt][d][3]));
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
         if (mine && 16 * d + 4 * q4 < A.D) {
           if (A.dk) store4<DT>(static_cast<E*>(A.dk) + row * A.D + 16 * d + 4 * q4, dk[kt][d]);
           if (A.dv) store4<DT>(static_cast<E*>(A.dv) + row * A.D + 16 * d + 4 * q4, dv[kt][d]);
         }
-      }
       uint64_t odd = __ballot(mine && !finite(all));
       odd |= odd >> 32, odd |= odd >> 16;
       for (uint32_t left = odd & 0xffffu; left; left &= left - 1)
@@ -573,17 +615,100 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(WindowBwdArgs A) {
   }
 }
 
+// The chunks' sums for first tokens added up in order, in the place of the first chunk: four values a thread, a workgroup 1024 of
+// a sequence, tile and key head.
+template <int BK>
+__global__ __launch_bounds__(256) void window_sink_sum(WindowBwdArgs A) {
+  const int64_t floats = int64_t{2} * A.sink_rows * A.D, blocks = (floats + 1023) / 1024;
+  const int64_t item = (A.first + blockIdx.x) / blocks, block = A.first + blockIdx.x - item * blocks;
+  const int64_t at = block * 1024 + threadIdx.x * 4, tiles = static_cast<int64_t>(A.sink_tiles) * A.G;
+  const int s = static_cast<int>(item / tiles), rest = static_cast<int>(item - s * tiles), tile = rest / A.G, g = rest - tile * A.G;
+  const int start = A.cu[s], n = A.cu[s + 1] - start;
+  const int64_t behind = static_cast<int64_t>(tile) * BK + BK - 1 + A.seen.window;
+  // (rows of the tile past the first tokens hold nothing and are not read)
+  const int row = static_cast<int>(at / A.D) % A.sink_rows;
+  if (behind >= n || at >= floats || tile * BK + row >= min(n, A.seen.sinks)) return;
+  const int first = static_cast<int>(behind) >> A.chunk_log2, end = (n - 1) >> A.chunk_log2;
+  float* part = sink_part(A, start, s, first, tile, g) + at;
+  const int64_t step = sink_chunk_floats(A);
+  f32x4 sum = *reinterpret_cast<const f32x4*>(part);
+#pragma unroll 8
+  for (int ch = 1; ch <= end - first; ++ch) sum += *reinterpret_cast<const f32x4*>(part + ch * step);
+  *reinterpret_cast<f32x4*>(part) = sum;
+}
+
+// The parts of a key's sums added up in order, a wave a key: those of its tile's splits, then that of the rows behind the
+// window, if it is a first token.
+template <int DT, int BK>
+__global__ __launch_bounds__(256) void window_dkv_join(WindowBwdArgs A) {
+  using E = typename Fragment<DT>::Element;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (A.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= A.tokens * A.G) return;
+  const int64_t t = row / A.G, plane = A.tokens * A.G * A.D;
+  const int g = static_cast<int>(row - t * A.G), d = 4 * lane;
+  const bool mine = d < A.D;
+  f32x4 dk = f32x4{0.f, 0.f, 0.f, 0.f}, dv = dk;
+  const float* part = A.split + row * A.D + (mine ? d : 0);
+#pragma unroll 4
+  for (int z = 0; z < A.splits; ++z, part += 2 * plane) {
+    dk += *reinterpret_cast<const f32x4*>(part);
+    dv += *reinterpret_cast<const f32x4*>(part + plane);
+  }
+  const int s = A.nseq == 1 ? 0 : wave_upper_index(A.nseq, t, [&](int i) { return static_cast<int64_t>(A.cu[i]); });
+  const int start = A.cu[s], n = A.cu[s + 1] - start, j = static_cast<int>(t - start), tile = j / BK;
+  const int64_t behind = static_cast<int64_t>(tile) * BK + BK - 1 + A.seen.window;  // tokens of the chunks: from here on
+  if (j < A.seen.sinks && behind < n) {
+    part = sink_part(A, start, s, static_cast<int>(behind) >> A.chunk_log2, tile, g) + static_cast<int64_t>(j - tile * BK) * A.D +
+           (mine ? d : 0);
+    dk += *reinterpret_cast<const f32x4*>(part);
+    dv += *reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(A.sink_rows) * A.D);
+  }
+  if (mine) {
+    if (A.dk) store4<DT>(static_cast<E*>(A.dk) + row * A.D + d, dk);
+    if (A.dv) store4<DT>(static_cast<E*>(A.dv) + row * A.D + d, dv);
+  }
+  const float all = ((dk[0] + dk[1]) + (dk[2] + dk[3])) + ((dv[0] + dv[1]) + (dv[2] + dv[3]));
+  if (__any(mine && !finite(all))) careful_dkv<DT>(A, start, n, g, j);
+}
+
 // Keys of a workgroup of the dK / dV kernels.
 int keys_per_tile(int32_t dtype, int64_t dim) { return dtype != kF32 && dim <= 128 ? 128 : 64; }
 
 // Tiles that hold first tokens, and their rows in one; 0 where no sequence has rows behind the window.
 struct SinkShape {
   int64_t tiles, rows;
+  int chunk_log2;
 };
-SinkShape sink_shape(int32_t dtype, int64_t dim, int64_t longest, int64_t window, int64_t sinks) {
-  if (window == 0 || sinks == 0 || longest <= window) return SinkShape{0, 0};
+SinkShape sink_shape(int32_t dtype, int64_t dim, int64_t tokens, int64_t longest, int64_t ratio, int64_t window, int64_t sinks) {
+  if (window == 0 || sinks == 0 || longest <= window) return SinkShape{0, 0, 0};
+  // 256 rows a chunk at least, and no more than 256 chunks in all
+  int chunk_log2 = 4;
+  while (ratio << chunk_log2 < 256 || tokens >> chunk_log2 > 256) ++chunk_log2;
   const int64_t keys = keys_per_tile(dtype, dim), most = sinks < longest ? sinks : longest;
-  return SinkShape{(most + keys - 1) / keys, most < keys ? (most + 15) / 16 * 16 : keys};
+  return SinkShape{(most + keys - 1) / keys, most < keys ? (most + 15) / 16 * 16 : keys, chunk_log2};
+}
+
+// Workgroups that share the rows of a tile of keys: so many that the largest share is not above what each of the workgroups
+// that run at once (512, or 256 of fp32) gets of all the work, which is at least that of the longest sequence and of
+// sequences of equal length; no more than give a share 128 rows, nor than fill 256 MiB with parts.
+int64_t split_count(int32_t dtype, int64_t tokens, int64_t nseq, int64_t longest, int64_t q_heads, int64_t groups, int64_t dim,
+                    int64_t window) {
+  const double keys = keys_per_tile(dtype, dim), w = window == 0 ? 1e18 : static_cast<double>(window);
+  const auto pairs = [&](double n) { return n <= w ? n * n / 2 : w * (n - w / 2); };
+  const double all = static_cast<double>(nseq) * pairs(static_cast<double>(tokens) / nseq), one = pairs(static_cast<double>(longest));
+  const double work = groups * (all > one ? all : one) / keys;  // tokens of rows that tiles go through
+  const double most = longest < w + keys ? longest : w + keys;
+  const int64_t even = static_cast<int64_t>(most * (dtype == kF32 ? 256 : 512) / (work < 1 ? 1 : work) + 0.5);
+  const int64_t by_rows = static_cast<int64_t>(most * (q_heads / groups) / 128), by_size = (int64_t{1} << 25) / (tokens * groups * dim);
+  int64_t n = even < by_rows ? even : by_rows;
+  n = n < by_size ? n : by_size;
+  return n < 1 ? 1 : n < 64 ? n : 64;
+}
+
+int64_t delta_floats(int64_t tokens, int64_t q_heads) { return (tokens * q_heads + 3) / 4 * 4; }
+int64_t sink_floats(const SinkShape& shape, int64_t tokens, int64_t nseq, int64_t groups, int64_t dim) {
+  return tile_numbers(tokens, nseq, 1, shape.chunk_log2) * shape.tiles * groups * 2 * shape.rows * dim;
 }
 
 }  // namespace
@@ -594,10 +719,13 @@ using namespace msa;
 extern "C" int64_t msa_window_attn_bwd_workspace_bytes(int32_t dtype, int64_t total_tokens, int64_t num_seqs,
                                                        int64_t longest, int64_t q_heads, int64_t kv_groups,
                                                        int64_t head_dim, int64_t window, int64_t sinks) {
-  if (total_tokens <= 0 || num_seqs <= 0 || q_heads <= 0 || kv_groups <= 0 || head_dim <= 0 || window < 0 || sinks < 0) return 0;
-  const SinkShape shape = sink_shape(dtype, head_dim, longest, window, sinks);
-  const int64_t rows = (total_tokens * q_heads + 3) / 4 * 4;
-  return 4 * (rows + tile_numbers(total_tokens, num_seqs, 1, kChunk) * shape.tiles * kv_groups * 2 * shape.rows * head_dim);
+  if (total_tokens <= 0 || num_seqs <= 0 || q_heads <= 0 || kv_groups <= 0 || q_heads % kv_groups || head_dim <= 0 || window < 0 ||
+      sinks < 0)
+    return 0;
+  const SinkShape shape = sink_shape(dtype, head_dim, total_tokens, longest, q_heads / kv_groups, window, sinks);
+  const int64_t splits = split_count(dtype, total_tokens, num_seqs, longest, q_heads, kv_groups, head_dim, window);
+  return 4 * (delta_floats(total_tokens, q_heads) + sink_floats(shape, total_tokens, num_seqs, kv_groups, head_dim) +
+              (splits > 1 ? splits * 2 * total_tokens * kv_groups * head_dim : 0));
 }
 
 extern "C" int msa_window_attn_bwd(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
@@ -611,18 +739,18 @@ extern "C" int msa_window_attn_bwd(const void* q, const void* k, const void* v, 
       !out || !lse || !grad_out || reinterpret_cast<uintptr_t>(grad_out) % 16 || longest < 0 || longest > total_tokens)
     return kErrInvalidArgument;
   const int unit = dtype == kF32 ? 4 : 8;
-  if (strides[6] % unit || strides[7] % unit) return kErrInvalidArgument;
+  if (strides[6] % unit || strides[7] % unit || !near_rows(strides + 6, q_heads / kv_groups)) return kErrInvalidArgument;
   if (!window_supported(dtype, head_dim, total_tokens, q_heads / kv_groups)) return kErrUnsupported;
   if (total_tokens == 0 || !(grad_q || grad_k || grad_v)) return kOk;
   if (!workspace || workspace_bytes < msa_window_attn_bwd_workspace_bytes(dtype, total_tokens, num_seqs, longest, q_heads,
                                                                           kv_groups, head_dim, window, sinks))
     return kErrInvalidArgument;
-  const SinkShape shape = sink_shape(dtype, head_dim, longest, window, sinks);
+  const SinkShape shape = sink_shape(dtype, head_dim, total_tokens, longest, q_heads / kv_groups, window, sinks);
   WindowBwdArgs A{};
-  A.q = PackedView{q, strides[0], strides[1]};
-  A.k = PackedView{k, strides[2], strides[3]};
-  A.v = PackedView{v, strides[4], strides[5]};
-  A.dout = PackedView{grad_out, strides[6], strides[7]};
+  A.q = packed_view(q, strides);
+  A.k = packed_view(k, strides + 2);
+  A.v = packed_view(v, strides + 4);
+  A.dout = packed_view(grad_out, strides + 6);
   A.cu = cu_seqlens;
   A.nseq = static_cast<int>(num_seqs);
   A.ratio = divisor_of(q_heads / kv_groups);
@@ -636,9 +764,12 @@ extern "C" int msa_window_attn_bwd(const void* q, const void* k, const void* v, 
   A.out_lo = out_lo;
   A.lse = lse;
   A.delta = static_cast<float*>(workspace);
-  A.part = A.delta + (total_tokens * q_heads + 3) / 4 * 4;
+  A.part = A.delta + delta_floats(total_tokens, q_heads);
+  A.split = A.part + sink_floats(shape, total_tokens, num_seqs, kv_groups, head_dim);
+  A.splits = static_cast<int>(split_count(dtype, total_tokens, num_seqs, longest, q_heads, kv_groups, head_dim, window));
   A.sink_tiles = static_cast<int>(shape.tiles);
   A.sink_rows = static_cast<int>(shape.rows);
+  A.chunk_log2 = shape.chunk_log2;
   A.dq = grad_q;
   A.dk = grad_k;
   A.dv = grad_v;
@@ -658,22 +789,32 @@ extern "C" int msa_window_attn_bwd(const void* q, const void* k, const void* v, 
 #define MSA_WINDOW_BWD(DT, NK, MT, KS, KT)                                                                                       \
   {                                                                                                                              \
     if (rc == kOk && grad_q)                                                                                                     \
-      MSA_WINDOW_LAUNCH((window_dq_kernel<DT, NK, MT, KS>), tile_numbers(total_tokens, num_seqs, A.ratio.d, 64 * MT) * kv_groups); \
+      MSA_WINDOW_LAUNCH((window_dq_kernel<DT, NK, MT, KS>), tile_numbers(total_tokens, num_seqs, A.ratio.d, log2_of(64 * MT)) * kv_groups); \
     if (rc == kOk && (grad_k || grad_v) && shape.tiles)                                                                          \
       MSA_WINDOW_LAUNCH((window_dkv_kernel<DT, NK, KT, true>),                                                                   \
-                        tile_numbers(total_tokens, num_seqs, 1, kChunk) * shape.tiles * kv_groups);                              \
+                        tile_numbers(total_tokens, num_seqs, 1, shape.chunk_log2) * shape.tiles * kv_groups);                    \
+    if (rc == kOk && (grad_k || grad_v) && shape.tiles)                                                                          \
+      MSA_WINDOW_LAUNCH((window_sink_sum<64 * KT>),                                                                              \
+                        num_seqs * shape.tiles * kv_groups * ((2 * shape.rows * head_dim + 1023) / 1024));                       \
     if (rc == kOk && (grad_k || grad_v))                                                                                         \
-      MSA_WINDOW_LAUNCH((window_dkv_kernel<DT, NK, KT, false>), tile_numbers(total_tokens, num_seqs, 1, 64 * KT) * kv_groups);   \
+      MSA_WINDOW_LAUNCH((window_dkv_kernel<DT, NK, KT, false>),                                                                  \
+                        tile_numbers(total_tokens, num_seqs, 1, log2_of(64 * KT)) * A.splits * kv_groups);                                \
+    if (rc == kOk && (grad_k || grad_v) && A.splits > 1)                                                                         \
+      MSA_WINDOW_LAUNCH((window_dkv_join<DT, 64 * KT>), (total_tokens * kv_groups + 3) / 4);                                     \
     return rc;                                                                                                                   \
   }
   if (dtype == kF32) {
     if (head_dim <= 64) MSA_WINDOW_BWD(kF32, 2, 1, 32, 1)
+    if (head_dim <= 96) MSA_WINDOW_BWD(kF32, 3, 1, 32, 1)
     if (head_dim <= 128) MSA_WINDOW_BWD(kF32, 4, 1, 32, 1)
+    if (head_dim <= 192) MSA_WINDOW_BWD(kF32, 6, 1, 32, 1)
     MSA_WINDOW_BWD(kF32, 8, 1, 32, 1)
   }
-#define MSA_WINDOW_BWD_DIM(DT)                        \
-  if (head_dim <= 64) MSA_WINDOW_BWD(DT, 2, 2, 32, 2) \
+#define MSA_WINDOW_BWD_DIM(DT)                         \
+  if (head_dim <= 64) MSA_WINDOW_BWD(DT, 2, 2, 32, 2)  \
+  if (head_dim <= 96) MSA_WINDOW_BWD(DT, 3, 2, 32, 2)  \
   if (head_dim <= 128) MSA_WINDOW_BWD(DT, 4, 2, 32, 2) \
+  if (head_dim <= 192) MSA_WINDOW_BWD(DT, 6, 1, 32, 1) \
   MSA_WINDOW_BWD(DT, 8, 1, 32, 1)
   if (dtype == kBF16) { MSA_WINDOW_BWD_DIM(kBF16) }
   MSA_WINDOW_BWD_DIM(kF16)

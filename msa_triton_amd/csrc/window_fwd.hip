@@ -37,16 +37,16 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
                                             float inv) {
   using E = typename Fragment<DT>::Element;
   const int lane = threadIdx.x & 63;
-  const E* q = static_cast<const E*>(A.q.base) + (start + static_cast<int64_t>(tok)) * A.q.token + head * A.q.head;
-  const E* k = static_cast<const E*>(A.k.base) + start * A.k.token + g * A.k.head;
-  const E* v = static_cast<const E*>(A.v.base) + start * A.v.token + g * A.v.head;
+  const E* q = static_cast<const E*>(A.q.base) + A.q.at(start + static_cast<int64_t>(tok), head);
+  const E* k = static_cast<const E*>(A.k.base) + A.k.at(start, g);
+  const E* v = static_cast<const E*>(A.v.base) + A.v.at(start, g);
   const int low = A.seen.low(tok);
   float o[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
   auto keys = [&](int from, int to) {
     for (int base = from; base < to; base += kWave) {
       const int j = min(base + lane, to - 1), count = min(kWave, to - base);
       float x = 0.f;
-      for (int d = 0; d < A.D; ++d) x = fmaf(value_at<DT>(q, d), value_at<DT>(k + j * A.k.token, d), x);
+      for (int d = 0; d < A.D; ++d) x = fmaf(value_at<DT>(q, d), value_at<DT>(k + static_cast<int64_t>(j) * A.k.token, d), x);
       x *= A.scale_log2;
       const float p = __builtin_amdgcn_exp2f(x + shift);
       for (int i = 0; i < count; ++i) {
@@ -56,7 +56,7 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
         for (int u = 0; u < 4; ++u) {
           const int d = lane + u * kWave;
           if (d >= A.D) break;
-          const float y = value_at<DT>(v + (base + i) * A.v.token, d);
+          const float y = value_at<DT>(v + static_cast<int64_t>(base + i) * A.v.token, d);
           if (finite(y)) o[u] = fmaf(p_i, y, o[u]);
           else odd[u] += x_i == -__builtin_inff() ? __builtin_nanf("") : y;
         }
@@ -80,7 +80,7 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
 }
 
 template <int DT, int NK, int MT, int KS>
-__global__ __launch_bounds__(256, 1) void window_fwd_kernel(WindowFwdArgs A) {
+__global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_fwd_kernel(WindowFwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
   constexpr float kUp = DT == kF16 ? 15.f : 0.f;
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256, 1) void window_fwd_kernel(WindowFwdArgs A) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t item = A.first + blockIdx.x;
   const int g = static_cast<int>(item % A.G);
-  const TilePlace at = tile_place<R>(A.cu, A.nseq, item / A.G, A.ratio);
+  const TilePlace at = tile_place(A.cu, A.nseq, item / A.G, A.ratio, log2_of(R));
   const int64_t rows = static_cast<int64_t>(at.n) * A.ratio, r0 = static_cast<int64_t>(at.tile) * R;
   if (r0 >= rows) return;
   const int live = static_cast<int>(min(rows - r0, int64_t{R}));
@@ -97,8 +97,8 @@ __global__ __launch_bounds__(256, 1) void window_fwd_kernel(WindowFwdArgs A) {
   const int off = static_cast<int>(r0 - static_cast<int64_t>(t0) * A.ratio);  // head of the first row
   auto token_of = [&](int r) { return t0 + (off + r) / A.ratio; };
 
-  const E* kbase = static_cast<const E*>(A.k.base) + at.start * A.k.token + g * A.k.head;
-  const E* vbase = static_cast<const E*>(A.v.base) + at.start * A.v.token + g * A.v.head;
+  const E* kbase = static_cast<const E*>(A.k.base) + A.k.at(at.start, g);
+  const E* vbase = static_cast<const E*>(A.v.base) + A.v.at(at.start, g);
   int tok[MT];
   Fragment<DT> qf[MT][NK];
 #pragma unroll
@@ -122,8 +122,8 @@ __global__ __launch_bounds__(256, 1) void window_fwd_kernel(WindowFwdArgs A) {
   TileLoad<DT, DP, KS> kload, vload;
   auto load_step = [&](int e) {
     const int j0 = first_key(e);
-    kload.load(A.D, [&](int r) { return kbase + min(j0 + r, t1) * A.k.token; });
-    vload.load(A.D, [&](int r) { return vbase + min(j0 + r, t1) * A.v.token; });
+    kload.load_near(A.D, kbase + static_cast<int64_t>(j0) * A.k.token, [&](int r) { return min(r, t1 - j0) * A.k.token; });
+    vload.load_near(A.D, vbase + static_cast<int64_t>(j0) * A.v.token, [&](int r) { return min(r, t1 - j0) * A.v.token; });
   };
   auto store_step = [&](int e) {
     kload.store(kbuf[e & 1], RS, A.D);
@@ -278,9 +278,9 @@ extern "C" int msa_window_attn_fwd(const void* q, const void* k, const void* v, 
   if (!window_supported(dtype, head_dim, total_tokens, q_heads / kv_groups)) return kErrUnsupported;
   if (total_tokens == 0) return kOk;
   WindowFwdArgs A{};
-  A.q = PackedView{q, strides[0], strides[1]};
-  A.k = PackedView{k, strides[2], strides[3]};
-  A.v = PackedView{v, strides[4], strides[5]};
+  A.q = packed_view(q, strides);
+  A.k = packed_view(k, strides + 2);
+  A.v = packed_view(v, strides + 4);
   A.cu = cu_seqlens;
   A.nseq = static_cast<int>(num_seqs);
   A.ratio = static_cast<int>(q_heads / kv_groups);
@@ -293,17 +293,19 @@ extern "C" int msa_window_attn_fwd(const void* q, const void* k, const void* v, 
   A.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define MSA_WINDOW_FWD(DT, NK, MT, KS)                                                                                 \
-  return launch_parts(tile_numbers(total_tokens, num_seqs, A.ratio, 64 * MT) * kv_groups, [&](int64_t first, unsigned count) { \
+  return launch_parts(tile_numbers(total_tokens, num_seqs, A.ratio, log2_of(64 * MT)) * kv_groups, [&](int64_t first, unsigned count) { \
     A.first = first;                                                                                                   \
     hipLaunchKernelGGL((window_fwd_kernel<DT, NK, MT, KS>), dim3(count), dim3(256), 0, st, A);                         \
   })
-#define MSA_WINDOW_FWD_DIM(DT, S2, S4, S8)         \
-  if (head_dim <= 64) MSA_WINDOW_FWD(DT, 2, 2, S2); \
-  if (head_dim <= 128) MSA_WINDOW_FWD(DT, 4, 2, S4); \
-  MSA_WINDOW_FWD(DT, 8, 1, S8)
-  if (dtype == kBF16) { MSA_WINDOW_FWD_DIM(kBF16, 64, 64, 32); }
-  if (dtype == kF16) { MSA_WINDOW_FWD_DIM(kF16, 64, 64, 32); }
-  MSA_WINDOW_FWD_DIM(kF32, 32, 32, 32);
+#define MSA_WINDOW_FWD_DIM(DT)                       \
+  if (head_dim <= 64) MSA_WINDOW_FWD(DT, 2, 2, 32);  \
+  if (head_dim <= 96) MSA_WINDOW_FWD(DT, 3, 2, 32);  \
+  if (head_dim <= 128) MSA_WINDOW_FWD(DT, 4, 2, 32); \
+  if (head_dim <= 192) MSA_WINDOW_FWD(DT, 6, 1, 32); \
+  MSA_WINDOW_FWD(DT, 8, 1, 32)
+  if (dtype == kBF16) { MSA_WINDOW_FWD_DIM(kBF16); }
+  if (dtype == kF16) { MSA_WINDOW_FWD_DIM(kF16); }
+  MSA_WINDOW_FWD_DIM(kF32);
 #undef MSA_WINDOW_FWD_DIM
 #undef MSA_WINDOW_FWD
 }

@@ -37,7 +37,8 @@ def check_window(window_size, sink_tokens):
 
 
 def aligned_rows(x):
-    """A rank-3 tensor whose rows are contiguous and 16-byte aligned, and its token and head strides."""
+    """A rank-3 tensor whose rows are contiguous, 16-byte aligned and near each other (33 tokens of all heads within 2^30
+    elements, as the kernels address them), and its token and head strides."""
     of_token, of_head, of_dim = x.stride()
     tokens, heads, dim = x.shape
     if tokens == 1:  # (a stride that nothing steps over may be anything)
@@ -45,7 +46,8 @@ def aligned_rows(x):
     if heads == 1:
         of_head = 0
     unit = 16 // x.element_size()
-    if (of_dim == 1 or dim == 1) and of_token % unit == 0 and of_head % unit == 0 and x.data_ptr() % 16 == 0:
+    if ((of_dim == 1 or dim == 1) and of_token % unit == 0 and of_head % unit == 0 and x.data_ptr() % 16 == 0
+            and 33 * of_token + heads * of_head < 1 << 30 and of_token < 1 << 25):
         return x, of_token, of_head
     x = x.contiguous()
     if x.data_ptr() % 16:
@@ -159,6 +161,8 @@ def _validate(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens, scale):
         raise ValueError("scale must be finite.")
     if dim > MAX_HEAD_DIM or dim % (4 if q.dtype == torch.float32 else 8):
         raise NotImplementedError("m3_window_attention takes head dims up to 256 whose rows are multiples of 16 bytes")
+    if heads * dim >= 1 << 24:
+        raise NotImplementedError("m3_window_attention takes fewer than 2^24 values a token")
     if total * (heads // k.shape[1]) >= 0x7FFF0000:
         raise NotImplementedError("m3_window_attention takes fewer than 2^31 rows of a key head")
     _lib.require_gpu(q, "m3_window_attention")
