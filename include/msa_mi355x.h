@@ -361,7 +361,7 @@ int64_t msa_window_attn_paged_workspace_bytes(int64_t total_tokens, int64_t num_
  * all) and the first `sinks`. Keys of missing pages do not exist; rows without a key, and rows of a sequence with a
  * negative context, get 0 and an lse of -inf. What is not finite: as in msa_attn_paged. strides (host array, elements):
  * k_cache page, head, slot; v_cache page, head, slot. head_dim: a multiple of 16 up to 256, T * Hq / G below 0x7fff0000,
- * longest up to 1024 with parents (status 2 otherwise); cache rows, q and workspace 16-byte aligned. Deterministic. */
+ * slot strides below 2^27, longest up to 512 with parents (status 2 otherwise); cache rows, q and workspace 16-byte aligned. Deterministic. */
 int msa_window_attn_paged(const void* q, const void* k_cache, const void* v_cache, int32_t dtype, int32_t cache_is_fp8,
                           const float* k_scale, const float* v_scale, const int64_t* strides, const int32_t* parents,
                           const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq, int64_t num_pages,

@@ -64,6 +64,33 @@ inline Divisor divisor_of(int64_t d) {
   return Divisor{static_cast<uint32_t>(((uint64_t{1} << (31 + bits)) + d - 1) / d), bits - 1, static_cast<int>(d)};
 }
 
+// The largest (the sum) of a value over the four quarters of a wave (lanes c, c + 16, c + 32, c + 48), by row swaps in the
+// vector unit.
+__device__ __forceinline__ float quarters_max(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// A running maximum is only raised when a row passes it by this much (log2): weights stay below 2^kSlack, sums and outputs are
+// rescaled in few steps. In fp16 weights are held times 2^(15 - kSlack), so that the largest is at most 2^15.
+constexpr float kSlack = 8.f;
+
+// A fragment, times -1 where `turn` says so.
+template <int DT, class F>
+__device__ __forceinline__ F turned(F f, bool turn) {
+  if (!turn) return f;
+  if constexpr (DT == kF32) {
+    f.a = -f.a, f.b = -f.b;
+  } else {
+    uint4 w = __builtin_bit_cast(uint4, f.v);
+    w.x ^= 0x80008000u, w.y ^= 0x80008000u, w.z ^= 0x80008000u, w.w ^= 0x80008000u;
+    f.v = __builtin_bit_cast(bf16x8, w);
+  }
+  return f;
+}
+
 // ---- fragments: eight values of a lane. In 16 bits one 16x16x32 product takes them; in fp32 eight 16x16x4 products do,
 // element j of all lanes in the j-th (its four k are those of the lanes' quarters, for both operands alike).
 
@@ -187,6 +214,11 @@ struct TileLoad {
     for (int p = 0; p < kPieces; ++p) r[p] = *reinterpret_cast<const uint4*>(at(row(p)) + (dim(p) < D ? dim(p) : 0));
   }
   __device__ __forceinline__ void store(E* tile, int stride, int D) const {
+    if (D == DP) {
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) *reinterpret_cast<uint4*>(tile + row(p) * stride + dim(p)) = r[p];
+      return;
+    }
 #pragma unroll
     for (int p = 0; p < kPieces; ++p)  // (a last piece that several threads hold is written by all of them alike)
       *reinterpret_cast<uint4*>(tile + row(p) * stride + dim(p)) = dim(p) < D ? r[p] : make_uint4(0u, 0u, 0u, 0u);

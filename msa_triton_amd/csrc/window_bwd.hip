@@ -195,8 +195,14 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dq_kernel(Wind
   TileLoad<DT, DP, KS> kload, vload;
   auto load_step = [&](int e) {
     const int j0 = first_key(e);
-    kload.load_near(A.D, kbase + static_cast<int64_t>(j0) * A.k.token, [&](int r) { return min(r, t1 - j0) * A.k.token; });
-    vload.load_near(A.D, vbase + static_cast<int64_t>(j0) * A.v.token, [&](int r) { return min(r, t1 - j0) * A.v.token; });
+    const E *k = kbase + static_cast<int64_t>(j0) * A.k.token, *v = vbase + static_cast<int64_t>(j0) * A.v.token;
+    if (j0 + KS - 1 <= t1) {
+      kload.load_near(A.D, k, [&](int r) { return r * A.k.token; });
+      vload.load_near(A.D, v, [&](int r) { return r * A.v.token; });
+    } else {
+      kload.load_near(A.D, k, [&](int r) { return min(r, t1 - j0) * A.k.token; });
+      vload.load_near(A.D, v, [&](int r) { return min(r, t1 - j0) * A.v.token; });
+    }
   };
   auto store_step = [&](int e) {
     kload.store(kbuf[e & 1], RS, A.D);
@@ -260,7 +266,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dq_kernel(Wind
           for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(ds[kt][i]));
-          big = quad_max(big);
+          big = quarters_max(big);
           if (__any(big >= range[m].cap && big != 0.f)) {
             const float factor = range[m].widen(big);
 #pragma unroll
@@ -540,7 +546,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dkv_kernel(Win
             }
           }
           if constexpr (DT == kF16) {
-            const float big = quad_max(fmaxf(fmaxf(fabsf(ds[0]), fabsf(ds[1])), fmaxf(fabsf(ds[2]), fabsf(ds[3]))));
+            const float big = quarters_max(fmaxf(fmaxf(fabsf(ds[0]), fabsf(ds[1])), fmaxf(fabsf(ds[2]), fabsf(ds[3]))));
             if (__any(big >= range[kt].cap && big != 0.f)) {
               const float factor = range[kt].widen(big);
 #pragma unroll

@@ -10,8 +10,8 @@
 // O^T = V^T P^T (values by transposed reads with the keys in that same order).
 //
 // Logits, statistics and outputs are fp32. The weights enter the second product rounded once to the input type (half a step
-// of 2^-8 in bf16, of the size of the output's own rounding and averaged over the keys; in fp16 times 2^15, so that weights
-// down to 2^-29 keep their bits). The sum of the weights is that of the unrounded ones.
+// of 2^-8 in bf16, of the size of the output's own rounding and averaged over the keys; in fp16 times 2^7, so that weights
+// down to 2^-21 keep their bits). The sum of the weights is that of the unrounded ones.
 #include "window.hpp"
 
 namespace msa {
@@ -83,7 +83,7 @@ template <int DT, int NK, int MT, int KS>
 __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_fwd_kernel(WindowFwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
-  constexpr float kUp = DT == kF16 ? 15.f : 0.f;
+  constexpr float kUp = DT == kF16 ? 15.f - kSlack : 0.f;
   __shared__ alignas(16) E kbuf[2][KS * RS], vbuf[2][KS * RS];
   const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -109,7 +109,9 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_
                    (g * A.ratio + (off + r) % A.ratio) * A.q.head;
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk)
-      qf[m][kk] = 32 * kk + 8 * q4 < A.D && A.scale_log2 != 0.f ? fragment_at<DT>(row + 32 * kk + 8 * q4) : no_fragment<DT>();
+      qf[m][kk] = 32 * kk + 8 * q4 < A.D && A.scale_log2 != 0.f
+                      ? turned<DT>(fragment_at<DT>(row + 32 * kk + 8 * q4), A.scale_log2 < 0.f)
+                      : no_fragment<DT>();
   }
   // keys of this workgroup: sinks in front of the first row's window, then from there to the last row
   const int low = A.seen.low(t0), sinks = min(A.seen.sinks, low);
@@ -122,16 +124,22 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_
   TileLoad<DT, DP, KS> kload, vload;
   auto load_step = [&](int e) {
     const int j0 = first_key(e);
-    kload.load_near(A.D, kbase + static_cast<int64_t>(j0) * A.k.token, [&](int r) { return min(r, t1 - j0) * A.k.token; });
-    vload.load_near(A.D, vbase + static_cast<int64_t>(j0) * A.v.token, [&](int r) { return min(r, t1 - j0) * A.v.token; });
+    const E *k = kbase + static_cast<int64_t>(j0) * A.k.token, *v = vbase + static_cast<int64_t>(j0) * A.v.token;
+    if (j0 + KS - 1 <= t1) {
+      kload.load_near(A.D, k, [&](int r) { return r * A.k.token; });
+      vload.load_near(A.D, v, [&](int r) { return r * A.v.token; });
+    } else {
+      kload.load_near(A.D, k, [&](int r) { return min(r, t1 - j0) * A.k.token; });
+      vload.load_near(A.D, v, [&](int r) { return min(r, t1 - j0) * A.v.token; });
+    }
   };
   auto store_step = [&](int e) {
     kload.store(kbuf[e & 1], RS, A.D);
     vload.store(vbuf[e & 1], RS, A.D);
   };
 
-  // A maximum is kept of the raw dots, whose sign is turned where the scale's is negative.
-  const float turn = A.scale_log2 < 0.f ? -1.f : 1.f, scale = fabsf(A.scale_log2);
+  // A maximum is kept of the raw dots (queries are turned where the scale is negative, and zero with a factor of 1 where it is 0).
+  const float factor = A.scale_log2 == 0.f ? 1.f : fabsf(A.scale_log2), slack = kSlack / factor;
   float top[MT], l[MT];
   f32x4 acc[MT][ND];
 #pragma unroll
@@ -162,12 +170,6 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_
           for (int m = 0; m < MT; ++m) s[m][kt] = product<DT>(kf, qf[m][kk], s[m][kt]);
         }
       }
-      if (turn < 0.f) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) s[m][kt] = -s[m][kt];
-      }
       const bool whole = of_sinks ? j0 + KS <= sinks : j0 + KS - 1 <= w0 && (w1 - j0 < A.seen.window || j0 + KS <= A.seen.sinks);
       if (!whole) {
 #pragma unroll
@@ -189,17 +191,14 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) high = fmaxf(high, s[m][kt][i]);
-        high = quad_max(high);
-        if (__any(high > top[m])) {
-          const float next = fmaxf(top[m], high);
-          const float keep = top[m] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((top[m] - next) * scale);
+        if (__any(high > top[m] + slack)) {
+          const float next = fmaxf(top[m], quarters_max(high));
+          const float keep = top[m] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((top[m] - next) * factor);
           top[m] = next;
           l[m] *= keep;
 #pragma unroll
           for (int d = 0; d < ND; ++d) acc[m][d] *= keep;
         }
-        // (masked logits stay -inf under a scale of 0, which has zero queries and a factor of 1 instead)
-        const float factor = A.scale_log2 == 0.f ? 1.f : scale;
         const float shift = kUp - (top[m] == -__builtin_inff() ? 0.f : top[m] * factor);
 #pragma unroll
         for (int u = 0; u < KT / 2; ++u) {
@@ -246,7 +245,6 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_
           if (A.out_lo) store4<DT>(lo + 16 * d + 4 * q4, left_out<DT>(o));
       }
     }
-    const float factor = A.scale_log2 == 0.f ? 1.f : scale;
     const float level = top[m] == -__builtin_inff() ? 0.f : top[m] * factor;
     if (mine && q4 == 0 && A.lse)
       A.lse[at_row] = l[m] == 0.f ? -__builtin_inff() : (level - kUp + __log2f(l[m])) * kLn2Window;

@@ -31,6 +31,12 @@ graph breaks and AOTAutograd differentiates it:
                                        block_size, scale, topk_blocks, local_blocks) -> (scores, indices)
     msa_mi355x::sparse_attention_paged(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, block_size,
                                        scale, k_scale, v_scale) -> (out, lse)
+    msa_mi355x::window_attention(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens, scale, save_state)
+        -> (out, lse, out_lo)                  out_lo: what the rounding of out left out, or empty when not saved
+    msa_mi355x::window_attention_backward(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens, scale, out, out_lo, lse,
+                                          grad_out, need_q, need_k, need_v) -> (dq, dk, dv)
+    msa_mi355x::window_attention_paged(q, k_cache, v_cache, page_table, cu_seqlens, context_lens, parents, window_size,
+                                       sink_tokens, scale, k_scale, v_scale) -> (out, lse)   parents: of a tree, or None
 
 A gradient that is not needed comes back as an empty tensor. ``m3_index_score``,
 ``m3_topk`` and ``m3_sparse_attention`` below keep the public signatures: their
@@ -62,6 +68,11 @@ from .paged_attention import m3_sparse_attention_paged as _eager_attention_paged
 from .paged_score import m3_index_score_topk_paged as _eager_score_paged
 from .sparse_attention import _attn_backward, _attn_forward
 from .topk import m3_topk as _eager_topk
+from .window_attention import _backward as _window_backward_call
+from .window_attention import _forward as _window_forward_call
+from .window_attention import _validate as _window_validate
+from .window_paged import m3_tree_attention_paged as _eager_tree_paged
+from .window_paged import m3_window_attention_paged as _eager_window_paged
 
 _NS = "msa_mi355x"
 
@@ -369,6 +380,75 @@ def _(q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, block_
     return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
 
 
+# ---------------------------------------------------------------------------- window and tree attention
+
+@torch.library.custom_op(f"{_NS}::window_attention", mutates_args=())
+def _window_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, max_seqlen: int, window_size: Optional[int],
+                      sink_tokens: int, scale: float, save_state: bool) -> tuple[Tensor, Tensor, Tensor]:
+    cu, num_seqs, _, window, sinks, scale = _window_validate(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens, scale)
+    out, lse, lo = _window_forward_call(q, k, v, cu, num_seqs, window, sinks, scale, True, save_state)
+    return out, lse, lo if lo is not None else q.new_empty(0)
+
+
+@_window_attention.register_fake
+def _(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens, scale, save_state):
+    saved = save_state and q.dtype != torch.float32
+    return (q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32), q.new_empty(q.shape if saved else (0,)))
+
+
+@torch.library.custom_op(f"{_NS}::window_attention_backward", mutates_args=())
+def _window_attention_backward(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, max_seqlen: int,
+                               window_size: Optional[int], sink_tokens: int, scale: float, out: Tensor, out_lo: Tensor,
+                               lse: Tensor, grad_out: Tensor, need_q: bool, need_k: bool,
+                               need_v: bool) -> tuple[Tensor, Tensor, Tensor]:
+    cu, num_seqs, longest, window, sinks, scale = _window_validate(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens,
+                                                                   scale)
+    grads = _window_backward_call(q, k, v, cu, num_seqs, longest, window, sinks, scale, out,
+                                  out_lo if q.dtype != torch.float32 else None, lse, grad_out, need_q, need_k, need_v)
+    dq, dk, dv = (g if g is not None else q.new_empty(0) for g in grads)
+    return dq, dk, dv
+
+
+@_window_attention_backward.register_fake
+def _(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens, scale, out, out_lo, lse, grad_out, need_q, need_k, need_v):
+    return tuple(x.new_empty(x.shape if need else (0,)) for x, need in ((q, need_q), (k, need_k), (v, need_v)))
+
+
+def _window_setup(ctx, inputs, output):
+    q, k, v, cu_seqlens, *ctx.call, _ = inputs
+    out, lse, lo = output
+    ctx.save_for_backward(q, k, v, cu_seqlens, out, lse, lo)
+    ctx.mark_non_differentiable(lse, lo)
+
+
+def _window_grad(ctx, grad_out, grad_lse, grad_lo):
+    q, k, v, cu_seqlens, out, lse, lo = ctx.saved_tensors
+    need = [bool(x) for x in ctx.needs_input_grad[:3]]
+    if grad_out is None:
+        grad_out = torch.zeros_like(out)
+    grads = torch.ops.msa_mi355x.window_attention_backward(q, k, v, cu_seqlens, *ctx.call, out, lo, lse, grad_out, *need)
+    return (*(g if n else None for g, n in zip(grads, need)), None, None, None, None, None, None)
+
+
+torch.library.register_autograd(f"{_NS}::window_attention", _window_grad, setup_context=_window_setup)
+
+
+@torch.library.custom_op(f"{_NS}::window_attention_paged", mutates_args=())
+def _window_attention_paged(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor, cu_seqlens: Tensor,
+                            context_lens: Tensor, parents: Optional[Tensor], window_size: Optional[int], sink_tokens: int,
+                            scale: float, k_scale: Optional[Tensor], v_scale: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    given = dict(window_size=window_size, sink_tokens=sink_tokens, scale=scale, k_scale=k_scale, v_scale=v_scale,
+                 return_lse=True)
+    if parents is None:
+        return _eager_window_paged(q, k_cache, v_cache, page_table, cu_seqlens, context_lens, **given)
+    return _eager_tree_paged(q, k_cache, v_cache, page_table, cu_seqlens, context_lens, parents, **given)
+
+
+@_window_attention_paged.register_fake
+def _(q, k_cache, v_cache, page_table, cu_seqlens, context_lens, parents, window_size, sink_tokens, scale, k_scale, v_scale):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
 # ---------------------------------------------------------------------------- public wrappers
 
 def m3_index_score(index_q, index_k, cu_seqlens, max_seqlen, *, block_size=128, scale=1.0):
@@ -504,5 +584,36 @@ def m3_sparse_attention_paged(q, k_cache, v_cache, indices, page_table, cu_seqle
     refuse_tangents("m3_sparse_attention_paged", q, k_cache, v_cache, k_scale, v_scale)
     out, lse = torch.ops.msa_mi355x.sparse_attention_paged(
         q, k_cache, v_cache, indices, page_table, cu_seqlens, context_lens, block_size,
+        q.shape[-1] ** -0.5 if scale is None else float(scale), k_scale, v_scale)
+    return (out, lse) if return_lse else out
+
+
+def m3_window_attention(q, k, v, cu_seqlens, max_seqlen, *, window_size, sink_tokens=0, scale=None, return_lse=False):
+    """``msa_triton_amd.m3_window_attention`` through the registered op."""
+    refuse_tangents("m3_window_attention", q, k, v)
+    save_state = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    out, lse, _ = torch.ops.msa_mi355x.window_attention(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens,
+                                                        q.shape[-1] ** -0.5 if scale is None else float(scale), save_state)
+    return (out, lse) if return_lse else out
+
+
+def m3_window_attention_paged(q, k_cache, v_cache, page_table, cu_seqlens, context_lens, *, window_size, sink_tokens=0,
+                              scale=None, k_scale=None, v_scale=None, return_lse=False):
+    """``msa_triton_amd.m3_window_attention_paged`` through the registered op."""
+    refuse_tangents("m3_window_attention_paged", q, k_cache, v_cache, k_scale, v_scale)
+    out, lse = torch.ops.msa_mi355x.window_attention_paged(
+        q, k_cache, v_cache, page_table, cu_seqlens, context_lens, None, window_size, sink_tokens,
+        q.shape[-1] ** -0.5 if scale is None else float(scale), k_scale, v_scale)
+    return (out, lse) if return_lse else out
+
+
+def m3_tree_attention_paged(q, k_cache, v_cache, page_table, cu_seqlens, context_lens, parents, *, window_size=None,
+                            sink_tokens=0, scale=None, k_scale=None, v_scale=None, return_lse=False):
+    """``msa_triton_amd.m3_tree_attention_paged`` through the registered op."""
+    if parents is None:
+        raise TypeError("parents must be int32")
+    refuse_tangents("m3_tree_attention_paged", q, k_cache, v_cache, k_scale, v_scale)
+    out, lse = torch.ops.msa_mi355x.window_attention_paged(
+        q, k_cache, v_cache, page_table, cu_seqlens, context_lens, parents, window_size, sink_tokens,
         q.shape[-1] ** -0.5 if scale is None else float(scale), k_scale, v_scale)
     return (out, lse) if return_lse else out

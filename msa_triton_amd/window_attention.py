@@ -12,8 +12,8 @@ out (delta = dO . O is formed from both).
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -55,8 +55,7 @@ def aligned_rows(x):
     return x, heads * dim, dim
 
 
-def _strides(*values):
-    return (ctypes.c_int64 * len(values))(*values)
+_pack6, _pack8 = struct.Struct("6q").pack, struct.Struct("8q").pack
 
 
 def _forward(q, k, v, cu, num_seqs, window, sinks, scale, need_lse, need_grad):
@@ -72,7 +71,7 @@ def _forward(q, k, v, cu, num_seqs, window, sinks, scale, need_lse, need_grad):
         v, *of_v = aligned_rows(v)
         with _lib.on_device(q.device):
             status = _lib.lib().msa_window_attn_fwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODE[q.dtype], _strides(*of_q, *of_k, *of_v),
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODE[q.dtype], _pack6(*of_q, *of_k, *of_v),
                 cu.data_ptr(), num_seqs, total, heads, groups, dim, window, sinks, scale, out.data_ptr(), _lib.ptr(lo),
                 _lib.ptr(lse), _lib.stream_of(q.device))
         _lib.check(status, "msa_window_attn_fwd")
@@ -100,7 +99,7 @@ def _backward(q, k, v, cu, num_seqs, longest, window, sinks, scale, out, lo, lse
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         with _lib.on_device(device):
             status = lib.msa_window_attn_bwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), code, _strides(*of_q, *of_k, *of_v, *of_grad), cu.data_ptr(),
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), code, _pack8(*of_q, *of_k, *of_v, *of_grad), cu.data_ptr(),
                 num_seqs, longest, total, heads, groups, dim, window, sinks, scale, out.data_ptr(), _lib.ptr(lo),
                 lse.data_ptr(), grad.data_ptr(), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), workspace.data_ptr(), size,
                 _lib.stream_of(device))

@@ -22,7 +22,7 @@ from .paged import check_kv_caches, check_pages, sixteen_bit
 from .window_attention import check_window
 
 _pack_strides = struct.Struct("6q").pack
-MAX_TREE_NODES = 1024
+MAX_TREE_NODES = 512
 
 
 def _attend(name, q, k_cache, v_cache, page_table, cu_seqlens, context_lens, parents, window_size, sink_tokens, scale,
@@ -56,6 +56,8 @@ def _attend(name, q, k_cache, v_cache, page_table, cu_seqlens, context_lens, par
         parents = parents.contiguous()
     if dim % 16 or dim > 256:
         raise NotImplementedError(f"{name} takes head dims that are multiples of 16 up to 256")
+    if max(k_cache.stride(2), v_cache.stride(2)) >= 1 << 27:
+        raise NotImplementedError(f"{name} takes caches whose slots lie fewer than 2^27 values apart")
     if total * (heads // groups) >= 0x7FFF0000:
         raise NotImplementedError(f"{name} takes fewer than 2^31 rows of a key head")
     if parents is not None and longest > MAX_TREE_NODES:
@@ -133,7 +135,7 @@ def m3_tree_attention_paged(
     front of their children, and anything outside ``[0, own place)`` (-1, say) is a child of the context. A node
     sees the cached tokens and, of the new ones, itself and its ancestors. It lies in slot ``context + place`` of the cache,
     and its position, by which window and first tokens are counted, is ``context + depth`` (the position to rotate it by).
-    Up to 1024 nodes a sequence."""
+    Up to 512 nodes a sequence."""
     if parents is None:
         raise TypeError("parents must be int32")
     return _attend("m3_tree_attention_paged", q, k_cache, v_cache, page_table, cu_seqlens, context_lens, parents,

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import msa_triton_amd as msa
 from tests.helpers import cu_tensor
@@ -148,3 +149,277 @@ def test_against_the_formula(case):
     assert torch.equal(plain, out)
     for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out.detach(), lse, *grads)):
         check(got, res[name], off[name], name)
+
+
+def run(q, k, v, lengths, do=None, window=40, sinks=3, **kw):
+    """out, lse and, with do, the gradients."""
+    leaves = [x.detach().requires_grad_(do is not None) for x in (q, k, v)]
+    out, lse = msa.m3_window_attention(*leaves, cu_tensor(lengths, "cuda"), max(lengths), window_size=window, sink_tokens=sinks,
+                                       return_lse=True, **kw)
+    return (out.detach(), lse, *(torch.autograd.grad(out, leaves, do) if do is not None else ()))
+
+
+def against(got, q, k, v, lengths, window, sinks, scale, do):
+    res, off = reference(q, k, v, lengths, window, sinks, scale, do)
+    for name, x in zip(("out", "lse", "dq", "dk", "dv"), got):
+        check(x, res[name], off[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_strides(dtype):
+    """Slices of one projection, heads in front, a shared key head, odd addresses; gradients that are views."""
+    lengths, hq, g, d = [70, 130], 4, 2, 64
+    q, k, v, do = inputs(lengths, hq, g, d, dtype)
+    want = run(q, k, v, lengths, do)
+    against(want, q, k, v, lengths, 40, 3, d ** -0.5, do)
+    fused = torch.cat([q, k, v], 1)
+    cases = [tuple(fused.split([hq, g, g], 1)), tuple(x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)),
+             tuple(torch.nn.functional.pad(x, (1, 7))[..., 1:d + 1] for x in (q, k, v)),  # rows off 16 bytes
+             tuple(x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v))]    # no unit stride
+    grads = [do, do.transpose(0, 1).contiguous().transpose(0, 1), torch.nn.functional.pad(do, (1, 7))[..., 1:d + 1], do]
+    for (a, b, c), y in zip(cases, grads):
+        assert all(torch.equal(x, z) for x, z in zip(run(a, b, c, lengths, y), want))
+    shared = k[:, :1].expand(-1, g, -1)  # stride 0
+    got = run(q, shared, shared, lengths, do)
+    assert all(torch.equal(x, z) for x, z in zip(got, run(q, shared.contiguous(), shared.contiguous(), lengths, do)))
+    ones = torch.ones((), dtype=dtype, device="cuda").expand_as(do)
+    assert all(torch.equal(x, z) for x, z in zip(run(q, k, v, lengths, ones), run(q, k, v, lengths, ones.contiguous())))
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.5, 1e-9])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_scales(dtype, scale):
+    lengths = [90, 33]
+    q, k, v, do = inputs(lengths, 4, 2, 64, dtype)
+    against(run(q, k, v, lengths, do, scale=scale), q, k, v, lengths, 40, 3, scale, do)
+
+
+def test_each_gradient_alone():
+    lengths = [150]
+    q, k, v, do = inputs(lengths, 8, 2, 128, torch.bfloat16)
+    want = run(q, k, v, lengths, do)[2:]
+    for keep in range(1, 8):
+        leaves = [x.detach().requires_grad_(bool(keep >> i & 1)) for i, x in enumerate((q, k, v))]
+        out = msa.m3_window_attention(*leaves, cu_tensor(lengths, "cuda"), 150, window_size=40, sink_tokens=3)
+        out.backward(do)
+        for i, x in enumerate(leaves):
+            assert torch.equal(x.grad, want[i]) if keep >> i & 1 else x.grad is None
+
+
+def test_gradients_against_differences():
+    """fp32: (f(x + s y) - f(x - s y)) / 2 s for f = <out, do>, along random y. The difference of third order is s^2 / 6 times
+    the third derivative; with logits of size 1 that is below s^2 sum |do| |out| 10, and the two f are off by their bounds over s."""
+    lengths, scale = [37, 20], 16 ** -0.5
+    q, k, v, do = (x * 0.5 for x in inputs(lengths, 4, 2, 16, torch.float32))
+    window, sinks, s = 9, 2, 2.0 ** -6
+    grads = run(q, k, v, lengths, do, window, sinks)[2:]
+    gen = torch.Generator().manual_seed(8)
+    for i in range(3):
+        y = torch.randn((q, k, v)[i].shape, generator=gen).cuda()
+        y /= y.norm() / 4
+        f = []
+        room = 0.0
+        for sign in (1, -1):
+            x = [a.clone() for a in (q, k, v)]
+            x[i] += sign * s * y
+            f.append((run(*x, lengths, None, window, sinks)[0].double() * do.double()).sum().item())
+            res, off = reference(*x, lengths, window, sinks, scale)
+            room += (off["out"] * do.abs().double()).sum().item() / (2 * s)
+        bound = room + 10 * s * s * (do.abs().double() * res["out"].abs()).sum().item()
+        assert abs((f[0] - f[1]) / (2 * s) - (grads[i].double() * y.double()).sum().item()) <= bound
+
+
+def test_fp16_gradients_of_any_size():
+    """Incoming gradients of 2^-20 and of 2^10, as without and with loss scaling: what fp16 holds of the results is theirs."""
+    lengths = [300]
+    q, k, v, do = inputs(lengths, 4, 2, 64, torch.float16)
+    for power in (-20, -12, 10):
+        y = (do.double() * 2.0 ** power).half()
+        against(run(q, k, v, lengths, y, 100, 4), q, k, v, lengths, 100, 4, 64 ** -0.5, y)
+    rows = torch.randint(-22, 9, (300, 4, 1), generator=torch.Generator().manual_seed(2)).double().exp2().cuda()
+    y = (do.double() * rows).half()  # rows of different size
+    against(run(q, k, v, lengths, y, 100, 4), q, k, v, lengths, 100, 4, 64 ** -0.5, y)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64), (torch.bfloat16, 256)])
+def test_what_is_not_finite_stays_with_the_rows_that_see_it(dtype, d):
+    lengths, window, sinks = [200, 90], 32, 2
+    q, k, v, do = inputs(lengths, 4, 2, d, dtype)
+    plain = run(q, k, v, lengths, do, window, sinks)
+    res, off = reference(q, k, v, lengths, window, sinks, d ** -0.5, do)
+    for what, value in ((0, float("nan")), (1, float("nan")), (1, float("inf")), (2, float("nan")), (2, float("inf")), (3, float("nan")),
+                        (3, float("-inf"))):
+        for at in (0, 1, 100, 199, 230):  # a first token, a later one, the last of a sequence, one of the second
+            x = [y.clone() for y in (q, k, v, do)]
+            x[what][at, 0, 3] = value
+            got = run(*x[:3], lengths, x[3], window, sinks)
+            start, end = (0, 200) if at < 200 else (200, 290)
+            sees = torch.zeros(290, dtype=torch.bool, device="cuda")  # rows that see token `at`
+            sees[at:end] = True if at - start < sinks else False
+            sees[at:min(end, at + window)] = True
+            keys = torch.zeros(290, dtype=torch.bool, device="cuda")  # keys that token `at` sees
+            keys[max(start, at - window + 1):at + 1] = True
+            keys[start:min(start + sinks, at + 1)] = True
+            heads = [0, 1] if what in (1, 2) else [0]
+            if what in (1, 2):  # a key's or value's: its rows, and the keys that those see
+                far = torch.zeros_like(keys)
+                for i in sees.nonzero().flatten().tolist():
+                    far[max(start, i - window + 1):i + 1] = True
+                    far[start:min(start + sinks, i + 1)] = True
+            else:
+                sees, far = torch.zeros_like(sees), keys
+                sees[at] = True
+            for name, a in zip(("out", "lse", "dq", "dk", "dv"), got):
+                other = torch.ones_like(a, dtype=torch.bool)
+                if name in ("out", "lse", "dq"):
+                    for h in heads:
+                        other[:, h] &= (~sees).view(-1, *[1] * (a.ndim - 2))
+                else:
+                    other[:, 0] &= (~far)[:, None]
+                # (tiles that met the value are formed again, key by key: within the same bound, not the same bits)
+                check(a[other], res[name][other], off[name][other], (what, value, at, name))
+            if what == 2:  # the value's dim alone, as the formula has it
+                out = got[0][sees][:, :2]
+                assert (torch.isnan(out[..., 3]).all() if value != value else (out[..., 3] == value).all())
+                keep = [i for i in range(d) if i != 3]
+                check(out[..., keep], res["out"][sees][:, :2][..., keep], off["out"][sees][:, :2][..., keep], (value, at))
+                assert torch.equal(got[1], plain[1])
+            if what == 3:
+                assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1])
+
+
+def test_an_infinity_counts_whatever_its_weight():
+    """A key so far from the row's best that its weight is 0 in fp32."""
+    q, k, v, _ = inputs([64], 1, 1, 64, torch.bfloat16)
+    k[5] = -200.0 * q[63, 0].sign()
+    v[5, 0, 7] = float("inf")
+    out = run(q, k, v, [64], None, 64, 0)[0]
+    assert out[63, 0, 7] == float("inf") and torch.isfinite(out[63, 0, :7]).all() and torch.isfinite(out[:5]).all()
+
+
+def test_all_of_a_batch_not_finite_ends():
+    q, k, v, do = inputs([600], 8, 2, 128, torch.bfloat16)
+    for i in range(4):
+        x = [y.clone() for y in (q, k, v, do)]
+        x[i].fill_(float("nan"))
+        got = run(*x[:3], [600], x[3], 256, 4)
+        assert torch.isnan(got[0]).all() == (i < 3) and torch.isnan(got[2]).all() and torch.isnan(got[3]).all()
+
+
+def test_larger_calls():
+    """Enough keys for tiles of keys that no workgroups share, with first tokens seen from behind the window."""
+    lengths, hq, g, d, window, sinks = [5000, 3001, 1], 16, 16, 64, 130, 5
+    q, k, v, do = inputs(lengths, hq, g, d, torch.bfloat16)
+    against(run(q, k, v, lengths, do, window, sinks), q, k, v, lengths, window, sinks, d ** -0.5, do)
+
+
+def test_streams_and_determinism():
+    q, k, v, do = inputs([700, 129], 8, 2, 128, torch.float16)
+    want = run(q, k, v, [700, 129], do, 200, 4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(q, k, v, [700, 129], do, 200, 4)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_captured_step_replays():
+    lengths = [300, 1, 77]
+    seqs = msa.prepare_sequences(cu_tensor(lengths, "cuda"))
+    q, k, v, do = inputs(lengths, 8, 2, 64, torch.bfloat16)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+
+    def step():
+        out, lse = msa.m3_window_attention(*leaves, seqs, 300, window_size=50, sink_tokens=4, return_lse=True)
+        return (out.detach(), lse, *torch.autograd.grad(out, leaves, do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for turn in range(3):
+        gen = torch.Generator(device="cuda").manual_seed(turn)
+        with torch.no_grad():
+            for x in (*leaves, do):
+                x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        graph.replay()
+        want = run(q, k, v, lengths, do, 50, 4)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_checkpointing_and_offloaded_saved_tensors():
+    lengths = [140]
+    q, k, v, do = inputs(lengths, 4, 2, 64, torch.bfloat16)
+    want = run(q, k, v, lengths, do)[2:]
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    f = lambda *x: msa.m3_window_attention(*x, cu_tensor(lengths, "cuda"), 140, window_size=40, sink_tokens=3)  # noqa: E731
+    torch.utils.checkpoint.checkpoint(f, *leaves, use_reentrant=False).backward(do)
+    assert all(torch.equal(x.grad, y) for x, y in zip(leaves, want))
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    with torch.autograd.graph.save_on_cpu():
+        out = f(*leaves)
+    out.backward(do)
+    assert all(torch.equal(x.grad, y) for x, y in zip(leaves, want))
+
+
+def test_an_input_changed_before_its_backward_pass_is_noticed():
+    q, k, v, do = inputs([30], 2, 1, 64, torch.bfloat16)
+    q.requires_grad_()
+    out = msa.m3_window_attention(q, k, v, cu_tensor([30], "cuda"), 30, window_size=None)
+    k.zero_()
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        out.backward(do)
+
+
+def test_no_tokens():
+    for dtype in (torch.bfloat16, torch.float32):
+        q, k = torch.zeros(0, 4, 64, dtype=dtype, device="cuda"), torch.zeros(0, 2, 64, dtype=dtype, device="cuda")
+        q.requires_grad_()
+        out, lse = msa.m3_window_attention(q, k, k, cu_tensor([0, 0], "cuda"), 1, window_size=3, return_lse=True)
+        out.sum().backward()
+        assert out.shape == q.shape and lse.shape == (0, 4) and q.grad.shape == q.shape
+
+
+def test_offsets_past_32_bits():
+    """2.3e9 values a tensor, checked at their ends and in between."""
+    tokens, hq, d, window = 140_000, 64, 256, 3
+    q = torch.empty(tokens, hq, d, dtype=torch.bfloat16, device="cuda")
+    assert q.numel() > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q.normal_(generator=gen)
+    k, v = (torch.randn(tokens, 1, d, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    q.requires_grad_(), k.requires_grad_(), v.requires_grad_()
+    out = msa.m3_window_attention(q, k, v, cu_tensor([tokens], "cuda"), tokens, window_size=window)
+    do = torch.empty_like(out).normal_(generator=gen)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    for a, b in ((0, 40), (69_000, 69_040), (tokens - 40, tokens)):
+        front = min(a, window - 1)  # (rows in front complete the windows of the checked ones)
+        back = min(tokens - b, window - 1)
+        rows = slice(a - front, b + back)
+        res, off = reference(*(x.detach()[rows] for x in (q, k, v)), [b - a + front + back], window, 0, d ** -0.5, do[rows])
+        mine = slice(front, front + b - a)
+        for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+            check(got.detach()[a:b], res[name][mine], off[name][mine], name)
+
+
+def test_calls_of_more_than_2_to_the_23_workgroups():
+    """Sequences of one token, in one call: out is v, with the gradients of that. dq = (dO . v - dO . out) k is nothing but the
+    errors of two sums of 8 products, each off by at most 16 u sum |dO||v|."""
+    from msa_triton_amd.window_attention import _backward, _forward
+
+    n = (1 << 23) + 77
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v, do = (torch.randn(n, 1, 8, generator=gen, device="cuda").bfloat16() for _ in range(4))
+    out, lse, lo = _forward(q, k, v, cu, n, 5, 0, 1.0, True, True)
+    dq, dk, dv = _backward(q, k, v, cu, n, 1, 5, 0, 1.0, out, lo, lse, do, True, True, True)
+    assert torch.equal(out, v) and torch.equal(dv, do)
+    most = 2 * 16 * U * (do.double().abs() * v.double().abs()).sum(2, keepdim=True) * (1 + 2.0 ** -7)
+    assert (dq.double().abs() <= most * k.double().abs()).all() and (dk.double().abs() <= most * q.double().abs()).all()

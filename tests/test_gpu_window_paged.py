@@ -3,7 +3,7 @@
 Tolerance, with h half a step of a type relative to the value: logits are fp32 products of exact terms, so a dot of D
 terms is off by D 2^-23 sum |q||k| at most, times the scale, and by 2^-22 of itself; a weight by twice that error d of a logit
 (its own and the maximum's) and its exponential's 2^-22. A weight enters the second product as two terms (2^-17 left
-out) where no sequence has more than 16 rows a key head or the head dim is above 128, and is rounded once otherwise (h
+out) where no sequence has more than 16 rows a key head, and is rounded once otherwise (h
 of the type of that product, bf16 for 8-bit caches). The second product and its sums, over waves and workgroups, add 2^-16.
 So |out - exact| <= (2 d + left out + 2^-16) max |v| + h |out|. The lse is off by d and 2^-20 of its size.
 """
@@ -77,7 +77,7 @@ def oracle(x, lengths, context, window, sinks, scale):
     pages, groups, page, _ = x["kc"].shape
     ratio = heads // groups
     fp8 = x["kc"].dtype == FP8
-    two = max(lengths) * ratio <= 16 or dim > 128
+    two = max(lengths) * ratio <= 16
     left_out = 2.0 ** -17 if two else torch.finfo(torch.bfloat16 if fp8 else x["q"].dtype).eps / 2
     out, tol = torch.zeros_like(q), torch.zeros_like(q)
     lse = torch.full((total, heads), float("-inf"), dtype=torch.float64, device=q.device)
@@ -187,7 +187,7 @@ TREES = [  # lengths, context, groups, ratio, dim, page, window, sinks, dtype, f
     ([64, 48, 0, 17, 1], [500, 0, 8, 3000, -1], 2, 5, 96, 64, 40, 4, torch.float16, True),
     ([130, 33], [1000, 31], 1, 4, 64, 16, 6, 33, torch.float16, False),  # windows that end inside the paths
     ([130, 33], [1000, 31], 1, 1, 256, 32, 3, 40, torch.bfloat16, False),
-    ([1024], [100], 1, 2, 64, 64, 90, 1, torch.bfloat16, False),
+    ([512], [100], 1, 2, 64, 64, 90, 1, torch.bfloat16, False),
     ([9] * 80, "mixed", 2, 2, 64, 16, None, 0, torch.float16, True),
 ]
 
@@ -201,3 +201,206 @@ def test_tree_against_the_formula(case):
     out, lse = check(x, lengths, context, window, sinks)
     again = call(x, window, sinks, msa.prepare_sequences(x["cu"]))
     assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+def test_scales_of_any_sign():
+    for lengths, fp8 in (([1, 2], False), ([1, 40], False), ([2, 1], True), ([3, 40], True)):
+        x = setup(lengths, [70, 300], 2, 4, 64, 16, torch.float16, fp8)
+        for scale in (-0.4, 0.0, 3.0):
+            check(x, lengths, [70, 300], 50, 4, scale=scale)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_that_do_not_exist(new, fp8):
+    """Entries of -1 and past the cache in the middle, in the window and in front of it, lengths behind the table, no table."""
+    lengths, context = [new, new, new, new], [500, 333, 700, 90]
+    x = setup(lengths, context, 2, 4, 64, 16, torch.bfloat16, fp8, width=50)
+    x["table"][0, 3:20] = -1
+    x["table"][1, 20] = x["kc"].shape[0]
+    x["table"][1, 5] = 1 << 30
+    x["table"][2, ::2] = -7
+    x["table"][3, :] = -1
+    for window, sinks in ((None, 0), (100, 4), (30, 70), (1, 0)):
+        check(x, lengths, context, window, sinks)
+    short = dict(x, table=x["table"][:, :21].contiguous())
+    check(short, lengths, context, None, 0)
+    check(short, lengths, context, 100, 4)
+    none = dict(x, table=x["table"][:, :0].contiguous())
+    out, lse = call(none, None, 0)
+    assert not out.any() and (lse == float("-inf")).all()
+    empty = dict(x, kc=x["kc"][:0], vc=x["vc"][:0], ks=x["ks"][:0] if fp8 else None, vs=x["vs"][:0] if fp8 else None)
+    out, lse = call(empty, 100, 4)
+    assert not out.any() and (lse == float("-inf")).all()
+    far = dict(x, context=torch.tensor([2 ** 31 - 1, 333, -1, -2 ** 31], dtype=torch.int32, device="cuda"))
+    out, lse = call(far, 100, 0)
+    assert (lse[:new] == float("-inf")).all() and not out[:new].any() and not out[2 * new:].any()
+    assert torch.isfinite(lse[new:2 * new]).all() and (lse[2 * new:] == float("-inf")).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lengths", [[1, 3, 2], [40, 3, 70]], ids=("few", "many"))
+def test_strided_caches_streams_and_a_table_of_columns(lengths, fp8):
+    context = [300, 17, 64]
+    x = setup(lengths, context, 2, 4, 64, 16, torch.bfloat16, fp8)
+    want = call(x, 60, 3)
+    moved = dict(x, table=x["table"].t().contiguous().t(), q=x["q"].transpose(0, 1).contiguous().transpose(0, 1))
+    for name in ("kc", "vc"):
+        c = x[name]
+        both = torch.zeros(c.shape[0], c.shape[2], c.shape[1], 2 * c.shape[3], device="cuda").to(c.dtype)  # slots in front of heads
+        both[..., :64] = c.transpose(1, 2)
+        moved[name] = both[..., :64].transpose(1, 2)
+    got = call(moved, 60, 3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call(x, 60, 3)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_offsets_past_32_bits():
+    """Pages whose first value is 2^31 values and more into the cache."""
+    pages, page, dim = 140_000, 128, 128
+    cache = torch.zeros(pages, 1, page, dim, dtype=torch.bfloat16, device="cuda")
+    assert cache.numel() > 2 ** 31
+    lengths, context = [1, 20], [700, 300]
+    small = setup(lengths, context, 1, 8, dim, page, torch.bfloat16, False)
+    x = dict(small, kc=cache, vc=torch.zeros_like(cache), table=torch.full_like(small["table"], -1))
+    at = pages - 1
+    for s in range(2):
+        for m in range(small["table"].shape[1]):
+            p = int(small["table"][s, m])
+            if p >= 0:
+                x["kc"][at], x["vc"][at] = small["kc"][p], small["vc"][p]
+                x["table"][s, m] = at
+                at -= 3
+    got, want = call(x, 500, 4), call(small, 500, 4)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lengths,context", [([1, 1], [900, 40]), ([40, 17], [900, 40]), ([1], [20000])], ids=("few", "many", "split"))
+def test_values_that_are_not_finite(lengths, context, fp8):
+    """An infinity and a NaN of one key's value: the dim of every row that sees it, whatever the weight, and nothing else."""
+    g, ratio, d, page = 2, 4, 64, 16
+    x = setup(lengths, context, g, ratio, d, page, torch.bfloat16, fp8)
+    want, want_lse, tol, lse_tol = oracle(x, lengths, context, 500, 2, d ** -0.5)
+    for at, value in ((context[0] - 3, float("inf")), (0, float("-inf")), (context[0] - 450, float("nan")), (context[0] - 600, float("nan")),
+                      (context[0], float("nan"))):
+        if fp8 and value == value:
+            value = float("nan")  # (e4m3 has no infinities)
+        y = dict(x, vc=x["vc"].clone())
+        p = int(x["table"][0, at // page])
+        y["vc"].view(torch.uint8 if fp8 else torch.bfloat16)[p, 1, at % page, 5] = 0x7F if fp8 else value
+        out, lse = call(y, 500, 2)
+        pos = torch.arange(context[0], context[0] + lengths[0], device="cuda")
+        sees = (pos >= at) & ((pos - at < 500) | (at < 2))
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        hit[:lengths[0], ratio:, 5] = sees[:, None]
+        assert (torch.isnan(out[hit]).all() if value != value else (out[hit] == value).all())
+        assert ((out.double() - want).abs() <= tol)[~hit].all()
+        assert ((lse.double() - want_lse).abs() <= lse_tol).all()
+
+
+def test_a_value_under_a_weight_of_zero():
+    """A key so far from the row's best that its weight is 0 in fp32, its value an infinity."""
+    for lengths in ([1], [40]):
+        x = setup(lengths, [300], 1, 4, 64, 16, torch.bfloat16, False)
+        p = int(x["table"][0, 0])
+        x["kc"][p, 0, 5] = (-100 * x["q"][0, 2].float().sign()).bfloat16()
+        x["vc"][p, 0, 5, 9] = float("inf")
+        out, lse = call(x, None, 0)
+        assert (out[:, :, 9] == float("inf")).all() and torch.isfinite(out[:, :, :9]).all() and torch.isfinite(lse).all()
+
+
+def test_keys_and_queries_that_are_not_finite():
+    lengths, context = [30, 2], [100, 50]
+    x = setup(lengths, context, 1, 4, 64, 16, torch.float16, False)
+    want = call(x, 40, 1)
+    y = dict(x, kc=x["kc"].clone())
+    p = int(x["table"][0, 110 // 16])
+    y["kc"][p, 0, 110 % 16, 0] = float("nan")  # seen by tokens 10 to 29 of the first sequence
+    out, lse = call(y, 40, 1)
+    assert torch.isnan(out[10:30]).all() and torch.isnan(lse[10:30]).all()
+    rest = torch.ones(32, dtype=torch.bool)
+    rest[10:30] = False
+    assert torch.equal(out[rest], want[0][rest]) and torch.equal(lse[rest], want[1][rest])
+    z = dict(x, q=x["q"].clone())
+    z["q"][3, 1, 7] = float("inf")
+    out, lse = call(z, 40, 1)
+    assert not torch.isfinite(out[3, 1]).any()
+    rest = torch.ones(32, 4, dtype=torch.bool)
+    rest[3, 1] = False
+    assert torch.equal(out[rest], want[0][rest]) and torch.equal(lse[rest], want[1][rest])
+
+
+def test_a_chain_is_a_drafted_run():
+    lengths, context = [9, 1, 40], [300, 5, 64]
+    for fp8 in (False, True):
+        x = setup(lengths, context, 2, 4, 64, 16, torch.bfloat16, fp8)
+        chain = torch.cat([torch.arange(n) - 1 for n in lengths]).to(torch.int32).cuda()
+        for window, sinks in ((None, 0), (20, 3)):
+            a, b = call(x, window, sinks), call(dict(x, parents=chain), window, sinks)
+            x["parents"] = None
+            want, _, tol, _ = oracle(x, lengths, context, window, sinks, 64 ** -0.5)
+            assert ((b[0].double() - want).abs() <= tol).all()
+            assert window or all(torch.equal(u, w) for u, w in zip(a, b))
+
+
+@pytest.mark.parametrize("lengths", [[1, 1, 1], [17, 5, 40]], ids=("single", "tree"))
+def test_captured_calls_replay_at_new_lengths_and_trees(lengths):
+    x = setup(lengths, [400, 200, 300], 2, 8, 64, 16, torch.bfloat16, True)
+    x["context"].copy_(torch.tensor([40, 20, 30]))
+    x["parents"] = tree(lengths)
+    seqs = msa.prepare_sequences(x["cu"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(x, 100, 4, seqs)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):  # two graphs, replayed in turn
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, call(x, 100, 4, seqs)))
+    for turn, context in enumerate(([40, 20, 30], [400, 200, 300], [0, 199, -1], [390, 1, 16])):
+        x["context"].copy_(torch.tensor(context))
+        x["parents"].copy_(tree(lengths, seed=turn))
+        graph, held = graphs[turn % 2]
+        graph.replay()
+        want = call(x, 100, 4)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_a_million_sequences():
+    """One call of 2^20 requests and 2^24 rows."""
+    n, hq, d, page = 1 << 20, 16, 16, 16
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(n, hq, d, generator=gen, device="cuda").bfloat16()
+    kc, vc = (torch.randn(4096, 1, page, d, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    table = torch.randint(0, 4096, (n, 2), generator=gen, device="cuda", dtype=torch.int32)
+    context = torch.randint(-1, 31, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    out, lse = msa.m3_window_attention_paged(q, kc, vc, table, cu, context, window_size=20, sink_tokens=1, return_lse=True)
+    for a in (0, 500_000, n - 20):
+        part = slice(a, a + 20)
+        x = dict(q=q[part], kc=kc, vc=vc, ks=None, vs=None, table=table[part], parents=None)
+        want, want_lse, tol, lse_tol = oracle(x, [1] * 20, context[part].tolist(), 20, 1, d ** -0.5)
+        assert ((out[part].double() - want).abs() <= tol).all()
+        none = want_lse == float("-inf")
+        assert torch.equal(lse[part] == float("-inf"), none)
+        assert ((lse[part].double() - want_lse).abs() <= lse_tol)[~none].all()
+
+
+def test_differentiating_raises():
+    x = setup([2], [20], 1, 2, 64, 16, torch.bfloat16, False)
+    x["q"].requires_grad_()
+    for parents in (None, tree([2])):
+        out, _ = call(dict(x, parents=parents), 4, 0)
+        with pytest.raises(RuntimeError, match="no gradients"):
+            out.float().sum().backward()
+        with torch.no_grad():
+            assert not call(dict(x, parents=parents), 4, 0)[0].requires_grad

@@ -115,5 +115,5 @@ def test_parents():
                            (torch.zeros(3, dtype=torch.int32, device="meta"), ValueError)):
         with pytest.raises(error):
             _serve(True, **x, parents=parents)
-    with pytest.raises(NotImplementedError, match="1024 nodes"):
-        _serve(True, **_paged(tokens=1026))
+    with pytest.raises(NotImplementedError, match="512 nodes"):
+        _serve(True, **_paged(tokens=514))
