@@ -326,7 +326,8 @@ int msa_attn_paged(const void* q, const void* k_cache, const void* v_cache, int3
  * i - j < window (0: all) or j < sinks. out [T,Hq,D] in `dtype`, out_lo (NULL: not wanted; fp32: unread) what its
  * rounding left out, rounded to `dtype` as well; lse [T,Hq] (NULL: none) natural log. strides (host array, elements):
  * q token, head; k token, head; v token, head; unit stride along D, rows 16-byte aligned, 33 token strides and Hq / G head
- * strides together below 2^30, a token stride below 2^25. head_dim: rows of multiples of 16 bytes, up to 256; T * Hq / G below 0x7fff0000 (status 2 otherwise). One launch. */
+ * strides together below 2^30, a token stride below 2^25. head_dim: a multiple of 8 up
+ * to 256; T * Hq / G below 0x7fff0000 (status 2 otherwise). One launch. */
 int msa_window_attn_fwd(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
                         const int32_t* cu_seqlens, int64_t num_seqs, int64_t total_tokens, int64_t q_heads,
                         int64_t kv_groups, int64_t head_dim, int64_t window, int64_t sinks, double scale, void* out,

@@ -170,7 +170,20 @@ __device__ __forceinline__ Fragment<DT> pack_fragment(const float (&x)[8]) {
   return f;
 }
 
-// The same in two halves: elements 4 half .. 4 half + 3 of f.
+// What that rounding left out, rounded to 16 bits as well: the second term of each value, to 2^-17 (fp16: 2^-22) of it.
+template <int DT>
+__device__ __forceinline__ Fragment<DT> second_terms(const Fragment<DT>& first, const float (&x)[8]) {
+  static_assert(DT != kF32, "nothing is left out");
+  const uint4 w = __builtin_bit_cast(uint4, first.v);
+  auto two = [](uint32_t h, float a, float b) {
+    return DT == kF16 ? cvt_pk_f16(sub_lo_half_f16(h, a), sub_hi_half_f16(h, b)) : cvt_pk_bf16(sub_lo_half(h, a), sub_hi_half(h, b));
+  };
+  Fragment<DT> f;
+  f.v = __builtin_bit_cast(bf16x8, make_uint4(two(w.x, x[0], x[1]), two(w.y, x[2], x[3]), two(w.z, x[4], x[5]), two(w.w, x[6], x[7])));
+  return f;
+}
+
+// pack_fragment in two halves: elements 4 half .. 4 half + 3 of f.
 template <int DT>
 __device__ __forceinline__ void pack_half(Fragment<DT>& f, int half, f32x4 x) {
   if constexpr (DT == kF32) {
@@ -279,8 +292,8 @@ inline bool valid_window_call(const void* q, const void* k, const void* v, int32
          reinterpret_cast<uintptr_t>(v) % 16 == 0;
 }
 // (rows of a key head are numbered in 32 bits)
-inline bool window_supported(int32_t dtype, int64_t dim, int64_t tokens, int64_t ratio) {
-  return dim % (dtype == kF32 ? 4 : 8) == 0 && dim <= 256 && tokens * ratio < 0x7fff0000;
+inline bool window_supported(int64_t dim, int64_t tokens, int64_t ratio) {
+  return dim % 8 == 0 && dim <= 256 && tokens * ratio < 0x7fff0000;
 }
 
 // window 0: none

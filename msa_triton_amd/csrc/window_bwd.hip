@@ -42,37 +42,31 @@ struct WindowBwdArgs {
   int chunk_log2;             // tokens of a chunk of the rows that see first tokens from behind the window
 };
 
-// ---- delta: 16 lanes a row
+// ---- delta: the diagonal of a product of 16 rows' outputs and gradients, a wave sixteen rows. By the matrix unit and in the
+// order of dP, so that a row that sees one key, whose output is its value, has dp - delta = 0 to the last bit.
 
 template <int DT>
 __global__ __launch_bounds__(256) void window_delta_kernel(WindowBwdArgs A) {
   using E = typename Fragment<DT>::Element;
-  constexpr int kPer = DT == kF32 ? 4 : 8;
-  const int heads = A.G * A.ratio.d;
-  const int64_t row = (A.first + blockIdx.x) * 16 + threadIdx.x / 16;
-  if (row >= A.tokens * heads) return;
-  const int64_t t = row / heads;
-  const E* dout = static_cast<const E*>(A.dout.base) + t * A.dout.token + (row - t * heads) * A.dout.head;
+  const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4, heads = A.G * A.ratio.d;
+  const int64_t all = A.tokens * heads, row0 = ((A.first + blockIdx.x) * 4 + (threadIdx.x >> 6)) * 16;
+  if (row0 >= all) return;
+  const int64_t row = min(row0 + c, all - 1), t = row / heads;
+  const E* dout = static_cast<const E*>(A.dout.base) + A.dout.at(t, static_cast<int>(row - t * heads));
   const E* out = static_cast<const E*>(A.out) + row * A.D;
   const E* lo = static_cast<const E*>(A.out_lo) + row * A.D;
-  float sum = 0.f;
-  for (int d = threadIdx.x % 16 * kPer; d < A.D; d += 16 * kPer) {
-    const uint4 x = *reinterpret_cast<const uint4*>(dout + d), y = *reinterpret_cast<const uint4*>(out + d);
-    const uint4 z = A.out_lo ? *reinterpret_cast<const uint4*>(lo + d) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == kF32) {
-        sum = fmaf(__uint_as_float(xs[i]), __uint_as_float(ys[i]), sum);
-      } else {
-        sum = fmaf(lo16_f32<DT>(xs[i]), lo16_f32<DT>(ys[i]) + lo16_f32<DT>(zs[i]), sum);
-        sum = fmaf(hi16_f32<DT>(xs[i]), hi16_f32<DT>(ys[i]) + hi16_f32<DT>(zs[i]), sum);
-      }
-    }
+  f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f}, left = sum;
+  for (int d0 = 0; d0 < A.D; d0 += 32) {
+    const int d = d0 + 8 * q4;
+    const Fragment<DT> g = d < A.D ? fragment_at<DT>(dout + d) : no_fragment<DT>();
+    sum = product<DT>(d < A.D ? fragment_at<DT>(out + d) : no_fragment<DT>(), g, sum);
+    if (DT != kF32 && A.out_lo) left = product<DT>(d < A.D ? fragment_at<DT>(lo + d) : no_fragment<DT>(), g, left);
   }
+  if (c >> 2 == q4 && row0 + c < all) {  // row c of the product is in the quarter c / 4
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
-  if (threadIdx.x % 16 == 0) A.delta[row] = sum;
+    for (int i = 0; i < 4; ++i)
+      if ((c & 3) == i) A.delta[row0 + c] = sum[i] + left[i];
+  }
 }
 
 // ---- fp16: the power of two that ds of a lane's row (or key) is multiplied by, so that the largest one so far stays below 2^15
@@ -746,7 +740,7 @@ extern "C" int msa_window_attn_bwd(const void* q, const void* k, const void* v, 
     return kErrInvalidArgument;
   const int unit = dtype == kF32 ? 4 : 8;
   if (strides[6] % unit || strides[7] % unit || !near_rows(strides + 6, q_heads / kv_groups)) return kErrInvalidArgument;
-  if (!window_supported(dtype, head_dim, total_tokens, q_heads / kv_groups)) return kErrUnsupported;
+  if (!window_supported(head_dim, total_tokens, q_heads / kv_groups)) return kErrUnsupported;
   if (total_tokens == 0 || !(grad_q || grad_k || grad_v)) return kOk;
   if (!workspace || workspace_bytes < msa_window_attn_bwd_workspace_bytes(dtype, total_tokens, num_seqs, longest, q_heads,
                                                                           kv_groups, head_dim, window, sinks))
@@ -781,7 +775,7 @@ extern "C" int msa_window_attn_bwd(const void* q, const void* k, const void* v, 
   A.dv = grad_v;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 block(256);
-  int rc = launch_parts((total_tokens * q_heads + 15) / 16, [&](int64_t first, unsigned count) {
+  int rc = launch_parts((total_tokens * q_heads + 63) / 64, [&](int64_t first, unsigned count) {
     A.first = first;
     if (dtype == kBF16) hipLaunchKernelGGL(window_delta_kernel<kBF16>, dim3(count), block, 0, st, A);
     else if (dtype == kF16) hipLaunchKernelGGL(window_delta_kernel<kF16>, dim3(count), block, 0, st, A);

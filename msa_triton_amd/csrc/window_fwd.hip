@@ -10,8 +10,10 @@
 // O^T = V^T P^T (values by transposed reads with the keys in that same order).
 //
 // Logits, statistics and outputs are fp32. The weights enter the second product rounded once to the input type (half a step
-// of 2^-8 in bf16, of the size of the output's own rounding and averaged over the keys; in fp16 times 2^7, so that weights
-// down to 2^-21 keep their bits). The sum of the weights is that of the unrounded ones.
+// of 2^-8 in bf16, of the size of the output's own rounding and averaged over the keys: 0.0021 of the output where its own
+// is 0.0017; in fp16 times 2^7, so that weights down to 2^-21 keep their bits). For a backward pass they are two terms: its
+// delta = dO . out goes into every ds of a row, and dq and dk would be off by 0.0026 instead of 0.0021. The
+// sum of the weights is that of the unrounded ones.
 #include "window.hpp"
 
 namespace msa {
@@ -79,11 +81,14 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
   }
 }
 
-template <int DT, int NK, int MT, int KS>
-__global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_fwd_kernel(WindowFwdArgs A) {
+// TWO: weights as two terms.
+template <int DT, int NK, int MT, int KS, bool TWO>
+__global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 && !TWO ? 3 : 2) void window_fwd_kernel(WindowFwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
   constexpr float kUp = DT == kF16 ? 15.f - kSlack : 0.f;
+  // The weight of a row's only key is 1 to the last bit, and its output the value (what delta relies on); one operation more.
+  constexpr bool kExact = TWO || DT == kF32;
   __shared__ alignas(16) E kbuf[2][KS * RS], vbuf[2][KS * RS];
   const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -183,7 +188,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_
               s[m][kt][i] = seen ? s[m][kt][i] : -__builtin_inff();
             }
       }
-      Fragment<DT> pf[MT][KT / 2];
+      Fragment<DT> pf[MT][KT / 2], pl[MT][KT / 2];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         float high = s[m][0][0];
@@ -199,16 +204,18 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_
 #pragma unroll
           for (int d = 0; d < ND; ++d) acc[m][d] *= keep;
         }
-        const float shift = kUp - (top[m] == -__builtin_inff() ? 0.f : top[m] * factor);
+        const float base = top[m] == -__builtin_inff() ? 0.f : top[m], shift = kUp - base * factor;
 #pragma unroll
         for (int u = 0; u < KT / 2; ++u) {
           float p[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(s[m][2 * u + (i >> 2)][i & 3], factor, shift));
+            const float x = s[m][2 * u + (i >> 2)][i & 3];
+            p[i] = __builtin_amdgcn_exp2f(kExact ? fmaf(x - base, factor, kUp) : fmaf(x, factor, shift));
             l[m] += p[i];
           }
           pf[m][u] = pack_fragment<DT>(p);
+          if constexpr (TWO) pl[m][u] = second_terms<DT>(pf[m][u], p);
         }
       }
 #pragma unroll
@@ -217,7 +224,10 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_
         for (int u = 0; u < KT / 2; ++u) {
           const Fragment<DT> vf = column_fragment<DT>(vt_, RS, 32 * u, 16 * d, c, q4);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) acc[m][d] = product<DT>(vf, pf[m][u], acc[m][d]);
+          for (int m = 0; m < MT; ++m) {
+            acc[m][d] = product<DT>(vf, pf[m][u], acc[m][d]);
+            if constexpr (TWO) acc[m][d] = product<DT>(vf, pl[m][u], acc[m][d]);
+          }
         }
     }
     if (e + 1 < steps) store_step(e + 1);
@@ -273,7 +283,7 @@ extern "C" int msa_window_attn_fwd(const void* q, const void* k, const void* v, 
                          sinks, scale) ||
       !out)
     return kErrInvalidArgument;
-  if (!window_supported(dtype, head_dim, total_tokens, q_heads / kv_groups)) return kErrUnsupported;
+  if (!window_supported(head_dim, total_tokens, q_heads / kv_groups)) return kErrUnsupported;
   if (total_tokens == 0) return kOk;
   WindowFwdArgs A{};
   A.q = packed_view(q, strides);
@@ -290,20 +300,25 @@ extern "C" int msa_window_attn_fwd(const void* q, const void* k, const void* v, 
   A.out_lo = out_lo;
   A.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define MSA_WINDOW_FWD(DT, NK, MT, KS)                                                                                 \
+#define MSA_WINDOW_FWD(DT, NK, MT, TWO)                                                                                 \
   return launch_parts(tile_numbers(total_tokens, num_seqs, A.ratio, log2_of(64 * MT)) * kv_groups, [&](int64_t first, unsigned count) { \
-    A.first = first;                                                                                                   \
-    hipLaunchKernelGGL((window_fwd_kernel<DT, NK, MT, KS>), dim3(count), dim3(256), 0, st, A);                         \
+    A.first = first;                                                                                                    \
+    hipLaunchKernelGGL((window_fwd_kernel<DT, NK, MT, 32, TWO>), dim3(count), dim3(256), 0, st, A);                     \
   })
-#define MSA_WINDOW_FWD_DIM(DT)                       \
-  if (head_dim <= 64) MSA_WINDOW_FWD(DT, 2, 2, 32);  \
-  if (head_dim <= 96) MSA_WINDOW_FWD(DT, 3, 2, 32);  \
-  if (head_dim <= 128) MSA_WINDOW_FWD(DT, 4, 2, 32); \
-  if (head_dim <= 192) MSA_WINDOW_FWD(DT, 6, 1, 32); \
-  MSA_WINDOW_FWD(DT, 8, 1, 32)
-  if (dtype == kBF16) { MSA_WINDOW_FWD_DIM(kBF16); }
-  if (dtype == kF16) { MSA_WINDOW_FWD_DIM(kF16); }
-  MSA_WINDOW_FWD_DIM(kF32);
+#define MSA_WINDOW_FWD_DIM(DT, TWO)                     \
+  {                                                     \
+    if (head_dim <= 64) MSA_WINDOW_FWD(DT, 2, 2, TWO);  \
+    if (head_dim <= 96) MSA_WINDOW_FWD(DT, 3, 2, TWO);  \
+    if (head_dim <= 128) MSA_WINDOW_FWD(DT, 4, 2, TWO); \
+    if (head_dim <= 192) MSA_WINDOW_FWD(DT, 6, 1, TWO); \
+    MSA_WINDOW_FWD(DT, 8, 1, TWO);                      \
+  }
+  // (out_lo is asked for where a backward pass takes the output)
+  if (dtype == kBF16 && out_lo) MSA_WINDOW_FWD_DIM(kBF16, true)
+  if (dtype == kBF16) MSA_WINDOW_FWD_DIM(kBF16, false)
+  if (dtype == kF16 && out_lo) MSA_WINDOW_FWD_DIM(kF16, true)
+  if (dtype == kF16) MSA_WINDOW_FWD_DIM(kF16, false)
+  MSA_WINDOW_FWD_DIM(kF32, false)
 #undef MSA_WINDOW_FWD_DIM
 #undef MSA_WINDOW_FWD
 }

@@ -15,7 +15,7 @@
 //
 // Logits, statistics and outputs are fp32. With one tile of 16 rows, where the products are not the bound, a weight
 // enters the second product as two 16-bit terms (2^-17 of it left out); with more it is rounded once, as in the packed
-// form. In fp16 both are of the weight times 2^7. Bytes of an 8-bit page are exact in bf16; its scales go into logits
+// form (fp16 queries over an 8-bit cache, whose products are bf16's, take two terms). In fp16 both are of the weight times 2^7. Bytes of an 8-bit page are exact in bf16; its scales go into logits
 // and weights.
 #include "window.hpp"
 
@@ -632,6 +632,7 @@ template <int DT, bool FP8, int NK, int MT>
 __global__ __launch_bounds__(256, 2) void window_paged_rows_kernel(PagedWindowArgs A) {
   constexpr int R = 64 * MT, DP = 32 * NK, RS = DP + 16, ND = DP / 16, ES = FP8 ? 1 : 2;
   constexpr int PT = FP8 ? kBF16 : DT;          // type of the second product
+  constexpr bool kTwo = DT != PT;               // terms of a weight: fp16 results from bf16 products
   constexpr float kUp = PT == kF16 ? 15.f - kSlack : 0.f;
   constexpr int VD = 16 / ES, VL = DP / VD, kAll = 32 * VL, NV = (kAll + 255) / 256;  // values and lanes of a row's pieces
   __shared__ alignas(16) uint16_t kbuf[2][32 * RS], vbuf[2][32 * RS];
@@ -786,7 +787,7 @@ __global__ __launch_bounds__(256, 2) void window_paged_rows_kernel(PagedWindowAr
           }
           const bool whole = now.p0 >= 0 && now.p1 >= 0 && now.key + 31 < common && now.key + 31 <= now.upto &&
                              (of_sinks || now.key >= low_most || now.key + 31 < A.seen.sinks);
-          Fragment<PT> pf[MT];
+          Fragment<PT> pf[MT], pl[MT];
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             // raw dots; of an 8-bit page times its scale
@@ -820,12 +821,16 @@ __global__ __launch_bounds__(256, 2) void window_paged_rows_kernel(PagedWindowAr
               if constexpr (FP8) x[j] *= j < 4 ? now.vs0 : now.vs1;
             }
             pf[m] = pack_fragment<PT>(x);
+            if constexpr (kTwo) pl[m] = second_terms<PT>(pf[m], x);
           }
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
             const Fragment<PT> vf = column_fragment<PT>(vt, RS, 0, 16 * d, c, q4);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][d] = product<PT>(vf, pf[m], acc[m][d]);
+            for (int m = 0; m < MT; ++m) {
+              acc[m][d] = product<PT>(vf, pf[m], acc[m][d]);
+              if constexpr (kTwo) acc[m][d] = product<PT>(vf, pl[m], acc[m][d]);
+            }
           }
         }
         if (e + 1 < stop) store_step(b ^ 1);

