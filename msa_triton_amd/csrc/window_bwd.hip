@@ -3,18 +3,23 @@
 //   delta[i, h] = dO . O,  p_ij = exp(scale q_i . k_j - lse_i),  ds_ij = p_ij (dO_i . v_j - delta_i),
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_{i, h} ds_ij q_i,  dv_j = sum_{i, h} p_ij dO_i.
 //
-// Three launches, all sums in fixed orders: delta; dQ by tiles of rows as in the forward (three products a pair); dK and dV by
-// tiles of keys (four products), each workgroup over the rows that see its keys, all query heads of the key head among
-// them. The seven products are two more than one pass with atomic sums of dQ needs. The first tokens are seen by
-// all later rows: what their rows behind the window give is summed in a launch of its own, in chunks of rows
-// side by side, before the tiles that hold them add those sums to their own.
+// All sums are in fixed orders: delta; dQ by tiles of rows as in the forward (three products a pair); dK and dV by tiles of keys
+// (four products), each workgroup over the rows that see its keys, all query heads of the key head among them. The seven
+// products are two more than one pass with atomic sums of dQ needs. Rows of a tile of keys are shared by several
+// workgroups where the tiles alone would leave the chip idle (split_count), whose sums another launch adds up. The first tokens
+// are seen by all later rows: what the rows behind the window give is summed in launches of its own, in chunks of
+// rows side by side, before the tiles that hold them add it to their own.
 //
-// Bound by the matrix products, which wait for LDS: a wave of 32 rows (or keys) reads 8 KB a product and 32 keys
-// (or rows) of 128 dims.
+// Bound by the matrix products, the vector work between them and the LDS reads that feed them: a wave of 32 rows (or keys)
+// reads 8 KB a product and 32 keys (or rows) of 128 dims. 32K tokens, 32 heads of 128 over 4, window 4096, bf16: dQ 3.6 ms, dK
+// and dV 6.4. Two waves a SIMD hide the waits (one: dQ 5.5, dK and dV 8.4); for dK and dV that takes the values
+// from LDS, the logits of 16 rows after those of the other 16, and 256 registers.
 //
-// Logits, p, ds and all sums are fp32; p and ds enter their products rounded once to the input type. fp16 has neither
-// range nor small values for a ds: its products take ds times a power of two, one a row (dQ) or key (dK) that
-// follows the largest so far, and p times 2^15. delta takes the output with what its rounding left out.
+// Logits, p, ds and all sums are fp32. p enters its product rounded once to the input type; a ds enters as two terms (2^-17 of
+// it left out): one would be of the size of the gradients' own rounding and bring dq and dk from 0.0018 to 0.0024 of
+// themselves (dQ 3.0 ms, dK and dV 6.1). fp16 has neither range nor small values for a ds: its products take ds times a
+// power of two, one a row (dQ) or key (dK) that follows the largest so far, and p times 2^15. delta takes the output with
+// what its rounding left out.
 #include "window.hpp"
 
 namespace msa {
@@ -39,6 +44,7 @@ struct WindowBwdArgs {
   float* split;               // [splits][2][T][G][D]
   int splits;                 // workgroups that share the rows of a tile of keys
   int sink_tiles, sink_rows;  // of a tile
+  bool whole_tiles;           // tiles that hold first tokens go through all rows: there are no chunks
   int chunk_log2;             // tokens of a chunk of the rows that see first tokens from behind the window
 };
 
@@ -145,6 +151,7 @@ template <int DT, int NK, int MT, int KS>
 __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dq_kernel(WindowBwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
+  constexpr bool kTwo = DT != kF32;  // terms of a ds
   __shared__ alignas(16) E kbuf[2][KS * RS], vbuf[2][KS * RS];
   const int lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -235,7 +242,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dq_kernel(Wind
         }
       }
       const bool whole = of_sinks ? j0 + KS <= sinks : j0 + KS - 1 <= w0 && (w1 - j0 < A.seen.window || j0 + KS <= A.seen.sinks);
-      Fragment<DT> df[MT][KT / 2];
+      Fragment<DT> df[MT][KT / 2], dl[MT][KT / 2];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         float ds[KT][4];
@@ -277,6 +284,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dq_kernel(Wind
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = ds[2 * u + (i >> 2)][i & 3];
           df[m][u] = pack_fragment<DT>(x);
+          if constexpr (kTwo) dl[m][u] = second_terms<DT>(df[m][u], x);
         }
       }
 #pragma unroll
@@ -285,7 +293,10 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dq_kernel(Wind
         for (int u = 0; u < KT / 2; ++u) {
           const Fragment<DT> kf = column_fragment<DT>(kt_, RS, 32 * u, 16 * d, c, q4);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) acc[m][d] = product<DT>(kf, df[m][u], acc[m][d]);
+          for (int m = 0; m < MT; ++m) {
+            acc[m][d] = product<DT>(kf, df[m][u], acc[m][d]);
+            if constexpr (kTwo) acc[m][d] = product<DT>(kf, dl[m][u], acc[m][d]);
+          }
         }
     }
     if (e + 1 < steps) store_step(e + 1);
@@ -382,6 +393,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dkv_kernel(Win
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, BK = 64 * KT, QS = 32;
   constexpr float kUp = DT == kF16 ? 15.f : 0.f;
   constexpr int kBuffers = NK <= 4 || DT == kF32 ? 2 : 1;  // (of LDS for two workgroups a CU)
+  constexpr bool kTwo = DT != kF32;        // terms of a ds
   constexpr bool kValuesInLds = DT != kF32;  // (in registers with the keys they would leave room for one wave a SIMD)
   __shared__ alignas(16) E qbuf[kBuffers][QS * RS], gbuf[kBuffers][QS * RS], values[kValuesInLds ? BK * RS : 8];
   __shared__ alignas(16) float shift_of[kBuffers][QS], delta_of[kBuffers][QS];
@@ -411,7 +423,8 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dkv_kernel(Win
     if (static_cast<int64_t>(at.tile) * BK >= at.n) return;
     j0 = at.tile * BK;
     from = j0;
-    to = static_cast<int>(min(static_cast<int64_t>(at.n), static_cast<int64_t>(j0) + BK - 1 + A.seen.window));
+    to = A.whole_tiles && j0 < A.seen.sinks ? at.n
+                                            : static_cast<int>(min(static_cast<int64_t>(at.n), static_cast<int64_t>(j0) + BK - 1 + A.seen.window));
   }
   int rb = from * ratio, re = to * ratio;
   if (!SINKS && A.splits > 1) {
@@ -499,9 +512,9 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dkv_kernel(Win
     if (has_keys && tb >= ka && (ta - kb < A.seen.window || ka < A.seen.sinks)) {
       const E *qt = qbuf[b], *gt = gbuf[b];
       const bool whole = r0 + QS <= re && ta >= kb && (tb - ka < A.seen.window || kb < A.seen.sinks);
-      Fragment<DT> pf[KT], df[KT];
+      Fragment<DT> pf[KT], df[KT], dl[KT];
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) pf[kt] = df[kt] = no_fragment<DT>();
+      for (int kt = 0; kt < KT; ++kt) pf[kt] = df[kt] = dl[kt] = no_fragment<DT>();
       // (16 rows after the other: both at once take more registers than two waves a SIMD have)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -545,12 +558,13 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dkv_kernel(Win
               const float factor = range[kt].widen(big);
 #pragma unroll
               for (int d = 0; d < ND; ++d) dk[kt][d] *= factor;
-              if (h == 1) rescale_half(df[kt], factor);
+              if (h == 1) rescale_half(df[kt], factor), rescale_half(dl[kt], factor);
             }
             ds *= range[kt].up, p *= 0x1p15f;
           }
           pack_half<DT>(pf[kt], h, p);
           pack_half<DT>(df[kt], h, ds);
+          if constexpr (kTwo) pack_half<DT>(dl[kt], h, left_out<DT>(ds));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -562,6 +576,7 @@ __global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dkv_kernel(Win
         for (int kt = 0; kt < KT; ++kt) {
           dv[kt][d] = product<DT>(gf, pf[kt], dv[kt][d]);
           dk[kt][d] = product<DT>(qf, df[kt], dk[kt][d]);
+          if constexpr (kTwo) dk[kt][d] = product<DT>(qf, dl[kt], dk[kt][d]);
         }
       }
     }
@@ -658,7 +673,7 @@ __global__ __launch_bounds__(256) void window_dkv_join(WindowBwdArgs A) {
   const int s = A.nseq == 1 ? 0 : wave_upper_index(A.nseq, t, [&](int i) { return static_cast<int64_t>(A.cu[i]); });
   const int start = A.cu[s], n = A.cu[s + 1] - start, j = static_cast<int>(t - start), tile = j / BK;
   const int64_t behind = static_cast<int64_t>(tile) * BK + BK - 1 + A.seen.window;  // tokens of the chunks: from here on
-  if (j < A.seen.sinks && behind < n) {
+  if (j < A.seen.sinks && behind < n && !A.whole_tiles) {
     part = sink_part(A, start, s, static_cast<int>(behind) >> A.chunk_log2, tile, g) + static_cast<int64_t>(j - tile * BK) * A.D +
            (mine ? d : 0);
     dk += *reinterpret_cast<const f32x4*>(part);
@@ -675,30 +690,38 @@ __global__ __launch_bounds__(256) void window_dkv_join(WindowBwdArgs A) {
 // Keys of a workgroup of the dK / dV kernels.
 int keys_per_tile(int32_t dtype, int64_t dim) { return dtype != kF32 && dim <= 128 ? 128 : 64; }
 
-// Tiles that hold first tokens, and their rows in one; 0 where no sequence has rows behind the window.
+// Tiles that hold first tokens, their rows in one, and the chunks of the rows behind the window; no tiles where no sequence has
+// such rows, or where the chunks' sums would take more than 256 MiB (many first tokens, or many short sequences: their tiles
+// go through all rows then).
 struct SinkShape {
   int64_t tiles, rows;
   int chunk_log2;
+  bool whole;  // tiles that hold first tokens go through all rows
 };
-SinkShape sink_shape(int32_t dtype, int64_t dim, int64_t tokens, int64_t longest, int64_t ratio, int64_t window, int64_t sinks) {
-  if (window == 0 || sinks == 0 || longest <= window) return SinkShape{0, 0, 0};
+int64_t sink_floats(const SinkShape& shape, int64_t tokens, int64_t nseq, int64_t groups, int64_t dim) {
+  return tile_numbers(tokens, nseq, 1, shape.chunk_log2) * shape.tiles * groups * 2 * shape.rows * dim;
+}
+SinkShape sink_shape(int32_t dtype, int64_t dim, int64_t tokens, int64_t nseq, int64_t longest, int64_t ratio, int64_t groups,
+                     int64_t window, int64_t sinks) {
+  if (window == 0 || sinks == 0 || longest <= window) return SinkShape{0, 0, 0, false};
   // 256 rows a chunk at least, and no more than 256 chunks in all
   int chunk_log2 = 4;
   while (ratio << chunk_log2 < 256 || tokens >> chunk_log2 > 256) ++chunk_log2;
   const int64_t keys = keys_per_tile(dtype, dim), most = sinks < longest ? sinks : longest;
-  return SinkShape{(most + keys - 1) / keys, most < keys ? (most + 15) / 16 * 16 : keys, chunk_log2};
+  const SinkShape shape{(most + keys - 1) / keys, most < keys ? (most + 15) / 16 * 16 : keys, chunk_log2, false};
+  return sink_floats(shape, tokens, nseq, groups, dim) <= int64_t{1} << 26 ? shape : SinkShape{0, 0, 0, true};
 }
 
 // Workgroups that share the rows of a tile of keys: so many that the largest share is not above what each of the workgroups
 // that run at once (512, or 256 of fp32) gets of all the work, which is at least that of the longest sequence and of
 // sequences of equal length; no more than give a share 128 rows, nor than fill 256 MiB with parts.
 int64_t split_count(int32_t dtype, int64_t tokens, int64_t nseq, int64_t longest, int64_t q_heads, int64_t groups, int64_t dim,
-                    int64_t window) {
+                    int64_t window, bool whole) {
   const double keys = keys_per_tile(dtype, dim), w = window == 0 ? 1e18 : static_cast<double>(window);
   const auto pairs = [&](double n) { return n <= w ? n * n / 2 : w * (n - w / 2); };
   const double all = static_cast<double>(nseq) * pairs(static_cast<double>(tokens) / nseq), one = pairs(static_cast<double>(longest));
   const double work = groups * (all > one ? all : one) / keys;  // tokens of rows that tiles go through
-  const double most = longest < w + keys ? longest : w + keys;
+  const double most = whole || longest < w + keys ? longest : w + keys;
   const int64_t even = static_cast<int64_t>(most * (dtype == kF32 ? 256 : 512) / (work < 1 ? 1 : work) + 0.5);
   const int64_t by_rows = static_cast<int64_t>(most * (q_heads / groups) / 128), by_size = (int64_t{1} << 25) / (tokens * groups * dim);
   int64_t n = even < by_rows ? even : by_rows;
@@ -707,9 +730,6 @@ int64_t split_count(int32_t dtype, int64_t tokens, int64_t nseq, int64_t longest
 }
 
 int64_t delta_floats(int64_t tokens, int64_t q_heads) { return (tokens * q_heads + 3) / 4 * 4; }
-int64_t sink_floats(const SinkShape& shape, int64_t tokens, int64_t nseq, int64_t groups, int64_t dim) {
-  return tile_numbers(tokens, nseq, 1, shape.chunk_log2) * shape.tiles * groups * 2 * shape.rows * dim;
-}
 
 }  // namespace
 }  // namespace msa
@@ -722,8 +742,9 @@ extern "C" int64_t msa_window_attn_bwd_workspace_bytes(int32_t dtype, int64_t to
   if (total_tokens <= 0 || num_seqs <= 0 || q_heads <= 0 || kv_groups <= 0 || q_heads % kv_groups || head_dim <= 0 || window < 0 ||
       sinks < 0)
     return 0;
-  const SinkShape shape = sink_shape(dtype, head_dim, total_tokens, longest, q_heads / kv_groups, window, sinks);
-  const int64_t splits = split_count(dtype, total_tokens, num_seqs, longest, q_heads, kv_groups, head_dim, window);
+  const SinkShape shape = sink_shape(dtype, head_dim, total_tokens, num_seqs, longest, q_heads / kv_groups, kv_groups, window, sinks);
+  const int64_t splits = split_count(dtype, total_tokens, num_seqs, longest, q_heads, kv_groups, head_dim, window,
+                                     shape.whole);
   return 4 * (delta_floats(total_tokens, q_heads) + sink_floats(shape, total_tokens, num_seqs, kv_groups, head_dim) +
               (splits > 1 ? splits * 2 * total_tokens * kv_groups * head_dim : 0));
 }
@@ -745,7 +766,7 @@ extern "C" int msa_window_attn_bwd(const void* q, const void* k, const void* v, 
   if (!workspace || workspace_bytes < msa_window_attn_bwd_workspace_bytes(dtype, total_tokens, num_seqs, longest, q_heads,
                                                                           kv_groups, head_dim, window, sinks))
     return kErrInvalidArgument;
-  const SinkShape shape = sink_shape(dtype, head_dim, total_tokens, longest, q_heads / kv_groups, window, sinks);
+  const SinkShape shape = sink_shape(dtype, head_dim, total_tokens, num_seqs, longest, q_heads / kv_groups, kv_groups, window, sinks);
   WindowBwdArgs A{};
   A.q = packed_view(q, strides);
   A.k = packed_view(k, strides + 2);
@@ -766,7 +787,8 @@ extern "C" int msa_window_attn_bwd(const void* q, const void* k, const void* v, 
   A.delta = static_cast<float*>(workspace);
   A.part = A.delta + delta_floats(total_tokens, q_heads);
   A.split = A.part + sink_floats(shape, total_tokens, num_seqs, kv_groups, head_dim);
-  A.splits = static_cast<int>(split_count(dtype, total_tokens, num_seqs, longest, q_heads, kv_groups, head_dim, window));
+  A.splits = static_cast<int>(split_count(dtype, total_tokens, num_seqs, longest, q_heads, kv_groups, head_dim, window, shape.whole));
+  A.whole_tiles = shape.whole;
   A.sink_tiles = static_cast<int>(shape.tiles);
   A.sink_rows = static_cast<int>(shape.rows);
   A.chunk_log2 = shape.chunk_log2;

@@ -8,7 +8,7 @@ Tolerances, with h half a step of the type relative to the value (``finfo.eps / 
 * weights enter the second product rounded once (h in 16 bits, 0 in fp32), or, for a backward pass, as two terms (h^2 left
   out), so out is off by (h + 2 e + (n + 8) u) sum p|v|, n keys, then by h of itself;
 * delta = dO . out takes the latter out, to 2 h^2;
-* ds = p (dp - delta) is off by p (D u sum |dO||v| + that of delta) and its weight's error of |ds|, and is rounded once;
+* ds = p (dp - delta) is off by p (D u sum |dO||v| + that of delta) and its weight's error of |ds|, and is two terms (h^2);
 * each gradient is a sum of products of these, off by the sum of their errors' magnitudes, then by h of itself.
 
 What falls below the type's range is off by its smallest step.
@@ -76,7 +76,7 @@ def reference(q, k, v, lengths, window, sinks, scale, do=None):
             dp, delta = y @ vv.T, (y * (p @ vv)).sum(1, keepdim=True)
             ds = p * (dp - delta)
             e_delta = (y.abs() * (off["trained"][rows, head] + (2 * h_in * h_in + (d + 8) * U) * size)).sum(1, keepdim=True)
-            e_ds = p * ((d + 8) * U * (y.abs() @ vv.abs().T) + e_delta) + (h_in + w) * (ds.abs() + 4 * U * p * delta.abs())
+            e_ds = p * ((d + 8) * U * (y.abs() @ vv.abs().T) + e_delta) + (h_in * h_in + w) * (ds.abs() + 4 * U * p * delta.abs())
             few = (n * ratio + 8) * U  # of a sum
             res["dq"][rows, head] = ds @ kk * scale
             off["dq"][rows, head] = (e_ds + few * ds.abs()) @ kk.abs() * abs(scale)
@@ -129,6 +129,8 @@ CASES = [  # lengths, hq, g, d, window, sinks, dtype
     ([2500], 2, 1, 64, 300, 4, torch.bfloat16),          # three chunks of rows behind the window
     ([2500], 2, 1, 64, 1, 70, torch.float16),
     ([2100, 1, 1030], 2, 1, 64, 1024, 16, torch.float32),
+    ([6000, 700], 2, 1, 64, 5, 900, torch.bfloat16),     # tiles of first tokens that go through all rows
+    ([2, 65] * 150, 2, 1, 256, 5, 64, torch.float16),    # the same: many short sequences
     ([64] * 40, 2, 2, 64, 8, 2, torch.bfloat16),
     ([3] * 200 + [90], 8, 2, 64, 2, 1, torch.bfloat16),  # more sequences than a wave has lanes
     ([400], 64, 1, 64, 31, 4, torch.bfloat16),           # one token a tile of rows

@@ -117,3 +117,19 @@ def test_parents():
             _serve(True, **x, parents=parents)
     with pytest.raises(NotImplementedError, match="512 nodes"):
         _serve(True, **_paged(tokens=514))
+
+
+def test_backward_workspace_is_bounded():
+    """Beyond delta: parts of sums of at most 256 MiB for each of the two kinds, whatever the window and the first tokens."""
+    from msa_triton_amd import _lib
+
+    size = _lib.lib().msa_window_attn_bwd_workspace_bytes
+    for code in (0, 1, 2):
+        for tokens, seqs, longest in ((1, 1, 1), (1280, 2, 768), (32768, 1, 32768), (32768, 500, 9000), (1 << 20, 10000, 3000),
+                                      (1 << 20, 1, 1 << 20)):
+            for hq, g, d in ((8, 2, 64), (32, 4, 128), (64, 8, 256), (128, 1, 80)):
+                for window in (0, 1, 100, 4096, 1 << 30):
+                    for sinks in (0, 1, 4, 130, 5000, 2147483647):
+                        got = size(code, tokens, seqs, longest, hq, g, d, window, sinks)
+                        delta = 4 * (tokens * hq + 3)
+                        assert 4 * tokens * hq <= got <= delta + (2 << 28), (code, tokens, seqs, longest, hq, g, d, window, sinks)
