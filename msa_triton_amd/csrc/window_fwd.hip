@@ -83,7 +83,7 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
 
 // TWO: weights as two terms.
 template <int DT, int NK, int MT, int KS, bool TWO>
-__global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 && !TWO ? 3 : 2) void window_fwd_kernel(WindowFwdArgs A) {
+__global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_fwd_kernel(WindowFwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
   constexpr float kUp = DT == kF16 ? 15.f - kSlack : 0.f;

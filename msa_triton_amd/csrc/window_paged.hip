@@ -730,8 +730,9 @@ __global__ __launch_bounds__(256, 2) void window_paged_rows_kernel(PagedWindowAr
 #pragma unroll
       for (int p = 0; p < NV; ++p) {
         const bool second = half_of(p) != 0;
-        kr[p] = *reinterpret_cast<const uint4*>(kbase + (second ? k1 : k0) + k_off[p]);
-        vr[p] = *reinterpret_cast<const uint4*>(vbase + (second ? v1 : v0) + v_off[p]);
+        const char *k = kbase + scalar(second ? k1 : k0), *v = vbase + scalar(second ? v1 : v0);
+        kr[p] = *reinterpret_cast<const uint4*>(k + k_off[p]);
+        vr[p] = *reinterpret_cast<const uint4*>(v + v_off[p]);
       }
       in_flight.ks0 = in_flight.ks1 = in_flight.vs0 = in_flight.vs1 = 1.f;
       if constexpr (FP8) {
@@ -881,17 +882,111 @@ __global__ __launch_bounds__(256, 2) void window_paged_rows_kernel(PagedWindowAr
   }
 }
 
-// The parts of a row that several workgroups share, added up by WAVES waves (four for few rows, one for many): every
-// WAVES-th part each, eight of them in flight, two dims a lane and pass.
-template <int DT, bool FP8, int R, int WAVES>
+// The parts of rows that several workgroups share, of many rows: a workgroup sixteen rows of a tile, a wave four of them, their
+// maxima and sums sixteen parts at a time, then the outputs with four parts of each row in flight, two dims a lane and pass.
+template <int DT, bool FP8, int R>
+__global__ __launch_bounds__(256) void window_paged_join_rows(PagedWindowArgs A, int64_t first) {
+  constexpr float kUp = !FP8 && DT == kF16 ? 15.f - kSlack : 0.f;
+  __shared__ float weights[4][4][kMostParts];
+  const int lane = threadIdx.x & 63, ratio = A.ratio.d;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t item = first + blockIdx.x;
+  const int row0 = static_cast<int>(item % (R / 16)) * 16 + 4 * wave;
+  item /= R / 16;
+  const int g = static_cast<int>(item % A.G);
+  const TilePlace at = tile_place(A.cu, A.nseq, item / A.G, ratio, log2_of(R));
+  const PagedPlan plan = *A.plan;
+  const int context = A.context[at.seq], live = min(R, at.n * ratio - at.tile * R);
+  if (row0 >= live) return;
+  const SeqPlan P = seq_plan<R>(A, at.start, at.start + at.n, context);
+  const int64_t begin = A.first_item[at.seq] + (static_cast<int64_t>(g) * P.tiles + at.tile) * P.steps;
+  const int64_t w0 = scalar(begin / plan.share);
+  const int parts = __builtin_amdgcn_readfirstlane(static_cast<int>((begin + P.steps - 1) / plan.share - w0) + 1);
+  if (parts == 1) return;
+  auto place_of = [&](int z) { return (w0 + z) * 2 + (z == 0 ? 1 : 0); };
+
+  const int i_own = lane >> 4, r_own = min(row0 + i_own, live - 1);  // the row that this lane weighs parts of
+  float top = -__builtin_inff(), sum = 0.f;
+  for (int z = lane & 15; z < parts; z += 16) {
+    const float high = A.stats[place_of(z) * 2 * R + r_own];
+    weights[wave][i_own][z] = high;
+    top = fmaxf(top, high);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+  for (int z = lane & 15; z < parts; z += 16) {
+    const float high = weights[wave][i_own][z];
+    const float w = high == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(high - top);
+    weights[wave][i_own][z] = w;
+    sum += w * A.stats[(place_of(z) * 2 + 1) * R + r_own];
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+  const float inv_own = sum == 0.f ? 0.f : 1.f / sum;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  float inv[4], all[4] = {0.f, 0.f, 0.f, 0.f};
+  int64_t out_row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int in_group = at.tile * R + min(row0 + i, live - 1), tok = A.ratio(in_group);
+    inv[i] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(inv_own), 16 * i));
+    out_row[i] = (at.start + static_cast<int64_t>(tok)) * (A.G * ratio) + g * ratio + in_group - tok * ratio;
+  }
+  for (int d0 = 0; d0 < A.D; d0 += 128) {
+    const int d = min(d0 + 2 * lane, A.D - 2);
+    float2 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = make_float2(0.f, 0.f);
+    for (int z0 = 0; z0 < parts; z0 += 4) {
+      float2 x[4][4];
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[z][i] = z0 + z < parts ? *reinterpret_cast<const float2*>(
+                                         A.part + (place_of(z0 + z) * R + min(row0 + i, live - 1)) * A.D + d)
+                                   : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f = z0 + z < parts ? weights[wave][i][z0 + z] : 0.f;
+          o[i].x = fmaf(f, x[z][i].x, o[i].x);
+          o[i].y = fmaf(f, x[z][i].y, o[i].y);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i].x *= inv[i], o[i].y *= inv[i];
+      all[i] += o[i].x + o[i].y;
+      if (row0 + i < live && d0 + 2 * lane < A.D)
+        *reinterpret_cast<uint32_t*>(A.out + out_row[i] * A.D + d) = DT == kF16 ? cvt_pk_f16(o[i].x, o[i].y) : cvt_pk_bf16(o[i].x, o[i].y);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float top_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), 16 * i));
+    const float sum_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sum), 16 * i));
+    if (row0 + i >= live) break;
+    if (lane == 0 && A.lse) A.lse[out_row[i]] = sum_i == 0.f ? -__builtin_inff() : (top_i - kUp + __log2f(sum_i)) * kLn2Window;
+    if (__any(!finite(all[i])) && sum_i == sum_i) {
+      const int in_group = at.tile * R + row0 + i, tok = A.ratio(in_group);
+      careful_row<DT, FP8>(A, at.seq, at.start, context, tok, g, g * ratio + in_group - tok * ratio, top_i - kUp, inv[i]);
+    }
+  }
+}
+
+// The same of few rows: four waves a row, every fourth part each, eight of them in flight.
+template <int DT, bool FP8, int R>
 __global__ __launch_bounds__(256) void window_paged_join(PagedWindowArgs A, int64_t first) {
   constexpr float kUp = !FP8 && DT == kF16 ? 15.f - kSlack : 0.f;
   __shared__ float weights[4][kMostParts], sums[4][128];
   const int lane = threadIdx.x & 63, ratio = A.ratio.d;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t out_row = WAVES == 4 ? first + blockIdx.x : (first + blockIdx.x) * 4 + wave;
+  const int64_t out_row = first + blockIdx.x;
   const int heads = A.G * ratio;
-  if (out_row >= A.tokens * heads) return;
   const int64_t t = out_row / heads;
   const int head = static_cast<int>(out_row - t * heads), g = A.ratio(head);
   const PagedPlan plan = *A.plan;
@@ -931,32 +1026,30 @@ __global__ __launch_bounds__(256) void window_paged_join(PagedWindowArgs A, int6
   for (int d0 = 0; d0 < A.D; d0 += 128) {
     const int d = min(d0 + 2 * lane, A.D - 2);
     float o0 = 0.f, o1 = 0.f;
-    for (int z0 = WAVES == 4 ? wave : 0; z0 < parts; z0 += 8 * WAVES) {
+    for (int z0 = wave; z0 < parts; z0 += 32) {
       float2 x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        x[i] = z0 + WAVES * i < parts ? *reinterpret_cast<const float2*>(A.part + (place_of(z0 + WAVES * i) * R + r) * A.D + d)
+        x[i] = z0 + 4 * i < parts ? *reinterpret_cast<const float2*>(A.part + (place_of(z0 + 4 * i) * R + r) * A.D + d)
                                       : make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float f = z0 + WAVES * i < parts ? weight[z0 + WAVES * i] : 0.f;
+        const float f = z0 + 4 * i < parts ? weight[z0 + 4 * i] : 0.f;
         o0 = fmaf(f, x[i].x, o0);
         o1 = fmaf(f, x[i].y, o1);
       }
     }
-    if constexpr (WAVES == 4) {
-      sums[wave][2 * lane] = o0, sums[wave][2 * lane + 1] = o1;
-      __syncthreads();
-      o0 = ((sums[0][2 * lane] + sums[1][2 * lane]) + (sums[2][2 * lane] + sums[3][2 * lane]));
-      o1 = ((sums[0][2 * lane + 1] + sums[1][2 * lane + 1]) + (sums[2][2 * lane + 1] + sums[3][2 * lane + 1]));
-      __syncthreads();
-    }
+    sums[wave][2 * lane] = o0, sums[wave][2 * lane + 1] = o1;
+    __syncthreads();
+    o0 = ((sums[0][2 * lane] + sums[1][2 * lane]) + (sums[2][2 * lane] + sums[3][2 * lane]));
+    o1 = ((sums[0][2 * lane + 1] + sums[1][2 * lane + 1]) + (sums[2][2 * lane + 1] + sums[3][2 * lane + 1]));
+    __syncthreads();
     o0 *= inv, o1 *= inv;
     all += o0 + o1;
-    if ((WAVES == 1 || wave == 0) && d0 + 2 * lane < A.D)
+    if (wave == 0 && d0 + 2 * lane < A.D)
       *reinterpret_cast<uint32_t*>(A.out + out_row * A.D + d) = DT == kF16 ? cvt_pk_f16(o0, o1) : cvt_pk_bf16(o0, o1);
   }
-  if (WAVES == 4 && wave != 0) return;
+  if (wave != 0) return;
   if (lane == 0 && A.lse) A.lse[out_row] = sum == 0.f ? -__builtin_inff() : (top - kUp + __log2f(sum)) * kLn2Window;
   if (__any(!finite(all)) && sum == sum)
     careful_row<DT, FP8>(A, s, start, context, tok, g, head, top - kUp, inv);
@@ -1065,21 +1158,31 @@ extern "C" int msa_window_attn_paged(const void* q, const void* k_cache, const v
   A.first_item = reinterpret_cast<int64_t*>(A.stats + 4 * S.workgroups * S.rows);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(S.workgroups)), block(256);
-#define MSA_WINDOW_PAGED(KERNEL, DT, F8, R, WAVES)                                                                        \
-  {                                                                                                                       \
-    hipLaunchKernelGGL(KERNEL, grid, block, 0, st, A);                                                                    \
-    const int rc = status_from(hipGetLastError());                                                                        \
-    if (rc != kOk) return rc;                                                                                             \
-    const int64_t all = total_tokens * q_heads;                                                                           \
-    return launch_parts(WAVES == 4 ? all : (all + 3) / 4, [&](int64_t first, unsigned count) {                            \
-      hipLaunchKernelGGL((window_paged_join<DT, F8, R, WAVES>), dim3(count), block, 0, st, A, first);                     \
-    });                                                                                                                   \
+  // rows that four waves each add up (480 rows of 16 parts 5.5 us, four rows a wave 9.5), or one wave four (26 000 rows of 2 or 3 16
+  // us, a wave each 26)
+  const bool few = total_tokens * q_heads <= 2048;
+#define MSA_WINDOW_PAGED(KERNEL, JOIN, PARTS)                                                           \
+  {                                                                                                     \
+    hipLaunchKernelGGL(KERNEL, grid, block, 0, st, A);                                                  \
+    const int rc = status_from(hipGetLastError());                                                      \
+    if (rc != kOk) return rc;                                                                           \
+    return launch_parts(PARTS, [&](int64_t first, unsigned count) {                                     \
+      hipLaunchKernelGGL(JOIN, dim3(count), block, 0, st, A, first);                                    \
+    });                                                                                                 \
   }
-#define MSA_WINDOW_PAGED_DIM(DT, F8, NK, MT)                                                                              \
-  {                                                                                                                       \
-    if (S.rows == 16) MSA_WINDOW_PAGED((window_paged_kernel<DT, F8, NK>), DT, F8, 16, 4)                                  \
-    if (S.rows == 64) MSA_WINDOW_PAGED((window_paged_rows_kernel<DT, F8, NK, 1>), DT, F8, 64, 1)                          \
-    MSA_WINDOW_PAGED((window_paged_rows_kernel<DT, F8, NK, MT>), DT, F8, 64 * MT, 1)                                      \
+#define MSA_WINDOW_PAGED_ROWS(DT, F8, NK, MT)                                                           \
+  {                                                                                                     \
+    if (few)                                                                                            \
+      MSA_WINDOW_PAGED((window_paged_rows_kernel<DT, F8, NK, MT>), (window_paged_join<DT, F8, 64 * MT>), total_tokens * q_heads) \
+    MSA_WINDOW_PAGED((window_paged_rows_kernel<DT, F8, NK, MT>), (window_paged_join_rows<DT, F8, 64 * MT>), \
+                     tile_numbers(total_tokens, num_seqs, ratio, log2_of(64 * MT)) * kv_groups * (4 * MT)) \
+  }
+#define MSA_WINDOW_PAGED_DIM(DT, F8, NK, MT)                                                            \
+  {                                                                                                     \
+    if (S.rows == 16)                                                                                   \
+      MSA_WINDOW_PAGED((window_paged_kernel<DT, F8, NK>), (window_paged_join<DT, F8, 16>), total_tokens * q_heads) \
+    if (S.rows == 64) MSA_WINDOW_PAGED_ROWS(DT, F8, NK, 1)                                              \
+    MSA_WINDOW_PAGED_ROWS(DT, F8, NK, MT)                                                               \
   }
 #define MSA_WINDOW_PAGED_TYPE(DT, F8)                       \
   {                                                         \
@@ -1095,5 +1198,6 @@ extern "C" int msa_window_attn_paged(const void* q, const void* k_cache, const v
   MSA_WINDOW_PAGED_TYPE(kF16, false)
 #undef MSA_WINDOW_PAGED_TYPE
 #undef MSA_WINDOW_PAGED_DIM
+#undef MSA_WINDOW_PAGED_ROWS
 #undef MSA_WINDOW_PAGED
 }
