@@ -148,7 +148,7 @@ __device__ __forceinline__ void careful_dq(const WindowBwdArgs& A, int start, in
 }
 
 template <int DT, int NK, int MT, int KS>
-__global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dq_kernel(WindowBwdArgs A) {
+__global__ __launch_bounds__(256, DT == kF32 && NK > 4 ? 1 : 2) void window_dq_kernel(WindowBwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
   constexpr bool kTwo = DT != kF32;  // terms of a ds
@@ -388,7 +388,7 @@ __device__ __forceinline__ float* sink_part(const WindowBwdArgs& A, int start, i
 
 // SINKS: the rows of one chunk that see the first tokens from behind the window; their sums go to A.part.
 template <int DT, int NK, int KT, bool SINKS>
-__global__ __launch_bounds__(256, DT == kF32 ? 1 : 2) void window_dkv_kernel(WindowBwdArgs A) {
+__global__ __launch_bounds__(256, DT == kF32 && NK > 4 ? 1 : 2) void window_dkv_kernel(WindowBwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, BK = 64 * KT, QS = 32;
   constexpr float kUp = DT == kF16 ? 15.f : 0.f;
@@ -713,7 +713,7 @@ SinkShape sink_shape(int32_t dtype, int64_t dim, int64_t tokens, int64_t nseq, i
 }
 
 // Workgroups that share the rows of a tile of keys: so many that the largest share is not above what each of the workgroups
-// that run at once (512, or 256 of fp32) gets of all the work, which is at least that of the longest sequence and of
+// that run at once (512, or 256 of more than 128 fp32 dims) gets of all the work, which is at least that of the longest sequence and of
 // sequences of equal length; no more than give a share 128 rows, nor than fill 256 MiB with parts.
 int64_t split_count(int32_t dtype, int64_t tokens, int64_t nseq, int64_t longest, int64_t q_heads, int64_t groups, int64_t dim,
                     int64_t window, bool whole) {
@@ -722,7 +722,7 @@ int64_t split_count(int32_t dtype, int64_t tokens, int64_t nseq, int64_t longest
   const double all = static_cast<double>(nseq) * pairs(static_cast<double>(tokens) / nseq), one = pairs(static_cast<double>(longest));
   const double work = groups * (all > one ? all : one) / keys;  // tokens of rows that tiles go through
   const double most = whole || longest < w + keys ? longest : w + keys;
-  const int64_t even = static_cast<int64_t>(most * (dtype == kF32 ? 256 : 512) / (work < 1 ? 1 : work) + 0.5);
+  const int64_t even = static_cast<int64_t>(most * (dtype == kF32 && dim > 128 ? 256 : 512) / (work < 1 ? 1 : work) + 0.5);
   const int64_t by_rows = static_cast<int64_t>(most * (q_heads / groups) / 128), by_size = (int64_t{1} << 25) / (tokens * groups * dim);
   int64_t n = even < by_rows ? even : by_rows;
   n = n < by_size ? n : by_size;

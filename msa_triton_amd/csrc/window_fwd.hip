@@ -83,7 +83,7 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
 
 // TWO: weights as two terms.
 template <int DT, int NK, int MT, int KS, bool TWO>
-__global__ __launch_bounds__(256, DT == kF32 ? 1 : NK <= 4 ? 3 : 2) void window_fwd_kernel(WindowFwdArgs A) {
+__global__ __launch_bounds__(256, NK > 4 ? (DT == kF32 ? 1 : 2) : DT == kF32 ? 2 : 3) void window_fwd_kernel(WindowFwdArgs A) {
   using E = typename Fragment<DT>::Element;
   constexpr int DP = 32 * NK, RS = DP + Fragment<DT>::kPad, ND = DP / 16, KT = KS / 16, R = 64 * MT;
   constexpr float kUp = DT == kF16 ? 15.f - kSlack : 0.f;
@@ -305,20 +305,20 @@ extern "C" int msa_window_attn_fwd(const void* q, const void* k, const void* v, 
     A.first = first;                                                                                                    \
     hipLaunchKernelGGL((window_fwd_kernel<DT, NK, MT, 32, TWO>), dim3(count), dim3(256), 0, st, A);                     \
   })
-#define MSA_WINDOW_FWD_DIM(DT, TWO)                     \
-  {                                                     \
-    if (head_dim <= 64) MSA_WINDOW_FWD(DT, 2, 2, TWO);  \
-    if (head_dim <= 96) MSA_WINDOW_FWD(DT, 3, 2, TWO);  \
-    if (head_dim <= 128) MSA_WINDOW_FWD(DT, 4, 2, TWO); \
-    if (head_dim <= 192) MSA_WINDOW_FWD(DT, 6, 1, TWO); \
-    MSA_WINDOW_FWD(DT, 8, 1, TWO);                      \
+#define MSA_WINDOW_FWD_DIM(DT, MT, TWO)                  \
+  {                                                      \
+    if (head_dim <= 64) MSA_WINDOW_FWD(DT, 2, MT, TWO);  \
+    if (head_dim <= 96) MSA_WINDOW_FWD(DT, 3, MT, TWO);  \
+    if (head_dim <= 128) MSA_WINDOW_FWD(DT, 4, MT, TWO); \
+    if (head_dim <= 192) MSA_WINDOW_FWD(DT, 6, 1, TWO);  \
+    MSA_WINDOW_FWD(DT, 8, 1, TWO);                       \
   }
   // (out_lo is asked for where a backward pass takes the output)
-  if (dtype == kBF16 && out_lo) MSA_WINDOW_FWD_DIM(kBF16, true)
-  if (dtype == kBF16) MSA_WINDOW_FWD_DIM(kBF16, false)
-  if (dtype == kF16 && out_lo) MSA_WINDOW_FWD_DIM(kF16, true)
-  if (dtype == kF16) MSA_WINDOW_FWD_DIM(kF16, false)
-  MSA_WINDOW_FWD_DIM(kF32, false)
+  if (dtype == kBF16 && out_lo) MSA_WINDOW_FWD_DIM(kBF16, 2, true)
+  if (dtype == kBF16) MSA_WINDOW_FWD_DIM(kBF16, 2, false)
+  if (dtype == kF16 && out_lo) MSA_WINDOW_FWD_DIM(kF16, 2, true)
+  if (dtype == kF16) MSA_WINDOW_FWD_DIM(kF16, 2, false)
+  MSA_WINDOW_FWD_DIM(kF32, 1, false)
 #undef MSA_WINDOW_FWD_DIM
 #undef MSA_WINDOW_FWD
 }
