@@ -244,6 +244,26 @@ __device__ __forceinline__ float value_at(const typename Fragment<DT>::Element* 
   return load_as_f32<DT>(p, i);
 }
 
+// The dot of two rows in memory, 16 bytes at a time.
+template <int DT>
+__device__ __forceinline__ float row_dot(const typename Fragment<DT>::Element* a, const typename Fragment<DT>::Element* b, int D) {
+  float x = 0.f;
+  for (int d = 0; d < D; d += DT == kF32 ? 4 : 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(a + d), w = *reinterpret_cast<const uint4*>(b + d);
+    const uint32_t us[4] = {u.x, u.y, u.z, u.w}, ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == kF32) {
+        x = fmaf(__uint_as_float(us[i]), __uint_as_float(ws[i]), x);
+      } else {
+        x = fmaf(lo16_f32<DT>(us[i]), lo16_f32<DT>(ws[i]), x);
+        x = fmaf(hi16_f32<DT>(us[i]), hi16_f32<DT>(ws[i]), x);
+      }
+    }
+  }
+  return x;
+}
+
 // Four results, rounded once, at p (8 or 16 bytes, aligned).
 template <int DT>
 __device__ __forceinline__ void store4(typename Fragment<DT>::Element* p, f32x4 x) {

@@ -117,15 +117,12 @@ __device__ __forceinline__ void careful_dq(const WindowBwdArgs& A, int start, in
   const float lse = A.lse[row], shift = lse * -kLog2e, delta = A.delta[row];
   const int low = A.seen.low(tok);
   float o[4] = {0.f, 0.f, 0.f, 0.f};
-  bool lost = false;  // a ds of NaN: no dim is left
+  bool lost = lse != lse || delta != delta;  // a ds of NaN: no dim is left
   auto keys = [&](int from, int to) {
     for (int base = from; base < to && !lost; base += kWave) {
       const int j = min(base + lane, to - 1), count = min(kWave, to - base);
-      float x = 0.f, dp = 0.f;
-      for (int d = 0; d < A.D; ++d) {
-        x = fmaf(value_at<DT>(q, d), value_at<DT>(k + static_cast<int64_t>(j) * A.k.token, d), x);
-        dp = fmaf(value_at<DT>(dout, d), value_at<DT>(v + static_cast<int64_t>(j) * A.v.token, d), dp);
-      }
+      const float x = row_dot<DT>(q, k + static_cast<int64_t>(j) * A.k.token, A.D);
+      const float dp = row_dot<DT>(dout, v + static_cast<int64_t>(j) * A.v.token, A.D);
       const float ds = __builtin_amdgcn_exp2f(fmaf(x, A.scale_log2, shift)) * (dp - delta);
       lost = __any(ds != ds);
       for (int i = 0; i < count && !lost; ++i) {
@@ -325,46 +322,81 @@ __global__ __launch_bounds__(256, DT == kF32 && NK > 4 ? 1 : 2) void window_dq_k
 
 // ---- dK and dV
 
-// The gradients of one key, row by row, by a wave: where a value that is not finite met the products of a tile, which
-// multiply the rows that do not see a key by 0.
+// The gradients of one key that came out not finite, by a wave: where a value that is not finite met the products of a tile,
+// which multiply the rows that do not see a key by 0. A row whose log sum is NaN leaves no dim of either, one whose delta is
+// none of dK; a dim in which a row's dO is not finite is these values' sum in dV. What is left is formed again row by row.
 template <int DT>
-__device__ __forceinline__ void careful_dkv(const WindowBwdArgs& A, int start, int n, int g, int j) {
+__device__ __forceinline__ void careful_dkv(const WindowBwdArgs& A, int start, int n, int g, int j, bool need_k, bool need_v) {
   using E = typename Fragment<DT>::Element;
   const int lane = threadIdx.x & 63, ratio = A.ratio.d;
-  const int64_t t = start + static_cast<int64_t>(j);
+  const int64_t t = start + static_cast<int64_t>(j), at = (t * A.G + g) * A.D;
   const E* k = static_cast<const E*>(A.k.base) + A.k.at(t, g);
   const E* v = static_cast<const E*>(A.v.base) + A.v.at(t, g);
-  const int end = (j < A.seen.sinks || A.seen.window >= n - j ? n : j + A.seen.window) * ratio;
-  float ok[4] = {0.f, 0.f, 0.f, 0.f}, ov[4] = {0.f, 0.f, 0.f, 0.f};
-  bool lost_k = false, lost_v = false;  // a ds (a p) of NaN: no dim is left
-  for (int base = j * ratio; base < end && !(lost_k && lost_v); base += kWave) {
-    const int r = min(base + lane, end - 1), count = min(kWave, end - base);
-    const int64_t tr = start + static_cast<int64_t>(A.ratio(r));
-    const int head = g * ratio + r - A.ratio(r) * ratio;
-    const E* q = static_cast<const E*>(A.q.base) + A.q.at(tr, head);
-    const E* dout = static_cast<const E*>(A.dout.base) + A.dout.at(tr, head);
-    const float lse = A.lse[tr * (A.G * ratio) + head];
-    float x = 0.f, dp = 0.f;
-    for (int d = 0; d < A.D; ++d) {
-      x = fmaf(value_at<DT>(q, d), value_at<DT>(k, d), x);
-      dp = fmaf(value_at<DT>(dout, d), value_at<DT>(v, d), dp);
+  const int begin = j * ratio, end = (j < A.seen.sinks || A.seen.window >= n - j ? n : j + A.seen.window) * ratio;
+  need_k &= A.dk != nullptr, need_v &= A.dv != nullptr;
+  auto token_of = [&](int r) { return start + static_cast<int64_t>(A.ratio(r)); };
+  auto head_of = [&](int r) { return g * ratio + r - A.ratio(r) * ratio; };
+  auto state_of = [&](int r) { return token_of(r) * (A.G * ratio) + head_of(r); };
+  bool lost_k = false, lost_v = false;
+  for (int base = begin; base < end && !(lost_v || (lost_k && !need_v)); base += kWave) {
+    const int64_t row = state_of(min(base + lane, end - 1));
+    const float lse = A.lse[row], delta = A.delta[row];
+    lost_v |= __any(lse != lse) != 0;
+    lost_k |= __any(lse != lse || delta != delta) != 0;
+  }
+  float ok[4] = {0.f, 0.f, 0.f, 0.f}, ov[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+  bool bad[4], again = false;
+  if (need_v && !lost_v) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");  // (what this wave's other lanes stored)
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+#pragma unroll
+    for (int u = 0; u < 4; ++u) bad[u] = lane + u * kWave < A.D && !finite(load_as_f32<DT>(A.dv, at + lane + u * kWave));
+    for (int base = begin; base < end; base += kWave) {
+      bool open = false;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) open |= bad[u] && odd[u] == odd[u];
+      if (!__any(open)) break;
+      uint64_t dead = 0;  // rows of a logit of -inf, looked for when a value is infinite
+      bool known = false;
+      for (int r = base; r < min(end, base + kWave); ++r) {
+        const E* y = static_cast<const E*>(A.dout.base) + A.dout.at(token_of(r), head_of(r));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float x = bad[u] ? value_at<DT>(y, lane + u * kWave) : 0.f;
+          if (!known && __any(!finite(x) && x == x)) {
+            const int i = min(base + lane, end - 1);
+            dead = __ballot(row_dot<DT>(static_cast<const E*>(A.q.base) + A.q.at(token_of(i), head_of(i)), k, A.D) * A.scale_log2 ==
+                            -__builtin_inff());
+            known = true;
+          }
+          if (!finite(x)) odd[u] += dead >> (r - base) & 1 ? __builtin_nanf("") : x;
+        }
+      }
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) again |= bad[u] && odd[u] == 0.f;
+  }
+  const bool sum_k = need_k && !lost_k, sum_v = need_v && !lost_v && __any(again);
+  for (int base = begin; base < end && ((sum_k && !lost_k) || sum_v); base += kWave) {
+    const int r = min(base + lane, end - 1), count = min(kWave, end - base);
+    const E* q = static_cast<const E*>(A.q.base) + A.q.at(token_of(r), head_of(r));
+    const E* dout = static_cast<const E*>(A.dout.base) + A.dout.at(token_of(r), head_of(r));
+    const float lse = A.lse[state_of(r)];
+    const float x = row_dot<DT>(q, k, A.D), dp = row_dot<DT>(dout, v, A.D);
     const float p = lse == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(fmaf(x, A.scale_log2, lse * -kLog2e));
-    const float ds = p * (dp - A.delta[tr * (A.G * ratio) + head]);
+    const float ds = p * (dp - A.delta[state_of(r)]);
     lost_k |= __any(ds != ds) != 0;
-    lost_v |= __any(p != p) != 0;
     for (int i = 0; i < count; ++i) {
       const float p_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), i));
       const float ds_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ds), i));
-      const int ti = A.ratio(base + i), hi = g * ratio + base + i - ti * ratio;
-      const E* qi = static_cast<const E*>(A.q.base) + A.q.at(start + static_cast<int64_t>(ti), hi);
-      const E* gi = static_cast<const E*>(A.dout.base) + A.dout.at(start + static_cast<int64_t>(ti), hi);
+      const E* qi = static_cast<const E*>(A.q.base) + A.q.at(token_of(base + i), head_of(base + i));
+      const E* gi = static_cast<const E*>(A.dout.base) + A.dout.at(token_of(base + i), head_of(base + i));
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int d = lane + u * kWave;
         if (d >= A.D) break;
-        ok[u] = fmaf(ds_i, value_at<DT>(qi, d), ok[u]);
-        ov[u] = fmaf(p_i, value_at<DT>(gi, d), ov[u]);
+        if (sum_k && !lost_k) ok[u] = fmaf(ds_i, value_at<DT>(qi, d), ok[u]);
+        if (sum_v) ov[u] = fmaf(p_i, value_at<DT>(gi, d), ov[u]);
       }
     }
   }
@@ -372,8 +404,9 @@ __device__ __forceinline__ void careful_dkv(const WindowBwdArgs& A, int start, i
   for (int u = 0; u < 4; ++u) {
     const int d = lane + u * kWave;
     if (d >= A.D) break;
-    if (A.dk) store_from_f32<DT>(A.dk, (t * A.G + g) * A.D + d, lost_k ? __builtin_nanf("") : ok[u] * A.scale);
-    if (A.dv) store_from_f32<DT>(A.dv, (t * A.G + g) * A.D + d, lost_v ? __builtin_nanf("") : ov[u]);
+    if (need_k) store_from_f32<DT>(A.dk, at + d, lost_k ? __builtin_nanf("") : ok[u] * A.scale);
+    if (need_v && lost_v) store_from_f32<DT>(A.dv, at + d, __builtin_nanf(""));
+    else if (need_v && bad[u]) store_from_f32<DT>(A.dv, at + d, odd[u] != 0.f ? odd[u] : ov[u]);
   }
 }
 
@@ -611,21 +644,24 @@ __global__ __launch_bounds__(256, DT == kF32 && NK > 4 ? 1 : 2) void window_dkv_
             dv[kt][d] += *reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(A.sink_rows) * A.D + 16 * d);
           }
       }
-      float all = 0.f;
+      float all_k = 0.f, all_v = 0.f;
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-        all += ((dk[kt][d][0] + dk[kt][d][1]) + (dk[kt][d][2] + dk[kt][d][3])) +
-               ((dv[kt][d][0] + dv[kt][d][1]) + (dv[kt][d][2] + dv[kt][d][3]));
+      for (int d = 0; d < ND; ++d) {
+        all_k += (dk[kt][d][0] + dk[kt][d][1]) + (dk[kt][d][2] + dk[kt][d][3]);
+        all_v += (dv[kt][d][0] + dv[kt][d][1]) + (dv[kt][d][2] + dv[kt][d][3]);
+      }
 #pragma unroll
       for (int d = 0; d < ND; ++d)
         if (mine && 16 * d + 4 * q4 < A.D) {
           if (A.dk) store4<DT>(static_cast<E*>(A.dk) + row * A.D + 16 * d + 4 * q4, dk[kt][d]);
           if (A.dv) store4<DT>(static_cast<E*>(A.dv) + row * A.D + 16 * d + 4 * q4, dv[kt][d]);
         }
-      uint64_t odd = __ballot(mine && !finite(all));
-      odd |= odd >> 32, odd |= odd >> 16;
-      for (uint32_t left = odd & 0xffffu; left; left &= left - 1)
-        careful_dkv<DT>(A, at.start, at.n, g, ka + 16 * kt + __builtin_ctz(left));
+      uint64_t odd_k = __ballot(mine && !finite(all_k)), odd_v = __ballot(mine && !finite(all_v));
+      odd_k |= odd_k >> 32, odd_k |= odd_k >> 16, odd_v |= odd_v >> 32, odd_v |= odd_v >> 16;
+      for (uint32_t left = (odd_k | odd_v) & 0xffffu; left; left &= left - 1) {
+        const int i = __builtin_ctz(left);
+        careful_dkv<DT>(A, at.start, at.n, g, ka + 16 * kt + i, odd_k >> i & 1, odd_v >> i & 1);
+      }
     }
   }
 }
@@ -683,8 +719,9 @@ __global__ __launch_bounds__(256) void window_dkv_join(WindowBwdArgs A) {
     if (A.dk) store4<DT>(static_cast<E*>(A.dk) + row * A.D + d, dk);
     if (A.dv) store4<DT>(static_cast<E*>(A.dv) + row * A.D + d, dv);
   }
-  const float all = ((dk[0] + dk[1]) + (dk[2] + dk[3])) + ((dv[0] + dv[1]) + (dv[2] + dv[3]));
-  if (__any(mine && !finite(all))) careful_dkv<DT>(A, start, n, g, j);
+  const bool odd_k = __any(mine && !finite((dk[0] + dk[1]) + (dk[2] + dk[3])));
+  const bool odd_v = __any(mine && !finite((dv[0] + dv[1]) + (dv[2] + dv[3])));
+  if (odd_k || odd_v) careful_dkv<DT>(A, start, n, g, j, odd_k, odd_v);
 }
 
 // Keys of a workgroup of the dK / dV kernels.

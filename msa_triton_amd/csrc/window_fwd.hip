@@ -31,9 +31,10 @@ struct WindowFwdArgs {
   float* lse;        // [T][Hq], or null
 };
 
-// The row of a token and head, key by key, by a wave: where a value that is not finite met the products of a tile,
-// which multiply the keys that a row does not see by 0. Such values count whatever their weight above 0; a weight of 0 under
-// a logit of -inf makes NaN of them. x2 = logit * log2(e); the weight is exp2(x2 + shift).
+// The dims of a row that came out not finite, by a wave: where a value that is not finite met the products of a tile, which
+// multiply the keys that a row does not see by 0. Such values count whatever their weight above 0; a weight of 0 under
+// a logit of -inf makes NaN of them. Dims in which the row sees one are these values' sum, which takes a look at their
+// column; the others are formed again key by key. The weight is exp2(logit * log2(e) + shift).
 template <int DT>
 __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, int g, int tok, int head, float shift,
                                             float inv) {
@@ -42,40 +43,69 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
   const E* q = static_cast<const E*>(A.q.base) + A.q.at(start + static_cast<int64_t>(tok), head);
   const E* k = static_cast<const E*>(A.k.base) + A.k.at(start, g);
   const E* v = static_cast<const E*>(A.v.base) + A.v.at(start, g);
-  const int low = A.seen.low(tok);
+  const int low = A.seen.low(tok), sinks = min(A.seen.sinks, low);
+  const int64_t at = ((start + static_cast<int64_t>(tok)) * (A.G * A.ratio) + head) * A.D;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");  // (what this wave's other lanes stored)
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   float o[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+  bool bad[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) bad[u] = lane + u * kWave < A.D && !finite(load_as_f32<DT>(A.out, at + lane + u * kWave));
+  auto open = [&]() {  // dims whose value may still change
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) any |= bad[u] && odd[u] == odd[u];
+    return __any(any);
+  };
+  auto column = [&](int from, int to) {
+    for (int base = from; base < to && open(); base += kWave) {
+      uint64_t dead = 0;  // keys of a logit of -inf, looked for when a value is infinite
+      bool known = false;
+      for (int j = base; j < min(to, base + kWave); ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float y = bad[u] ? value_at<DT>(v + static_cast<int64_t>(j) * A.v.token, lane + u * kWave) : 0.f;
+          if (!known && __any(!finite(y) && y == y)) {
+            dead = __ballot(row_dot<DT>(q, k + static_cast<int64_t>(min(base + lane, to - 1)) * A.k.token, A.D) * A.scale_log2 ==
+                            -__builtin_inff());
+            known = true;
+          }
+          if (!finite(y)) odd[u] += dead >> (j - base) & 1 ? __builtin_nanf("") : y;
+        }
+    }
+  };
+  column(0, sinks);
+  column(low, tok + 1);
+  bool again = false;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) again |= bad[u] && odd[u] == 0.f;
   auto keys = [&](int from, int to) {
     for (int base = from; base < to; base += kWave) {
       const int j = min(base + lane, to - 1), count = min(kWave, to - base);
-      float x = 0.f;
-      for (int d = 0; d < A.D; ++d) x = fmaf(value_at<DT>(q, d), value_at<DT>(k + static_cast<int64_t>(j) * A.k.token, d), x);
-      x *= A.scale_log2;
+      const float x = row_dot<DT>(q, k + static_cast<int64_t>(j) * A.k.token, A.D) * A.scale_log2;
       const float p = __builtin_amdgcn_exp2f(x + shift);
       for (int i = 0; i < count; ++i) {
         const float p_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), i));
-        const float x_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i));
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int d = lane + u * kWave;
-          if (d >= A.D) break;
-          const float y = value_at<DT>(v + static_cast<int64_t>(base + i) * A.v.token, d);
-          if (finite(y)) o[u] = fmaf(p_i, y, o[u]);
-          else odd[u] += x_i == -__builtin_inff() ? __builtin_nanf("") : y;
-        }
+        for (int u = 0; u < 4; ++u)
+          if (bad[u] && odd[u] == 0.f) o[u] = fmaf(p_i, value_at<DT>(v + static_cast<int64_t>(base + i) * A.v.token, lane + u * kWave), o[u]);
       }
     }
   };
-  keys(0, min(A.seen.sinks, low));
-  keys(low, tok + 1);
-  const int64_t at = ((start + static_cast<int64_t>(tok)) * (A.G * A.ratio) + head) * A.D;
+  if (__any(again)) {
+    keys(0, sinks);
+    keys(low, tok + 1);
+  }
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
+    if (!bad[u]) continue;
     const int d = lane + u * kWave;
-    if (d >= A.D) break;
     const float y = odd[u] != 0.f ? odd[u] : o[u] * inv;
     store_from_f32<DT>(A.out, at + d, y);
     if (DT != kF32 && A.out_lo) {
-      const float lo = y - load_as_f32<DT>(A.out, at + d);
+      uint16_t high;
+      store_from_f32<DT>(&high, 0, y);
+      const float lo = y - load_as_f32<DT>(&high, 0);
       store_from_f32<DT>(A.out_lo, at + d, lo == lo ? lo : 0.f);
     }
   }
@@ -260,6 +290,18 @@ __global__ __launch_bounds__(256, NK > 4 ? (DT == kF32 ? 1 : 2) : DT == kF32 ? 2
       A.lse[at_row] = l[m] == 0.f ? -__builtin_inff() : (level - kUp + __log2f(l[m])) * kLn2Window;
     // (a sum of NaN makes the row NaN)
     uint64_t odd = __ballot(mine && !finite(all) && l[m] == l[m]);
+    if constexpr (DT != kF32)
+      if (odd && A.out_lo) {  // (the two terms above come from pairs of values: one that is not finite spoils its neighbour's)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = acc[m][d][i] * inv;
+            uint16_t high;
+            store_from_f32<DT>(&high, 0, x);
+            if (mine && 16 * d + 4 * q4 < A.D) store_from_f32<DT>(lo, 16 * d + 4 * q4 + i, x - load_as_f32<DT>(&high, 0));
+          }
+      }
     odd |= odd >> 32, odd |= odd >> 16;
     for (uint32_t left = odd & 0xffffu; left; left &= left - 1) {
       const int from = __builtin_ctz(left);

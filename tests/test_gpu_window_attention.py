@@ -439,3 +439,48 @@ def test_calls_of_more_than_2_to_the_23_workgroups():
     assert torch.equal(out, v) and torch.equal(dv, do)
     most = 2 * 16 * U * (do.double().abs() * v.double().abs()).sum(2, keepdim=True) * (1 + 2.0 ** -7)
     assert (dq.double().abs() <= most * k.double().abs()).all() and (dk.double().abs() <= most * q.double().abs()).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 72)])
+def test_several_values_that_are_not_finite(dtype, d):
+    """Infinities that meet, beside NaN, under a logit of -inf, and in more than one dim: NaN, +inf and -inf stand where the
+    formula over the visible tokens has them, and the rest is within the bound."""
+    n, window, sinks, scale = 150, 20, 2, d ** -0.5
+    q, k, v, do = inputs([n], 2, 1, d, dtype)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    res, off = reference(q, k, v, [n], window, sinks, scale, do)
+    inf = float("inf")
+    x = [y.clone() for y in (q, k, v, do)]
+    x[2][60, 0, 5], x[2][62, 0, 5], x[2][64, 0, 6], x[2][64, 0, 7] = inf, -inf, float("nan"), inf
+    x[2][100, 0, 9], x[1][100, 0, 0] = inf, -inf  # a weight of 0 under an infinity
+    out = run(*x[:3], [n], None, window, sinks)[0]
+    for i in range(n):
+        seen = [j for j in range(i + 1) if i - j < window or j < sinks]
+        for h in range(2):
+            p = torch.softmax(x[0][i, h].double() @ x[1][seen, 0].double().T * scale, -1)
+            want = (p[:, None] * x[2][seen, 0].double()).sum(0)
+            for name in (torch.isnan, torch.isposinf, torch.isneginf):
+                assert torch.equal(name(out[i, h]), name(want)), (i, h, name)
+    far = torch.ones(n, dtype=torch.bool, device="cuda")
+    far[60:120] = False
+    check(out[far], res["out"][far], off["out"][far], "out")
+    x = [y.clone() for y in (q, k, v, do)]
+    x[3][60, 0, 5], x[3][62, 0, 5], x[3][64, 1, 6], x[3][64, 1, 7] = inf, -inf, float("nan"), inf
+    _, _, dq, dk, dv = run(*x[:3], [n], x[3], window, sinks)
+    lse = res["lse"]
+    for j in range(n):
+        rows = [i for i in range(j, n) if i - j < window or j < sinks]
+        p = torch.exp(x[0][rows].double() @ x[1][j, 0].double() * scale - lse[rows])
+        want = (p[..., None] * x[3][rows].double()).sum((0, 1))
+        for name in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(name(dv[j, 0]), name(want)), (j, name)
+        clean = torch.isfinite(want)
+        check(dv[j, 0][clean], res["dv"][j, 0][clean], off["dv"][j, 0][clean], ("dv", j))
+    other = [i for i in range(n) if i not in (60, 62, 64)]
+    check(dq[other], res["dq"][other], off["dq"][other], "dq")
+    x = [y.clone() for y in (q, k, v, do)]
+    x[2].fill_(float("nan"))
+    out, lse, dq, dk, dv = run(*x[:3], [n], x[3], window, sinks)
+    assert all(torch.isnan(y).all() for y in (out, dq, dk))
+    check(lse, res["lse"], off["lse"], "lse")
+    check(dv, res["dv"], off["dv"], "dv")
