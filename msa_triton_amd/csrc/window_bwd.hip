@@ -16,7 +16,7 @@
 // from LDS, the logits of 16 rows after those of the other 16, and 256 registers.
 //
 // Logits, p, ds and all sums are fp32. p enters its product rounded once to the input type; a ds enters as two terms (2^-17 of
-// it left out): one would be of the size of the gradients' own rounding and bring dq and dk from 0.0018 to 0.0024 of
+// it left out): one would be of the size of the gradients' own rounding and bring dq and dk from 0.0017 to 0.0024 of
 // themselves (dQ 3.0 ms, dK and dV 6.1). fp16 has neither range nor small values for a ds: its products take ds times a
 // power of two, one a row (dQ) or key (dK) that follows the largest so far, and p times 2^15. delta takes the output with
 // what its rounding left out.
@@ -24,8 +24,6 @@
 
 namespace msa {
 namespace {
-
-constexpr int kChunk = 256;  // tokens of a chunk of the rows that see first tokens from behind the window
 
 struct WindowBwdArgs {
   PackedView q, k, v, dout;

@@ -11,12 +11,13 @@
 // one of 60): a workgroup takes a stretch of them, its four waves every fourth step of a tile each on their own, as in
 // the block-sparse form: key fragments straight from memory, S^T = K Q^T, weights as they come out of it, values through
 // the wave's LDS tile. A tile that lies in one stretch is finished there; the parts of the others, maxima, sums and fp32
-// outputs, are joined by a second launch in a fixed order.
+// outputs, are joined by a second launch in a fixed order. 64 requests of 60 to 30 000 tokens, 4 key heads of 128, 16 bits, no
+// window: 131 + 10 us, 4.8 TB/s; 512, 300 and 1 new tokens behind 8192, 1000 and 5000, window 2048, 32 heads: 61 + 16 us.
 //
 // Logits, statistics and outputs are fp32. With one tile of 16 rows, where the products are not the bound, a weight
 // enters the second product as two 16-bit terms (2^-17 of it left out); with more it is rounded once, as in the packed
-// form (fp16 queries over an 8-bit cache, whose products are bf16's, take two terms). In fp16 both are of the weight times 2^7. Bytes of an 8-bit page are exact in bf16; its scales go into logits
-// and weights.
+// form (fp16 queries over an 8-bit cache, whose products are bf16's, take two terms). In fp16 both are of the weight times
+// 2^7. Bytes of an 8-bit page are exact in bf16; its scales go into logits and weights.
 #include "window.hpp"
 
 namespace msa {
