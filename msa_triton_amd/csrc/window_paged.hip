@@ -122,9 +122,10 @@ __device__ __forceinline__ int64_t quotient(int64_t a, uint32_t b) {
 // The parent of node i among its sequence's new tokens, or -1: anything that is not in front of it is none.
 __device__ __forceinline__ int parent_of(int p, int i) { return p >= 0 && p < i ? p : -1; }
 
-// One row, key by key, by a wave: where a value that is not finite met the products of a tile, which multiply the keys that
-// a row does not see by 0. Such values count whatever their weight above 0; a weight of 0 under a logit of -inf
-// makes NaN of them. The weight is exp2(logit * log2(e) - top).
+// The dims of a row that came out not finite, by a wave: where a value that is not finite met the products of a tile, which
+// multiply the keys that a row does not see by 0. Such values count whatever their weight above 0; a weight of 0 under
+// a logit of -inf makes NaN of them. Dims in which the row sees one are these values' sum, which takes a look at their
+// column; the others are formed again key by key. The weight is exp2(logit * log2(e) - top).
 template <int DT, bool FP8>
 __device__ __forceinline__ void careful_row(const PagedWindowArgs& A, int s, int start, int context, int tok, int g, int head,
                                             float top, float inv) {
@@ -141,67 +142,85 @@ __device__ __forceinline__ void careful_row(const PagedWindowArgs& A, int s, int
     for (int i = parent_of(parents[tok], tok); i >= 0; i = parent_of(parents[i], i)) ++pos;
   }
   const int64_t hi = min(context + static_cast<int64_t>(tok), A.pages.last_position()), low = max(int64_t{0}, pos - A.seen.window + 1);
+  const int d = 4 * lane;  // (at most 256 dims)
   float o[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+  bool bad[4] = {false, false, false, false}, look = true;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");  // (what this wave's other lanes stored)
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  if (d < A.D) {
+    float y[4];
+    load4<DT, false>(reinterpret_cast<const char*>(A.out + row * A.D + d), y);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) bad[u] = !finite(y[u]);
+  }
+  auto wanted = [&](int u) { return bad[u] && (look ? odd[u] == odd[u] : odd[u] == 0.f); };
   auto keys = [&](int64_t from, int64_t to) {  // both below 2^31; cached tokens and new ones never in one go
     for (int64_t base = from; base < to; base += kWave) {
+      const bool mine = wanted(0) || wanted(1) || wanted(2) || wanted(3);
+      if (!__any(mine)) return;
       const int64_t j = min(base + lane, to - 1);
       bool seen = base + lane < to;
       if (parents && base >= context) {  // new tokens on the way up
-        const int mine = static_cast<int>(j - context);
+        const int own = static_cast<int>(j - context);
         bool on_path = false;
         int64_t place = pos;
         for (int i = tok; i >= 0; i = parent_of(parents[i], i), --place)
-          on_path |= i == mine && (pos - place < A.seen.window || place < A.seen.sinks);
+          on_path |= i == own && (pos - place < A.seen.window || place < A.seen.sinks);
         seen &= on_path;
       }
       const int page = A.pages.page_of(s, j);
       seen &= page >= 0;
-      const int64_t p0 = page < 0 ? 0 : page, slot = j & slot_mask;
-      const char* kp = kbase + (p0 * A.k.stride_page + slot * A.k.stride_slot) * ES;
-      float x = 0.f;
-      for (int d = 0; d < A.D; d += 4) {
-        float y[4], z[4];
-        load4<DT, false>(reinterpret_cast<const char*>(q + d), y);
-        load4<DT, FP8>(kp + d * ES, z);
+      auto logit = [&]() {
+        const int64_t p0 = page < 0 ? 0 : page;
+        const char* kp = kbase + (p0 * A.k.stride_page + (j & slot_mask) * A.k.stride_slot) * ES;
+        float x = 0.f;
+        for (int e = 0; e < A.D; e += 4) {
+          float y[4], z[4];
+          load4<DT, false>(reinterpret_cast<const char*>(q + e), y);
+          load4<DT, FP8>(kp + e * ES, z);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x = fmaf(y[i], z[i], x);
-      }
-      x *= A.scale_log2 * (FP8 ? A.k_scale[p0 * A.G + g] : 1.f);
-      const float p = __builtin_amdgcn_exp2f(x - top);
-      uint64_t left = __ballot(seen);
-      for (; left; left &= left - 1) {
+          for (int i = 0; i < 4; ++i) x = fmaf(y[i], z[i], x);
+        }
+        return x * (A.scale_log2 * (FP8 ? A.k_scale[p0 * A.G + g] : 1.f));
+      };
+      const float p = look ? 0.f : __builtin_amdgcn_exp2f(logit() - top);
+      uint64_t dead = 0;  // keys of a logit of -inf, looked for when a value is infinite
+      bool known = false;
+      for (uint64_t left = __ballot(seen); left; left &= left - 1) {
         const int i = __builtin_ctzll(left);
         const float p_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), i));
-        const float x_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i));
         const int64_t page_i = __builtin_amdgcn_readlane(page, i);
         const char* vp = vbase + (page_i * A.v.stride_page + ((base + i) & slot_mask) * A.v.stride_slot) * ES;
         const float vs = FP8 ? A.v_scale[page_i * A.G + g] : 1.f;
-        const int d = 4 * lane;  // (at most 256 dims)
-        if (d < A.D) {
-          float y[4];
-          load4<DT, FP8>(vp + d * ES, y);
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+        if (mine) load4<DT, FP8>(vp + d * ES, y);
+        if (look) {
+          bool infinite = false;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            y[u] *= vs;
-            if (finite(y[u])) o[u] = fmaf(p_i, y[u], o[u]);
-            else odd[u] += x_i == -__builtin_inff() ? __builtin_nanf("") : y[u];
-          }
+          for (int u = 0; u < 4; ++u) y[u] = bad[u] ? y[u] * vs : 0.f, infinite |= !finite(y[u]) && y[u] == y[u];
+          if (!known && __any(infinite)) dead = __ballot(logit() == -__builtin_inff()), known = true;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (!finite(y[u])) odd[u] += dead >> i & 1 ? __builtin_nanf("") : y[u];
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (wanted(u)) o[u] = fmaf(p_i, y[u] * vs, o[u]);
         }
       }
     }
   };
   if (context >= 0 && A.pages.num_pages > 0) {
     const int64_t cached = parents ? min(static_cast<int64_t>(context), hi + 1) : hi + 1;
-    keys(0, min(static_cast<int64_t>(A.seen.sinks), min(low, cached)));
-    keys(min(low, cached), cached);
-    if (parents) keys(context, hi + 1);
+    for (int pass = 0; pass < 2; ++pass, look = false) {
+      keys(0, min(static_cast<int64_t>(A.seen.sinks), min(low, cached)));
+      keys(min(low, cached), cached);
+      if (parents) keys(context, hi + 1);
+    }
   }
-  const int d = 4 * lane;
-  if (d >= A.D) return;
-  f32x4 y;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) y[u] = odd[u] != 0.f ? odd[u] : o[u] * inv;
-  store4<DT>(A.out + row * A.D + d, y);
+  for (int u = 0; u < 4; ++u)
+    if (bad[u]) store_from_f32<DT>(A.out, row * A.D + d + u, odd[u] != 0.f ? odd[u] : o[u] * inv);
 }
 
 // Which keys a row sees: `low` the first of its window, `slot` its own.
