@@ -316,6 +316,47 @@ def test_a_value_under_a_weight_of_zero():
         assert (out[:, :, 9] == float("inf")).all() and torch.isfinite(out[:, :, :9]).all() and torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float16, 256)])
+@pytest.mark.parametrize("n", [3, 24])
+@pytest.mark.parametrize("drafted", [False, True])
+def test_several_values_that_are_not_finite(dtype, dim, n, drafted):
+    """Infinities that meet, beside NaN, among cached tokens, under a logit of -inf and among a tree's nodes: NaN, +inf and
+    -inf stand where the formula over the visible tokens has them, and the other dims are within the bound."""
+    page, context, window, inf = 16, 200, 150, float("inf")
+    x = setup([n], [context], 1, 4, dim, page, dtype, False)
+    x["q"][:, :, 0] = x["q"][:, :, 0].abs() + 0.5
+    x["parents"] = tree([n]) if drafted else None
+
+    def put(cache, at, d, value):
+        cache[x["table"][0, at // page].item(), 0, at % page, d] = value
+
+    x["kc"], x["vc"] = x["kc"].clone(), x["vc"].clone()
+    for at, d, value in ((120, 5, inf), (130, 5, -inf), (140, 6, float("nan")), (140, 7, inf), (141, 7, inf), (0, 8, -inf), (20, 10, inf),
+                         (60, 11, inf), (context + 1, 12, inf), (context + 2, 12, -inf), (context + n - 1, 13, -inf)):
+        put(x["vc"], at, d, value)
+    put(x["kc"], 150, 0, -inf)
+    put(x["vc"], 150, 9, inf)
+    out, lse = call(x, window, 2)
+    # (the bound's terms: of the cache with zeros for what is not finite, a logit of 0 in place of -inf)
+    _, _, tol, _ = oracle(dict(x, kc=x["kc"].nan_to_num(0.0, 0.0, 0.0), vc=x["vc"].nan_to_num(0.0, 0.0, 0.0)), [n], [context], window, 2,
+                          dim ** -0.5)
+    own = None if x["parents"] is None else x["parents"].tolist()
+    rows = x["q"].double()
+    ids = x["table"][0].long()
+    j = torch.arange(context + n, device="cuda")
+    k, v = (x[c][ids[j // page], 0, j % page].double() for c in ("kc", "vc"))
+    for i, path in enumerate(paths(own, n)):
+        low = context + len(path) - window
+        seen = [t for t in range(context) if t >= low or t < 2] + [context + node for node in path]
+        for h in range(4):
+            p = torch.softmax(k[seen] @ rows[i, h] * dim ** -0.5, 0)
+            z = (p[:, None] * v[seen]).sum(0)
+            for name in (torch.isnan, torch.isposinf, torch.isneginf):
+                assert torch.equal(name(out[i, h]), name(z)), (i, h, name)
+            clean = torch.isfinite(z)
+            assert ((out[i, h].double() - z).abs() <= tol[i, h])[clean].all()
+
+
 def test_keys_and_queries_that_are_not_finite():
     lengths, context = [30, 2], [100, 50]
     x = setup(lengths, context, 1, 4, 64, 16, torch.float16, False)
