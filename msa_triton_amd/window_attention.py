@@ -186,8 +186,9 @@ def m3_window_attention(
     first ``sink_tokens`` keys. Each contiguous group of ``Hq / G`` query heads shares a key head. Rows must be
     contiguous and 16-byte aligned to be read in place (slices of a fused projection are); others are copied. The
     optional natural-log LSE is FP32 and non-differentiable. What is not finite reaches the rows that see it and
-    no others: a value that is an infinity makes its dim one whatever the weight (NaN where both signs meet). Head dims are
-    multiples of 8 up to 256."""
+    no others: a value that is an infinity makes its dim one whatever the weight (NaN where both signs meet). A row whose
+    logits are all -inf has an output of 0 and an LSE of -inf, as in ``m3_sparse_attention``. Head dims are multiples of 8 up to
+    256."""
     cu, num_seqs, longest, window, sinks, effective_scale = _validate(q, k, v, cu_seqlens, max_seqlen, window_size,
                                                                       sink_tokens, scale)
     if wanted(q, k, v):

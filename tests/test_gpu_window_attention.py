@@ -484,3 +484,16 @@ def test_several_values_that_are_not_finite(dtype, d):
     assert all(torch.isnan(y).all() for y in (out, dq, dk))
     check(lse, res["lse"], off["lse"], "lse")
     check(dv, res["dv"], off["dv"], "dv")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_row_whose_logits_are_all_minus_infinity(dtype):
+    q, k, v, do = inputs([70], 2, 1, 64, dtype)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    k[0, 0, 0] = float("-inf")  # the first token's only key; the others' weight of 0
+    out, lse, dq, dk, dv = run(q, k, v, [70], do, window=8, sinks=0)
+    assert not out[0].any() and (lse[0] == float("-inf")).all()
+    assert torch.isfinite(out).all() and torch.isfinite(lse[1:]).all() and torch.isfinite(dk).all() and torch.isfinite(dv).all()
+    assert not dk[0].any() and not dv[0].any() and torch.isfinite(dq[8:]).all()
+    other, _ = run(q, k, v, [70], None, window=8, sinks=0)
+    assert not other[0].any()
