@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256, DT == kF32 && NK > 4 ? 1 : 2) void window_dkv_
   if constexpr (kValuesInLds) {
     TileLoad<DT, DP, BK> load;
     load.load(A.D, [&](int r) {
-      return static_cast<const E*>(A.v.base) + (at.start + static_cast<int64_t>(min(j0 + r, at.n - 1))) * A.v.token + g * A.v.head;
+      return static_cast<const E*>(A.v.base) + A.v.at(at.start + static_cast<int64_t>(min(j0 + r, at.n - 1)), g);
     });
     load.store(values, RS, A.D);
   }

@@ -141,8 +141,8 @@ __global__ __launch_bounds__(256, NK > 4 ? (DT == kF32 ? 1 : 2) : DT == kF32 ? 2
   for (int m = 0; m < MT; ++m) {
     const int r = min(16 * (MT * wave + m) + c, live - 1);
     tok[m] = token_of(r);
-    const E* row = static_cast<const E*>(A.q.base) + (at.start + static_cast<int64_t>(tok[m])) * A.q.token +
-                   (g * A.ratio + (off + r) % A.ratio) * A.q.head;
+    const E* row = static_cast<const E*>(A.q.base) +
+                   A.q.at(at.start + static_cast<int64_t>(tok[m]), g * A.ratio + (off + r) % A.ratio);
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk)
       qf[m][kk] = 32 * kk + 8 * q4 < A.D && A.scale_log2 != 0.f
