@@ -130,6 +130,7 @@ template <int DT, bool FP8>
 __device__ __forceinline__ void careful_row(const PagedWindowArgs& A, int s, int start, int context, int tok, int g, int head,
                                             float top, float inv) {
   constexpr int ES = FP8 ? 1 : 2;
+  if (top == -__builtin_inff()) top = 0.f;  // (all logits -inf: weights 0)
   const int lane = threadIdx.x & 63, slot_mask = (1 << A.pages.shift) - 1;
   const int64_t row = (start + static_cast<int64_t>(tok)) * (A.G * A.ratio.d) + head;
   const uint16_t* q = A.q + row * A.D;
