@@ -112,7 +112,8 @@ __device__ __forceinline__ void careful_dq(const WindowBwdArgs& A, int start, in
   const E* dout = static_cast<const E*>(A.dout.base) + A.dout.at(t, head);
   const E* k = static_cast<const E*>(A.k.base) + A.k.at(start, g);
   const E* v = static_cast<const E*>(A.v.base) + A.v.at(start, g);
-  const float lse = A.lse[row], shift = lse * -kLog2e, delta = A.delta[row];
+  const float lse = A.lse[row], delta = A.delta[row];
+  const float shift = lse == -__builtin_inff() ? lse : lse * -kLog2e;  // (all logits -inf: no weights)
   const int low = A.seen.low(tok);
   float o[4] = {0.f, 0.f, 0.f, 0.f};
   bool lost = lse != lse || delta != delta;  // a ds of NaN: no dim is left

@@ -1,6 +1,6 @@
-"""Rows whose visible logits are all -inf, beside values that are not finite and that these rows do not see.
+"""Rows whose visible logits are all -inf, beside values and keys that are not finite and that these rows do not see.
 
-Such a row has an output of 0 and a log sum of -inf, whatever the rest of its tile holds.
+Such a row has an output of 0 and a log sum of -inf, weights of 0 and so a dq of 0, whatever the rest of its tile holds.
 """
 
 from __future__ import annotations
@@ -8,11 +8,13 @@ from __future__ import annotations
 import pytest
 import torch
 
+from tests.test_gpu_window_attention import inputs, run
 from tests.test_gpu_window_paged import call, oracle, setup
 
 pytestmark = pytest.mark.gpu
 
 INF = float("inf")
+
 
 PAGED = [  # new tokens, cached tokens, ratio, dim
     (3, 40, 4, 64),       # 16 rows a tile
@@ -57,3 +59,23 @@ def test_over_a_paged_cache(new, context, ratio, dim, dtype, fp8, drafted):
         assert ((out.double() - want).abs() <= tol)[other].all()
         hit = out[sees, :, 3]
         assert torch.isnan(hit).all() if fp8 or value != value else (hit == INF).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(8, 0), (None, 0), (5, 3)])
+def test_gradients_of_queries(dtype, dim, window, sinks):
+    """The key that is not finite is later than the row, or in front of its window."""
+    n, row = 70, 20
+    q, k, v, do = inputs([n], 2, 1, dim, dtype)
+    k[..., 0] = k[..., 0].abs() + 0.5
+    q[row, 1, 0] = -INF
+    want = run(q, k, v, [n], do, window, sinks)
+    assert not want[0][row, 1].any() and (want[1][row, 1] == -INF) and not want[2][row, 1].any()
+    for at in (row + 5, n - 1, *([row - 9] if window else [])):
+        for value in (INF, float("nan")):
+            y = k.clone()
+            y[at, 0, 3] = value
+            out, lse, dq, _, _ = run(q, y, v, [n], do, window, sinks)
+            assert not out[row, 1].any() and lse[row, 1] == -INF
+            assert not dq[row, 1].any(), (at, value, dq[row, 1])
