@@ -76,6 +76,8 @@ __device__ __forceinline__ float quarters_max(float x) {
 // A running maximum is only raised when a row passes it by this much (log2): weights stay below 2^kSlack, sums and outputs are
 // rescaled in few steps. In fp16 weights are held times 2^(15 - kSlack), so that the largest is at most 2^15.
 constexpr float kSlack = 8.f;
+// The same of raw dots, which are times `factor` in log2; finite, so that a first key raises a maximum of -inf.
+__device__ __forceinline__ float raw_slack(float factor) { return fminf(kSlack / factor, 3.402823466e38f); }
 
 // A fragment, times -1 where `turn` says so.
 template <int DT, class F>

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256, NK > 4 ? (DT == kF32 ? 1 : 2) : DT == kF32 ? 2
   };
 
   // A maximum is kept of the raw dots (queries are turned where the scale is negative, and zero with a factor of 1 where it is 0).
-  const float factor = A.scale_log2 == 0.f ? 1.f : fabsf(A.scale_log2), slack = kSlack / factor;
+  const float factor = A.scale_log2 == 0.f ? 1.f : fabsf(A.scale_log2), slack = raw_slack(factor);
   float top[MT], l[MT];
   f32x4 acc[MT][ND];
 #pragma unroll
