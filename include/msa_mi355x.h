@@ -325,8 +325,8 @@ int msa_attn_paged(const void* q, const void* k_cache, const void* v_cache, int3
  * attention alone). q [T,Hq,D], k and v [T,G,D], fp32, fp16 or bf16; token i of a sequence sees the keys j <= i with
  * i - j < window (0: all) or j < sinks. out [T,Hq,D] in `dtype`, out_lo (NULL: not wanted; fp32: unread) what its
  * rounding left out, rounded to `dtype` as well; lse [T,Hq] (NULL: none) natural log. strides (host array, elements):
- * q token, head; k token, head; v token, head; unit stride along D, rows 16-byte aligned, 33 token strides and Hq / G head
- * strides together below 2^30, a token stride below 2^25. head_dim: a multiple of 8 up
+ * q token, head; k token, head; v token, head; unit stride along D, rows 16-byte aligned. A token stride is below 2^25, a head
+ * stride below 2^30, 33 token strides (of q: and Hq / G head strides with them) are below 2^30. head_dim: a multiple of 8 up
  * to 256; T * Hq / G below 0x7fff0000 (status 2 otherwise). One launch. */
 int msa_window_attn_fwd(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
                         const int32_t* cu_seqlens, int64_t num_seqs, int64_t total_tokens, int64_t q_heads,
@@ -339,7 +339,7 @@ int64_t msa_window_attn_bwd_workspace_bytes(int32_t dtype, int64_t total_tokens,
                                             int64_t sinks);
 
 /* Gradients of msa_window_attn_fwd from its out, out_lo (NULL: taken as 0) and lse; grad_out in `dtype`.
- * strides: the forward's six, then grad_out token, head. grad_q [T,Hq,D], grad_k and grad_v [T,G,D] in `dtype`,
+ * strides: the forward's six, then grad_out token, head (within q's limits). grad_q [T,Hq,D], grad_k and grad_v [T,G,D] in `dtype`,
  * contiguous; NULL: not wanted. Deterministic (sums in fixed orders). Limits as in the forward. */
 int msa_window_attn_bwd(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
                         const int32_t* cu_seqlens, int64_t num_seqs, int64_t longest, int64_t total_tokens,

@@ -10,8 +10,9 @@
 
 namespace msa {
 
-// A packed tensor [T, heads, D] with free strides over tokens and heads, so small that 33 tokens and the heads of a key head lie
-// within 2^30 elements: a tile's rows are at 32-bit offsets from an address that the whole wave shares.
+// A packed tensor [T, heads, D] with free strides over tokens and heads. A tile's rows are at 32-bit offsets from an address
+// that the whole wave shares, so 33 tokens lie within 2^30 elements, of queries and their gradients with the heads of a key head
+// (near_rows); from one key head to the next, offsets are 64 bits.
 struct PackedView {
   const void* base;
   int token, head;  // elements
@@ -292,9 +293,10 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_in
 
 constexpr float kLn2Window = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
 
-inline bool near_rows(const int64_t* strides, int64_t ratio) {
+// heads: those of a tile's rows (0: all rows are of one).
+inline bool near_rows(const int64_t* strides, int64_t heads) {
   return strides[0] >= 0 && strides[1] >= 0 && strides[0] < (1 << 25) && strides[1] < (1 << 30) &&
-         33 * strides[0] + ratio * strides[1] < (1 << 30);
+         33 * strides[0] + heads * strides[1] < (1 << 30);
 }
 
 // What the packed entry points check. strides: token and head strides of q, k, v (elements).
@@ -309,7 +311,7 @@ inline bool valid_window_call(const void* q, const void* k, const void* v, int32
   for (int i = 0; i < 6; ++i)
     if (strides[i] % unit) return false;
   for (int i = 0; i < 6; i += 2)
-    if (!near_rows(strides + i, q_heads / groups)) return false;
+    if (!near_rows(strides + i, i == 0 ? q_heads / groups : 0)) return false;
   return reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 &&
          reinterpret_cast<uintptr_t>(v) % 16 == 0;
 }

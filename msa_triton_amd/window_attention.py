@@ -36,9 +36,9 @@ def check_window(window_size, sink_tokens):
     return 0 if window_size is None or window_size >= most else window_size, min(sink_tokens, most)
 
 
-def aligned_rows(x):
-    """A rank-3 tensor whose rows are contiguous, 16-byte aligned and near each other (33 tokens of all heads within 2^30
-    elements, as the kernels address them), and its token and head strides."""
+def aligned_rows(x, near_heads=0):
+    """A rank-3 tensor whose rows are contiguous, 16-byte aligned and near each other, as the kernels address them, and its token
+    and head strides: 33 tokens within 2^30 elements, with ``near_heads`` heads where a tile's rows are of so many."""
     of_token, of_head, of_dim = x.stride()
     tokens, heads, dim = x.shape
     if tokens == 1:  # (a stride that nothing steps over may be anything)
@@ -47,7 +47,7 @@ def aligned_rows(x):
         of_head = 0
     unit = 16 // x.element_size()
     if ((of_dim == 1 or dim == 1) and of_token % unit == 0 and of_head % unit == 0 and x.data_ptr() % 16 == 0
-            and 33 * of_token + heads * of_head < 1 << 30 and of_token < 1 << 25):
+            and of_token < 1 << 25 and of_head < 1 << 30 and 33 * of_token + near_heads * of_head < 1 << 30):
         return x, of_token, of_head
     x = x.contiguous()
     if x.data_ptr() % 16:
@@ -66,7 +66,7 @@ def _forward(q, k, v, cu, num_seqs, window, sinks, scale, need_lse, need_grad):
     lse = torch.empty((total, heads), dtype=torch.float32, device=q.device) if need_lse or need_grad else None
     lo = torch.empty_like(out) if need_grad and q.dtype != torch.float32 else None
     if total:
-        q, *of_q = aligned_rows(q)
+        q, *of_q = aligned_rows(q, heads // groups)
         k, *of_k = aligned_rows(k)
         v, *of_v = aligned_rows(v)
         with _lib.on_device(q.device):
@@ -87,10 +87,10 @@ def _backward(q, k, v, cu, num_seqs, longest, window, sinks, scale, out, lo, lse
     dv = torch.empty(v.shape, dtype=q.dtype, device=device) if need_v else None
     if total and (need_q or need_k or need_v):
         lib = _lib.lib()
-        q, *of_q = aligned_rows(q)
+        q, *of_q = aligned_rows(q, heads // groups)
         k, *of_k = aligned_rows(k)
         v, *of_v = aligned_rows(v)
-        grad, *of_grad = aligned_rows(grad)
+        grad, *of_grad = aligned_rows(grad, heads // groups)
         out = out.contiguous()
         lse = lse.contiguous()
         lo = lo if lo is None else lo.contiguous()

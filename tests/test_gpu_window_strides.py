@@ -7,8 +7,9 @@ import struct
 import pytest
 import torch
 
+import msa_triton_amd as msa
 from msa_triton_amd import _lib
-from msa_triton_amd.window_attention import _backward, _forward
+from msa_triton_amd.window_attention import _backward, _forward, aligned_rows
 from tests.helpers import cu_tensor
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +58,28 @@ def test_heads_more_than_2_to_the_31_values_apart(q_heads, groups):
                                      *(x.data_ptr() for x in grads), workspace.data_ptr(), size, stream)
     assert status == 0
     assert all(torch.equal(a, b) for a, b in zip(grads, want_grads))
+
+
+@pytest.mark.parametrize("q_heads,groups,far", [(64, 4, "kv"), (64, 8, "qkv"), (40, 40, "qkv"), (64, 2, "qkv")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_heads_in_front_through_the_operator(q_heads, groups, far, dtype):
+    """Keys and values of far heads are read in place whatever the heads that share them; queries where a key head's lie near
+    enough, and copied otherwise (64 over 2)."""
+    tokens, dim, ratio = 90, 64, q_heads // groups
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    q, do = (torch.randn(tokens, q_heads, dim, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    k, v = (torch.randn(tokens, groups, dim, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    cu = cu_tensor([tokens], "cuda")
+
+    def run(*leaves, grad):
+        leaves = [x.detach().requires_grad_() for x in leaves]
+        out, lse = msa.m3_window_attention(*leaves, cu, tokens, window_size=30, sink_tokens=2, return_lse=True)
+        return out.detach(), lse, *torch.autograd.grad(out, leaves, grad)
+
+    want = run(q, k, v, grad=do)
+    k, v = far_heads(k), far_heads(v)
+    assert aligned_rows(k)[0] is k and aligned_rows(v)[0] is v
+    if "q" in far:
+        q, do = far_heads(q), far_heads(do)
+        assert (aligned_rows(q, ratio)[0] is q) == (ratio < 16)
+    assert all(torch.equal(a, b) for a, b in zip(run(q, k, v, grad=do), want))
