@@ -87,10 +87,11 @@ __device__ __forceinline__ TileKeys tile_keys(const PagedWindowArgs& A, int n, i
   const int64_t last = A.pages.last_position(), c = context;
   K.hi = context < 0 ? -1 : static_cast<int>(min(c + K.b, last));
   const int64_t low = max(int64_t{0}, c + (A.parents ? 0 : K.a) - A.seen.window + 1);
-  K.low = static_cast<int>(min(low, static_cast<int64_t>(K.hi) + 32)) & ~31;  // (past hi: none)
+  // (past hi: none; a table may reach up to 2^31 - 17)
+  K.low = static_cast<int>(min(low, min(static_cast<int64_t>(K.hi) + 32, int64_t{0x7fffffff}))) & ~31;
   if (context < 0) K.low = 0;
   K.sinks = min(A.seen.sinks, min(K.low, K.hi + 1));
-  K.sink_steps = (K.sinks + 31) >> 5;
+  K.sink_steps = (K.sinks >> 5) + ((K.sinks & 31) != 0);
   K.steps = K.sink_steps + (K.hi >= K.low ? (K.hi >> 5) - (K.low >> 5) + 1 : 0);
   return K;
 }
@@ -703,7 +704,7 @@ __global__ __launch_bounds__(256, 2) void window_paged_rows_kernel(PagedWindowAr
     const int64_t c64 = P.context;
     const int common = scalar_int(A.parents ? c64 : min(c64 + first_tok, static_cast<int64_t>(K.hi)) + 1);
     const int low_most = scalar_int(c64 + (A.parents ? K.b : last_tok) - A.seen.window + 1);
-    const int low_least = scalar_int(c64 + (A.parents ? 0 : first_tok) - A.seen.window + 1);
+    const int low_least = scalar_int(max(c64 + (A.parents ? 0 : first_tok) - A.seen.window + 1, int64_t{0}));
     const int last_slot = scalar_int(min(c64 + last_tok, static_cast<int64_t>(K.hi)));
 
     // a maximum is kept of the raw dots (queries are turned where the scale is negative, and zero with a factor of 1 where it is 0)
@@ -793,7 +794,7 @@ __global__ __launch_bounds__(256, 2) void window_paged_rows_kernel(PagedWindowAr
         if (e + 1 < stop) load_step(e + 1);
         const bool of_sinks = e < K.sink_steps;
         if (has_rows && (now.p0 >= 0 || now.p1 >= 0) &&
-            (of_sinks || (now.key <= last_slot && (now.key + 32 > low_least || now.key < A.seen.sinks)))) {
+            (of_sinks || (now.key <= last_slot && (now.key > low_least - 32 || now.key < A.seen.sinks)))) {
           const uint16_t *kt = kbuf[b], *vt = vbuf[b];
           f32x4 sc[MT][2];
 #pragma unroll
