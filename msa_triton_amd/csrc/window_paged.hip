@@ -44,7 +44,6 @@ struct PagedWindowArgs {
   int G, D;
   Visible seen;
   float scale_log2;  // scale * log2(e)
-  int64_t tokens;
   uint16_t* out;  // [T][Hq][D]
   float* lse;     // [T][Hq], or null
   PagedPlan* plan;
@@ -1171,7 +1170,6 @@ extern "C" int msa_window_attn_paged(const void* q, const void* k_cache, const v
   A.D = static_cast<int>(head_dim);
   A.seen = visible_of(window, sinks);
   A.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  A.tokens = total_tokens;
   A.out = static_cast<uint16_t*>(out);
   A.lse = lse;
   A.plan = static_cast<PagedPlan*>(workspace);
