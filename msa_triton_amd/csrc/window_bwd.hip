@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WindowBwdArgs A) {
   if (c >> 2 == q4 && row0 + c < all) {  // row c of the product is in the quarter c / 4
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if ((c & 3) == i) A.delta[row0 + c] = sum[i] + left[i];
+      if ((c & 3) == i) A.delta[row0 + c] = finite(sum[i]) ? sum[i] + left[i] : sum[i];  // (an infinity times what is left out: any sign, or NaN)
   }
 }
 
