@@ -35,7 +35,8 @@ struct WindowFwdArgs {
 // The dims of a row that came out not finite, by a wave: where a value that is not finite met the products of a tile, which
 // multiply the keys that a row does not see by 0. Such values count whatever their weight above 0; a weight of 0 under
 // a logit of -inf makes NaN of them. Dims in which the row sees one are these values' sum, which takes a look at their
-// column; the others are formed again key by key. The weight is exp2(logit * log2(e) + shift).
+// column; the others are formed again key by key, from weights whose sum is 1 (values next to the end of fp32's range, of
+// which a tile's sums are infinities, have a finite mean). The weight is exp2(logit * log2(e) + shift) inv.
 template <int DT>
 __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, int g, int tok, int head, float shift,
                                             float inv) {
@@ -84,7 +85,7 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
     for (int base = from; base < to; base += kWave) {
       const int j = min(base + lane, to - 1), count = min(kWave, to - base);
       const float x = row_dot<DT>(q, k + static_cast<int64_t>(j) * A.k.token, A.D) * A.scale_log2;
-      const float p = __builtin_amdgcn_exp2f(x + shift);
+      const float p = __builtin_amdgcn_exp2f(x + shift) * inv;
       for (int i = 0; i < count; ++i) {
         const float p_i = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), i));
 #pragma unroll
@@ -101,7 +102,7 @@ __device__ __forceinline__ void careful_row(const WindowFwdArgs& A, int start, i
   for (int u = 0; u < 4; ++u) {
     if (!bad[u]) continue;
     const int d = lane + u * kWave;
-    const float y = odd[u] != 0.f ? odd[u] : o[u] * inv;
+    const float y = odd[u] != 0.f ? odd[u] : o[u];
     store_from_f32<DT>(A.out, at + d, y);
     if (DT != kF32 && A.out_lo) {
       uint16_t high;

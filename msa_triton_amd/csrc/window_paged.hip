@@ -125,7 +125,8 @@ __device__ __forceinline__ int parent_of(int p, int i) { return p >= 0 && p < i 
 // The dims of a row that came out not finite, by a wave: where a value that is not finite met the products of a tile, which
 // multiply the keys that a row does not see by 0. Such values count whatever their weight above 0; a weight of 0 under
 // a logit of -inf makes NaN of them. Dims in which the row sees one are these values' sum, which takes a look at their
-// column; the others are formed again key by key. The weight is exp2(logit * log2(e) - top).
+// column; the others are formed again key by key, from weights whose sum is 1 (values next to the end of fp32's range, of
+// which a tile's sums are infinities, have a finite mean). The weight is exp2(logit * log2(e) - top) inv.
 template <int DT, bool FP8>
 __device__ __forceinline__ void careful_row(const PagedWindowArgs& A, int s, int start, int context, int tok, int g, int head,
                                             float top, float inv) {
@@ -184,7 +185,7 @@ __device__ __forceinline__ void careful_row(const PagedWindowArgs& A, int s, int
         }
         return x * (A.scale_log2 * (FP8 ? A.k_scale[p0 * A.G + g] : 1.f));
       };
-      const float p = look ? 0.f : __builtin_amdgcn_exp2f(logit() - top);
+      const float p = look ? 0.f : __builtin_amdgcn_exp2f(logit() - top) * inv;
       uint64_t dead = 0;  // keys of a logit of -inf, looked for when a value is infinite
       bool known = false;
       for (uint64_t left = __ballot(seen); left; left &= left - 1) {
@@ -221,7 +222,7 @@ __device__ __forceinline__ void careful_row(const PagedWindowArgs& A, int s, int
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    if (bad[u]) store_from_f32<DT>(A.out, row * A.D + d + u, odd[u] != 0.f ? odd[u] : o[u] * inv);
+    if (bad[u]) store_from_f32<DT>(A.out, row * A.D + d + u, odd[u] != 0.f ? odd[u] : o[u]);
 }
 
 // Which keys a row sees: `low` the first of its window, `slot` its own.
