@@ -13,7 +13,11 @@
 // Bound by the matrix products, the vector work between them and the LDS reads that feed them: a wave of 32 rows (or keys)
 // reads 8 KB a product and 32 keys (or rows) of 128 dims. 32K tokens, 32 heads of 128 over 4, window 4096, bf16: dQ 3.6 ms, dK
 // and dV 6.4. Two waves a SIMD hide the waits (one: dQ 5.5, dK and dV 8.4); for dK and dV that takes the values
-// from LDS, the logits of 16 rows after those of the other 16, and 256 registers.
+// from LDS, the logits of 16 rows after those of the other 16, and 256 registers, of which bf16 at 128 dims spills 4 and at 256 dims
+// 14. fp16, whose keys also hold their ranges, spills 77 and 109, in the loop: dK and dV 15.2 ms for the case above where bf16 takes
+// 6.8 in the same run, 2.34 for 0.92 at 8192 tokens, 16 heads of 256 over 2, window 2048 (none at 64, 96 dims; one at 192). fp32 spills
+// 196 at 96 dims, behind the loop. careful_dkv, which is inlined, goes with 54 to 105 scalar registers spilled (the kernel of the first
+// tokens' rows, which has none of it: 0).
 //
 // Logits, p, ds and all sums are fp32. p enters its product rounded once to the input type; a ds enters as two terms (2^-17 of
 // it left out): one would be of the size of the gradients' own rounding and bring dq and dk from 0.0017 to 0.0024 of
@@ -748,9 +752,12 @@ SinkShape sink_shape(int32_t dtype, int64_t dim, int64_t tokens, int64_t nseq, i
   return sink_floats(shape, tokens, nseq, groups, dim) <= int64_t{1} << 26 ? shape : SinkShape{0, 0, 0, true};
 }
 
-// Workgroups that share the rows of a tile of keys: so many that the largest share is not above what each of the workgroups
-// that run at once (512, or 256 of more than 128 fp32 dims) gets of all the work, which is at least that of the longest sequence and of
-// sequences of equal length; no more than give a share 128 rows, nor than fill 256 MiB with parts.
+// Workgroups that share the rows of a tile of keys: the number next to the quotient of the largest tile's work and what each of the
+// workgroups that run at once (512, or 256 of more than 128 fp32 dims) gets of all the work, which is at least that of the longest
+// sequence and of sequences of equal length; no more than give a share 128 rows, nor than fill 256 MiB with parts. Rounding down leaves
+// a largest share of up to 1.5 times the even one, and rounds of workgroups that run at once are not counted: six fp16 sequences of
+// 1 to 6151 tokens, 16 heads of 96 over 4, window 1024 have a quotient of 1.39, one workgroup a tile, 524 in all, 12 of them in a second
+// round (414 us); two fp32 ones of 701 and 1347, 16 heads of 128 over 2, window 500 have 792 in 1.5 rounds (151 us).
 int64_t split_count(int32_t dtype, int64_t tokens, int64_t nseq, int64_t longest, int64_t q_heads, int64_t groups, int64_t dim,
                     int64_t window, bool whole) {
   const double keys = keys_per_tile(dtype, dim), w = window == 0 ? 1e18 : static_cast<double>(window);

@@ -12,7 +12,9 @@
 // the block-sparse form: key fragments straight from memory, S^T = K Q^T, weights as they come out of it, values through
 // the wave's LDS tile. A tile that lies in one stretch is finished there; the parts of the others, maxima, sums and fp32
 // outputs, are joined by a second launch in a fixed order. 64 requests of 60 to 30 000 tokens, 4 key heads of 128, 16 bits, no
-// window: 131 + 10 us, 4.8 TB/s; 512, 300 and 1 new tokens behind 8192, 1000 and 5000, window 2048, 32 heads: 61 + 16 us.
+// window: 131 + 11 us, 4.8 TB/s; 512, 300 and 1 new tokens behind 8192, 1000 and 5000, window 2048, 32 heads: 60 + 16 us.
+// The attention kernels spill 102 to 179 scalar registers into lanes of vector registers (careful_row is inlined in them); of vector
+// registers e4m3 at 256 dims spills 38 a lane, and 16 bits at 256 dims with 16 rows a tile takes 430, one wave a SIMD.
 //
 // Logits, statistics and outputs are fp32. With one tile of 16 rows, where the products are not the bound, a weight
 // enters the second product as two 16-bit terms (2^-17 of it left out); with more it is rounded once, as in the packed
@@ -292,7 +294,8 @@ struct Batch {
       items = S.first_item[256];
     }
     most = __builtin_amdgcn_readfirstlane(most);
-    // four steps at least, and no tile in more than kMostParts stretches
+    // four steps at least (one a wave of the kernel of 16 rows; the one of many rows takes them one after the other: 15 nodes behind
+    // 1999 tokens, 4 key heads, in 64 workgroups 24 us), and no tile in more than kMostParts stretches
     items = scalar(items);
     const int64_t share = scalar(max(max(int64_t{4}, quotient(items + gridDim.x - 1, gridDim.x)),
                                      static_cast<int64_t>((most + kMostParts - 2) / (kMostParts - 1))));
@@ -1078,7 +1081,8 @@ __global__ __launch_bounds__(256) void window_paged_join(PagedWindowArgs A, int6
 }
 
 // Rows of a tile: 16, gone through by the waves of a workgroup key by key, where no sequence has more of them a key head;
-// otherwise 64, or 128 (of more than 128 dims a wave's registers hold 16).
+// otherwise 64, or 128 (of more than 128 dims a wave's registers hold 16). One size for all sequences of a call: a long one among
+// single tokens takes those to its own tiles and to weights that are rounded once.
 int tile_rows(int64_t longest, int64_t ratio, int64_t dim) { return longest * ratio <= 16 ? 16 : longest * ratio <= 64 || dim > 128 ? 64 : 128; }
 
 // Workgroups of a call at most. 512 run at once; with 16 rows twice as many, whose waves' waits differ, draw more of HBM (64 requests

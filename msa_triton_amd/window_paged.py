@@ -107,8 +107,9 @@ def m3_window_attention_paged(
     ``sink_tokens``. 8-bit caches (``torch.float8_e4m3fn``) come with ``k_scale`` and ``v_scale`` (fp32 ``[P,G]``). Keys
     in missing pages do not exist (pages that lie wholly between the first tokens and the window may be given
     back); rows without keys, and those of an absent sequence (negative ``context_lens``), give zero output and an LSE of
-    -inf. Values that are not finite give what the formula gives, as in ``m3_sparse_attention_paged``. ``D`` is a
-    multiple of 16 up to 256."""
+    -inf. Values that are not finite give what the formula gives, as in ``m3_sparse_attention_paged``; a row whose logits are
+    all -inf has an output of 0. ``D`` is a multiple of 16 up to 256. How softmax weights are rounded goes by the
+    longest sequence of the call, so a request's last bits depend on its batch."""
     return _attend("m3_window_attention_paged", q, k_cache, v_cache, page_table, cu_seqlens, context_lens, None, window_size,
                    sink_tokens, scale, k_scale, v_scale, return_lse)
 
