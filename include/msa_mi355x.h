@@ -327,7 +327,7 @@ int msa_attn_paged(const void* q, const void* k_cache, const void* v_cache, int3
  * rounding left out, rounded to `dtype` as well; lse [T,Hq] (NULL: none) natural log. strides (host array, elements):
  * q token, head; k token, head; v token, head; unit stride along D, rows 16-byte aligned. A token stride is below 2^25, a head
  * stride below 2^30, 33 token strides (of q: and Hq / G head strides with them) are below 2^30. head_dim: a multiple of 8 up
- * to 256; T * Hq / G below 0x7fff0000 (status 2 otherwise). One launch. */
+ * to 256; T * Hq / G below 0x7fff0000 (status 2 otherwise); a scale of at most 2e38. One launch. */
 int msa_window_attn_fwd(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
                         const int32_t* cu_seqlens, int64_t num_seqs, int64_t total_tokens, int64_t q_heads,
                         int64_t kv_groups, int64_t head_dim, int64_t window, int64_t sinks, double scale, void* out,

@@ -299,13 +299,16 @@ inline bool near_rows(const int64_t* strides, int64_t heads) {
          33 * strides[0] + heads * strides[1] < (1 << 30);
 }
 
+// scale * log2(e) is held in fp32
+inline bool valid_scale(double scale) { return scale >= -2e38 && scale <= 2e38; }
+
 // What the packed entry points check. strides: token and head strides of q, k, v (elements).
 inline bool valid_window_call(const void* q, const void* k, const void* v, int32_t dtype, const int64_t* strides,
                               const int32_t* cu, int64_t num_seqs, int64_t tokens, int64_t q_heads, int64_t groups,
                               int64_t dim, int64_t window, int64_t sinks, double scale) {
   if (!q || !k || !v || !strides || !cu || num_seqs <= 0 || num_seqs > 0x3fffffff || tokens < 0 || tokens > 0x7fffffff ||
       groups <= 0 || q_heads <= 0 || q_heads % groups || q_heads >= (1 << 20) || dim <= 0 || window < 0 || sinks < 0 ||
-      !__builtin_isfinite(scale) || (dtype != kF32 && dtype != kF16 && dtype != kBF16))
+      !valid_scale(scale) || (dtype != kF32 && dtype != kF16 && dtype != kBF16))
     return false;
   const int unit = dtype == kF32 ? 4 : 8;  // 16 bytes
   for (int i = 0; i < 6; ++i)

@@ -1137,7 +1137,7 @@ extern "C" int msa_window_attn_paged(const void* q, const void* k_cache, const v
                                      void* stream) {
   if (!q || !out || !strides || !cu_seqlens || !context_lens || num_seqs <= 0 || num_seqs > 0x3fffffff || total_tokens < 0 ||
       total_tokens > 0x7fffffff || longest < 0 || longest > total_tokens || q_heads <= 0 || kv_groups <= 0 ||
-      q_heads % kv_groups || q_heads >= (1 << 20) || head_dim <= 0 || window < 0 || sinks < 0 || !__builtin_isfinite(scale) ||
+      q_heads % kv_groups || q_heads >= (1 << 20) || head_dim <= 0 || window < 0 || sinks < 0 || !valid_scale(scale) ||
       (dtype != kBF16 && dtype != kF16) || !valid_pages(page_table, table_stride, pages_per_seq, num_pages, page_size) ||
       (num_pages > 0 && (!k_cache || !v_cache || (cache_is_fp8 && (!k_scale || !v_scale)))))
     return kErrInvalidArgument;

@@ -12,7 +12,6 @@ out (delta = dO . O is formed from both).
 
 from __future__ import annotations
 
-import math
 import struct
 
 import torch
@@ -34,6 +33,14 @@ def check_window(window_size, sink_tokens):
         raise ValueError("sink_tokens must be a nonnegative integer")
     most = 2147483647
     return 0 if window_size is None or window_size >= most else window_size, min(sink_tokens, most)
+
+
+def check_scale(scale, dim):
+    """The scale of a call. Kernels hold scale * log2(e) in fp32, where it has to be finite as well."""
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= 2e38:
+        raise ValueError("scale must be finite, of at most 2e38.")
+    return scale
 
 
 def aligned_rows(x, near_heads=0):
@@ -155,9 +162,7 @@ def _validate(q, k, v, cu_seqlens, max_seqlen, window_size, sink_tokens, scale):
         cu, num_seqs, longest = cu_seqlens.contiguous(), len(lengths), max(lengths)
     if longest > max_seqlen:
         raise ValueError("max_seqlen is smaller than an actual sequence.")
-    effective_scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(effective_scale):
-        raise ValueError("scale must be finite.")
+    effective_scale = check_scale(scale, dim)
     if dim > MAX_HEAD_DIM or dim % 8:
         raise NotImplementedError("m3_window_attention takes head dims that are multiples of 8 up to 256")
     if heads * dim >= 1 << 24:
@@ -187,8 +192,8 @@ def m3_window_attention(
     contiguous and 16-byte aligned to be read in place (slices of a fused projection are); others are copied. The
     optional natural-log LSE is FP32 and non-differentiable. What is not finite reaches the rows that see it and
     no others: a value that is an infinity makes its dim one whatever the weight (NaN where both signs meet). A row whose
-    logits are all -inf has an output of 0 and an LSE of -inf, as in ``m3_sparse_attention``. Head dims are multiples of 8 up to
-    256."""
+    logits are all -inf has an output of 0 and an LSE of -inf, as in ``m3_sparse_attention``. ``scale`` (default ``D ** -0.5``) is at
+    most 2e38 in magnitude. Head dims are multiples of 8 up to 256."""
     cu, num_seqs, longest, window, sinks, effective_scale = _validate(q, k, v, cu_seqlens, max_seqlen, window_size,
                                                                       sink_tokens, scale)
     if wanted(q, k, v):

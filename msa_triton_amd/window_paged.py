@@ -10,7 +10,6 @@ only. No gradients: differentiating the outputs raises.
 
 from __future__ import annotations
 
-import math
 import struct
 
 import torch
@@ -19,7 +18,7 @@ from . import _lib
 from .derivatives import NoBackward, wanted
 from .layout import PackedSequences
 from .paged import check_kv_caches, check_pages, sixteen_bit
-from .window_attention import check_window
+from .window_attention import check_scale, check_window
 
 _pack_strides = struct.Struct("6q").pack
 MAX_TREE_NODES = 512
@@ -37,9 +36,7 @@ def _attend(name, q, k_cache, v_cache, page_table, cu_seqlens, context_lens, par
         raise ValueError("k_cache must be [pages, G, page size, D] with Hq a positive multiple of G")
     page, strides, fp8 = check_kv_caches(k_cache, v_cache, k_scale, v_scale, groups, dim, dtype, device)
     window, sinks = check_window(window_size, sink_tokens)
-    effective_scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(effective_scale):
-        raise ValueError("scale must be finite")
+    effective_scale = check_scale(scale, dim)
     pages, cu, num_seqs, context, page_map = check_pages(page_table, cu_seqlens, context_lens, total, page, k_cache, device)
     if isinstance(cu_seqlens, PackedSequences):
         longest = cu_seqlens.max_seqlen
